@@ -1,0 +1,92 @@
+// attn.cu - entry point of the paged attention (ftb_attention): argument checks, tensor maps,
+// and the choice between the kernels.
+#include <cudaTypedefs.h>
+
+#include <cmath>
+#include <mutex>
+
+#include "attn.cuh"
+
+namespace ftb {
+
+PFN_cuTensorMapEncodeTiled encode_fn();  // moe_decode_tma.cu
+
+CUtensorMapDataType attn_dtype(int type) {
+  return type == FTB_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+}
+
+int attn_cache_map(CUtensorMap* m, const void* base, const ftb_attn_args& a,
+                   const int64_t (&strides)[3], uint32_t box_rows, uint32_t halves) {
+  PFN_cuTensorMapEncodeTiled fn = encode_fn();
+  if (!fn) return FTB_ERR_CUDA;
+  const bool split = halves > 1;  // the halves of a head as a dimension of their own
+  const cuuint64_t dims[5] = {split ? 64u : (cuuint64_t)a.D, (cuuint64_t)a.page,
+                              (cuuint64_t)a.Hkv, (cuuint64_t)a.num_pages, halves};
+  const cuuint64_t st[4] = {(cuuint64_t)strides[1] * 2, (cuuint64_t)strides[2] * 2,
+                            (cuuint64_t)strides[0] * 2, 128};
+  const cuuint32_t box[5] = {64, box_rows, 1, 1, halves};
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  const CUresult r = fn(m, attn_dtype(a.type), 5, const_cast<void*>(base), dims, st, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? FTB_OK : FTB_ERR_CUDA;
+}
+
+}  // namespace ftb
+
+using namespace ftb;
+
+extern "C" {
+
+size_t ftb_attention_workspace_bytes(int64_t total_q, int batch, int max_q, int Hq, int Hkv, int D) {
+  if (total_q < 0 || batch < 0 || max_q < 0 || Hkv < 1 || Hq < Hkv || D < 8) return 0;
+  return FTB_ATTN_ZERO_BYTES + attn_stream_partial_bytes((int64_t)max_q * (Hq / Hkv), D);
+}
+
+int ftb_attention(const ftb_attn_args* a, ftb_stream_t stream) {
+  if (!a) return FTB_ERR_ARG;
+  if (a->type != FTB_TYPE_BF16 && a->type != FTB_TYPE_F16) return FTB_ERR_ARG;
+  if (a->total_q < 0 || a->total_q > 0x7fffffff || a->batch < 0 || a->max_q < 0 || a->Hkv < 1 ||
+      a->Hq < 1 || a->Hq % a->Hkv || a->Hq / a->Hkv > 128 || a->D < 8 || a->D > 128 || a->D % 8 ||
+      a->page < 8 || (a->page & (a->page - 1)) || a->num_pages < 1 ||
+      a->num_pages > 0x7fffffff - 1 || a->table_width < 0 || a->window < 0 ||
+      (int64_t)a->table_width * a->page > 0x7fffff00)
+    return FTB_ERR_SHAPE;
+  if (a->total_q == 0 || a->batch == 0 || a->max_q == 0) return FTB_OK;
+  if (!a->q || !a->k_cache || !a->v_cache || !a->block_table || !a->kv_len || !a->out)
+    return FTB_ERR_ARG;
+  if (!a->cu_q && a->total_q != a->batch) return FTB_ERR_SHAPE;
+  if (!std::isfinite(a->scale)) return FTB_ERR_ARG;
+  if (!aligned16(a->q) || !aligned16(a->k_cache) || !aligned16(a->v_cache) || !aligned16(a->out))
+    return FTB_ERR_ALIGN;
+  for (int i = 0; i < 3; ++i)
+    if (a->k_strides[i] % 8 || a->v_strides[i] % 8 || a->k_strides[i] < 0 || a->v_strides[i] < 0)
+      return FTB_ERR_ALIGN;
+  for (int i = 0; i < 2; ++i)
+    if (a->q_strides[i] % 8 || a->q_strides[i] < 0) return FTB_ERR_ALIGN;
+  if (!a->workspace ||
+      a->workspace_bytes < ftb_attention_workspace_bytes(a->total_q, a->batch, a->max_q, a->Hq,
+                                                         a->Hkv, a->D))
+    return FTB_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(a->workspace) & 255u) return FTB_ERR_ALIGN;
+  AttnParams P{};
+  P.q = a->q, P.out = a->out, P.lse = a->lse;
+  P.block_table = a->block_table, P.kv_len = a->kv_len, P.cu_q = a->cu_q;
+  char* ws = static_cast<char*>(a->workspace);
+  P.status = reinterpret_cast<uint32_t*>(ws);
+  P.counters = reinterpret_cast<int32_t*>(ws + 16);
+  P.partial = reinterpret_cast<float*>(ws + FTB_ATTN_ZERO_BYTES);
+  P.q_st = a->q_strides[0], P.q_sh = a->q_strides[1];
+  P.total_q = a->total_q, P.table_stride = a->table_stride, P.num_pages = a->num_pages;
+  P.batch = a->batch, P.max_q = a->max_q, P.table_width = a->table_width;
+  int lg = 0;
+  while ((1 << lg) < a->page) ++lg;
+  P.page_log2 = lg;
+  P.Hq = a->Hq, P.Hkv = a->Hkv, P.G = a->Hq / a->Hkv, P.D = a->D;
+  P.causal = a->causal != 0, P.window = a->window;
+  P.keys_max = a->table_width * a->page;
+  P.scale_log2 = a->scale * 1.44269504088896341f;
+  return launch_attn_stream(*a, P, (cudaStream_t)stream);
+}
+
+}  // extern "C"

@@ -734,6 +734,9 @@ __global__ void __launch_bounds__((NW + 1) * kWarp, CPS)
 // ---------------------------------------------------------------------------------------
 // host: tensor maps (cached by address and shape) and launches
 
+}  // namespace
+
+// cuTensorMapEncodeTiled, looked up once (NULL where the driver has none).
 PFN_cuTensorMapEncodeTiled encode_fn() {
   static PFN_cuTensorMapEncodeTiled fn = nullptr;
   static std::once_flag once;
@@ -747,6 +750,8 @@ PFN_cuTensorMapEncodeTiled encode_fn() {
   });
   return fn;
 }
+
+namespace {
 
 struct MapKey {
   const void* base;

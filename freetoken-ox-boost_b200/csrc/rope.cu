@@ -1,0 +1,261 @@
+// rope.cu - rotary positions on one or several axes, with the write of the new tokens' keys and
+// values into the paged cache.
+//
+// Frequency i of a head turns the pair (a, b) = (x[i], x[i + rot/2]) ("half" pairs) or
+// (x[2i], x[2i+1]) ("adjacent") by the angle of position[axis(i)]:
+//   a' = a cos - b sin,  b' = b cos + a sin            (fp32, rounded once)
+// cos and sin come from a table [positions, rot] (cos in its first rot/2 columns); elements past
+// rot are copied. q goes to q_out, k (rotated) and v (copied) to the cache row of the token's
+// slot, or to k_out without a cache.
+//
+// Bound: DRAM, 2 * (Hq + 2 Hkv) * D * 2 bytes per token. One block per token; a thread owns one
+// column of VEC pairs in every head it visits, so it reads the token's cos and sin once into
+// registers and needs no shared memory or barrier.
+#include "ftb_common.cuh"
+
+namespace ftb {
+namespace {
+
+constexpr int kMaxPairs = 128;  // rot <= 256
+
+struct RopeParams {
+  const uint16_t *q, *k, *v;
+  uint16_t *q_out, *k_dst, *v_dst;
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;      // token and head strides, elements
+  int64_t kc_page, kc_tok, kc_head;                // cache strides (k_out: kc_tok, kc_head)
+  int64_t vc_page, vc_tok, vc_head;
+  const void* positions;  // [axes, tokens], axis stride pos_stride
+  int64_t pos_stride;
+  const float* table;
+  int64_t table_rows;
+  const void* slots;  // NULL: k_dst holds a row per token
+  int64_t tokens, n_slots;
+  int pos64, slot64, page, Hq, Hkv, D, rot, adjacent, axes;
+  uint32_t axis[kMaxPairs / 16];  // 2 bits per frequency
+};
+
+template <int VEC>
+struct Chunk;
+template <>
+struct Chunk<8> { using type = uint4; };
+template <>
+struct Chunk<4> { using type = uint2; };
+template <>
+struct Chunk<1> { using type = uint16_t; };
+
+template <typename T>
+__device__ __forceinline__ float elem_f32(uint16_t b);
+template <>
+__device__ __forceinline__ float elem_f32<__nv_bfloat16>(uint16_t b) { return bf16_bits_to_f32(b); }
+template <>
+__device__ __forceinline__ float elem_f32<__half>(uint16_t b) { return __half2float(__ushort_as_half(b)); }
+template <typename T>
+__device__ __forceinline__ uint16_t elem_bits(float f);
+template <>
+__device__ __forceinline__ uint16_t elem_bits<__nv_bfloat16>(float f) { return f32_to_bf16_bits(f); }
+template <>
+__device__ __forceinline__ uint16_t elem_bits<__half>(float f) { return __half_as_ushort(__float2half_rn(f)); }
+
+template <int VEC>
+__device__ __forceinline__ void load_bits(const uint16_t* p, uint16_t (&v)[VEC]) {
+  // a plain load: q_out may be q itself
+  const typename Chunk<VEC>::type w = *reinterpret_cast<const typename Chunk<VEC>::type*>(p);
+  memcpy(v, &w, sizeof(w));
+}
+template <int VEC>
+__device__ __forceinline__ void store_bits(uint16_t* p, const uint16_t (&v)[VEC]) {
+  typename Chunk<VEC>::type w;
+  memcpy(&w, v, sizeof(w));
+  *reinterpret_cast<typename Chunk<VEC>::type*>(p) = w;
+}
+
+// Block (cols, heads per sweep): column threadIdx.x of 2 VEC elements, of each head.
+template <typename T, int VEC>
+__global__ void k_rope(const __grid_constant__ RopeParams P) {
+  pdl_launch_dependents();
+  const int col = threadIdx.x;
+  const int half = P.rot / 2, rot_cols = half / VEC;
+  const bool turns = col < rot_cols;
+  // element offsets of this column's two chunks in a rotated head and in a copied one
+  int e0, e1;
+  if (!turns) {
+    e0 = P.rot + (col - rot_cols) * 2 * VEC;
+    e1 = e0 + VEC;
+  } else if (P.adjacent) {
+    e0 = col * 2 * VEC;
+    e1 = e0 + VEC;
+  } else {
+    e0 = col * VEC;
+    e1 = e0 + half;
+  }
+  const int c0 = col * 2 * VEC;
+  pdl_wait();
+  const int64_t tok = blockIdx.x;
+  float cs[VEC], sn[VEC];
+  if (turns) {
+    int64_t at[4];
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      at[a] = 0;
+      if (a < P.axes)
+        at[a] = P.pos64 ? static_cast<const int64_t*>(P.positions)[a * P.pos_stride + tok]
+                        : static_cast<const int32_t*>(P.positions)[a * P.pos_stride + tok];
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const int i = col * VEC + j;
+      const int a = (P.axis[i >> 4] >> (2 * (i & 15))) & 3;
+      const int64_t p = a == 0 ? at[0] : a == 1 ? at[1] : a == 2 ? at[2] : at[3];
+      // a position outside the table has no angle: the outputs are NaN, not another position's
+      const bool in = p >= 0 && p < P.table_rows;
+      const float* row = P.table + (in ? p : 0) * P.rot;
+      cs[j] = in ? __ldg(row + i) : __int_as_float(0x7fffffff);
+      sn[j] = in ? __ldg(row + half + i) : __int_as_float(0x7fffffff);
+    }
+  }
+  int64_t slot = tok, page = 0;
+  bool keep = true;
+  if (P.slots) {
+    slot = P.slot64 ? static_cast<const int64_t*>(P.slots)[tok]
+                    : static_cast<const int32_t*>(P.slots)[tok];
+    keep = slot >= 0 && slot < P.n_slots;  // -1: a padded token, not stored
+    page = slot / P.page;
+    slot -= page * P.page;
+  }
+  const int heads = P.Hq + 2 * P.Hkv;
+  for (int hh = threadIdx.y; hh < heads; hh += blockDim.y) {
+    const uint16_t* src;
+    uint16_t* dst;
+    bool copy = !turns;
+    int f0 = e0, f1 = e1;
+    if (hh < P.Hq) {
+      src = P.q + tok * P.q_st + hh * P.q_sh;
+      dst = P.q_out + (tok * P.Hq + hh) * P.D;
+    } else if (hh < P.Hq + P.Hkv) {
+      if (!keep) continue;
+      const int h = hh - P.Hq;
+      src = P.k + tok * P.k_st + h * P.k_sh;
+      dst = P.k_dst + page * P.kc_page + slot * P.kc_tok + h * P.kc_head;
+    } else {
+      if (!keep || !P.v_dst) continue;
+      const int h = hh - P.Hq - P.Hkv;
+      src = P.v + tok * P.v_st + h * P.v_sh;
+      dst = P.v_dst + page * P.vc_page + slot * P.vc_tok + h * P.vc_head;
+      copy = true;
+      f0 = c0;
+      f1 = c0 + VEC;
+    }
+    uint16_t a[VEC], b[VEC];
+    load_bits<VEC>(src + f0, a);
+    load_bits<VEC>(src + f1, b);
+    if (!copy) {
+      if (P.adjacent) {
+        uint16_t w[2 * VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) w[j] = a[j], w[VEC + j] = b[j];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float u = elem_f32<T>(w[2 * j]), v = elem_f32<T>(w[2 * j + 1]);
+          w[2 * j] = elem_bits<T>(u * cs[j] - v * sn[j]);
+          w[2 * j + 1] = elem_bits<T>(v * cs[j] + u * sn[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) a[j] = w[j], b[j] = w[VEC + j];
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float u = elem_f32<T>(a[j]), v = elem_f32<T>(b[j]);
+          a[j] = elem_bits<T>(u * cs[j] - v * sn[j]);
+          b[j] = elem_bits<T>(v * cs[j] + u * sn[j]);
+        }
+      }
+    }
+    store_bits<VEC>(dst + f0, a);
+    store_bits<VEC>(dst + f1, b);
+  }
+}
+
+template <typename T, int VEC>
+int launch_rope(const RopeParams& P, cudaStream_t stream) {
+  const int cols = P.D / (2 * VEC), heads = P.Hq + 2 * P.Hkv;
+  const int most = 256 / cols < 1 ? 1 : 256 / cols;
+  const int sweeps = (heads + most - 1) / most;
+  const dim3 block(cols, (heads + sweeps - 1) / sweeps);
+  return cuda_status(launch_pdl(k_rope<T, VEC>, dim3((unsigned)P.tokens), block, 0, stream, P));
+}
+
+template <typename T>
+int pick_rope(const RopeParams& P, int vec, cudaStream_t stream) {
+  return vec == 8   ? launch_rope<T, 8>(P, stream)
+         : vec == 4 ? launch_rope<T, 4>(P, stream)
+                    : launch_rope<T, 1>(P, stream);
+}
+
+}  // namespace
+}  // namespace ftb
+
+using namespace ftb;
+
+extern "C" int ftb_rope(const ftb_rope_args* a, ftb_stream_t stream) {
+  if (!a) return FTB_ERR_ARG;
+  if (a->tokens < 0 || a->tokens > 0x7fffffff || a->Hq < 1 || a->Hkv < 1 || a->D < 2 ||
+      a->D > 512 || a->D % 2 || a->rot < 2 || a->rot % 2 || a->rot > a->D ||
+      a->rot > 2 * kMaxPairs || a->axes < 1 || a->axes > 4 || a->table_rows < 1)
+    return FTB_ERR_SHAPE;
+  if (a->type != FTB_TYPE_BF16 && a->type != FTB_TYPE_F16) return FTB_ERR_ARG;
+  if (a->pairs != FTB_PAIRS_HALF && a->pairs != FTB_PAIRS_ADJACENT) return FTB_ERR_ARG;
+  if (a->order != FTB_AXES_BLOCKS && a->order != FTB_AXES_CYCLIC) return FTB_ERR_ARG;
+  const int half = a->rot / 2;
+  RopeParams P{};
+  int sum = 0;
+  for (int x = 0; x < a->axes; ++x) {
+    if (a->sections[x] < 0) return FTB_ERR_SHAPE;
+    sum += a->sections[x];
+  }
+  if (sum != half) return FTB_ERR_SHAPE;
+  for (int i = 0, x = 0, used = 0; i < half; ++i) {
+    int axis;
+    if (a->order == FTB_AXES_BLOCKS) {
+      while (used == a->sections[x]) ++x, used = 0;
+      ++used;
+      axis = x;
+    } else {  // the axes in turn while an axis has frequencies left, axis 0 for the rest
+      axis = i % a->axes;
+      if (i / a->axes >= a->sections[axis]) axis = 0;
+    }
+    P.axis[i >> 4] |= (uint32_t)axis << (2 * (i & 15));
+  }
+  if (a->tokens == 0) return FTB_OK;
+  if (!a->q || !a->k || !a->q_out || !a->k_dst || !a->positions || !a->table) return FTB_ERR_ARG;
+  if (a->slots ? (!a->v || !a->v_dst || a->page < 1) : (a->v_dst != nullptr)) return FTB_ERR_ARG;
+  P.q = a->q, P.k = a->k, P.v = a->v, P.q_out = a->q_out, P.k_dst = a->k_dst, P.v_dst = a->v_dst;
+  P.q_st = a->q_strides[0], P.q_sh = a->q_strides[1];
+  P.k_st = a->k_strides[0], P.k_sh = a->k_strides[1];
+  P.v_st = a->v_strides[0], P.v_sh = a->v_strides[1];
+  P.kc_page = a->k_dst_strides[0], P.kc_tok = a->k_dst_strides[1], P.kc_head = a->k_dst_strides[2];
+  P.vc_page = a->v_dst_strides[0], P.vc_tok = a->v_dst_strides[1], P.vc_head = a->v_dst_strides[2];
+  P.positions = a->positions, P.pos_stride = a->pos_stride, P.table = a->table;
+  P.table_rows = a->table_rows, P.slots = a->slots, P.tokens = a->tokens;
+  P.n_slots = a->n_slots, P.pos64 = a->pos64, P.slot64 = a->slot64, P.page = a->page;
+  P.Hq = a->Hq, P.Hkv = a->Hkv, P.D = a->D, P.rot = a->rot;
+  P.adjacent = a->pairs == FTB_PAIRS_ADJACENT, P.axes = a->axes;
+  // the widest chunk that divides the rotated and the copied part, and that every head of every
+  // operand starts aligned to
+  auto fits = [&](int n) {
+    if (half % n || (a->D - a->rot) % (2 * n) || a->D % (2 * n)) return false;
+    uint64_t m = 0;
+    const void* ptrs[] = {a->q, a->k, a->q_out, a->k_dst, a->v_dst ? a->v : nullptr, a->v_dst};
+    for (const void* p : ptrs) m |= reinterpret_cast<uintptr_t>(p);
+    int64_t st = 0;
+    for (int i = 0; i < 2; ++i) st |= a->q_strides[i] | a->k_strides[i];
+    for (int i = 0; i < 3; ++i) st |= a->k_dst_strides[i];
+    if (a->v_dst) {
+      for (int i = 0; i < 2; ++i) st |= a->v_strides[i];
+      for (int i = 0; i < 3; ++i) st |= a->v_dst_strides[i];
+    }
+    return (m | (uint64_t)(st * 2)) % (2 * n) == 0;
+  };
+  const int vec = fits(8) ? 8 : fits(4) ? 4 : 1;
+  return a->type == FTB_TYPE_BF16 ? pick_rope<__nv_bfloat16>(P, vec, (cudaStream_t)stream)
+                                  : pick_rope<__half>(P, vec, (cudaStream_t)stream);
+}

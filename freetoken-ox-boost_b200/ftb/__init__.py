@@ -3,7 +3,9 @@
 Host code is Python/PyTorch; all device work runs in ``libftb.so`` (hand-written CUDA,
 C ABI in ``include/ftb.h``), loaded through ctypes. There is no CPU or Triton fallback.
 """
+from .attention import paged_attention
 from .banks import Nvfp4Bank, bank_bytes_per_expert
+from .block import block_norm, rms_norm, rope, rope_append, rope_table
 from .checkpoint import bank_from_modelopt, bank_to_modelopt, moe_layers_in
 from .ds_fp4 import DsFp4Bank, fused_experts_ds_fp4, nvfp4_from_ds_fp4
 from .ep import EpGroup, ExpertParallelMoE
@@ -20,5 +22,6 @@ __all__ = [
     "moe_align_block_size", "moe_decode", "moe_prefill", "moe_prefill_fp4", "quant_nvfp4",
     "fused_route", "fused_route_ranked", "fused_topk", "router_logits",
     "bank_from_modelopt", "bank_to_modelopt", "moe_layers_in", "EpGroup", "ExpertParallelMoE",
+    "paged_attention", "block_norm", "rms_norm", "rope", "rope_append", "rope_table",
     "DsFp4Bank", "fused_experts_ds_fp4", "nvfp4_from_ds_fp4",
 ]

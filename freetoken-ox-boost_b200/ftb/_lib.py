@@ -75,6 +75,51 @@ class MoeArgsStruct(ctypes.Structure):
         ("shared_out", _vp), ("h_quant", _i32),
     ]
 
+FTB_TYPE_BF16, FTB_TYPE_F16, FTB_TYPE_F32 = 0, 1, 2
+FTB_GATE_NONE, FTB_GATE_CHANNEL, FTB_GATE_TOKEN, FTB_GATE_FULL = 0, 1, 2, 3
+FTB_GATE_LINEAR, FTB_GATE_SIGMOID = 0, 1
+FTB_PAIRS_HALF, FTB_PAIRS_ADJACENT = 0, 1
+FTB_AXES_BLOCKS, FTB_AXES_CYCLIC = 0, 1
+FTB_ATTN_ZERO_BYTES = 65536
+ATTN_BAD_PAGE, ATTN_BAD_ROWS, ATTN_TIMEOUT = 1, 2, 4
+
+
+class NormArgsStruct(ctypes.Structure):
+    """``ftb_norm_args``"""
+    _fields_ = [
+        ("x", _vp), ("y", _vp), ("gate", _vp), ("post", _vp), ("pre", _vp), ("r", _vp),
+        ("h", _vp), ("rows", _i64), ("x_stride", _i64), ("y_stride", _i64),
+        ("gate_stride", _i64), ("H", _i32), ("type", _i32), ("residual_type", _i32),
+        ("weights_f32", _i32), ("gate_kind", _i32), ("gate_act", _i32), ("scale", _f32),
+        ("eps", _f32),
+    ]
+
+
+class RopeArgsStruct(ctypes.Structure):
+    """``ftb_rope_args``"""
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("v", _vp), ("q_out", _vp), ("k_dst", _vp), ("v_dst", _vp),
+        ("q_strides", _i64 * 2), ("k_strides", _i64 * 2), ("v_strides", _i64 * 2),
+        ("k_dst_strides", _i64 * 3), ("v_dst_strides", _i64 * 3), ("positions", _vp),
+        ("pos_stride", _i64), ("table", _vp), ("table_rows", _i64), ("slots", _vp),
+        ("n_slots", _i64), ("tokens", _i64), ("pos64", _i32), ("slot64", _i32), ("page", _i32),
+        ("Hq", _i32), ("Hkv", _i32), ("D", _i32), ("rot", _i32), ("axes", _i32),
+        ("sections", _i32 * 4), ("order", _i32), ("pairs", _i32), ("type", _i32),
+    ]
+
+
+class AttnArgsStruct(ctypes.Structure):
+    """``ftb_attn_args``"""
+    _fields_ = [
+        ("q", _vp), ("k_cache", _vp), ("v_cache", _vp), ("block_table", _vp), ("kv_len", _vp),
+        ("cu_q", _vp), ("out", _vp), ("lse", _vp), ("workspace", _vp), ("workspace_bytes", _sz),
+        ("q_strides", _i64 * 2), ("k_strides", _i64 * 3), ("v_strides", _i64 * 3),
+        ("total_q", _i64), ("num_pages", _i64), ("table_stride", _i64), ("batch", _i32),
+        ("max_q", _i32), ("table_width", _i32), ("page", _i32), ("Hq", _i32), ("Hkv", _i32),
+        ("D", _i32), ("causal", _i32), ("window", _i32), ("type", _i32), ("scale", _f32),
+    ]
+
+
 SIGNATURES = {
     "ftb_status_string": (ctypes.c_char_p, [_i32]),
     "ftb_version": (_i32, []),
@@ -118,6 +163,10 @@ SIGNATURES = {
                                      _vp, _vp]),
     "ftb_ep_status": (_i32, [_vp, _i32, _vp]),
     "ftb_ep_destroy": (_i32, [_vp]),
+    "ftb_block_norm": (_i32, [ctypes.POINTER(NormArgsStruct), _vp]),
+    "ftb_rope": (_i32, [ctypes.POINTER(RopeArgsStruct), _vp]),
+    "ftb_attention_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32, _i32, _i32]),
+    "ftb_attention": (_i32, [ctypes.POINTER(AttnArgsStruct), _vp]),
     "ftb_profile_begin": (_i32, []),
     "ftb_profile_end": (_i32, [_vp, _vp, _i32]),
 }

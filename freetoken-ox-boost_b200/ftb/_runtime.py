@@ -46,6 +46,17 @@ def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     return t
 
 
+def zeroed_workspace(nbytes: int, device: torch.device) -> torch.Tensor:
+    """A cached buffer like :func:`workspace`, of its own and zero-filled when it is made: for
+    calls whose counters start at zero and are left at zero."""
+    key = (device.index, torch.cuda.current_stream(device).cuda_stream, "zeroed")
+    t = _WS.get(key)
+    if t is None or t.numel() < nbytes:
+        t = torch.zeros(int(nbytes), dtype=torch.uint8, device=device)
+        _WS[key] = t
+    return t
+
+
 def read_status(ws: torch.Tensor) -> int:
     """The device status word (first 4 bytes of a workspace); synchronises the stream."""
     return int(ws[:4].view(torch.int32).item())

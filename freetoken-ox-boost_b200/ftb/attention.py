@@ -1,0 +1,88 @@
+"""Attention of new tokens over a paged cache, on libftb (``ftb_attention`` in ``include/ftb.h``)."""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from ._runtime import read_status, require_cuda, stream_handle, zeroed_workspace
+from .block import _TYPE
+
+
+def _int32(t, name, shape, dev):
+    if t.dtype != torch.int32 or t.device != dev or tuple(t.shape) != shape or (
+            t.shape[-1] > 1 and t.stride(-1) != 1):
+        raise ValueError(f"{name}: {tuple(t.shape)} {t.dtype} on {t.device}, expected int32 "
+                         f"{shape} on {dev} with contiguous rows")
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                    block_table: torch.Tensor, kv_len: torch.Tensor,
+                    cu_q: torch.Tensor | None = None, max_q: int = 1, *,
+                    scale: float | None = None, causal: bool = True, window: int = 0,
+                    out: torch.Tensor | None = None, return_lse: bool = False,
+                    check_status: bool = False):
+    """Attention of the new tokens of a batch over their sequences' pages; their own keys and
+    values are in the caches already (``rope_append``).
+
+    ``q`` [total, q heads, D]; caches [pages, page, kv heads, D] (any strides with contiguous
+    heads); ``block_table`` int32 [batch, width]; ``kv_len`` int32 [batch], keys of each sequence
+    with the new ones. ``cu_q`` int32 [batch + 1] gives the rows of each sequence in ``q`` and
+    ``max_q`` the most of them; without ``cu_q`` every sequence has one new token (decode).
+    Token i of n sees the keys up to its own position ``kv_len - n + i`` (``causal``), and no more
+    than the last ``window`` of them (0: all). A token that sees none gets 0 (lse -inf).
+    Returns out [total, q heads, D], with ``return_lse`` also the natural log of the sum of the
+    exponentials, float32 [total, q heads]. ``check_status`` reads the device status word
+    (synchronises) and raises on page ids, lengths or starts outside the tensors."""
+    dev = require_cuda(q)
+    if q.dim() != 3 or q.dtype not in _TYPE or q.stride(2) != 1:
+        raise ValueError(f"q: {tuple(q.shape)} {q.dtype}, expected [total, heads, D] bf16 or f16 "
+                         "with contiguous heads")
+    total, Hq, D = q.shape
+    for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if c.dim() != 4 or c.dtype != q.dtype or c.device != dev or c.shape[3] != D or (
+                c.stride(3) != 1) or c.shape != k_cache.shape:
+            raise ValueError(f"{name}: {tuple(c.shape)} {c.dtype} on {c.device}, expected [pages, "
+                             f"page, kv heads, {D}] {q.dtype} with contiguous heads on {dev}")
+    pages, page, Hkv, _ = k_cache.shape
+    if Hkv < 1 or Hq % Hkv:
+        raise ValueError(f"{Hq} query heads do not divide into {Hkv} kv heads")
+    if block_table.dim() != 2:
+        raise ValueError("block_table must be [batch, width]")
+    batch, width = block_table.shape
+    _int32(block_table, "block_table", (batch, width), dev)
+    _int32(kv_len, "kv_len", (batch,), dev)
+    if cu_q is not None:
+        _int32(cu_q, "cu_q", (batch + 1,), dev)
+    elif batch != total or max_q != 1:
+        raise ValueError(f"without cu_q q has one row per sequence (got {total} rows, batch {batch}, "
+                         f"max_q {max_q})")
+    if window < 0:
+        raise ValueError(f"window={window}")
+    if out is None:
+        out = torch.empty(total, Hq, D, dtype=q.dtype, device=dev)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
+        raise ValueError("out must be contiguous, of q's shape and dtype")
+    lse = torch.empty(total, Hq, dtype=torch.float32, device=dev) if return_lse else None
+    lib = _lib.load()
+    nbytes = lib.ftb_attention_workspace_bytes(total, batch, max_q, Hq, Hkv, D)
+    ws = zeroed_workspace(nbytes, dev)
+    a = _lib.AttnArgsStruct(
+        q=q.data_ptr(), k_cache=k_cache.data_ptr(), v_cache=v_cache.data_ptr(),
+        block_table=block_table.data_ptr(), kv_len=kv_len.data_ptr(),
+        cu_q=0 if cu_q is None else cu_q.data_ptr(), out=out.data_ptr(),
+        lse=0 if lse is None else lse.data_ptr(), workspace=ws.data_ptr(),
+        workspace_bytes=ws.numel(), q_strides=q.stride()[:2], k_strides=k_cache.stride()[:3],
+        v_strides=v_cache.stride()[:3], total_q=total, num_pages=pages,
+        table_stride=block_table.stride(0), batch=batch, max_q=int(max_q), table_width=width,
+        page=page, Hq=Hq, Hkv=Hkv, D=D, causal=int(causal), window=int(window),
+        type=_TYPE[q.dtype], scale=D ** -0.5 if scale is None else scale)
+    _lib.check("ftb_attention", lib.ftb_attention(ctypes.byref(a), stream_handle(dev)))
+    if check_status:
+        status = read_status(ws)
+        if status:
+            ws[:4].zero_()
+            raise ValueError(f"paged_attention: device status {status} (1: page id or kv_len "
+                             "outside the cache, 2: cu_q outside q or above max_q, 4: timeout)")
+    return (out, lse) if return_lse else out

@@ -382,6 +382,136 @@ FTB_API int ftb_ep_status(ftb_ep* ep, int clear, ftb_stream_t stream);
 FTB_API int ftb_ep_destroy(ftb_ep* ep);
 
 /*
+ * ---- The operators of a decoder block around the MoE layer -------------------------------
+ * (no counterparts among the reference's own kernels: its model blocks take them from the
+ * upstream project). Element types of these calls:
+ */
+enum { FTB_TYPE_BF16 = 0, FTB_TYPE_F16 = 1, FTB_TYPE_F32 = 2 };
+
+/*
+ * Norms before and after a block, fused with its gate and residual scale, per row of H:
+ *   n = post ? y * rsqrt(mean(y^2) + eps) * post : y
+ *   r = x + scale * act(gate) * n
+ *   h = r * rsqrt(mean(r^2) + eps) * pre          (from r before its rounding)
+ * fp32 inside, each output rounded once. y NULL: h is the norm of x, and r, gate and post are
+ * NULL too. pre NULL: only r. x and r have residual_type (= type, or FTB_TYPE_F32), y and h have
+ * type (BF16 or F16); gate, post and pre have type, or F32 when weights_f32 != 0. Strides are in
+ * elements between rows; r and h are contiguous. r may be x, h may be y.
+ * gate_kind: NONE; CHANNEL gate[H]; TOKEN gate[rows] (gate_stride apart); FULL gate[rows, H].
+ * gate_act: LINEAR, or SIGMOID (the gate goes through 1 / (1 + exp(-g))).
+ * 1 <= H <= 16384.
+ */
+enum { FTB_GATE_NONE = 0, FTB_GATE_CHANNEL = 1, FTB_GATE_TOKEN = 2, FTB_GATE_FULL = 3 };
+enum { FTB_GATE_LINEAR = 0, FTB_GATE_SIGMOID = 1 };
+typedef struct ftb_norm_args {
+  const void* x;
+  const void* y;
+  const void* gate;
+  const void* post;
+  const void* pre;
+  void* r;
+  void* h;
+  int64_t rows;
+  int64_t x_stride, y_stride, gate_stride;
+  int H;
+  int type, residual_type, weights_f32;
+  int gate_kind, gate_act;
+  float scale, eps;
+} ftb_norm_args;
+FTB_API int ftb_block_norm(const ftb_norm_args* args, ftb_stream_t stream);
+
+/*
+ * Rotary positions on 1..4 axes (text: one; images and video: time, height, width), and the
+ * write of the new tokens' keys and values into the paged cache.
+ *   q [tokens, Hq, D], k, v [tokens, Hkv, D] with token and head strides (elements; a head is
+ *   contiguous); q_out [tokens, Hq, D] contiguous (may be q where q is contiguous).
+ *   positions [axes, tokens] int32 or int64 (pos64), axes pos_stride apart.
+ *   table [table_rows, rot] fp32: row p holds cos(p w_i), i < rot/2, then sin(p w_i).
+ *   sections[a] = frequencies of axis a, summing to rot/2. order BLOCKS: axis 0's frequencies
+ *   first, then axis 1's, ...; CYCLIC: frequency i belongs to axis i % axes while that axis has
+ *   frequencies left (i / axes < sections[axis]), else to axis 0.
+ *   pairs HALF: (x[i], x[i + rot/2]); ADJACENT: (x[2i], x[2i+1]). Elements past rot are copied.
+ *   With slots [tokens] (int32 or int64): k_dst, v_dst are the caches, token t goes to row
+ *   slots[t] % page of page slots[t] / page, strides {page, row, head} in elements; a slot
+ *   outside [0, n_slots) is not stored (-1: padding). Without slots: k_dst [tokens, Hkv, D] by
+ *   k_dst_strides {0, token, head}; v and v_dst are NULL.
+ * A position outside the table gives NaN. D even, <= 512; rot even, <= min(D, 256).
+ */
+enum { FTB_PAIRS_HALF = 0, FTB_PAIRS_ADJACENT = 1 };
+enum { FTB_AXES_BLOCKS = 0, FTB_AXES_CYCLIC = 1 };
+typedef struct ftb_rope_args {
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  uint16_t* q_out;
+  uint16_t* k_dst;
+  uint16_t* v_dst;
+  int64_t q_strides[2], k_strides[2], v_strides[2];
+  int64_t k_dst_strides[3], v_dst_strides[3];
+  const void* positions;
+  int64_t pos_stride;
+  const float* table;
+  int64_t table_rows;
+  const void* slots;
+  int64_t n_slots;
+  int64_t tokens;
+  int pos64, slot64, page;
+  int Hq, Hkv, D, rot;
+  int axes, sections[4];
+  int order, pairs, type;
+} ftb_rope_args;
+FTB_API int ftb_rope(const ftb_rope_args* args, ftb_stream_t stream);
+
+/*
+ * Attention of the new tokens of a batch over their sequences' paged caches.
+ * Sequence b has n = cu_q[b+1] - cu_q[b] new tokens (rows cu_q[b].. of q; cu_q NULL: one token
+ * each, row b) and kv_len[b] keys in all, the new tokens' own among them, so token i has position
+ * p = kv_len[b] - n + i. It sees the keys j with j < kv_len[b], j <= p when causal, and
+ * j > p - window when window > 0. Key j is row j % page of page block_table[b, j / page].
+ *   out = sum_j softmax_j(scale q.k_j) v_j,   lse = log sum_j exp(scale q.k_j)   (natural log)
+ * A token that sees no key gets out = 0 and lse = -inf. Cache rows at or past kv_len, or below
+ * every token's window, are never used, whatever they hold.
+ *   q [total_q, Hq, D] with token and head strides; out [total_q, Hq, D] contiguous; lse
+ *   [total_q, Hq] fp32 or NULL; caches [num_pages, page, Hkv, D] by strides {page, row, head}
+ *   (any order of page rows and heads). Query head h reads kv head h / (Hq / Hkv).
+ *   block_table int32 [batch, table_width] (table_stride apart), kv_len int32 [batch], cu_q int32
+ *   [batch + 1].
+ *   max_q: no sequence has more new tokens (tokens past it are not computed, status bit 1).
+ * D % 8 == 0, D <= 128; Hq / Hkv <= 128; page a power of two, >= 8; strides multiples of 8
+ * elements, pointers 16-byte aligned; type BF16 or F16. Softmax, sums and accumulators are fp32;
+ * the probabilities are rounded to `type` as the tensor cores' operand.
+ * workspace: ftb_attention_workspace_bytes() bytes, 256-byte aligned, for calls of one stream
+ * order. Its first FTB_ATTN_ZERO_BYTES bytes are zero before the first use (the caller's
+ * memset), and every call leaves the counters there zero again. Bytes [0, 4) are the
+ * status word, sticky until the caller clears it: bit 0 = a page id outside [0, num_pages) or a
+ * kv_len outside [0, table_width * page] (read as zero keys, or clamped), bit 1 = more new tokens
+ * than max_q, or cu_q outside [0, total_q]; bit 2 = a bounded device-side wait gave up.
+ */
+#define FTB_ATTN_ZERO_BYTES 65536
+typedef struct ftb_attn_args {
+  const uint16_t* q;
+  const uint16_t* k_cache;
+  const uint16_t* v_cache;
+  const int32_t* block_table;
+  const int32_t* kv_len;
+  const int32_t* cu_q;
+  uint16_t* out;
+  float* lse;
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t q_strides[2];
+  int64_t k_strides[3], v_strides[3];
+  int64_t total_q, num_pages, table_stride;
+  int batch, max_q, table_width, page;
+  int Hq, Hkv, D;
+  int causal, window, type;
+  float scale;
+} ftb_attn_args;
+FTB_API size_t ftb_attention_workspace_bytes(int64_t total_q, int batch, int max_q, int Hq, int Hkv,
+                                             int D);
+FTB_API int ftb_attention(const ftb_attn_args* args, ftb_stream_t stream);
+
+/*
  * Measurement hooks (no counterpart in the reference): between ftb_profile_begin() and
  * ftb_profile_end() the library records a CUDA event pair on the launching stream around
  * each of its kernel launches (ids: FTB_KERNEL_*). ftb_profile_end() synchronises those
