@@ -11,9 +11,15 @@ namespace ftb {
 
 PFN_cuTensorMapEncodeTiled encode_fn();  // moe_decode_tma.cu
 
+namespace {
 CUtensorMapDataType attn_dtype(int type) {
   return type == FTB_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
 }
+
+// Up to 16 query rows per kv head go to the streaming kernel, more to the tensor-core kernel.
+constexpr int kStreamRows = 16;
+bool streams(int64_t rows) { return rows <= kStreamRows; }
+}  // namespace
 
 int attn_cache_map(CUtensorMap* m, const void* base, const ftb_attn_args& a,
                    const int64_t (&strides)[3], uint32_t box_rows, uint32_t halves) {
@@ -32,6 +38,20 @@ int attn_cache_map(CUtensorMap* m, const void* base, const ftb_attn_args& a,
   return r == CUDA_SUCCESS ? FTB_OK : FTB_ERR_CUDA;
 }
 
+int attn_q_map(CUtensorMap* m, const ftb_attn_args& a, uint32_t group, uint32_t tokens) {
+  PFN_cuTensorMapEncodeTiled fn = encode_fn();
+  if (!fn) return FTB_ERR_CUDA;
+  const cuuint64_t dims[4] = {(cuuint64_t)a.D, group, (cuuint64_t)a.Hkv, (cuuint64_t)a.total_q};
+  const cuuint64_t st[3] = {(cuuint64_t)a.q_strides[1] * 2, (cuuint64_t)a.q_strides[1] * 2 * group,
+                            (cuuint64_t)a.q_strides[0] * 2};
+  const cuuint32_t box[4] = {64, group, 1, tokens};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r = fn(m, attn_dtype(a.type), 4, const_cast<uint16_t*>(a.q), dims, st, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? FTB_OK : FTB_ERR_CUDA;
+}
+
 }  // namespace ftb
 
 using namespace ftb;
@@ -40,7 +60,11 @@ extern "C" {
 
 size_t ftb_attention_workspace_bytes(int64_t total_q, int batch, int max_q, int Hq, int Hkv, int D) {
   if (total_q < 0 || batch < 0 || max_q < 0 || Hkv < 1 || Hq < Hkv || D < 8) return 0;
-  return FTB_ATTN_ZERO_BYTES + attn_stream_partial_bytes((int64_t)max_q * (Hq / Hkv), D);
+  const int G = Hq / Hkv;
+  if (G > 128) return 0;
+  return FTB_ATTN_ZERO_BYTES +
+         (streams((int64_t)max_q * G) ? attn_stream_partial_bytes((int64_t)max_q * G, D)
+                                      : attn_chunk_workspace_bytes(total_q, batch, Hkv, G, D));
 }
 
 int ftb_attention(const ftb_attn_args* a, ftb_stream_t stream) {
@@ -86,7 +110,8 @@ int ftb_attention(const ftb_attn_args* a, ftb_stream_t stream) {
   P.causal = a->causal != 0, P.window = a->window;
   P.keys_max = a->table_width * a->page;
   P.scale_log2 = a->scale * 1.44269504088896341f;
-  return launch_attn_stream(*a, P, (cudaStream_t)stream);
+  return streams((int64_t)a->max_q * P.G) ? launch_attn_stream(*a, P, (cudaStream_t)stream)
+                                          : launch_attn_chunk(*a, P, (cudaStream_t)stream);
 }
 
 }  // extern "C"

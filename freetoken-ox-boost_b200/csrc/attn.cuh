@@ -3,6 +3,8 @@
 
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "ftb_common.cuh"
 
 namespace ftb {
@@ -39,10 +41,13 @@ struct AttnMaps {
 
 int attn_cache_map(CUtensorMap* m, const void* base, const ftb_attn_args& a,
                    const int64_t (&strides)[3], uint32_t box_rows, uint32_t halves);
-CUtensorMapDataType attn_dtype(int type);
+// Query rows of one kv head: boxes of `tokens` tokens x `group` heads x 64 elements.
+int attn_q_map(CUtensorMap* m, const ftb_attn_args& a, uint32_t group, uint32_t tokens);
 
 int launch_attn_stream(const ftb_attn_args& a, AttnParams P, cudaStream_t stream);
 size_t attn_stream_partial_bytes(int64_t rows_max, int D);
+int launch_attn_chunk(const ftb_attn_args& a, AttnParams P, cudaStream_t stream);
+size_t attn_chunk_workspace_bytes(int64_t total_q, int batch, int Hkv, int G, int D);
 
 __device__ __forceinline__ void tma_5d(uint32_t dst, const CUtensorMap* map, int x, int row,
                                        int head, int page, int half, uint64_t* bar) {
@@ -61,6 +66,17 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap* m) {
 __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// Two fp32 values rounded to a packed pair.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t r;
+  if constexpr (std::is_same<T, __half>::value)
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
 

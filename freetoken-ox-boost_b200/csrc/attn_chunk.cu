@@ -1,0 +1,958 @@
+// attn_chunk.cu - paged attention for many query rows per kv head (prompts, chunks of a prefill)
+// on the 5th-generation tensor cores.
+//
+// The rows of a sequence and kv head are its new tokens x the G query heads that share the kv
+// head. An item is two tiles A and B of up to 128 rows (whole tokens, floor(128 / G) each), one
+// kv head and a range of 128-key tiles, computed by one persistent block:
+//   S = Q K^T   tcgen05.mma M = 128, N = 128 keys, Q and K from shared memory, S in tensor memory
+//   P = 2^(s - ref), l += sum P     one thread per row, all 128 scores in registers
+//   O += P V    tcgen05.mma M = 128, N = D, P from tensor memory (it takes S's place), V from
+//               shared memory (its rows are keys: the MN-major operand layout)
+// ref is the row's reference maximum. It moves only when a tile's maximum exceeds it by more than
+// 2^8 (the sums are fp32, and a P of up to 2^8 keeps its relative precision in bf16 and f16), so
+// O, in tensor memory, is rescaled rarely.
+//
+// Bound: the tensor cores, 4 D per visible (row, key), with the exponentials next: a 128 x 128
+// tile costs 1024 cycles of MMA at D = 128 and as many of the special-function unit. Two tiles
+// are in flight so that A's softmax runs beside B's MMAs.
+//
+// Warps: 0-3 softmax and output of tile A, 4-7 of tile B (one thread per row), 8 issues the MMAs,
+// 9 the TMA copies, 10 clears V rows that no token of the item may see (their weight is 0, but
+// 0 x NaN is not). K and V tiles share a ring in the order of their use: K0 V0 K1 V1 ...
+//
+// k_attn_plan lists the pieces of a call (an item, or a part of its keys where items are too few
+// or too long to fill the SMs evenly), largest first; parts leave (ref, l, O) in the workspace and
+// k_attn_join puts them together in their order in the sequence.
+#include "attn.cuh"
+
+namespace ftb {
+namespace {
+
+constexpr int kTileK = 128;   // keys per tile
+constexpr int kTileM = 128;   // rows per tile
+constexpr int kThreadsC = 384;
+constexpr int kWarpMma = 8, kWarpLoad = 9, kWarpFix = 10;
+// registers: softmax 2 x 128 threads x 216 + 128 x 72 = 64512 = 384 x 168 at launch
+constexpr int kRegsLaunch = 168, kRegsSoftmax = 216, kRegsOther = 72;
+static_assert(2 * 128 * kRegsSoftmax + 128 * kRegsOther <= kThreadsC * kRegsLaunch, "registers");
+constexpr int kTmemS = 0, kTmemO = 256;  // + 128 for tile B
+constexpr float kLazy = 8.f;             // log2 of what a score may exceed the reference by
+
+// ---- plan --------------------------------------------------------------------------------------
+
+struct Piece {
+  int q_tok;    // row of q of the first token
+  int n_tok;    // tokens
+  int seq, head;
+  int pos;      // position of the first token
+  int len;      // keys of the sequence
+  int lo, hi;   // keys that the item's tokens see between them
+  int t0, t1;   // key tiles of this piece
+  int slot;     // part number in the workspace, -1: the whole item
+  int pad;
+};
+static_assert(sizeof(Piece) == 48, "three 16-byte loads");
+
+struct Join {
+  int q_tok, n_tok, head, slot, parts;
+  int pad[3];
+};
+
+struct Plan {
+  int* head;     // kPlan* counts
+  Piece* pieces;
+  Join* joins;
+  int4* groups;  // per group (sequence, two row tiles): sequence, first token, tiles [z, w)
+  int* pos;      // per group: place among its size class
+  int* part0;    // per group that is cut: its first part's number among one kv head's parts
+  int max_pieces, max_parts, max_joins, max_groups;
+};
+enum { kPlanPieces = 0, kPlanJoins = 1, kPlanInts = 64 };
+constexpr int kClasses = 8;
+constexpr int kPlanThreads = 1024;
+constexpr int kPartsPerSm = 8;
+
+// Parts of split items: their number, not the sizes of the call, bounds the workspace.
+int plan_parts() { return kPartsPerSm * sm_count(); }
+
+Plan carve_plan(char* base, int64_t groups, int Hkv, size_t* bytes) {
+  size_t off = 0;
+  auto take = [&](size_t n) {
+    char* p = base ? base + off : nullptr;
+    off += (n + 255) / 256 * 256;
+    return p;
+  };
+  Plan p;
+  p.max_parts = plan_parts();
+  p.max_joins = p.max_parts / 2;
+  p.max_groups = (int)groups;
+  p.max_pieces = (int)(groups * Hkv + p.max_parts);
+  p.head = reinterpret_cast<int*>(take(kPlanInts * 4));
+  p.pieces = reinterpret_cast<Piece*>(take((size_t)p.max_pieces * sizeof(Piece)));
+  p.joins = reinterpret_cast<Join*>(take((size_t)p.max_joins * sizeof(Join)));
+  p.groups = reinterpret_cast<int4*>(take((size_t)groups * sizeof(int4)));
+  p.pos = reinterpret_cast<int*>(take((size_t)groups * 4));
+  p.part0 = reinterpret_cast<int*>(take((size_t)groups * 4));
+  *bytes = off;
+  return p;
+}
+
+// Inclusive sum over the block; *total gets the block's sum.
+__device__ __forceinline__ int block_scan(int v, int* red, int* total) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  __syncthreads();
+  if (lane == 31) red[warp] = v;
+  __syncthreads();
+  int w = red[lane];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += u;
+  }
+  *total = __shfl_sync(0xffffffffu, w, 31);
+  const int before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
+  return v + (warp ? before : 0);
+}
+
+// How a group of `tiles` key tiles is cut: into `parts` pieces of at most `size` tiles.
+struct Cut {
+  int parts, size;
+};
+__device__ __forceinline__ Cut cut_group(int tiles, int most) {
+  Cut c{1, tiles};
+  if (tiles > most) {
+    c.parts = (tiles + most - 1) / most;
+    c.size = (tiles + c.parts - 1) / c.parts;
+    c.parts = (tiles + c.size - 1) / c.size;
+  }
+  return c;
+}
+
+// One block. tok = tokens per group (two row tiles).
+__global__ void __launch_bounds__(kPlanThreads)
+    k_attn_plan(const __grid_constant__ AttnParams P, Plan plan, int tok, int blocks) {
+  extern __shared__ int first_group[];  // [batch + 1]
+  __shared__ int red[32];
+  __shared__ int class_n[kClasses];
+  __shared__ unsigned long long sum_tiles;
+  __shared__ int n_parts, n_joins, biggest;
+  const int tid = threadIdx.x;
+  pdl_launch_dependents();
+  if (tid == 0) sum_tiles = 0, biggest = 0, n_joins = 0;
+  pdl_wait();
+  int base = 0;
+  for (int b0 = 0; b0 < P.batch; b0 += kPlanThreads) {
+    const int b = b0 + tid;
+    int n = 0;
+    if (b < P.batch) {
+      const AttnSeq s = attn_seq(P, b);
+      if (s.bad_len || s.bad_rows)
+        atomicOr(P.status, (s.bad_len ? kAttnBadPage : 0u) | (s.bad_rows ? kAttnBadRows : 0u));
+      n = (s.n + tok - 1) / tok;
+    }
+    int total;
+    const int incl = block_scan(n, red, &total);
+    if (b < P.batch) first_group[b] = base + incl - n;
+    base += total;
+  }
+  if (tid == 0) first_group[P.batch] = base;
+  __syncthreads();
+  // (lengths that overlap, bad_rows, could make more groups than the rows allow)
+  const int groups = base < plan.max_groups ? base : plan.max_groups;
+  unsigned long long mine = 0;
+  int big = 0;
+  for (int g = tid; g < groups; g += kPlanThreads) {
+    int a = 0, z = P.batch;  // the sequence with first_group[a] <= g < first_group[a + 1]
+    while (z - a > 1) {
+      const int mid = (a + z) >> 1;
+      if (first_group[mid] <= g)
+        a = mid;
+      else
+        z = mid;
+    }
+    const AttnSeq s = attn_seq(P, a);
+    const int i0 = (g - first_group[a]) * tok;
+    const int i1 = i0 + tok < s.n ? i0 + tok : s.n;
+    const KeyRange r = attn_range(P, s, i0, i1 - 1);
+    int4 v = make_int4(a, i0, 0, 0);
+    if (r.lo < r.hi) v.z = r.lo / kTileK, v.w = (r.hi + kTileK - 1) / kTileK;
+    plan.groups[g] = v;
+    mine += v.w - v.z;
+    big = max(big, v.w - v.z);
+  }
+  if (mine) atomicAdd(&sum_tiles, mine);
+  if (big) atomicMax(&biggest, big);
+  __syncthreads();
+  // Pieces of at most `most` tiles: a quarter of an even share of the work, so that the last
+  // pieces end close together, but no shorter than 16 tiles (or the share itself, where that is
+  // less): a piece pays for its Q copy and its output.
+  const unsigned long long all = sum_tiles * P.Hkv;
+  const int share = (int)min((all + blocks - 1) / blocks, 1ull << 29);
+  int most = max(share / 4, min(16, max(2, share)));
+  for (;;) {
+    __syncthreads();
+    if (tid == 0) n_parts = 0;
+    if (tid < kClasses) class_n[tid] = 0;
+    __syncthreads();
+    const int top = min(most, max(biggest, 1));
+    for (int g = tid; g < groups; g += kPlanThreads) {
+      const int4 v = plan.groups[g];
+      const Cut c = cut_group(v.w - v.z, most);
+      if (c.parts > 1) atomicAdd(&n_parts, c.parts * P.Hkv);
+      atomicAdd(&class_n[min(kClasses - 1, (top - c.size) * kClasses / top)], c.parts);
+    }
+    __syncthreads();
+    if (n_parts <= plan.max_parts) break;
+    most *= 2;
+  }
+  const int top = min(most, max(biggest, 1));
+  // place of each group among its class, and the parts' numbers
+  for (int k = 0; k <= kClasses; ++k) {  // the last round numbers the parts
+    int run = 0;
+    for (int g0 = 0; g0 < groups; g0 += kPlanThreads) {
+      const int g = g0 + tid;
+      int n = 0;
+      bool in = false;
+      if (g < groups) {
+        const int4 v = plan.groups[g];
+        const Cut c = cut_group(v.w - v.z, most);
+        in = k == kClasses ? c.parts > 1
+                           : min(kClasses - 1, (top - c.size) * kClasses / top) == k;
+        n = in ? c.parts : 0;
+      }
+      int total;
+      const int incl = block_scan(n, red, &total);
+      if (in) (k < kClasses ? plan.pos : plan.part0)[g] = run + incl - n;
+      run += total;
+    }
+  }
+  __syncthreads();
+  // emission: a warp per group, a lane per piece; in a class one kv head after another, so that
+  // blocks that run at the same time share keys
+  const int warp = tid >> 5, lane = tid & 31;
+  for (int g = warp; g < groups; g += kPlanThreads / 32) {
+    const int4 v = plan.groups[g];
+    const AttnSeq s = attn_seq(P, v.x);
+    const int tiles = v.w - v.z;
+    const Cut c = cut_group(tiles, most);
+    const int k = min(kClasses - 1, (top - c.size) * kClasses / top);
+    int start = 0;
+    for (int i = 0; i < k; ++i) start += class_n[i] * P.Hkv;
+    const int i1 = v.y + tok < s.n ? v.y + tok : s.n;
+    const KeyRange r = attn_range(P, s, v.y, i1 - 1);
+    const int slot0 = c.parts > 1 ? plan.part0[g] : 0;
+    Piece p;
+    p.q_tok = s.q0 + v.y, p.n_tok = i1 - v.y, p.seq = v.x;
+    p.pos = s.len - s.n + v.y, p.len = s.len, p.lo = r.lo, p.hi = r.hi, p.pad = 0;
+    for (int i = lane; i < c.parts * P.Hkv; i += 32) {
+      const int head = i / c.parts, part = i % c.parts;
+      p.head = head;
+      p.t0 = v.z + part * c.size;
+      p.t1 = min(p.t0 + c.size, v.w);
+      p.slot = c.parts > 1 ? slot0 * P.Hkv + i : -1;
+      plan.pieces[start + head * class_n[k] + plan.pos[g] + part] = p;
+      if (c.parts > 1 && part == 0) {
+        const int j = atomicAdd(&n_joins, 1);
+        Join o{};
+        o.q_tok = p.q_tok, o.n_tok = p.n_tok, o.head = head, o.slot = p.slot, o.parts = c.parts;
+        plan.joins[j] = o;
+      }
+    }
+  }
+  __syncthreads();
+  if (tid == 0) {
+    int n = 0;
+    for (int k = 0; k < kClasses; ++k) n += class_n[k] * P.Hkv;
+    plan.head[kPlanPieces] = n;
+    plan.head[kPlanJoins] = n_joins;
+  }
+}
+
+// ---- tensor-core helpers -----------------------------------------------------------------------
+
+// Shared-memory operand descriptors, 128-byte swizzle, 8-row atoms 1024 bytes apart. K-major (Q,
+// K): rows of 64 elements. MN-major (V): a row is a key; blocks of 64 of the D columns are
+// kTileK * 128 bytes apart.
+__device__ __forceinline__ uint64_t desc_base(uint32_t saddr, uint32_t lbo) {
+  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) |
+         ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// Instruction descriptor, kind::f16: fp32 D, A and B bf16 or f16, M = 128, B K-major or MN-major.
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t idesc(int n, bool b_mn) {
+  const uint32_t f = std::is_same<T, __half>::value ? 0u : 1u;
+  return (1u << 4) | (f << 7) | (f << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(kTileM >> 4) << 24);
+}
+// Issued by one elected lane of the converged warp.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id,
+                                       uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(id), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id,
+                                       uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(id), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit1(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
+          smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tc_before() {
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void tc_after() {
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+// 32 columns of this warp's 32 lanes (no wait).
+__device__ __forceinline__ void tm_ld32(uint32_t t, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+      "%30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(t)
+      : "memory");
+}
+__device__ __forceinline__ void tm_ld_wait() {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tm_st32(uint32_t t, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+      "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, "
+      "%29, %30, %31, %32};" ::"r"(t),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+      "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+      "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
+      "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tm_st_wait() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tma_4d(uint32_t dst, const CUtensorMap* map, int x, int g, int head,
+                                       int tok, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(g), "r"(head), "r"(tok), "r"(smem_u32(bar))
+      : "memory");
+}
+// ---- the kernel --------------------------------------------------------------------------------
+
+constexpr int chunk_stages(int DP) { return DP == 128 ? 5 : 8; }
+template <int DP>
+struct ChunkSmem {
+  static constexpr int kStages = chunk_stages(DP);
+  static constexpr int kTileBytes = kTileK * DP * 2;
+  alignas(1024) uint8_t q[2][kTileBytes];          // [half][row][64]
+  alignas(1024) uint8_t ring[kStages][kTileBytes];  // [half][key][64]
+  uint64_t full[kStages], empty[kStages];
+  uint64_t land[kStages];  // a V tile that the fixer completes has landed
+  uint64_t q_full[2], q_empty[2];
+  uint64_t s_full[2], p_ready[2], o_full[2];
+  uint64_t drain;
+  uint32_t tmem;
+  int abort;
+};
+
+template <int DP>
+struct ChunkSync {
+  ChunkSmem<DP>* sh;
+  uint32_t* status;
+  __device__ bool wait(uint64_t* bar, uint32_t parity) const {
+    if (mbar_try_wait(bar, parity)) return true;
+    volatile int* ab = &sh->abort;
+    for (uint32_t i = 0; i < kSpinLimit; ++i) {
+      if (*ab) return false;
+      if (mbar_try_wait(bar, parity)) return true;
+      if (i > (1u << 16)) __nanosleep(64);
+    }
+    *ab = 1;
+    atomicOr(status, kAttnTimeout);
+    return false;
+  }
+  __device__ bool wait_warp(uint64_t* bar, uint32_t parity) const {
+    return __all_sync(0xffffffffu, wait(bar, parity));
+  }
+};
+
+// Block x takes pieces x, 2B - 1 - x, 2B + x, ... (B blocks): the list is sorted by size, and
+// turning around each time evens out the sums.
+__device__ __forceinline__ int piece_at(int round) {
+  const int B = gridDim.x;
+  return round * B + ((round & 1) ? B - 1 - (int)blockIdx.x : (int)blockIdx.x);
+}
+__device__ __forceinline__ Piece load_piece(const Piece* p) {
+  Piece r;
+  const int4* s = reinterpret_cast<const int4*>(p);
+  int4* d = reinterpret_cast<int4*>(&r);
+  d[0] = __ldcg(s), d[1] = __ldcg(s + 1), d[2] = __ldcg(s + 2);
+  return r;
+}
+// Rows and key tiles of tile X of a piece: its first and last token, tiles [t0, t0 + n).
+struct RowTile {
+  int tok0, toks, n;
+};
+__device__ __forceinline__ RowTile row_tile(const AttnParams& P, const Piece& p, int x, int tok1) {
+  RowTile r;
+  r.tok0 = x * tok1;
+  r.toks = min(tok1, p.n_tok - r.tok0);
+  r.n = 0;
+  if (r.toks <= 0) {
+    r.toks = 0;
+    return r;
+  }
+  int hi = p.hi;
+  if (P.causal) hi = min(hi, p.pos + r.tok0 + r.toks);
+  const int t1 = min(p.t1, (hi + kTileK - 1) / kTileK);  // hi may be <= 0
+  r.n = max(0, t1 - p.t0);
+  return r;
+}
+
+template <int DP>
+__device__ void chunk_load(const AttnParams& P, const AttnMaps& M, const Plan& plan, int n_pieces,
+                           int tok1, ChunkSmem<DP>* sh) {
+  constexpr int kStages = ChunkSmem<DP>::kStages, kH = DP / 64;
+  const int lane = threadIdx.x & 31;
+  const ChunkSync<DP> sy{sh, P.status};
+  const int page = 1 << P.page_log2;
+  const int r = page < kTileK ? page : kTileK;
+  const int boxes = kTileK / r;  // <= 16
+  const uint32_t box_bytes = (uint32_t)r * 128 * kH;
+  const uint32_t q_bytes = (uint32_t)(tok1 * P.G) * 128 * kH;
+  int stage = 0;
+  uint32_t parity = 1, q_par[2] = {1, 1};
+  // phases issued so far on each barrier, for the exit after a timeout
+  uint32_t n_full[kStages] = {}, n_land[kStages] = {}, n_q[2] = {};
+  bool ok = true;
+  for (int round = 0; ok; ++round) {
+    const int at = piece_at(round);
+    if (at >= n_pieces) break;
+    const Piece p = load_piece(plan.pieces + at);
+    const RowTile ra = row_tile(P, p, 0, tok1), rb = row_tile(P, p, 1, tok1);
+    const int n = max(ra.n, rb.n);
+    const int32_t* table = P.block_table + (int64_t)p.seq * P.table_stride;
+    for (int j = 0; j < 2 * n && ok; ++j) {  // K0 V0 K1 V1 ...
+      const bool v = j & 1;
+      const int key0 = (p.t0 + (j >> 1)) * kTileK;
+      const int b0 = p.lo > key0 ? (p.lo - key0) / r : 0;
+      const int b1 = min(boxes, (p.hi - key0 + r - 1) / r);
+      const bool mine = lane >= b0 && lane < b1;
+      int id = 0, row = 0;
+      if (mine) {
+        const int key = key0 + lane * r;
+        id = __ldg(table + (key >> P.page_log2));
+        row = key & (page - 1);
+        if (id < 0 || id >= P.num_pages) {
+          atomicOr(P.status, kAttnBadPage);
+          id = (int)P.num_pages;  // outside the tensor: reads zeros
+        }
+      }
+      ok = sy.wait_warp(&sh->empty[stage], parity);
+      if (!ok) break;
+      const bool fix = v && (key0 < p.lo || key0 + kTileK > p.hi);
+      uint64_t* bar = fix ? &sh->land[stage] : &sh->full[stage];
+#pragma unroll
+      for (int i = 0; i < kStages; ++i)
+        if (i == stage) n_full[i] += !fix, n_land[i] += fix;
+      if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(b1 - b0) * box_bytes);
+      __syncwarp();
+      if (mine) {
+        const uint32_t dst = smem_u32(sh->ring[stage]) + lane * r * 128;
+#pragma unroll
+        for (int h = 0; h < kH; ++h)
+          tma_5d(dst + h * kTileK * 128, v ? &M.v : &M.k, h * 64, row, p.head, id, 0, bar);
+      }
+      if (++stage == kStages) stage = 0, parity ^= 1u;
+      if (j == 0) {  // Q after the first K: its buffers come free last
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const RowTile& rt = x ? rb : ra;
+          if (rt.n == 0 || !ok) continue;
+          ok = sy.wait_warp(&sh->q_empty[x], q_par[x]);
+          if (!ok) break;
+          q_par[x] ^= 1u;
+          ++n_q[x];
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&sh->q_full[x], q_bytes);
+#pragma unroll
+            for (int h = 0; h < kH; ++h)
+              tma_4d(smem_u32(sh->q[x]) + h * kTileM * 128, &M.q, h * 64, 0, p.head,
+                     p.q_tok + rt.tok0, &sh->q_full[x]);
+          }
+          __syncwarp();
+        }
+      }
+    }
+  }
+  if (!ok) {  // a wait gave up: stay until the copies in flight have landed (again bounded)
+    for (int i = 0; i < kStages; ++i) {
+      for (uint32_t k = 0; n_land[i] && k < kSpinLimit; ++k)
+        if (mbar_try_wait(&sh->land[i], (n_land[i] - 1) & 1u)) break;
+      // full[] also takes the fixer's arrivals, one for each land[] phase
+      for (uint32_t k = 0; n_full[i] && k < kSpinLimit; ++k)
+        if (mbar_try_wait(&sh->full[i], (n_full[i] + n_land[i] - 1) & 1u)) break;
+    }
+    for (int x = 0; x < 2; ++x)
+      for (uint32_t k = 0; n_q[x] && k < kSpinLimit; ++k)
+        if (mbar_try_wait(&sh->q_full[x], (n_q[x] - 1) & 1u)) break;
+  }
+}
+
+// Clears the rows of V tiles that no token of the piece's item sees.
+template <int DP>
+__device__ void chunk_fix(const AttnParams& P, const Plan& plan, int n_pieces, int tok1,
+                          ChunkSmem<DP>* sh) {
+  constexpr int kStages = ChunkSmem<DP>::kStages, kH = DP / 64;
+  const int lane = threadIdx.x & 31;
+  const ChunkSync<DP> sy{sh, P.status};
+  int stage = 0;
+  uint32_t land_par = 0;  // a bit per stage
+  for (int round = 0;; ++round) {
+    const int at = piece_at(round);
+    if (at >= n_pieces) return;
+    const Piece p = load_piece(plan.pieces + at);
+    const RowTile ra = row_tile(P, p, 0, tok1), rb = row_tile(P, p, 1, tok1);
+    const int n = max(ra.n, rb.n);
+    for (int j = 0; j < n; ++j) {
+      if (++stage == kStages) stage = 0;  // past K
+      const int key0 = (p.t0 + j) * kTileK;
+      if (key0 < p.lo || key0 + kTileK > p.hi) {
+        if (!sy.wait_warp(&sh->land[stage], (land_par >> stage) & 1u)) return;
+        land_par ^= 1u << stage;
+        const int below = max(0, p.lo - key0), above = min(kTileK, p.hi - key0);
+        const int rows = below + kTileK - above;
+        for (int i = lane; i < rows * 8 * kH; i += 32) {
+          const int c = i & 7, k = (i >> 3) % rows, h = (i >> 3) / rows;
+          const int key = k < below ? k : above + k - below;
+          *reinterpret_cast<uint4*>(sh->ring[stage] + h * kTileK * 128 + key * 128 + c * 16) =
+              make_uint4(0, 0, 0, 0);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->full[stage]);
+      }
+      if (++stage == kStages) stage = 0;  // past V
+    }
+  }
+}
+
+template <typename T, int DP>
+__device__ void chunk_mma(const AttnParams& P, const Plan& plan, int n_pieces, int tok1,
+                          ChunkSmem<DP>* sh) {
+  constexpr int kStages = ChunkSmem<DP>::kStages;
+  constexpr int kTileBytes = ChunkSmem<DP>::kTileBytes;
+  const ChunkSync<DP> sy{sh, P.status};
+  const uint32_t tb = sh->tmem;
+  const uint64_t qd = desc_base(smem_u32(sh->q[0]), 16);
+  const uint64_t kd = desc_base(smem_u32(sh->ring[0]), 16);
+  const uint64_t vd = desc_base(smem_u32(sh->ring[0]), kTileK * 128);
+  constexpr uint32_t kIdS = idesc<T>(kTileK, false), kIdO = idesc<T>(DP, true);
+  int stage = 0;
+  uint32_t parity = 0, q_par[2] = {0, 0}, p_par[2] = {0, 0};
+  // tile x's P V of the last step: not issued yet; whether it adds to O, ends its row tile
+  bool pend[2] = {false, false}, acc[2] = {false, false}, last[2] = {false, false};
+  int v_stage = -1;
+  uint32_t v_par = 0;
+  bool v_there = false, ok = true, issued = false;
+
+  auto pv = [&](int x) {
+    ok = sy.wait_warp(&sh->p_ready[x], p_par[x]);
+    if (!ok) return;
+    p_par[x] ^= 1u;
+    if (!v_there) {
+      ok = sy.wait_warp(&sh->full[v_stage], v_par);
+      if (!ok) return;
+      v_there = true;
+    }
+    tc_after();
+    const uint32_t d = tb + kTmemO + x * 128, a = tb + kTmemS + x * 128;
+    const uint64_t b = vd + (uint64_t)((v_stage * kTileBytes) >> 4);
+#pragma unroll
+    for (int k = 0; k < kTileK / 16; ++k)
+      mma_ts(d, a + k * 8, b + (uint64_t)((k * 16 * 128) >> 4), kIdO, (k > 0 || acc[x]) ? 1u : 0u);
+    if (last[x]) mma_commit1(&sh->o_full[x]);
+    pend[x] = false;
+  };
+
+  for (int round = 0; ok; ++round) {
+    const int at = piece_at(round);
+    if (at >= n_pieces) break;
+    const Piece p = load_piece(plan.pieces + at);
+    const int nx[2] = {row_tile(P, p, 0, tok1).n, row_tile(P, p, 1, tok1).n};
+    const int n = max(nx[0], nx[1]);
+    for (int j = 0; j < n && ok; ++j) {
+      ok = sy.wait_warp(&sh->full[stage], parity);
+      if (!ok) break;
+      issued = true;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        if (pend[x]) pv(x);
+        if (!ok) break;
+        if (j >= nx[x]) continue;
+        if (j == 0) {
+          ok = sy.wait_warp(&sh->q_full[x], q_par[x]);
+          if (!ok) break;
+          q_par[x] ^= 1u;
+        }
+        tc_after();
+        const uint64_t a = qd + (uint64_t)((x * kTileBytes) >> 4);
+        const uint64_t b = kd + (uint64_t)((stage * kTileBytes) >> 4);
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+          const uint64_t o = (uint64_t)(((k >> 2) * kTileK * 128 + (k & 3) * 32) >> 4);
+          mma_ss(tb + kTmemS + x * 128, a + o, b + o, kIdS, k > 0 ? 1u : 0u);
+        }
+        mma_commit1(&sh->s_full[x]);
+        if (j == nx[x] - 1) mma_commit1(&sh->q_empty[x]);
+        pend[x] = true, acc[x] = j > 0, last[x] = j == nx[x] - 1;
+      }
+      if (!ok) break;
+      if (v_stage >= 0) mma_commit1(&sh->empty[v_stage]);
+      mma_commit1(&sh->empty[stage]);
+      if (++stage == kStages) stage = 0, parity ^= 1u;
+      v_stage = stage, v_par = parity, v_there = false;
+      if (++stage == kStages) stage = 0, parity ^= 1u;
+    }
+  }
+#pragma unroll
+  for (int x = 0; x < 2; ++x)
+    if (ok && pend[x]) pv(x);
+  if (issued) {  // every MMA has finished once the drain barrier completes
+    mma_commit1(&sh->drain);
+    for (uint32_t k = 0; k < kSpinLimit; ++k)
+      if (mbar_try_wait(&sh->drain, 0)) break;
+  }
+}
+
+template <typename T, int DP>
+__device__ void chunk_softmax(const AttnParams& P, const Plan& plan, int n_pieces, int tok1, int x,
+                              ChunkSmem<DP>* sh) {
+  const ChunkSync<DP> sy{sh, P.status};
+  const int row = threadIdx.x & 127, lane = threadIdx.x & 31;
+  const uint32_t lanes = (uint32_t)(row & ~31) << 16;
+  const uint32_t ts = sh->tmem + kTmemS + x * 128 + lanes, to = sh->tmem + kTmemO + x * 128 + lanes;
+  const int tok = row / P.G, g = row % P.G;
+  // scores are multiplied by |scale|; a negative scale flips their sign first. A scale of 0
+  // becomes one that is small enough to be flat and keeps a masked -inf at -inf.
+  const bool flip = P.scale_log2 < 0.f;
+  const float sc = fmaxf(fabsf(P.scale_log2), 1e-30f);
+  uint32_t s_par = 0, o_par = 0;
+  constexpr int kSlot = 2 * kTileM * (DP + 2);
+  for (int round = 0;; ++round) {
+    const int at = piece_at(round);
+    if (at >= n_pieces) return;
+    const Piece p = load_piece(plan.pieces + at);
+    const RowTile rt = row_tile(P, p, x, tok1);
+    if (rt.toks == 0) continue;
+    const bool live = tok < rt.toks;
+    // keys this row sees: [kmin, kmax); the tile's rows all see [tile_min, tile_max)
+    const int pos0 = p.pos + rt.tok0;
+    const int kmax = !live ? 0 : P.causal ? min(p.len, pos0 + tok + 1) : p.len;
+    const int kmin = P.window > 0 ? max(0, pos0 + tok - P.window + 1) : 0;
+    const int all_max = P.causal ? min(p.len, pos0 + 1) : p.len;
+    const int all_min = P.window > 0 ? max(0, pos0 + rt.toks - 1 - P.window + 1) : 0;
+    float ref = -INFINITY, l = 0.f;
+    for (int j = 0; j < rt.n; ++j) {
+      if (!sy.wait_warp(&sh->s_full[x], s_par)) return;
+      s_par ^= 1u;
+      tc_after();
+      float s[kTileK];
+#pragma unroll
+      for (int c = 0; c < kTileK; c += 32) tm_ld32(ts + c, s + c);
+      tm_ld_wait();
+      if (flip) {
+#pragma unroll
+        for (int c = 0; c < kTileK; ++c) s[c] = -s[c];
+      }
+      const int key0 = (p.t0 + j) * kTileK;
+      if (key0 < all_min || key0 + kTileK > all_max) {
+        const int a = kmin - key0, b = kmax - key0;
+#pragma unroll
+        for (int c = 0; c < kTileK; ++c) s[c] = c >= a && c < b ? s[c] : -INFINITY;
+      }
+      float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
+#pragma unroll
+      for (int c = 4; c < kTileK; c += 4) {
+        m0 = fmaxf(m0, s[c]), m1 = fmaxf(m1, s[c + 1]);
+        m2 = fmaxf(m2, s[c + 2]), m3 = fmaxf(m3, s[c + 3]);
+      }
+      const float mx = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+      const bool move = (mx - ref) * sc > kLazy;  // from -inf always (NaN where both are)
+      if (__any_sync(0xffffffffu, move)) {
+        const float f = move ? ex2((ref - mx) * sc) : 1.f;
+        if (move) ref = mx;
+        l *= f;
+        if (j > 0) {  // P V of the tiles before has finished: S of this one came after it
+#pragma unroll
+          for (int c = 0; c < DP; c += 32) {
+            float o[32];
+            tm_ld32(to + c, o);
+            tm_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] *= f;
+            tm_st32(to + c, reinterpret_cast<uint32_t*>(o));
+          }
+        }
+      }
+      const float off = ref == -INFINITY ? 0.f : -ref * sc;
+      float l0 = 0.f, l1 = 0.f, l2 = 0.f, l3 = 0.f;
+      uint32_t pk[kTileK / 2];
+#pragma unroll
+      for (int c = 0; c < kTileK; c += 4) {
+        const float p0 = ex2(fmaf(s[c], sc, off)), p1 = ex2(fmaf(s[c + 1], sc, off));
+        const float p2 = ex2(fmaf(s[c + 2], sc, off)), p3 = ex2(fmaf(s[c + 3], sc, off));
+        l0 += p0, l1 += p1, l2 += p2, l3 += p3;
+        pk[c / 2] = pack2<T>(p0, p1);
+        pk[c / 2 + 1] = pack2<T>(p2, p3);
+      }
+      tm_st32(ts, pk);
+      tm_st32(ts + 32, pk + 32);
+      l += (l0 + l1) + (l2 + l3);
+      tm_st_wait();
+      tc_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->p_ready[x]);
+    }
+    // output of the row tile
+    const int64_t out_row = (int64_t)(p.q_tok + rt.tok0 + tok) * P.Hq + p.head * P.G + g;
+    if (rt.n > 0) {
+      if (!sy.wait_warp(&sh->o_full[x], o_par)) return;
+      o_par ^= 1u;
+      tc_after();
+    }
+    if (p.slot >= 0) {
+      float* part = P.partial + (int64_t)p.slot * kSlot + (int64_t)x * kTileM * (DP + 2);
+      if (live) {
+        part[kTileM * DP + row] = ref == -INFINITY ? -INFINITY : ref * sc;
+        part[kTileM * DP + kTileM + row] = l;
+      }
+      for (int c = 0; c < DP && rt.n > 0; c += 32) {
+        float o[32];
+        tm_ld32(to + c, o);
+        tm_ld_wait();
+        if (live) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<float4*>(part + row * DP + c + i) =
+                make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        }
+      }
+    } else {
+      const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+      for (int c = 0; c < DP; c += 32) {
+        float o[32];
+        if (rt.n > 0) {
+          tm_ld32(to + c, o);
+          tm_ld_wait();
+        }
+        if (live) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            if (c + i < P.D) {
+              uint32_t w[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                w[k] = l == 0.f ? 0u : pack2<T>(o[i + 2 * k] * inv, o[i + 2 * k + 1] * inv);
+              *reinterpret_cast<uint4*>(P.out + out_row * P.D + c + i) =
+                  make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+        }
+      }
+      if (live && P.lse)
+        P.lse[out_row] =
+            l == 0.f ? -INFINITY : (ref * sc + log2f(l)) * 0.69314718055994531f;
+    }
+    tc_before();  // O has been read before the next item's P is announced
+  }
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreadsC, 1)
+    k_attn_chunk(const __grid_constant__ AttnMaps M, const __grid_constant__ AttnParams P,
+                 const __grid_constant__ Plan plan, int tok1) {
+  extern __shared__ uint8_t smem_raw[];
+  ChunkSmem<DP>* sh = reinterpret_cast<ChunkSmem<DP>*>(
+      smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023));
+  const int warp = threadIdx.x >> 5;
+  pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ChunkSmem<DP>::kStages; ++i) {
+      mbar_init(&sh->full[i], 1);
+      mbar_init(&sh->empty[i], 1);
+      mbar_init(&sh->land[i], 1);
+    }
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&sh->q_full[x], 1);
+      mbar_init(&sh->q_empty[x], 1);
+      mbar_init(&sh->s_full[x], 1);
+      mbar_init(&sh->p_ready[x], 4);
+      mbar_init(&sh->o_full[x], 1);
+    }
+    mbar_init(&sh->drain, 1);
+    sh->abort = 0;
+    fence_mbar_init();
+    prefetch_map(&M.k);
+    prefetch_map(&M.v);
+    prefetch_map(&M.q);
+  }
+  if (warp == kWarpMma) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
+                     smem_u32(&sh->tmem))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_before();
+  __syncthreads();
+  tc_after();
+  pdl_wait();
+  const int n_pieces = __ldcg(plan.head + kPlanPieces);
+  if (warp < kWarpMma) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+    chunk_softmax<T, DP>(P, plan, n_pieces, tok1, warp >> 2, sh);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+    if (warp == kWarpMma)
+      chunk_mma<T, DP>(P, plan, n_pieces, tok1, sh);
+    else if (warp == kWarpLoad)
+      chunk_load<DP>(P, M, plan, n_pieces, tok1, sh);
+    else if (warp == kWarpFix)
+      chunk_fix<DP>(P, plan, n_pieces, tok1, sh);
+  }
+  tc_before();
+  __syncthreads();
+  tc_after();
+  if (warp == kWarpMma)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(sh->tmem));
+}
+
+// Joins the parts of split items: a warp per row, a lane per 4 columns.
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) k_attn_join(const __grid_constant__ AttnParams P,
+                                                   const __grid_constant__ Plan plan, int tok1) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int joins = __ldcg(plan.head + kPlanJoins);
+  const int lane = threadIdx.x & 31;
+  constexpr int kSlot = 2 * kTileM * (DP + 2);
+  const int64_t warps = (int64_t)gridDim.x * 8;
+  for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < (int64_t)joins * 2 * kTileM;
+       i += warps) {
+    const Join& jn = plan.joins[i / (2 * kTileM)];
+    const int r = (int)(i % (2 * kTileM)), x = r / kTileM, row = r % kTileM;
+    const int tok = row / P.G;
+    if (tok >= tok1 || x * tok1 + tok >= jn.n_tok) continue;
+    const float* base = P.partial + (int64_t)jn.slot * kSlot + (int64_t)x * kTileM * (DP + 2);
+    float m = -INFINITY;
+    for (int k = 0; k < jn.parts; ++k) m = fmaxf(m, base[(int64_t)k * kSlot + kTileM * DP + row]);
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < jn.parts; ++k) {
+      const float* b = base + (int64_t)k * kSlot;
+      const float mk = b[kTileM * DP + row];
+      if (mk == -INFINITY) continue;  // a part without keys of this row left no O
+      const float f = ex2(mk - m);
+      l += f * b[kTileM * DP + kTileM + row];
+      if (lane * 4 < DP) {
+        const float4 v = *reinterpret_cast<const float4*>(b + row * DP + lane * 4);
+        o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;
+      }
+    }
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    const int64_t out_row =
+        (int64_t)(jn.q_tok + x * tok1 + tok) * P.Hq + jn.head * P.G + row % P.G;
+    if (lane * 4 < P.D)
+      *reinterpret_cast<uint2*>(P.out + out_row * P.D + lane * 4) =
+          make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
+    if (lane == 0 && P.lse)
+      P.lse[out_row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+  }
+}
+
+int64_t chunk_groups(int64_t total_q, int batch, int G) {
+  return total_q / (2 * (kTileM / G)) + batch;
+}
+
+template <typename T, int DP>
+int run_chunk(const AttnMaps& M, const AttnParams& P, const Plan& plan, int tok1, int64_t groups,
+              cudaStream_t stream) {
+  constexpr size_t smem = sizeof(ChunkSmem<DP>) + 1024;
+  static_assert(smem <= 227 * 1024, "shared memory");
+  cudaFuncAttributes at;
+  cudaError_t err = cudaFuncGetAttributes(&at, k_attn_chunk<T, DP>);
+  if (err != cudaSuccess) return cuda_status(err);
+  // the warpgroups' shares must add up to what a block is launched with
+  if (at.numRegs < kRegsLaunch) return FTB_ERR_NOT_BUILT;
+  err = cudaFuncSetAttribute(k_attn_chunk<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)smem);
+  if (err != cudaSuccess) return cuda_status(err);
+  const int sms = sm_count();
+  const size_t plan_smem = ((size_t)P.batch + 1) * sizeof(int);
+  err = cudaFuncSetAttribute(k_attn_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+  if (err != cudaSuccess) return cuda_status(err);
+  err = launch_pdl(k_attn_plan, dim3(1), dim3(kPlanThreads), plan_smem, stream, P, plan, 2 * tok1,
+                   sms);
+  if (err != cudaSuccess) return cuda_status(err);
+  err = launch_pdl(k_attn_chunk<T, DP>, dim3((unsigned)sms), dim3(kThreadsC), smem, stream, M, P,
+                   plan, tok1);
+  if (err != cudaSuccess) return cuda_status(err);
+  return cuda_status(launch_pdl(k_attn_join<T, DP>, dim3((unsigned)sms * 2), dim3(256), 0, stream,
+                                P, plan, tok1));
+}
+
+}  // namespace
+
+size_t attn_chunk_workspace_bytes(int64_t total_q, int batch, int Hkv, int G, int D) {
+  size_t bytes;
+  const int64_t groups = chunk_groups(total_q, batch, G);
+  carve_plan(nullptr, groups, Hkv, &bytes);
+  const int dp = D <= 64 ? 64 : 128;
+  return bytes + (size_t)plan_parts() * 2 * kTileM * (dp + 2) * sizeof(float);
+}
+
+int launch_attn_chunk(const ftb_attn_args& a, AttnParams P, cudaStream_t stream) {
+  const int tok1 = kTileM / P.G;
+  const int64_t groups = chunk_groups(a.total_q, a.batch, P.G);
+  if (a.batch > 49152 || groups * a.Hkv > 0x3fffffff) return FTB_ERR_SHAPE;
+  AttnMaps M;
+  const uint32_t r = a.page < kTileK ? a.page : kTileK;
+  int st = attn_cache_map(&M.k, a.k_cache, a, a.k_strides, r, 1);
+  if (!st) st = attn_cache_map(&M.v, a.v_cache, a, a.v_strides, r, 1);
+  if (!st) st = attn_q_map(&M.q, a, (uint32_t)P.G, (uint32_t)tok1);
+  if (st) return st;
+  size_t bytes;
+  const Plan plan = carve_plan(reinterpret_cast<char*>(P.partial), groups, a.Hkv, &bytes);
+  P.partial = reinterpret_cast<float*>(reinterpret_cast<char*>(P.partial) + bytes);
+  const int dp = a.D <= 64 ? 64 : 128;
+  if (a.type == FTB_TYPE_BF16)
+    return dp == 64 ? run_chunk<__nv_bfloat16, 64>(M, P, plan, tok1, groups, stream)
+                    : run_chunk<__nv_bfloat16, 128>(M, P, plan, tok1, groups, stream);
+  return dp == 64 ? run_chunk<__half, 64>(M, P, plan, tok1, groups, stream)
+                  : run_chunk<__half, 128>(M, P, plan, tok1, groups, stream);
+}
+
+}  // namespace ftb
