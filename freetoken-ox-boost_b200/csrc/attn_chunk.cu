@@ -32,8 +32,8 @@ constexpr int kTileK = 128;   // keys per tile
 constexpr int kTileM = 128;   // rows per tile
 constexpr int kThreadsC = 384;
 constexpr int kWarpMma = 8, kWarpLoad = 9, kWarpFix = 10;
-// registers: softmax 2 x 128 threads x 216 + 128 x 72 = 64512 = 384 x 168 at launch
-constexpr int kRegsLaunch = 168, kRegsSoftmax = 216, kRegsOther = 72;
+// registers: softmax 2 x 128 threads x 200 + 128 x 104 = 64512 = 384 x 168 at launch
+constexpr int kRegsLaunch = 168, kRegsSoftmax = 200, kRegsOther = 104;
 static_assert(2 * 128 * kRegsSoftmax + 128 * kRegsOther <= kThreadsC * kRegsLaunch, "registers");
 constexpr int kTmemS = 0, kTmemO = 256;  // + 128 for tile B
 constexpr float kLazy = 8.f;             // log2 of what a score may exceed the reference by
@@ -278,9 +278,10 @@ __global__ void __launch_bounds__(kPlanThreads)
 // Shared-memory operand descriptors, 128-byte swizzle, 8-row atoms 1024 bytes apart. K-major (Q,
 // K): rows of 64 elements. MN-major (V): a row is a key; blocks of 64 of the D columns are
 // kTileK * 128 bytes apart.
-__device__ __forceinline__ uint64_t desc_base(uint32_t saddr, uint32_t lbo) {
-  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) |
-         ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+// The high word is the same for all: the helpers below take the low one.
+constexpr uint32_t kDescHigh = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_low(uint32_t saddr, uint32_t lbo) {
+  return ((saddr & 0x3FFFFu) >> 4) | ((lbo >> 4) << 16);
 }
 // Instruction descriptor, kind::f16: fp32 D, A and B bf16 or f16, M = 128, B K-major or MN-major.
 template <typename T>
@@ -290,20 +291,22 @@ __device__ __forceinline__ constexpr uint32_t idesc(int n, bool b_mn) {
          ((uint32_t)(kTileM >> 4) << 24);
 }
 // Issued by one elected lane of the converged warp.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id,
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t id,
                                        uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(id), "r"(acc)
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 x, {%1, %5};\n\tmov.b64 y, {%2, %5};\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(id), "r"(acc), "r"(kDescHigh)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id,
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t id,
                                        uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(id), "r"(acc)
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 y, {%2, %5};\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(id), "r"(acc), "r"(kDescHigh)
       : "memory");
 }
 __device__ __forceinline__ void mma_commit1(uint64_t* bar) {
@@ -334,19 +337,27 @@ __device__ __forceinline__ void tm_ld32(uint32_t t, float* v) {
       : "r"(t)
       : "memory");
 }
+// 16 columns of this warp's 32 lanes (no wait).
+__device__ __forceinline__ void tm_ld16(uint32_t t, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(t)
+      : "memory");
+}
 __device__ __forceinline__ void tm_ld_wait() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void tm_st32(uint32_t t, const uint32_t* r) {
+__device__ __forceinline__ void tm_st16(uint32_t t, const uint32_t* r) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
-      "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, "
-      "%29, %30, %31, %32};" ::"r"(t),
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+      "%11, %12, %13, %14, %15, %16};" ::"r"(t),
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-      "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
-      "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
-      "r"(r[30]), "r"(r[31])
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 __device__ __forceinline__ void tm_st_wait() {
@@ -360,6 +371,31 @@ __device__ __forceinline__ void tma_4d(uint32_t dst, const CUtensorMap* map, int
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(g), "r"(head), "r"(tok), "r"(smem_u32(bar))
       : "memory");
 }
+// Two fp32 values as one operand of the packed instructions.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // ---- the kernel --------------------------------------------------------------------------------
 
 constexpr int chunk_stages(int DP) { return DP == 128 ? 5 : 8; }
@@ -445,9 +481,9 @@ __device__ void chunk_load(const AttnParams& P, const AttnMaps& M, const Plan& p
   const uint32_t q_bytes = (uint32_t)(tok1 * P.G) * 128 * kH;
   int stage = 0;
   uint32_t parity = 1, q_par[2] = {1, 1};
-  // phases issued so far on each barrier, for the exit after a timeout
-  uint32_t n_full[kStages] = {}, n_land[kStages] = {}, n_q[2] = {};
-  bool ok = true;
+  // for the exit after a timeout: stages whose last copy signals land[], a bit each
+  uint32_t on_land = 0, land_par = 0;  // parity of a stage's next phase on land[]
+  bool ok = true, first_round = true;
   for (int round = 0; ok; ++round) {
     const int at = piece_at(round);
     if (at >= n_pieces) break;
@@ -475,9 +511,8 @@ __device__ void chunk_load(const AttnParams& P, const AttnMaps& M, const Plan& p
       if (!ok) break;
       const bool fix = v && (key0 < p.lo || key0 + kTileK > p.hi);
       uint64_t* bar = fix ? &sh->land[stage] : &sh->full[stage];
-#pragma unroll
-      for (int i = 0; i < kStages; ++i)
-        if (i == stage) n_full[i] += !fix, n_land[i] += fix;
+      on_land = fix ? on_land | 1u << stage : on_land & ~(1u << stage);
+      land_par ^= (uint32_t)fix << stage;
       if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(b1 - b0) * box_bytes);
       __syncwarp();
       if (mine) {
@@ -486,7 +521,7 @@ __device__ void chunk_load(const AttnParams& P, const AttnMaps& M, const Plan& p
         for (int h = 0; h < kH; ++h)
           tma_5d(dst + h * kTileK * 128, v ? &M.v : &M.k, h * 64, row, p.head, id, 0, bar);
       }
-      if (++stage == kStages) stage = 0, parity ^= 1u;
+      if (++stage == kStages) stage = 0, parity ^= 1u, first_round = false;
       if (j == 0) {  // Q after the first K: its buffers come free last
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
@@ -495,7 +530,6 @@ __device__ void chunk_load(const AttnParams& P, const AttnMaps& M, const Plan& p
           ok = sy.wait_warp(&sh->q_empty[x], q_par[x]);
           if (!ok) break;
           q_par[x] ^= 1u;
-          ++n_q[x];
           if (lane == 0) {
             mbar_arrive_expect_tx(&sh->q_full[x], q_bytes);
 #pragma unroll
@@ -510,15 +544,16 @@ __device__ void chunk_load(const AttnParams& P, const AttnMaps& M, const Plan& p
   }
   if (!ok) {  // a wait gave up: stay until the copies in flight have landed (again bounded)
     for (int i = 0; i < kStages; ++i) {
-      for (uint32_t k = 0; n_land[i] && k < kSpinLimit; ++k)
-        if (mbar_try_wait(&sh->land[i], (n_land[i] - 1) & 1u)) break;
-      // full[] also takes the fixer's arrivals, one for each land[] phase
-      for (uint32_t k = 0; n_full[i] && k < kSpinLimit; ++k)
-        if (mbar_try_wait(&sh->full[i], (n_full[i] + n_land[i] - 1) & 1u)) break;
+      // the last use of stage i: this round of the ring before `stage`, the one before after it
+      const bool land = on_land >> i & 1u;
+      const uint32_t par = land ? (land_par >> i & 1u) ^ 1u : i < stage ? parity ^ 1u : parity;
+      if (!land && i >= stage && first_round) continue;  // never used
+      for (uint32_t k = 0; k < kSpinLimit; ++k)
+        if (mbar_try_wait(land ? &sh->land[i] : &sh->full[i], par)) break;
     }
     for (int x = 0; x < 2; ++x)
-      for (uint32_t k = 0; n_q[x] && k < kSpinLimit; ++k)
-        if (mbar_try_wait(&sh->q_full[x], (n_q[x] - 1) & 1u)) break;
+      for (uint32_t k = 0; k < kSpinLimit; ++k)  // (before its first copy: passes at once)
+        if (mbar_try_wait(&sh->q_full[x], q_par[x])) break;
   }
 }
 
@@ -567,9 +602,9 @@ __device__ void chunk_mma(const AttnParams& P, const Plan& plan, int n_pieces, i
   constexpr int kTileBytes = ChunkSmem<DP>::kTileBytes;
   const ChunkSync<DP> sy{sh, P.status};
   const uint32_t tb = sh->tmem;
-  const uint64_t qd = desc_base(smem_u32(sh->q[0]), 16);
-  const uint64_t kd = desc_base(smem_u32(sh->ring[0]), 16);
-  const uint64_t vd = desc_base(smem_u32(sh->ring[0]), kTileK * 128);
+  const uint32_t qd = desc_low(smem_u32(sh->q[0]), 16);
+  const uint32_t kd = desc_low(smem_u32(sh->ring[0]), 16);
+  const uint32_t vd = desc_low(smem_u32(sh->ring[0]), kTileK * 128);
   constexpr uint32_t kIdS = idesc<T>(kTileK, false), kIdO = idesc<T>(DP, true);
   int stage = 0;
   uint32_t parity = 0, q_par[2] = {0, 0}, p_par[2] = {0, 0};
@@ -590,10 +625,10 @@ __device__ void chunk_mma(const AttnParams& P, const Plan& plan, int n_pieces, i
     }
     tc_after();
     const uint32_t d = tb + kTmemO + x * 128, a = tb + kTmemS + x * 128;
-    const uint64_t b = vd + (uint64_t)((v_stage * kTileBytes) >> 4);
+    const uint32_t b = vd + (uint32_t)((v_stage * kTileBytes) >> 4);
 #pragma unroll
     for (int k = 0; k < kTileK / 16; ++k)
-      mma_ts(d, a + k * 8, b + (uint64_t)((k * 16 * 128) >> 4), kIdO, (k > 0 || acc[x]) ? 1u : 0u);
+      mma_ts(d, a + k * 8, b + (uint32_t)((k * 16 * 128) >> 4), kIdO, (k > 0 || acc[x]) ? 1u : 0u);
     if (last[x]) mma_commit1(&sh->o_full[x]);
     pend[x] = false;
   };
@@ -619,11 +654,11 @@ __device__ void chunk_mma(const AttnParams& P, const Plan& plan, int n_pieces, i
           q_par[x] ^= 1u;
         }
         tc_after();
-        const uint64_t a = qd + (uint64_t)((x * kTileBytes) >> 4);
-        const uint64_t b = kd + (uint64_t)((stage * kTileBytes) >> 4);
+        const uint32_t a = qd + (uint32_t)((x * kTileBytes) >> 4);
+        const uint32_t b = kd + (uint32_t)((stage * kTileBytes) >> 4);
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k) {
-          const uint64_t o = (uint64_t)(((k >> 2) * kTileK * 128 + (k & 3) * 32) >> 4);
+          const uint32_t o = (uint32_t)(((k >> 2) * kTileK * 128 + (k & 3) * 32) >> 4);
           mma_ss(tb + kTmemS + x * 128, a + o, b + o, kIdS, k > 0 ? 1u : 0u);
         }
         mma_commit1(&sh->s_full[x]);
@@ -696,42 +731,50 @@ __device__ void chunk_softmax(const AttnParams& P, const Plan& plan, int n_piece
       }
       float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
 #pragma unroll
-      for (int c = 4; c < kTileK; c += 4) {
-        m0 = fmaxf(m0, s[c]), m1 = fmaxf(m1, s[c + 1]);
-        m2 = fmaxf(m2, s[c + 2]), m3 = fmaxf(m3, s[c + 3]);
+      for (int c = 4; c + 8 <= kTileK; c += 8) {
+        m0 = max3(m0, s[c], s[c + 1]), m1 = max3(m1, s[c + 2], s[c + 3]);
+        m2 = max3(m2, s[c + 4], s[c + 5]), m3 = max3(m3, s[c + 6], s[c + 7]);
       }
-      const float mx = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+      m0 = max3(m0, s[kTileK - 4], s[kTileK - 3]), m1 = max3(m1, s[kTileK - 2], s[kTileK - 1]);
+      const float mx = fmaxf(max3(m0, m1, m2), m3);
       const bool move = (mx - ref) * sc > kLazy;  // from -inf always (NaN where both are)
       if (__any_sync(0xffffffffu, move)) {
         const float f = move ? ex2((ref - mx) * sc) : 1.f;
         if (move) ref = mx;
         l *= f;
         if (j > 0) {  // P V of the tiles before has finished: S of this one came after it
-#pragma unroll
-          for (int c = 0; c < DP; c += 32) {
-            float o[32];
-            tm_ld32(to + c, o);
+#pragma unroll 1
+          for (int c = 0; c < DP; c += 16) {  // 16 at a time: the scores stay in registers
+            float o[16];
+            tm_ld16(to + c, o);
             tm_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] *= f;
-            tm_st32(to + c, reinterpret_cast<uint32_t*>(o));
+            for (int i = 0; i < 16; ++i) o[i] *= f;
+            tm_st16(to + c, reinterpret_cast<uint32_t*>(o));
           }
         }
       }
       const float off = ref == -INFINITY ? 0.f : -ref * sc;
-      float l0 = 0.f, l1 = 0.f, l2 = 0.f, l3 = 0.f;
-      uint32_t pk[kTileK / 2];
+      const uint64_t sc2 = pair(sc, sc), off2 = pair(off, off);
+      uint64_t l0 = 0, l1 = 0;
 #pragma unroll
-      for (int c = 0; c < kTileK; c += 4) {
-        const float p0 = ex2(fmaf(s[c], sc, off)), p1 = ex2(fmaf(s[c + 1], sc, off));
-        const float p2 = ex2(fmaf(s[c + 2], sc, off)), p3 = ex2(fmaf(s[c + 3], sc, off));
-        l0 += p0, l1 += p1, l2 += p2, l3 += p3;
-        pk[c / 2] = pack2<T>(p0, p1);
-        pk[c / 2 + 1] = pack2<T>(p2, p3);
+      for (int h = 0; h < kTileK / 32; ++h) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const int c = h * 32 + 2 * i;
+          float a0, a1, a2, a3;
+          unpair(fma2(pair(s[c], s[c + 1]), sc2, off2), a0, a1);
+          unpair(fma2(pair(s[c + 2], s[c + 3]), sc2, off2), a2, a3);
+          a0 = ex2(a0), a1 = ex2(a1), a2 = ex2(a2), a3 = ex2(a3);
+          l0 = add2(l0, pair(a0, a1)), l1 = add2(l1, pair(a2, a3));
+          pk[i] = pack2<T>(a0, a1), pk[i + 1] = pack2<T>(a2, a3);
+        }
+        tm_st16(ts + h * 16, pk);
       }
-      tm_st32(ts, pk);
-      tm_st32(ts + 32, pk + 32);
-      l += (l0 + l1) + (l2 + l3);
+      float la, lb;
+      unpair(add2(l0, l1), la, lb);
+      l += la + lb;
       tm_st_wait();
       tc_before();
       __syncwarp();
