@@ -71,6 +71,7 @@ enum { kPlanPieces = 0, kPlanJoins = 1, kPlanInts = 64 };
 constexpr int kClasses = 8;
 constexpr int kPlanThreads = 1024;
 constexpr int kPartsPerSm = 8;
+constexpr int kPlanSmem = 200 * 1024, kMaxBatch = kPlanSmem / 4 - 1;
 
 // Parts of split items: their number, not the sizes of the call, bounds the workspace.
 int plan_parts() { return kPartsPerSm * sm_count(); }
@@ -945,18 +946,19 @@ int run_chunk(const AttnMaps& M, const AttnParams& P, const Plan& plan, int tok1
               cudaStream_t stream) {
   constexpr size_t smem = sizeof(ChunkSmem<DP>) + 1024;
   static_assert(smem <= 227 * 1024, "shared memory");
-  cudaFuncAttributes at;
-  cudaError_t err = cudaFuncGetAttributes(&at, k_attn_chunk<T, DP>);
-  if (err != cudaSuccess) return cuda_status(err);
   // the warpgroups' shares must add up to what a block is launched with
-  if (at.numRegs < kRegsLaunch) return FTB_ERR_NOT_BUILT;
-  err = cudaFuncSetAttribute(k_attn_chunk<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)smem);
+  static const bool fits = [] {
+    cudaFuncAttributes at;
+    return cudaFuncGetAttributes(&at, k_attn_chunk<T, DP>) == cudaSuccess &&
+           at.numRegs >= kRegsLaunch;
+  }();
+  if (!fits) return FTB_ERR_NOT_BUILT;
+  static std::atomic<uint64_t> done{0}, plan_done{0};
+  cudaError_t err = allow_smem(k_attn_chunk<T, DP>, smem, done);
+  if (err == cudaSuccess) err = allow_smem(k_attn_plan, kPlanSmem, plan_done);
   if (err != cudaSuccess) return cuda_status(err);
   const int sms = sm_count();
   const size_t plan_smem = ((size_t)P.batch + 1) * sizeof(int);
-  err = cudaFuncSetAttribute(k_attn_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
-  if (err != cudaSuccess) return cuda_status(err);
   err = launch_pdl(k_attn_plan, dim3(1), dim3(kPlanThreads), plan_smem, stream, P, plan, 2 * tok1,
                    sms);
   if (err != cudaSuccess) return cuda_status(err);
@@ -980,7 +982,7 @@ size_t attn_chunk_workspace_bytes(int64_t total_q, int batch, int Hkv, int G, in
 int launch_attn_chunk(const ftb_attn_args& a, AttnParams P, cudaStream_t stream) {
   const int tok1 = kTileM / P.G;
   const int64_t groups = chunk_groups(a.total_q, a.batch, P.G);
-  if (a.batch > 49152 || groups * a.Hkv > 0x3fffffff) return FTB_ERR_SHAPE;
+  if (a.batch > kMaxBatch || groups * a.Hkv > 0x3fffffff) return FTB_ERR_SHAPE;
   AttnMaps M;
   const uint32_t r = a.page < kTileK ? a.page : kTileK;
   int st = attn_cache_map(&M.k, a.k_cache, a, a.k_strides, r, 1);

@@ -556,8 +556,8 @@ template <typename T, int DP>
 int run_stream(const AttnMaps& M, const AttnParams& P, dim3 grid, cudaStream_t stream) {
   constexpr size_t smem = sizeof(StreamSmem<DP>) + 1024;
   static_assert(smem <= 113 * 1024, "two blocks per SM");
-  cudaError_t err = cudaFuncSetAttribute(k_attn_stream<T, DP>,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static std::atomic<uint64_t> done{0};
+  cudaError_t err = allow_smem(k_attn_stream<T, DP>, smem, done);
   if (err != cudaSuccess) return cuda_status(err);
   return cuda_status(launch_pdl(k_attn_stream<T, DP>, grid, dim3(kThreads), smem, stream, M, P));
 }

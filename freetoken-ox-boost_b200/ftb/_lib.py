@@ -192,6 +192,8 @@ _lib = None
 def load(path: str = LIB_PATH):
     """Load libftb.so once; raise if it is absent (no CPU or Python fallback exists)."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib

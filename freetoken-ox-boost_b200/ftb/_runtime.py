@@ -10,7 +10,13 @@ from . import _lib
 _WS: dict = {}
 
 
+# The current stream's handle without a Stream object around it (2.3 us less per call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_handle(device: torch.device) -> int:
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 
@@ -33,12 +39,34 @@ def require(t: torch.Tensor, name: str, dtype=None, shape=None, contiguous=True)
         raise ValueError(f"{name} must be contiguous")
 
 
+def signature(*tensors) -> tuple:
+    """What the argument checks of a call look at: shape, strides, dtype and device of each tensor
+    (or the None in its place)."""
+    return tuple([None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+                  for t in tensors])
+
+
+_ARGS: dict = {}
+
+
+def checked_args(key: tuple, make):
+    """A copy of the argument block that ``make()`` built, all but its pointers, when a call of this
+    ``key`` (its signature and options) was first checked. The checks cost more than the launch."""
+    a = _ARGS.get(key)
+    if a is None:
+        a = make()
+        if len(_ARGS) >= 4096:
+            _ARGS.clear()
+        _ARGS[key] = a
+    return type(a).from_buffer_copy(a)
+
+
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     """A cached uint8 device buffer of at least ``nbytes`` for the current stream.
 
     Grown (never shrunk) on demand; call once eagerly before CUDA-graph capture so capture
     does not allocate. Calls on one stream are ordered, so sharing it per stream is safe."""
-    key = (device.index, torch.cuda.current_stream(device).cuda_stream)
+    key = (device.index, stream_handle(device))
     t = _WS.get(key)
     if t is None or t.numel() < nbytes:
         t = torch.empty(max(int(nbytes), 1 << 16), dtype=torch.uint8, device=device)
@@ -49,7 +77,7 @@ def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
 def zeroed_workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     """A cached buffer like :func:`workspace`, of its own and zero-filled when it is made: for
     calls whose counters start at zero and are left at zero."""
-    key = (device.index, torch.cuda.current_stream(device).cuda_stream, "zeroed")
+    key = (device.index, stream_handle(device), "zeroed")
     t = _WS.get(key)
     if t is None or t.numel() < nbytes:
         t = torch.zeros(int(nbytes), dtype=torch.uint8, device=device)

@@ -6,35 +6,20 @@ import ctypes
 import torch
 
 from . import _lib
-from ._runtime import read_status, require_cuda, stream_handle, zeroed_workspace
-from .block import _TYPE
+from ._runtime import (checked_args, read_status, require_cuda, signature, stream_handle,
+                       zeroed_workspace)
+from .block import _TYPE, _new
 
 
 def _int32(t, name, shape, dev):
-    if t.dtype != torch.int32 or t.device != dev or tuple(t.shape) != shape or (
-            t.shape[-1] > 1 and t.stride(-1) != 1):
+    if t.dtype != torch.int32 or t.device != dev or t.shape != shape or (
+            not t.is_contiguous() and t.shape[-1] > 1 and t.stride(-1) != 1):
         raise ValueError(f"{name}: {tuple(t.shape)} {t.dtype} on {t.device}, expected int32 "
                          f"{shape} on {dev} with contiguous rows")
 
 
-def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
-                    block_table: torch.Tensor, kv_len: torch.Tensor,
-                    cu_q: torch.Tensor | None = None, max_q: int = 1, *,
-                    scale: float | None = None, causal: bool = True, window: int = 0,
-                    out: torch.Tensor | None = None, return_lse: bool = False,
-                    check_status: bool = False):
-    """Attention of the new tokens of a batch over their sequences' pages; their own keys and
-    values are in the caches already (``rope_append``).
-
-    ``q`` [total, q heads, D]; caches [pages, page, kv heads, D] (any strides with contiguous
-    heads); ``block_table`` int32 [batch, width]; ``kv_len`` int32 [batch], keys of each sequence
-    with the new ones. ``cu_q`` int32 [batch + 1] gives the rows of each sequence in ``q`` and
-    ``max_q`` the most of them; without ``cu_q`` every sequence has one new token (decode).
-    Token i of n sees the keys up to its own position ``kv_len - n + i`` (``causal``), and no more
-    than the last ``window`` of them (0: all). A token that sees none gets 0 (lse -inf).
-    Returns out [total, q heads, D], with ``return_lse`` also the natural log of the sum of the
-    exponentials, float32 [total, q heads]. ``check_status`` reads the device status word
-    (synchronises) and raises on page ids, lengths or starts outside the tensors."""
+def _args(q, k_cache, v_cache, block_table, kv_len, cu_q, max_q, scale, causal, window):
+    """The checks of a call, and its arguments without the pointers."""
     dev = require_cuda(q)
     if q.dim() != 3 or q.dtype not in _TYPE or q.stride(2) != 1:
         raise ValueError(f"q: {tuple(q.shape)} {q.dtype}, expected [total, heads, D] bf16 or f16 "
@@ -60,25 +45,54 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                          f"max_q {max_q})")
     if window < 0:
         raise ValueError(f"window={window}")
-    if out is None:
-        out = torch.empty(total, Hq, D, dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
-        raise ValueError("out must be contiguous, of q's shape and dtype")
-    lse = torch.empty(total, Hq, dtype=torch.float32, device=dev) if return_lse else None
-    lib = _lib.load()
-    nbytes = lib.ftb_attention_workspace_bytes(total, batch, max_q, Hq, Hkv, D)
-    ws = zeroed_workspace(nbytes, dev)
-    a = _lib.AttnArgsStruct(
-        q=q.data_ptr(), k_cache=k_cache.data_ptr(), v_cache=v_cache.data_ptr(),
-        block_table=block_table.data_ptr(), kv_len=kv_len.data_ptr(),
-        cu_q=0 if cu_q is None else cu_q.data_ptr(), out=out.data_ptr(),
-        lse=0 if lse is None else lse.data_ptr(), workspace=ws.data_ptr(),
-        workspace_bytes=ws.numel(), q_strides=q.stride()[:2], k_strides=k_cache.stride()[:3],
+    nbytes = _lib.load().ftb_attention_workspace_bytes(total, batch, max_q, Hq, Hkv, D)
+    return _lib.AttnArgsStruct(
+        workspace_bytes=nbytes, q_strides=q.stride()[:2], k_strides=k_cache.stride()[:3],
         v_strides=v_cache.stride()[:3], total_q=total, num_pages=pages,
         table_stride=block_table.stride(0), batch=batch, max_q=int(max_q), table_width=width,
         page=page, Hq=Hq, Hkv=Hkv, D=D, causal=int(causal), window=int(window),
         type=_TYPE[q.dtype], scale=D ** -0.5 if scale is None else scale)
-    _lib.check("ftb_attention", lib.ftb_attention(ctypes.byref(a), stream_handle(dev)))
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                    block_table: torch.Tensor, kv_len: torch.Tensor,
+                    cu_q: torch.Tensor | None = None, max_q: int = 1, *,
+                    scale: float | None = None, causal: bool = True, window: int = 0,
+                    out: torch.Tensor | None = None, return_lse: bool = False,
+                    check_status: bool = False):
+    """Attention of the new tokens of a batch over their sequences' pages; their own keys and
+    values are in the caches already (``rope_append``).
+
+    ``q`` [total, q heads, D]; caches [pages, page, kv heads, D] (any strides with contiguous
+    heads); ``block_table`` int32 [batch, width]; ``kv_len`` int32 [batch], keys of each sequence
+    with the new ones. ``cu_q`` int32 [batch + 1] gives the rows of each sequence in ``q`` and
+    ``max_q`` the most of them; without ``cu_q`` every sequence has one new token (decode).
+    Token i of n sees the keys up to its own position ``kv_len - n + i`` (``causal``), and no more
+    than the last ``window`` of them (0: all). A token that sees none gets 0 (lse -inf).
+    Returns out [total, q heads, D], with ``return_lse`` also the natural log of the sum of the
+    exponentials, float32 [total, q heads]. ``check_status`` reads the device status word
+    (synchronises) and raises on page ids, lengths or starts outside the tensors."""
+    a = checked_args(
+        ("attention", signature(q, k_cache, v_cache, block_table, kv_len, cu_q), max_q, scale,
+         causal, window),
+        lambda: _args(q, k_cache, v_cache, block_table, kv_len, cu_q, max_q, scale, causal, window))
+    dev = q.device
+    if out is None:
+        out = _new(q, q.dtype)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
+        raise ValueError("out must be contiguous, of q's shape and dtype")
+    lse = q.new_empty(q.shape[:2], dtype=torch.float32) if return_lse else None
+    ws = zeroed_workspace(a.workspace_bytes, dev)
+    a.q, a.k_cache, a.v_cache = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+    a.block_table, a.kv_len, a.out = block_table.data_ptr(), kv_len.data_ptr(), out.data_ptr()
+    a.workspace = ws.data_ptr()
+    if cu_q is not None:
+        a.cu_q = cu_q.data_ptr()
+    if lse is not None:
+        a.lse = lse.data_ptr()
+    st = _lib.load().ftb_attention(ctypes.byref(a), stream_handle(dev))
+    if st:
+        _lib.check("ftb_attention", st)
     if check_status:
         status = read_status(ws)
         if status:
