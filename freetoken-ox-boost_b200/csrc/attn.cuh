@@ -3,7 +3,6 @@
 
 #include <cuda.h>
 
-#include <atomic>
 #include <type_traits>
 
 #include "ftb_common.cuh"
@@ -49,20 +48,6 @@ int launch_attn_stream(const ftb_attn_args& a, AttnParams P, cudaStream_t stream
 size_t attn_stream_partial_bytes(int64_t rows_max, int D);
 int launch_attn_chunk(const ftb_attn_args& a, AttnParams P, cudaStream_t stream);
 size_t attn_chunk_workspace_bytes(int64_t total_q, int batch, int Hkv, int G, int D);
-
-// Raises a kernel's dynamic shared memory limit once per device (a call to the driver costs
-// microseconds). `done`: a bit per device, one word per kernel.
-template <typename K>
-cudaError_t allow_smem(K kernel, size_t bytes, std::atomic<uint64_t>& done) {
-  int dev = 0;
-  cudaError_t err = cudaGetDevice(&dev);
-  if (err != cudaSuccess) return err;
-  const uint64_t bit = 1ull << (dev & 63);
-  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
-  err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-  if (err == cudaSuccess && dev < 64) done.fetch_or(bit, std::memory_order_release);
-  return err;
-}
 
 __device__ __forceinline__ void tma_5d(uint32_t dst, const CUtensorMap* map, int x, int row,
                                        int head, int page, int half, uint64_t* bar) {

@@ -286,3 +286,17 @@ def test_rope_in_place_and_refusals():
     refuse(q_out=torch.empty(5, 4, 64, device="cuda"))
     got = ftb.rope_append(**{**args, "q_out": q})
     assert got is q and torch.equal(q, want)
+
+
+@pytest.mark.parametrize("H", [9, 63, 257, 2041, 2042, 4099, 8185, 8190, 16377, 16383])
+@pytest.mark.parametrize("rows", [3, 700])
+def test_block_norm_odd_widths_with_gates(H, rows):
+    """Rows that follow one another at a width that is no multiple of 8, and views of them that
+    start off a 16-byte boundary."""
+    run_norm(rows, H, BF, F32, "full")
+    run_norm(rows, H, F16, F16, "channel", "sigmoid")
+    run_norm(rows, H, BF, BF, "token", post=False)
+    x = torch.randn(rows * H + 1, device="cuda").to(BF)[1:].view(rows, H)
+    w = torch.ones(H, dtype=BF, device="cuda")
+    _, _, ref, b = ref_norm(x, None, None, None, 1, w, 1e-6, None)
+    near(ftb.rms_norm(x, w), ref, b)
