@@ -32,8 +32,8 @@ constexpr int kTileK = 128;   // keys per tile
 constexpr int kTileM = 128;   // rows per tile
 constexpr int kThreadsC = 384;
 constexpr int kWarpMma = 8, kWarpLoad = 9, kWarpFix = 10;
-// registers: softmax 2 x 128 threads x 200 + 128 x 104 = 64512 = 384 x 168 at launch
-constexpr int kRegsLaunch = 168, kRegsSoftmax = 200, kRegsOther = 104;
+// registers: softmax 2 x 128 threads x 208 + 128 x 88 = 64512 = 384 x 168 at launch
+constexpr int kRegsLaunch = 168, kRegsSoftmax = 208, kRegsOther = 88;
 static_assert(2 * 128 * kRegsSoftmax + 128 * kRegsOther <= kThreadsC * kRegsLaunch, "registers");
 constexpr int kTmemS = 0, kTmemO = 256;  // + 128 for tile B
 constexpr float kLazy = 8.f;             // log2 of what a score may exceed the reference by
@@ -57,21 +57,20 @@ struct Join {
   int q_tok, n_tok, head, slot, parts;
   int pad[3];
 };
+static_assert(sizeof(Join) == 32, "two 16-byte loads");
 
 struct Plan {
-  int* head;     // kPlan* counts
+  int* head;        // kPlan* counts
   Piece* pieces;
   Join* joins;
-  int4* groups;  // per group (sequence, two row tiles): sequence, first token, tiles [z, w)
-  int* pos;      // per group: place among its size class
-  int* part0;    // per group that is cut: its first part's number among one kv head's parts
+  int* scratch;     // 3 ints per group, where they do not fit the plan block's shared memory
   int max_pieces, max_parts, max_joins, max_groups;
 };
 enum { kPlanPieces = 0, kPlanJoins = 1, kPlanInts = 64 };
-constexpr int kClasses = 8;
+constexpr int kClasses = 4;
 constexpr int kPlanThreads = 1024;
 constexpr int kPartsPerSm = 8;
-constexpr int kPlanSmem = 200 * 1024, kMaxBatch = kPlanSmem / 4 - 1;
+constexpr int kPlanSmem = 200 * 1024, kMaxBatch = kPlanSmem / 8;
 
 // Parts of split items: their number, not the sizes of the call, bounds the workspace.
 int plan_parts() { return kPartsPerSm * sm_count(); }
@@ -91,33 +90,43 @@ Plan carve_plan(char* base, int64_t groups, int Hkv, size_t* bytes) {
   p.head = reinterpret_cast<int*>(take(kPlanInts * 4));
   p.pieces = reinterpret_cast<Piece*>(take((size_t)p.max_pieces * sizeof(Piece)));
   p.joins = reinterpret_cast<Join*>(take((size_t)p.max_joins * sizeof(Join)));
-  p.groups = reinterpret_cast<int4*>(take((size_t)groups * sizeof(int4)));
-  p.pos = reinterpret_cast<int*>(take((size_t)groups * 4));
-  p.part0 = reinterpret_cast<int*>(take((size_t)groups * 4));
+  p.scratch = reinterpret_cast<int*>(take((size_t)groups * 12));
   *bytes = off;
   return p;
 }
 
-// Inclusive sum over the block; *total gets the block's sum.
-__device__ __forceinline__ int block_scan(int v, int* red, int* total) {
+// Inclusive sums of N counts over the block; total[] gets the block's sums.
+template <int N>
+__device__ __forceinline__ void block_scan(int (&v)[N], int (&total)[N], int (*red)[32]) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += u;
-  }
-  __syncthreads();
-  if (lane == 31) red[warp] = v;
-  __syncthreads();
-  int w = red[lane];
+  for (int o = 1; o < 32; o <<= 1)
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(0xffffffffu, w, o);
-    if (lane >= o) w += u;
+    for (int k = 0; k < N; ++k) {
+      const int u = __shfl_up_sync(0xffffffffu, v[k], o);
+      if (lane >= o) v[k] += u;
+    }
+  __syncthreads();
+  if (lane == 31)
+#pragma unroll
+    for (int k = 0; k < N; ++k) red[k][warp] = v[k];
+  __syncthreads();
+  int w[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) w[k] = red[k][lane];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int u = __shfl_up_sync(0xffffffffu, w[k], o);
+      if (lane >= o) w[k] += u;
+    }
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    total[k] = __shfl_sync(0xffffffffu, w[k], 31);
+    const int before = __shfl_sync(0xffffffffu, w[k], (warp + 31) & 31);
+    v[k] += warp ? before : 0;
   }
-  *total = __shfl_sync(0xffffffffu, w, 31);
-  const int before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
-  return v + (warp ? before : 0);
 }
 
 // How a group of `tiles` key tiles is cut: into `parts` pieces of at most `size` tiles.
@@ -134,37 +143,51 @@ __device__ __forceinline__ Cut cut_group(int tiles, int most) {
   return c;
 }
 
-// One block. tok = tokens per group (two row tiles).
+// One block. tok = tokens per group (two row tiles); blocks = blocks that will take the pieces.
 __global__ void __launch_bounds__(kPlanThreads)
-    k_attn_plan(const __grid_constant__ AttnParams P, Plan plan, int tok, int blocks) {
-  extern __shared__ int first_group[];  // [batch + 1]
-  __shared__ int red[32];
-  __shared__ int class_n[kClasses];
+    k_attn_plan(const __grid_constant__ AttnParams P, const __grid_constant__ Plan plan, int tok,
+                int blocks) {
+  extern __shared__ int dyn[];
+  __shared__ int red[kClasses + 1][32];
   __shared__ unsigned long long sum_tiles;
-  __shared__ int n_parts, n_joins, biggest;
-  const int tid = threadIdx.x;
+  __shared__ int biggest, n_joins, most_best, parts_of[32];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int* first_group = dyn;  // [batch + 1]
   pdl_launch_dependents();
   if (tid == 0) sum_tiles = 0, biggest = 0, n_joins = 0;
+  if (tid < 32) parts_of[tid] = 0;
   pdl_wait();
-  int base = 0;
+  int groups = 0;
   for (int b0 = 0; b0 < P.batch; b0 += kPlanThreads) {
     const int b = b0 + tid;
-    int n = 0;
+    int n[1] = {0}, total[1];
     if (b < P.batch) {
       const AttnSeq s = attn_seq(P, b);
       if (s.bad_len || s.bad_rows)
         atomicOr(P.status, (s.bad_len ? kAttnBadPage : 0u) | (s.bad_rows ? kAttnBadRows : 0u));
-      n = (s.n + tok - 1) / tok;
+      n[0] = (s.n + tok - 1) / tok;
     }
-    int total;
-    const int incl = block_scan(n, red, &total);
-    if (b < P.batch) first_group[b] = base + incl - n;
-    base += total;
+    const int mine = n[0];
+    block_scan<1>(n, total, red);
+    if (b < P.batch) first_group[b] = groups + n[0] - mine;
+    groups += total[0];
   }
-  if (tid == 0) first_group[P.batch] = base;
+  // (sequences that overlap, status bit 1, could make more groups than the rows allow)
+  groups = min(groups, plan.max_groups);
+  if (tid == 0) first_group[P.batch] = groups;
   __syncthreads();
-  // (lengths that overlap, bad_rows, could make more groups than the rows allow)
-  const int groups = base < plan.max_groups ? base : plan.max_groups;
+  // per group: sequence, place among its size class, number of its first part
+  int* seq_of = dyn + P.batch + 1;
+  if ((size_t)(P.batch + 1 + 3 * groups) * 4 > kPlanSmem) seq_of = plan.scratch;
+  int* pos = seq_of + groups;
+  int* part0 = pos + groups;
+  auto key_tiles = [&](const AttnSeq& s, int i0, KeyRange& r) {
+    const int i1 = min(i0 + tok, s.n);
+    r = attn_range(P, s, i0, i1 - 1);
+    int2 t = make_int2(0, 0);
+    if (r.lo < r.hi) t = make_int2(r.lo / kTileK, (r.hi + kTileK - 1) / kTileK);
+    return t;
+  };
   unsigned long long mine = 0;
   int big = 0;
   for (int g = tid; g < groups; g += kPlanThreads) {
@@ -176,99 +199,111 @@ __global__ void __launch_bounds__(kPlanThreads)
       else
         z = mid;
     }
-    const AttnSeq s = attn_seq(P, a);
-    const int i0 = (g - first_group[a]) * tok;
-    const int i1 = i0 + tok < s.n ? i0 + tok : s.n;
-    const KeyRange r = attn_range(P, s, i0, i1 - 1);
-    int4 v = make_int4(a, i0, 0, 0);
-    if (r.lo < r.hi) v.z = r.lo / kTileK, v.w = (r.hi + kTileK - 1) / kTileK;
-    plan.groups[g] = v;
-    mine += v.w - v.z;
-    big = max(big, v.w - v.z);
+    seq_of[g] = a;
+    KeyRange r;
+    const int2 t = key_tiles(attn_seq(P, a), (g - first_group[a]) * tok, r);
+    pos[g] = t.y - t.x;  // for now
+    mine += t.y - t.x;
+    big = max(big, t.y - t.x);
   }
   if (mine) atomicAdd(&sum_tiles, mine);
   if (big) atomicMax(&biggest, big);
   __syncthreads();
-  // Pieces of at most `most` tiles: a quarter of an even share of the work, so that the last
-  // pieces end close together, but no shorter than 16 tiles (or the share itself, where that is
-  // less): a piece pays for its Q copy and its output.
-  const unsigned long long all = sum_tiles * P.Hkv;
-  const int share = (int)min((all + blocks - 1) / blocks, 1ull << 29);
-  int most = max(share / 4, min(16, max(2, share)));
-  for (;;) {
-    __syncthreads();
-    if (tid == 0) n_parts = 0;
-    if (tid < kClasses) class_n[tid] = 0;
-    __syncthreads();
-    const int top = min(most, max(biggest, 1));
-    for (int g = tid; g < groups; g += kPlanThreads) {
-      const int4 v = plan.groups[g];
-      const Cut c = cut_group(v.w - v.z, most);
-      if (c.parts > 1) atomicAdd(&n_parts, c.parts * P.Hkv);
-      atomicAdd(&class_n[min(kClasses - 1, (top - c.size) * kClasses / top)], c.parts);
+  // The longest piece: the longest item cut into 1, 2, ... parts (lane by lane), whichever ends
+  // first by an estimate: rounds of pieces of the mean size, kPieceTiles for the start and end of
+  // a piece, kJoinTiles more for a part that has to be joined.
+  constexpr int kPieceTiles = 2, kJoinTiles = 1, kFewest = 2;
+  const int top = max(biggest, 1);
+  const int ways = lane < 16 ? lane + 1 : (lane - 13) * (lane - 13) / 2 + 12;  // 1..16, 16.., 174
+  const int most = max((top + ways - 1) / ways, kFewest);
+  int n_mine = 0;
+  for (int g = warp; g < groups; g += kPlanThreads / 32)
+    n_mine += cut_group(pos[g], most).parts;
+  if (n_mine) atomicAdd(&parts_of[lane], n_mine);
+  __syncthreads();
+  if (warp == 0) {
+    const int64_t n = (int64_t)parts_of[lane] * P.Hkv;
+    const int64_t rounds = (n + blocks - 1) / blocks;
+    const float mean = n ? (float)(sum_tiles * P.Hkv) / (float)n : 0.f;
+    float cost = fmaxf((float)most, mean * rounds) + kPieceTiles * rounds;
+    if (n > (int64_t)groups * P.Hkv) cost += kJoinTiles * rounds;
+    if (n - (int64_t)groups * P.Hkv > plan.max_parts / 2) cost = INFINITY;  // parts <= 2 (n - items)
+    int best = lane;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float c = __shfl_xor_sync(0xffffffffu, cost, o);
+      const int b = __shfl_xor_sync(0xffffffffu, best, o);
+      if (c < cost || (c == cost && b < best)) cost = c, best = b;
     }
-    __syncthreads();
-    if (n_parts <= plan.max_parts) break;
-    most *= 2;
+    const int m = __shfl_sync(0xffffffffu, most, best);
+    if (lane == 0) most_best = m;
   }
-  const int top = min(most, max(biggest, 1));
-  // place of each group among its class, and the parts' numbers
-  for (int k = 0; k <= kClasses; ++k) {  // the last round numbers the parts
-    int run = 0;
-    for (int g0 = 0; g0 < groups; g0 += kPlanThreads) {
-      const int g = g0 + tid;
-      int n = 0;
-      bool in = false;
-      if (g < groups) {
-        const int4 v = plan.groups[g];
-        const Cut c = cut_group(v.w - v.z, most);
-        in = k == kClasses ? c.parts > 1
-                           : min(kClasses - 1, (top - c.size) * kClasses / top) == k;
-        n = in ? c.parts : 0;
-      }
-      int total;
-      const int incl = block_scan(n, red, &total);
-      if (in) (k < kClasses ? plan.pos : plan.part0)[g] = run + incl - n;
-      run += total;
+  __syncthreads();
+  const int limit = min(most_best, top);
+  // places: largest pieces first, by class
+  int run[kClasses + 1] = {};
+  for (int g0 = 0; g0 < groups; g0 += kPlanThreads) {
+    const int g = g0 + tid;
+    int v[kClasses + 1] = {}, total[kClasses + 1];
+    int k = 0, parts = 0;
+    if (g < groups) {
+      const Cut c = cut_group(pos[g], limit);
+      k = min(kClasses - 1, (limit - c.size) * kClasses / limit);
+      parts = c.parts;
+#pragma unroll
+      for (int i = 0; i < kClasses; ++i) v[i] = i == k ? parts : 0;
+      v[kClasses] = parts > 1 ? parts : 0;
     }
+    block_scan<kClasses + 1>(v, total, red);
+    if (g < groups) {
+      int at = 0;
+#pragma unroll
+      for (int i = 0; i < kClasses; ++i)
+        if (i == k) at = run[i] + v[i] - parts;
+      pos[g] = at;
+      part0[g] = run[kClasses] + v[kClasses] - (parts > 1 ? parts : 0);
+    }
+#pragma unroll
+    for (int i = 0; i <= kClasses; ++i) run[i] += total[i];
   }
   __syncthreads();
   // emission: a warp per group, a lane per piece; in a class one kv head after another, so that
   // blocks that run at the same time share keys
-  const int warp = tid >> 5, lane = tid & 31;
   for (int g = warp; g < groups; g += kPlanThreads / 32) {
-    const int4 v = plan.groups[g];
-    const AttnSeq s = attn_seq(P, v.x);
-    const int tiles = v.w - v.z;
-    const Cut c = cut_group(tiles, most);
-    const int k = min(kClasses - 1, (top - c.size) * kClasses / top);
-    int start = 0;
-    for (int i = 0; i < k; ++i) start += class_n[i] * P.Hkv;
-    const int i1 = v.y + tok < s.n ? v.y + tok : s.n;
-    const KeyRange r = attn_range(P, s, v.y, i1 - 1);
-    const int slot0 = c.parts > 1 ? plan.part0[g] : 0;
+    const int seq = seq_of[g], i0 = (g - first_group[seq]) * tok;
+    const AttnSeq s = attn_seq(P, seq);
+    KeyRange r;
+    const int2 t = key_tiles(s, i0, r);
+    const Cut c = cut_group(t.y - t.x, limit);
+    const int k = min(kClasses - 1, (limit - c.size) * kClasses / limit);
+    int start = 0, per_head = 0;
+#pragma unroll
+    for (int i = 0; i < kClasses; ++i) {
+      if (i < k) start += run[i] * P.Hkv;
+      if (i == k) per_head = run[i];
+    }
     Piece p;
-    p.q_tok = s.q0 + v.y, p.n_tok = i1 - v.y, p.seq = v.x;
-    p.pos = s.len - s.n + v.y, p.len = s.len, p.lo = r.lo, p.hi = r.hi, p.pad = 0;
+    p.q_tok = s.q0 + i0, p.n_tok = min(tok, s.n - i0), p.seq = seq;
+    p.pos = s.len - s.n + i0, p.len = s.len, p.lo = r.lo, p.hi = r.hi, p.pad = 0;
     for (int i = lane; i < c.parts * P.Hkv; i += 32) {
-      const int head = i / c.parts, part = i % c.parts;
+      const int head = i / c.parts, part = i - head * c.parts;
       p.head = head;
-      p.t0 = v.z + part * c.size;
-      p.t1 = min(p.t0 + c.size, v.w);
-      p.slot = c.parts > 1 ? slot0 * P.Hkv + i : -1;
-      plan.pieces[start + head * class_n[k] + plan.pos[g] + part] = p;
+      p.t0 = t.x + part * c.size;
+      p.t1 = min(p.t0 + c.size, t.y);
+      p.slot = c.parts > 1 ? part0[g] * P.Hkv + i : -1;
+      plan.pieces[start + head * per_head + pos[g] + part] = p;
       if (c.parts > 1 && part == 0) {
-        const int j = atomicAdd(&n_joins, 1);
         Join o{};
         o.q_tok = p.q_tok, o.n_tok = p.n_tok, o.head = head, o.slot = p.slot, o.parts = c.parts;
-        plan.joins[j] = o;
+        plan.joins[atomicAdd(&n_joins, 1)] = o;
       }
     }
   }
   __syncthreads();
   if (tid == 0) {
     int n = 0;
-    for (int k = 0; k < kClasses; ++k) n += class_n[k] * P.Hkv;
+#pragma unroll
+    for (int i = 0; i < kClasses; ++i) n += run[i] * P.Hkv;
     plan.head[kPlanPieces] = n;
     plan.head[kPlanJoins] = n_joins;
   }
@@ -381,14 +416,29 @@ __device__ __forceinline__ uint64_t pair(float a, float b) {
 __device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) {
   asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
 }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+// Packed and special-function instructions as volatile statements, which keep their order.
+__device__ __forceinline__ uint64_t fma2v(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  asm volatile("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+__device__ __forceinline__ uint64_t add2v(uint64_t a, uint64_t b) {
   uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  asm volatile("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float ex2v(float x) {
+  float r;
+  asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2v(float lo, float hi) {
+  uint32_t r;
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm volatile("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -409,7 +459,7 @@ struct ChunkSmem {
   uint64_t full[kStages], empty[kStages];
   uint64_t land[kStages];  // a V tile that the fixer completes has landed
   uint64_t q_full[2], q_empty[2];
-  uint64_t s_full[2], p_ready[2], o_full[2];
+  uint64_t s_full[2], p_ready[2][2], o_full[2];  // p_ready: by halves of the keys
   uint64_t drain;
   uint32_t tmem;
   int abort;
@@ -616,9 +666,8 @@ __device__ void chunk_mma(const AttnParams& P, const Plan& plan, int n_pieces, i
   bool v_there = false, ok = true, issued = false;
 
   auto pv = [&](int x) {
-    ok = sy.wait_warp(&sh->p_ready[x], p_par[x]);
+    ok = sy.wait_warp(&sh->p_ready[x][0], p_par[x]);
     if (!ok) return;
-    p_par[x] ^= 1u;
     if (!v_there) {
       ok = sy.wait_warp(&sh->full[v_stage], v_par);
       if (!ok) return;
@@ -628,8 +677,15 @@ __device__ void chunk_mma(const AttnParams& P, const Plan& plan, int n_pieces, i
     const uint32_t d = tb + kTmemO + x * 128, a = tb + kTmemS + x * 128;
     const uint32_t b = vd + (uint32_t)((v_stage * kTileBytes) >> 4);
 #pragma unroll
-    for (int k = 0; k < kTileK / 16; ++k)
+    for (int k = 0; k < kTileK / 16; ++k) {
+      if (k == kTileK / 32) {
+        ok = sy.wait_warp(&sh->p_ready[x][1], p_par[x]);
+        if (!ok) return;
+        tc_after();
+      }
       mma_ts(d, a + k * 8, b + (uint32_t)((k * 16 * 128) >> 4), kIdO, (k > 0 || acc[x]) ? 1u : 0u);
+    }
+    p_par[x] ^= 1u;
     if (last[x]) mma_commit1(&sh->o_full[x]);
     pend[x] = false;
   };
@@ -716,28 +772,35 @@ __device__ void chunk_softmax(const AttnParams& P, const Plan& plan, int n_piece
       if (!sy.wait_warp(&sh->s_full[x], s_par)) return;
       s_par ^= 1u;
       tc_after();
-      float s[kTileK];
-#pragma unroll
-      for (int c = 0; c < kTileK; c += 32) tm_ld32(ts + c, s + c);
-      tm_ld_wait();
-      if (flip) {
-#pragma unroll
-        for (int c = 0; c < kTileK; ++c) s[c] = -s[c];
-      }
+      float s[kTileK], m0 = -INFINITY, m1 = -INFINITY;
       const int key0 = (p.t0 + j) * kTileK;
-      if (key0 < all_min || key0 + kTileK > all_max) {
-        const int a = kmin - key0, b = kmax - key0;
+      const bool masked = key0 < all_min || key0 + kTileK > all_max;
+      const int a = kmin - key0, b = kmax - key0;
+      // sign, mask and maximum of half the scores while the other half is loading
+      auto look = [&](int c0) {
+        if (flip) {
 #pragma unroll
-        for (int c = 0; c < kTileK; ++c) s[c] = c >= a && c < b ? s[c] : -INFINITY;
-      }
-      float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
+          for (int c = c0; c < c0 + kTileK / 2; ++c) s[c] = -s[c];
+        }
+        if (masked) {
 #pragma unroll
-      for (int c = 4; c + 8 <= kTileK; c += 8) {
-        m0 = max3(m0, s[c], s[c + 1]), m1 = max3(m1, s[c + 2], s[c + 3]);
-        m2 = max3(m2, s[c + 4], s[c + 5]), m3 = max3(m3, s[c + 6], s[c + 7]);
-      }
-      m0 = max3(m0, s[kTileK - 4], s[kTileK - 3]), m1 = max3(m1, s[kTileK - 2], s[kTileK - 1]);
-      const float mx = fmaxf(max3(m0, m1, m2), m3);
+          for (int c = c0; c < c0 + kTileK / 2; ++c) s[c] = c >= a && c < b ? s[c] : -INFINITY;
+        }
+        float m2 = -INFINITY, m3 = -INFINITY;
+#pragma unroll
+        for (int c = c0; c < c0 + kTileK / 2; c += 8) {
+          m0 = max3(m0, s[c], s[c + 1]), m1 = max3(m1, s[c + 2], s[c + 3]);
+          m2 = max3(m2, s[c + 4], s[c + 5]), m3 = max3(m3, s[c + 6], s[c + 7]);
+        }
+        m0 = fmaxf(m0, m2), m1 = fmaxf(m1, m3);
+      };
+      tm_ld32(ts, s), tm_ld32(ts + 32, s + 32);
+      tm_ld_wait();
+      tm_ld32(ts + 64, s + 64), tm_ld32(ts + 96, s + 96);
+      look(0);
+      tm_ld_wait();
+      look(kTileK / 2);
+      const float mx = fmaxf(m0, m1);
       const bool move = (mx - ref) * sc > kLazy;  // from -inf always (NaN where both are)
       if (__any_sync(0xffffffffu, move)) {
         const float f = move ? ex2((ref - mx) * sc) : 1.f;
@@ -757,29 +820,43 @@ __device__ void chunk_softmax(const AttnParams& P, const Plan& plan, int n_piece
       }
       const float off = ref == -INFINITY ? 0.f : -ref * sc;
       const uint64_t sc2 = pair(sc, sc), off2 = pair(off, off);
+      // The instructions of neighbouring pairs are laid between the exponentials of a pair, which
+      // keep the special-function unit busy for 16 cycles: the product and sum of a pair kAhead
+      // later, rounding and summing of one kAhead before. In program order (volatile): left to
+      // itself the compiler does all of a kind in a row, and the unit waits.
+      // P goes out in two halves: the MMAs of the first run beside the exponentials of the second.
       uint64_t l0 = 0, l1 = 0;
+      constexpr int kPairs = kTileK / 2, kAhead = 4;
+      uint32_t pk[16];
+      auto scaled = [&](int i) {
+        unpair(fma2v(pair(s[2 * i], s[2 * i + 1]), sc2, off2), s[2 * i], s[2 * i + 1]);
+      };
 #pragma unroll
-      for (int h = 0; h < kTileK / 32; ++h) {
-        uint32_t pk[16];
+      for (int i = 0; i < kAhead; ++i) scaled(i);
 #pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          const int c = h * 32 + 2 * i;
-          float a0, a1, a2, a3;
-          unpair(fma2(pair(s[c], s[c + 1]), sc2, off2), a0, a1);
-          unpair(fma2(pair(s[c + 2], s[c + 3]), sc2, off2), a2, a3);
-          a0 = ex2(a0), a1 = ex2(a1), a2 = ex2(a2), a3 = ex2(a3);
-          l0 = add2(l0, pair(a0, a1)), l1 = add2(l1, pair(a2, a3));
-          pk[i] = pack2<T>(a0, a1), pk[i + 1] = pack2<T>(a2, a3);
+      for (int i = 0; i < kPairs + kAhead; ++i) {
+        if (i < kPairs) s[2 * i] = ex2v(s[2 * i]);
+        if (i + kAhead < kPairs) scaled(i + kAhead);
+        if (i < kPairs) s[2 * i + 1] = ex2v(s[2 * i + 1]);
+        const int d = i - kAhead;  // done
+        if (d >= 0) {
+          pk[d % 16] = pack2v<T>(s[2 * d], s[2 * d + 1]);
+          uint64_t& sum = d & 1 ? l1 : l0;
+          sum = add2v(sum, pair(s[2 * d], s[2 * d + 1]));
+          if (d % 16 == 15) {
+            tm_st16(ts + (d / 16) * 16, pk);
+            if (d % 32 == 31) {
+              tm_st_wait();
+              tc_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&sh->p_ready[x][d / 32]);
+            }
+          }
         }
-        tm_st16(ts + h * 16, pk);
       }
       float la, lb;
-      unpair(add2(l0, l1), la, lb);
+      unpair(add2v(l0, l1), la, lb);
       l += la + lb;
-      tm_st_wait();
-      tc_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh->p_ready[x]);
     }
     // output of the row tile
     const int64_t out_row = (int64_t)(p.q_tok + rt.tok0 + tok) * P.Hq + p.head * P.G + g;
@@ -854,7 +931,8 @@ __global__ void __launch_bounds__(kThreadsC, 1)
       mbar_init(&sh->q_full[x], 1);
       mbar_init(&sh->q_empty[x], 1);
       mbar_init(&sh->s_full[x], 1);
-      mbar_init(&sh->p_ready[x], 4);
+      mbar_init(&sh->p_ready[x][0], 4);
+      mbar_init(&sh->p_ready[x][1], 4);
       mbar_init(&sh->o_full[x], 1);
     }
     mbar_init(&sh->drain, 1);
@@ -894,7 +972,8 @@ __global__ void __launch_bounds__(kThreadsC, 1)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(sh->tmem));
 }
 
-// Joins the parts of split items: a warp per row, a lane per 4 columns.
+// Joins the parts of split items: a warp per row, a lane per 4 columns. The parts' ref and l come
+// with one load per lane, their O rows several at a time.
 template <typename T, int DP>
 __global__ void __launch_bounds__(256) k_attn_join(const __grid_constant__ AttnParams P,
                                                    const __grid_constant__ Plan plan, int tok1) {
@@ -902,33 +981,54 @@ __global__ void __launch_bounds__(256) k_attn_join(const __grid_constant__ AttnP
   pdl_wait();
   const int joins = __ldcg(plan.head + kPlanJoins);
   const int lane = threadIdx.x & 31;
-  constexpr int kSlot = 2 * kTileM * (DP + 2);
+  constexpr int64_t kSlot = 2 * kTileM * (DP + 2);
   const int64_t warps = (int64_t)gridDim.x * 8;
   for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < (int64_t)joins * 2 * kTileM;
        i += warps) {
-    const Join& jn = plan.joins[i / (2 * kTileM)];
+    const int4 j0 = __ldcg(reinterpret_cast<const int4*>(plan.joins + i / (2 * kTileM)));
+    const int parts = __ldcg(&plan.joins[i / (2 * kTileM)].parts);
+    const int q_tok = j0.x, n_tok = j0.y, head = j0.z, slot = j0.w;
     const int r = (int)(i % (2 * kTileM)), x = r / kTileM, row = r % kTileM;
     const int tok = row / P.G;
-    if (tok >= tok1 || x * tok1 + tok >= jn.n_tok) continue;
-    const float* base = P.partial + (int64_t)jn.slot * kSlot + (int64_t)x * kTileM * (DP + 2);
-    float m = -INFINITY;
-    for (int k = 0; k < jn.parts; ++k) m = fmaxf(m, base[(int64_t)k * kSlot + kTileM * DP + row]);
-    float l = 0.f;
+    if (tok >= tok1 || x * tok1 + tok >= n_tok) continue;
+    const float* base = P.partial + slot * kSlot + (int64_t)x * kTileM * (DP + 2);
+    float m = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k = 0; k < jn.parts; ++k) {
-      const float* b = base + (int64_t)k * kSlot;
-      const float mk = b[kTileM * DP + row];
-      if (mk == -INFINITY) continue;  // a part without keys of this row left no O
-      const float f = ex2(mk - m);
-      l += f * b[kTileM * DP + kTileM + row];
-      if (lane * 4 < DP) {
-        const float4 v = *reinterpret_cast<const float4*>(b + row * DP + lane * 4);
-        o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;
+    for (int k0 = 0; k0 < parts; k0 += 32) {  // (one round, but for very long sequences)
+      const float* mine = base + (k0 + lane) * kSlot + kTileM * DP + row;
+      const bool in = k0 + lane < parts;
+      const float mk = in ? __ldcg(mine) : -INFINITY, lk = in ? __ldcg(mine + kTileM) : 0.f;
+      float mx = fmaxf(mk, m);
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+      if (mx == -INFINITY) continue;
+      const float keep = ex2(m - mx);  // of what came before this round
+      m = mx;
+      l *= keep, o.x *= keep, o.y *= keep, o.z *= keep, o.w *= keep;
+      const float fk = ex2(mk - mx);  // 0 for a part without keys of this row, which left no O
+      float add = fk * lk;
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) add += __shfl_xor_sync(0xffffffffu, add, d);
+      l += add;
+      const int n = min(32, parts - k0);
+      for (int k = 0; k < n; k += 4) {
+        float4 v[4];
+        float f[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          f[u] = __shfl_sync(0xffffffffu, fk, (k + u) & 31);
+          if (k + u >= n || lane * 4 >= DP) f[u] = 0.f;
+          v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (f[u] != 0.f)
+            v[u] = __ldcg(reinterpret_cast<const float4*>(base + (k0 + k + u) * kSlot + row * DP) + lane);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          o.x += f[u] * v[u].x, o.y += f[u] * v[u].y, o.z += f[u] * v[u].z, o.w += f[u] * v[u].w;
       }
     }
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-    const int64_t out_row =
-        (int64_t)(jn.q_tok + x * tok1 + tok) * P.Hq + jn.head * P.G + row % P.G;
+    const int64_t out_row = (int64_t)(q_tok + x * tok1 + tok) * P.Hq + head * P.G + row % P.G;
     if (lane * 4 < P.D)
       *reinterpret_cast<uint2*>(P.out + out_row * P.D + lane * 4) =
           make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
@@ -958,14 +1058,16 @@ int run_chunk(const AttnMaps& M, const AttnParams& P, const Plan& plan, int tok1
   if (err == cudaSuccess) err = allow_smem(k_attn_plan, kPlanSmem, plan_done);
   if (err != cudaSuccess) return cuda_status(err);
   const int sms = sm_count();
-  const size_t plan_smem = ((size_t)P.batch + 1) * sizeof(int);
+  // the plan's arrays by sequence and by group, the latter in the workspace where they are too many
+  size_t plan_smem = ((size_t)P.batch + 1 + 3 * (size_t)groups) * sizeof(int);
+  if (plan_smem > (size_t)kPlanSmem) plan_smem = kPlanSmem;
   err = launch_pdl(k_attn_plan, dim3(1), dim3(kPlanThreads), plan_smem, stream, P, plan, 2 * tok1,
                    sms);
   if (err != cudaSuccess) return cuda_status(err);
   err = launch_pdl(k_attn_chunk<T, DP>, dim3((unsigned)sms), dim3(kThreadsC), smem, stream, M, P,
                    plan, tok1);
   if (err != cudaSuccess) return cuda_status(err);
-  return cuda_status(launch_pdl(k_attn_join<T, DP>, dim3((unsigned)sms * 2), dim3(256), 0, stream,
+  return cuda_status(launch_pdl(k_attn_join<T, DP>, dim3((unsigned)sms * 8), dim3(256), 0, stream,
                                 P, plan, tok1));
 }
 
