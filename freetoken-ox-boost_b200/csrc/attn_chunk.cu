@@ -441,9 +441,9 @@ __device__ __forceinline__ uint32_t pack2v(float lo, float hi) {
     asm volatile("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
+__device__ __forceinline__ float max3v(float a, float b, float c) {
   float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm volatile("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
@@ -740,6 +740,13 @@ __device__ void chunk_mma(const AttnParams& P, const Plan& plan, int n_pieces, i
   }
 }
 
+// 32 bytes, one sector.
+__device__ __forceinline__ void st_sector(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]),
+               "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
 template <typename T, int DP>
 __device__ void chunk_softmax(const AttnParams& P, const Plan& plan, int n_pieces, int tok1, int x,
                               ChunkSmem<DP>* sh) {
@@ -752,6 +759,7 @@ __device__ void chunk_softmax(const AttnParams& P, const Plan& plan, int n_piece
   // becomes one that is small enough to be flat and keeps a masked -inf at -inf.
   const bool flip = P.scale_log2 < 0.f;
   const float sc = fmaxf(fabsf(P.scale_log2), 1e-30f);
+  const bool sectors = P.D % 16 == 0 && (reinterpret_cast<uintptr_t>(P.out) & 31) == 0;
   uint32_t s_par = 0, o_par = 0;
   constexpr int kSlot = 2 * kTileM * (DP + 2);
   for (int round = 0;; ++round) {
@@ -772,87 +780,115 @@ __device__ void chunk_softmax(const AttnParams& P, const Plan& plan, int n_piece
       if (!sy.wait_warp(&sh->s_full[x], s_par)) return;
       s_par ^= 1u;
       tc_after();
-      float s[kTileK], m0 = -INFINITY, m1 = -INFINITY;
+      float s[kTileK];
       const int key0 = (p.t0 + j) * kTileK;
       const bool masked = key0 < all_min || key0 + kTileK > all_max;
-      const int a = kmin - key0, b = kmax - key0;
-      // sign, mask and maximum of half the scores while the other half is loading
-      auto look = [&](int c0) {
+      auto load = [&] {
+#pragma unroll
+        for (int c = 0; c < kTileK; c += 32) tm_ld32(ts + c, s + c);
+        tm_ld_wait();
         if (flip) {
 #pragma unroll
-          for (int c = c0; c < c0 + kTileK / 2; ++c) s[c] = -s[c];
+          for (int c = 0; c < kTileK; ++c) s[c] = -s[c];
         }
-        if (masked) {
-#pragma unroll
-          for (int c = c0; c < c0 + kTileK / 2; ++c) s[c] = c >= a && c < b ? s[c] : -INFINITY;
-        }
-        float m2 = -INFINITY, m3 = -INFINITY;
-#pragma unroll
-        for (int c = c0; c < c0 + kTileK / 2; c += 8) {
-          m0 = max3(m0, s[c], s[c + 1]), m1 = max3(m1, s[c + 2], s[c + 3]);
-          m2 = max3(m2, s[c + 4], s[c + 5]), m3 = max3(m3, s[c + 6], s[c + 7]);
-        }
-        m0 = fmaxf(m0, m2), m1 = fmaxf(m1, m3);
       };
-      tm_ld32(ts, s), tm_ld32(ts + 32, s + 32);
-      tm_ld_wait();
-      tm_ld32(ts + 64, s + 64), tm_ld32(ts + 96, s + 96);
-      look(0);
-      tm_ld_wait();
-      look(kTileK / 2);
-      const float mx = fmaxf(m0, m1);
-      const bool move = (mx - ref) * sc > kLazy;  // from -inf always (NaN where both are)
-      if (__any_sync(0xffffffffu, move)) {
+      // moves the reference of the rows that exceed it, and what was summed with the old one
+      auto move_to = [&](float mx) {
+        const bool move = (mx - ref) * sc > kLazy;  // from -inf always (NaN where both are)
+        if (!__any_sync(0xffffffffu, move)) return;
         const float f = move ? ex2((ref - mx) * sc) : 1.f;
         if (move) ref = mx;
         l *= f;
-        if (j > 0) {  // P V of the tiles before has finished: S of this one came after it
+        if (j == 0) return;
+        // (P V of the tiles before has finished: S of this one came after it)
 #pragma unroll 1
-          for (int c = 0; c < DP; c += 16) {  // 16 at a time: the scores stay in registers
-            float o[16];
-            tm_ld16(to + c, o);
-            tm_ld_wait();
+        for (int c = 0; c < DP; c += 16) {  // 16 at a time: the scores stay in registers
+          float o[16];
+          tm_ld16(to + c, o);
+          tm_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] *= f;
-            tm_st16(to + c, reinterpret_cast<uint32_t*>(o));
-          }
+          for (int i = 0; i < 16; ++i) o[i] *= f;
+          tm_st16(to + c, reinterpret_cast<uint32_t*>(o));
         }
-      }
-      const float off = ref == -INFINITY ? 0.f : -ref * sc;
-      const uint64_t sc2 = pair(sc, sc), off2 = pair(off, off);
-      // The instructions of neighbouring pairs are laid between the exponentials of a pair, which
-      // keep the special-function unit busy for 16 cycles: the product and sum of a pair kAhead
-      // later, rounding and summing of one kAhead before. In program order (volatile): left to
-      // itself the compiler does all of a kind in a row, and the unit waits.
-      // P goes out in two halves: the MMAs of the first run beside the exponentials of the second.
-      uint64_t l0 = 0, l1 = 0;
-      constexpr int kPairs = kTileK / 2, kAhead = 4;
-      uint32_t pk[16];
-      auto scaled = [&](int i) {
-        unpair(fma2v(pair(s[2 * i], s[2 * i + 1]), sc2, off2), s[2 * i], s[2 * i + 1]);
       };
+      auto highest = [&] {
+        float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) scaled(i);
+        for (int c = 4; c < kTileK; c += 4) {
+          m0 = fmaxf(m0, s[c]), m1 = fmaxf(m1, s[c + 1]);
+          m2 = fmaxf(m2, s[c + 2]), m3 = fmaxf(m3, s[c + 3]);
+        }
+        return fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+      };
+      load();
+      // The maximum is rarely news after the first tile. It is taken beside the exponentials with
+      // the reference so far, and looked at before any of P is announced; only the first tile and
+      // masked ones take it beforehand.
+      bool known = j > 0 && !masked;
+      if (!known) {
+        if (masked) {
+          const int a = kmin - key0, b = kmax - key0;
 #pragma unroll
-      for (int i = 0; i < kPairs + kAhead; ++i) {
-        if (i < kPairs) s[2 * i] = ex2v(s[2 * i]);
-        if (i + kAhead < kPairs) scaled(i + kAhead);
-        if (i < kPairs) s[2 * i + 1] = ex2v(s[2 * i + 1]);
-        const int d = i - kAhead;  // done
-        if (d >= 0) {
-          pk[d % 16] = pack2v<T>(s[2 * d], s[2 * d + 1]);
+          for (int c = 0; c < kTileK; ++c) s[c] = c >= a && c < b ? s[c] : -INFINITY;
+        }
+        move_to(highest());
+      }
+      // The instructions of other pairs are laid between the two exponentials of a pair, which keep
+      // the special-function unit busy for 16 cycles: the products of pairs to come (all of them,
+      // and so the maximum, within the first half), rounding and summing of one kAhead before. In
+      // program order (volatile): left to itself the compiler does all of a kind in a row, and the
+      // unit waits. P goes out in two halves: the MMAs of the first run beside the exponentials of
+      // the second.
+      constexpr int kPairs = kTileK / 2, kAhead = 4;
+      uint64_t l0, l1;
+      for (;;) {
+        const float off = ref == -INFINITY ? 0.f : -ref * sc;
+        const uint64_t sc2 = pair(sc, sc), off2 = pair(off, off);
+        uint32_t pk[kPairs / 2];
+        float m0 = -INFINITY, m1 = -INFINITY;
+        l0 = l1 = 0;
+        auto scaled = [&](int i, float& m) {
+          unpair(fma2v(pair(s[2 * i], s[2 * i + 1]), sc2, off2), s[2 * i], s[2 * i + 1]);
+          m = max3v(m, s[2 * i], s[2 * i + 1]);
+        };
+        auto done = [&](int d) {
+          pk[d % (kPairs / 2)] = pack2v<T>(s[2 * d], s[2 * d + 1]);
           uint64_t& sum = d & 1 ? l1 : l0;
           sum = add2v(sum, pair(s[2 * d], s[2 * d + 1]));
-          if (d % 16 == 15) {
-            tm_st16(ts + (d / 16) * 16, pk);
-            if (d % 32 == 31) {
-              tm_st_wait();
-              tc_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&sh->p_ready[x][d / 32]);
-            }
-          }
+        };
+        auto announce = [&](int half) {
+          tm_st16(ts + half * 32, pk);
+          tm_st16(ts + half * 32 + 16, pk + 16);
+          tm_st_wait();
+          tc_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh->p_ready[x][half]);
+        };
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) scaled(i, m0);
+#pragma unroll
+        for (int i = 0; i < kPairs / 2; ++i) {
+          s[2 * i] = ex2v(s[2 * i]);
+          if (kAhead + 2 * i < kPairs) scaled(kAhead + 2 * i, m0);
+          s[2 * i + 1] = ex2v(s[2 * i + 1]);
+          if (kAhead + 2 * i + 1 < kPairs) scaled(kAhead + 2 * i + 1, m1);
+          if (i >= kAhead) done(i - kAhead);
         }
+        if (known && __any_sync(0xffffffffu, fmaxf(m0, m1) > kLazy)) {
+          known = false;  // rare: from the scores again, with the new maximum
+          load();
+          move_to(highest());
+          continue;
+        }
+#pragma unroll
+        for (int i = kPairs / 2; i < kPairs + kAhead; ++i) {
+          if (i < kPairs) s[2 * i] = ex2v(s[2 * i]);
+          done(i - kAhead);
+          if (i < kPairs) s[2 * i + 1] = ex2v(s[2 * i + 1]);
+          if (i - kAhead == kPairs / 2 - 1) announce(0);
+        }
+        announce(1);
+        break;
       }
       float la, lb;
       unpair(add2v(l0, l1), la, lb);
@@ -878,7 +914,7 @@ __device__ void chunk_softmax(const AttnParams& P, const Plan& plan, int n_piece
         if (live) {
 #pragma unroll
           for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<float4*>(part + row * DP + c + i) =
+            *reinterpret_cast<float4*>(part + ((c + i) / 4 * kTileM + row) * 4) =
                 make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
         }
       }
@@ -892,14 +928,18 @@ __device__ void chunk_softmax(const AttnParams& P, const Plan& plan, int n_piece
         }
         if (live) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-            if (c + i < P.D) {
-              uint32_t w[4];
+          for (int i = 0; i < 32; i += 16) {  // a sector at a time where rows are whole sectors
+            uint32_t w[8];
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                w[k] = l == 0.f ? 0u : pack2<T>(o[i + 2 * k] * inv, o[i + 2 * k + 1] * inv);
-              *reinterpret_cast<uint4*>(P.out + out_row * P.D + c + i) =
-                  make_uint4(w[0], w[1], w[2], w[3]);
+            for (int k = 0; k < 8; ++k)
+              w[k] = l == 0.f ? 0u : pack2<T>(o[i + 2 * k] * inv, o[i + 2 * k + 1] * inv);
+            uint16_t* op = P.out + out_row * P.D + c + i;
+            if (sectors) {
+              if (c + i < P.D) st_sector(op, w);
+            } else {
+              if (c + i < P.D) *reinterpret_cast<uint4*>(op) = make_uint4(w[0], w[1], w[2], w[3]);
+              if (c + i + 8 < P.D)
+                *reinterpret_cast<uint4*>(op + 8) = make_uint4(w[4], w[5], w[6], w[7]);
             }
           }
         }
@@ -972,8 +1012,8 @@ __global__ void __launch_bounds__(kThreadsC, 1)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(sh->tmem));
 }
 
-// Joins the parts of split items: a warp per row, a lane per 4 columns. The parts' ref and l come
-// with one load per lane, their O rows several at a time.
+// Joins the parts of split items. A part's O is [D / 4][row][4]: a warp takes 32 rows (a lane
+// each) and 16 columns, so that it reads whole lines and writes whole sectors.
 template <typename T, int DP>
 __global__ void __launch_bounds__(256) k_attn_join(const __grid_constant__ AttnParams P,
                                                    const __grid_constant__ Plan plan, int tok1) {
@@ -982,57 +1022,70 @@ __global__ void __launch_bounds__(256) k_attn_join(const __grid_constant__ AttnP
   const int joins = __ldcg(plan.head + kPlanJoins);
   const int lane = threadIdx.x & 31;
   constexpr int64_t kSlot = 2 * kTileM * (DP + 2);
+  constexpr int kCols = 16, kUnits = 2 * (kTileM / 32) * (DP / kCols);  // per join
+  const bool sectors = P.D % 16 == 0 && (reinterpret_cast<uintptr_t>(P.out) & 31) == 0;
   const int64_t warps = (int64_t)gridDim.x * 8;
-  for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < (int64_t)joins * 2 * kTileM;
+  for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < (int64_t)joins * kUnits;
        i += warps) {
-    const int4 j0 = __ldcg(reinterpret_cast<const int4*>(plan.joins + i / (2 * kTileM)));
-    const int parts = __ldcg(&plan.joins[i / (2 * kTileM)].parts);
+    const Join* jn = plan.joins + i / kUnits;
+    const int4 j0 = __ldcg(reinterpret_cast<const int4*>(jn));
+    const int parts = __ldcg(&jn->parts);
     const int q_tok = j0.x, n_tok = j0.y, head = j0.z, slot = j0.w;
-    const int r = (int)(i % (2 * kTileM)), x = r / kTileM, row = r % kTileM;
-    const int tok = row / P.G;
-    if (tok >= tok1 || x * tok1 + tok >= n_tok) continue;
+    const int u = (int)(i % kUnits), c0 = u % (DP / kCols) * kCols, r = u / (DP / kCols) * 32 + lane;
+    const int x = r / kTileM, row = r % kTileM, tok = row / P.G;
+    const bool live = tok < tok1 && x * tok1 + tok < n_tok;
+    if (!__any_sync(0xffffffffu, live) || c0 >= P.D) continue;
     const float* base = P.partial + slot * kSlot + (int64_t)x * kTileM * (DP + 2);
-    float m = -INFINITY, l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k0 = 0; k0 < parts; k0 += 32) {  // (one round, but for very long sequences)
-      const float* mine = base + (k0 + lane) * kSlot + kTileM * DP + row;
-      const bool in = k0 + lane < parts;
-      const float mk = in ? __ldcg(mine) : -INFINITY, lk = in ? __ldcg(mine + kTileM) : 0.f;
-      float mx = fmaxf(mk, m);
+    float m = -INFINITY, l = 0.f, o[kCols] = {};
+    constexpr int kTogether = 4;  // parts whose loads are in flight together
+    for (int k0 = 0; k0 < parts; k0 += kTogether) {
+      float mk[kTogether], lk[kTogether];
+      float4 v[kTogether][kCols / 4];
 #pragma unroll
-      for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+      for (int k = 0; k < kTogether; ++k) {
+        const float* b = base + (k0 + k) * kSlot;
+        const bool in = live && k0 + k < parts;
+        mk[k] = in ? __ldcg(b + kTileM * DP + row) : -INFINITY;
+        lk[k] = in ? __ldcg(b + kTileM * DP + kTileM + row) : 0.f;
+#pragma unroll
+        for (int q = 0; q < kCols / 4; ++q)
+          if (in) v[k][q] = __ldcg(reinterpret_cast<const float4*>(b) + (c0 / 4 + q) * kTileM + row);
+      }
+      float mx = m;
+#pragma unroll
+      for (int k = 0; k < kTogether; ++k) mx = fmaxf(mx, mk[k]);
       if (mx == -INFINITY) continue;
-      const float keep = ex2(m - mx);  // of what came before this round
+      const float keep = ex2(m - mx);  // of the parts before
       m = mx;
-      l *= keep, o.x *= keep, o.y *= keep, o.z *= keep, o.w *= keep;
-      const float fk = ex2(mk - mx);  // 0 for a part without keys of this row, which left no O
-      float add = fk * lk;
+      l *= keep;
 #pragma unroll
-      for (int d = 16; d > 0; d >>= 1) add += __shfl_xor_sync(0xffffffffu, add, d);
-      l += add;
-      const int n = min(32, parts - k0);
-      for (int k = 0; k < n; k += 4) {
-        float4 v[4];
-        float f[4];
+      for (int c = 0; c < kCols; ++c) o[c] *= keep;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          f[u] = __shfl_sync(0xffffffffu, fk, (k + u) & 31);
-          if (k + u >= n || lane * 4 >= DP) f[u] = 0.f;
-          v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (f[u] != 0.f)
-            v[u] = __ldcg(reinterpret_cast<const float4*>(base + (k0 + k + u) * kSlot + row * DP) + lane);
+      for (int k = 0; k < kTogether; ++k) {
+        if (mk[k] == -INFINITY) continue;  // a part without keys of this row left no O
+        const float f = ex2(mk[k] - mx);
+        l += f * lk[k];
+#pragma unroll
+        for (int q = 0; q < kCols / 4; ++q) {
+          o[4 * q] += f * v[k][q].x, o[4 * q + 1] += f * v[k][q].y;
+          o[4 * q + 2] += f * v[k][q].z, o[4 * q + 3] += f * v[k][q].w;
         }
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          o.x += f[u] * v[u].x, o.y += f[u] * v[u].y, o.z += f[u] * v[u].z, o.w += f[u] * v[u].w;
       }
     }
+    if (!live) continue;
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
     const int64_t out_row = (int64_t)(q_tok + x * tok1 + tok) * P.Hq + head * P.G + row % P.G;
-    if (lane * 4 < P.D)
-      *reinterpret_cast<uint2*>(P.out + out_row * P.D + lane * 4) =
-          make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
-    if (lane == 0 && P.lse)
+    uint16_t* op = P.out + out_row * P.D + c0;
+    uint32_t w[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) w[k] = pack2<T>(o[2 * k] * inv, o[2 * k + 1] * inv);
+    if (sectors) {
+      st_sector(op, w);
+    } else {
+      *reinterpret_cast<uint4*>(op) = make_uint4(w[0], w[1], w[2], w[3]);
+      if (c0 + 8 < P.D) *reinterpret_cast<uint4*>(op + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+    if (c0 == 0 && P.lse)
       P.lse[out_row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
   }
 }
