@@ -2,6 +2,7 @@
 // and the choice between the kernels.
 #include <cudaTypedefs.h>
 
+#include <algorithm>
 #include <cmath>
 #include <mutex>
 
@@ -16,9 +17,22 @@ CUtensorMapDataType attn_dtype(int type) {
   return type == FTB_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
 }
 
-// Up to 16 query rows per kv head go to the streaming kernel, more to the tensor-core kernel.
+// Which kernel: the streaming one for up to 16 query rows per kv head (one mma.sync row tile, bound
+// by DRAM), and for small work, where the tensor-core kernel's plan and join cost more than its
+// rate gives: at most 2 GFLOP by the bound that the host knows (every token against the whole
+// table, or its window). On one B200, us (streaming / tensor cores), 32 heads over 8 of 128: 64 new
+// tokens of a prompt 7.4 / 19.3, 256 18.2 / 21.9, 512 49 / 25; 16 tokens at 2048 keys 14.1 / 20.3, 64
+// 28.9 / 24.9.
 constexpr int kStreamRows = 16;
-bool streams(int64_t rows) { return rows <= kStreamRows; }
+constexpr double kStreamFlops = 2e9;
+bool streams(int64_t total_q, int max_q, int Hq, int Hkv, int D, int64_t keys) {
+  return (int64_t)max_q * (Hq / Hkv) <= kStreamRows ||
+         4.0 * D * Hq * (double)total_q * (double)keys <= kStreamFlops;
+}
+int64_t keys_bound(const ftb_attn_args& a) {
+  const int64_t all = (int64_t)a.table_width * a.page;
+  return a.window > 0 ? std::min<int64_t>(all, a.window) : all;
+}
 }  // namespace
 
 int attn_cache_map(CUtensorMap* m, const void* base, const ftb_attn_args& a,
@@ -62,9 +76,12 @@ size_t ftb_attention_workspace_bytes(int64_t total_q, int batch, int max_q, int 
   if (total_q < 0 || batch < 0 || max_q < 0 || Hkv < 1 || Hq < Hkv || D < 8) return 0;
   const int G = Hq / Hkv;
   if (G > 128) return 0;
+  const int64_t rows = (int64_t)max_q * G;
+  const size_t stream = attn_stream_partial_bytes(rows, D);
+  if (rows <= kStreamRows) return FTB_ATTN_ZERO_BYTES + stream;
+  // (more rows: either kernel, by the lengths)
   return FTB_ATTN_ZERO_BYTES +
-         (streams((int64_t)max_q * G) ? attn_stream_partial_bytes((int64_t)max_q * G, D)
-                                      : attn_chunk_workspace_bytes(total_q, batch, Hkv, G, D));
+         std::max(stream, attn_chunk_workspace_bytes(total_q, batch, Hkv, G, D));
 }
 
 int ftb_attention(const ftb_attn_args* a, ftb_stream_t stream) {
@@ -110,8 +127,9 @@ int ftb_attention(const ftb_attn_args* a, ftb_stream_t stream) {
   P.causal = a->causal != 0, P.window = a->window;
   P.keys_max = a->table_width * a->page;
   P.scale_log2 = a->scale * 1.44269504088896341f;
-  return streams((int64_t)a->max_q * P.G) ? launch_attn_stream(*a, P, (cudaStream_t)stream)
-                                          : launch_attn_chunk(*a, P, (cudaStream_t)stream);
+  return streams(a->total_q, a->max_q, a->Hq, a->Hkv, a->D, keys_bound(*a))
+             ? launch_attn_stream(*a, P, (cudaStream_t)stream)
+             : launch_attn_chunk(*a, P, (cudaStream_t)stream);
 }
 
 }  // extern "C"

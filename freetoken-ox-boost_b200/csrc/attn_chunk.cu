@@ -66,7 +66,7 @@ struct Plan {
   int* scratch;     // 3 ints per group, where they do not fit the plan block's shared memory
   int max_pieces, max_parts, max_joins, max_groups;
 };
-enum { kPlanPieces = 0, kPlanJoins = 1, kPlanInts = 64 };
+enum { kPlanPieces = 0, kPlanJoins = 1, kPlanNext = 2, kPlanInts = 64 };
 constexpr int kClasses = 4;
 constexpr int kPlanThreads = 1024;
 constexpr int kPartsPerSm = 8;
@@ -306,6 +306,7 @@ __global__ void __launch_bounds__(kPlanThreads)
     for (int i = 0; i < kClasses; ++i) n += run[i] * P.Hkv;
     plan.head[kPlanPieces] = n;
     plan.head[kPlanJoins] = n_joins;
+    plan.head[kPlanNext] = blocks;
   }
 }
 
@@ -449,6 +450,7 @@ __device__ __forceinline__ float max3v(float a, float b, float c) {
 
 // ---- the kernel --------------------------------------------------------------------------------
 
+constexpr int kPieceRing = 4, kPieceReaders = 8 + 2;  // softmax warps, MMA, fixer
 constexpr int chunk_stages(int DP) { return DP == 128 ? 5 : 8; }
 template <int DP>
 struct ChunkSmem {
@@ -460,6 +462,8 @@ struct ChunkSmem {
   uint64_t land[kStages];  // a V tile that the fixer completes has landed
   uint64_t q_full[2], q_empty[2];
   uint64_t s_full[2], p_ready[2][2], o_full[2];  // p_ready: by halves of the keys
+  Piece piece[kPieceRing];
+  uint64_t piece_full[kPieceRing], piece_empty[kPieceRing];
   uint64_t drain;
   uint32_t tmem;
   int abort;
@@ -486,12 +490,8 @@ struct ChunkSync {
   }
 };
 
-// Block x takes pieces x, 2B - 1 - x, 2B + x, ... (B blocks): the list is sorted by size, and
-// turning around each time evens out the sums.
-__device__ __forceinline__ int piece_at(int round) {
-  const int B = gridDim.x;
-  return round * B + ((round & 1) ? B - 1 - (int)blockIdx.x : (int)blockIdx.x);
-}
+// Blocks take pieces from the list as they come free: block x starts with piece x, the next ones
+// go by a counter. The copying warp fetches them and passes them on through a ring.
 __device__ __forceinline__ Piece load_piece(const Piece* p) {
   Piece r;
   const int4* s = reinterpret_cast<const int4*>(p);
@@ -499,6 +499,20 @@ __device__ __forceinline__ Piece load_piece(const Piece* p) {
   d[0] = __ldcg(s), d[1] = __ldcg(s + 1), d[2] = __ldcg(s + 2);
   return r;
 }
+template <int DP>
+struct PieceReader {
+  int at = 0;
+  uint32_t parity = 0;
+  // the next piece; false at the end of the list or after a timeout
+  __device__ bool next(const ChunkSync<DP>& sy, Piece& p) {
+    if (!sy.wait_warp(&sy.sh->piece_full[at], parity)) return false;
+    p = sy.sh->piece[at];
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(&sy.sh->piece_empty[at]);
+    if (++at == kPieceRing) at = 0, parity ^= 1u;
+    return p.seq >= 0;
+  }
+};
 // Rows and key tiles of tile X of a piece: its first and last token, tiles [t0, t0 + n).
 struct RowTile {
   int tok0, toks, n;
@@ -520,8 +534,8 @@ __device__ __forceinline__ RowTile row_tile(const AttnParams& P, const Piece& p,
 }
 
 template <int DP>
-__device__ void chunk_load(const AttnParams& P, const AttnMaps& M, const Plan& plan, int n_pieces,
-                           int tok1, ChunkSmem<DP>* sh) {
+__device__ void chunk_load(const AttnParams& P, const AttnMaps& M, const Plan& plan, int tok1,
+                           ChunkSmem<DP>* sh) {
   constexpr int kStages = ChunkSmem<DP>::kStages, kH = DP / 64;
   const int lane = threadIdx.x & 31;
   const ChunkSync<DP> sy{sh, P.status};
@@ -535,10 +549,21 @@ __device__ void chunk_load(const AttnParams& P, const AttnMaps& M, const Plan& p
   // for the exit after a timeout: stages whose last copy signals land[], a bit each
   uint32_t on_land = 0, land_par = 0;  // parity of a stage's next phase on land[]
   bool ok = true, first_round = true;
-  for (int round = 0; ok; ++round) {
-    const int at = piece_at(round);
-    if (at >= n_pieces) break;
-    const Piece p = load_piece(plan.pieces + at);
+  // (the first piece is loaded before the length of the list is known: there is one at least)
+  Piece p = load_piece(plan.pieces + blockIdx.x);
+  const int n_pieces = __ldcg(plan.head + kPlanPieces);
+  if ((int)blockIdx.x >= n_pieces) p.seq = -1;
+  int slot = 0;
+  uint32_t slot_parity = 1;
+  for (;;) {
+    ok = sy.wait_warp(&sh->piece_empty[slot], slot_parity);
+    if (!ok) break;
+    if (lane == 0) {
+      sh->piece[slot] = p;
+      mbar_arrive(&sh->piece_full[slot]);
+    }
+    if (++slot == kPieceRing) slot = 0, slot_parity ^= 1u;
+    if (p.seq < 0) break;
     const RowTile ra = row_tile(P, p, 0, tok1), rb = row_tile(P, p, 1, tok1);
     const int n = max(ra.n, rb.n);
     const int32_t* table = P.block_table + (int64_t)p.seq * P.table_stride;
@@ -592,6 +617,15 @@ __device__ void chunk_load(const AttnParams& P, const AttnMaps& M, const Plan& p
         }
       }
     }
+    if (!ok) break;
+    // (taken only now: a block that took its next piece early could hold it while others idle)
+    int next = 0;
+    if (lane == 0) next = atomicAdd(plan.head + kPlanNext, 1);
+    next = __shfl_sync(0xffffffffu, next, 0);
+    if (next < n_pieces)
+      p = load_piece(plan.pieces + next);
+    else
+      p.seq = -1;
   }
   if (!ok) {  // a wait gave up: stay until the copies in flight have landed (again bounded)
     for (int i = 0; i < kStages; ++i) {
@@ -610,17 +644,14 @@ __device__ void chunk_load(const AttnParams& P, const AttnMaps& M, const Plan& p
 
 // Clears the rows of V tiles that no token of the piece's item sees.
 template <int DP>
-__device__ void chunk_fix(const AttnParams& P, const Plan& plan, int n_pieces, int tok1,
-                          ChunkSmem<DP>* sh) {
+__device__ void chunk_fix(const AttnParams& P, int tok1, ChunkSmem<DP>* sh) {
   constexpr int kStages = ChunkSmem<DP>::kStages, kH = DP / 64;
   const int lane = threadIdx.x & 31;
   const ChunkSync<DP> sy{sh, P.status};
   int stage = 0;
   uint32_t land_par = 0;  // a bit per stage
-  for (int round = 0;; ++round) {
-    const int at = piece_at(round);
-    if (at >= n_pieces) return;
-    const Piece p = load_piece(plan.pieces + at);
+  PieceReader<DP> pieces;
+  for (Piece p; pieces.next(sy, p);) {
     const RowTile ra = row_tile(P, p, 0, tok1), rb = row_tile(P, p, 1, tok1);
     const int n = max(ra.n, rb.n);
     for (int j = 0; j < n; ++j) {
@@ -647,8 +678,7 @@ __device__ void chunk_fix(const AttnParams& P, const Plan& plan, int n_pieces, i
 }
 
 template <typename T, int DP>
-__device__ void chunk_mma(const AttnParams& P, const Plan& plan, int n_pieces, int tok1,
-                          ChunkSmem<DP>* sh) {
+__device__ void chunk_mma(const AttnParams& P, int tok1, ChunkSmem<DP>* sh) {
   constexpr int kStages = ChunkSmem<DP>::kStages;
   constexpr int kTileBytes = ChunkSmem<DP>::kTileBytes;
   const ChunkSync<DP> sy{sh, P.status};
@@ -690,10 +720,8 @@ __device__ void chunk_mma(const AttnParams& P, const Plan& plan, int n_pieces, i
     pend[x] = false;
   };
 
-  for (int round = 0; ok; ++round) {
-    const int at = piece_at(round);
-    if (at >= n_pieces) break;
-    const Piece p = load_piece(plan.pieces + at);
+  PieceReader<DP> pieces;
+  for (Piece p; ok && pieces.next(sy, p);) {
     const int nx[2] = {row_tile(P, p, 0, tok1).n, row_tile(P, p, 1, tok1).n};
     const int n = max(nx[0], nx[1]);
     for (int j = 0; j < n && ok; ++j) {
@@ -748,8 +776,7 @@ __device__ __forceinline__ void st_sector(void* p, const uint32_t (&w)[8]) {
 }
 
 template <typename T, int DP>
-__device__ void chunk_softmax(const AttnParams& P, const Plan& plan, int n_pieces, int tok1, int x,
-                              ChunkSmem<DP>* sh) {
+__device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP>* sh) {
   const ChunkSync<DP> sy{sh, P.status};
   const int row = threadIdx.x & 127, lane = threadIdx.x & 31;
   const uint32_t lanes = (uint32_t)(row & ~31) << 16;
@@ -762,10 +789,8 @@ __device__ void chunk_softmax(const AttnParams& P, const Plan& plan, int n_piece
   const bool sectors = P.D % 16 == 0 && (reinterpret_cast<uintptr_t>(P.out) & 31) == 0;
   uint32_t s_par = 0, o_par = 0;
   constexpr int kSlot = 2 * kTileM * (DP + 2);
-  for (int round = 0;; ++round) {
-    const int at = piece_at(round);
-    if (at >= n_pieces) return;
-    const Piece p = load_piece(plan.pieces + at);
+  PieceReader<DP> pieces;
+  for (Piece p; pieces.next(sy, p);) {
     const RowTile rt = row_tile(P, p, x, tok1);
     if (rt.toks == 0) continue;
     const bool live = tok < rt.toks;
@@ -975,6 +1000,10 @@ __global__ void __launch_bounds__(kThreadsC, 1)
       mbar_init(&sh->p_ready[x][1], 4);
       mbar_init(&sh->o_full[x], 1);
     }
+    for (int i = 0; i < kPieceRing; ++i) {
+      mbar_init(&sh->piece_full[i], 1);
+      mbar_init(&sh->piece_empty[i], kPieceReaders);
+    }
     mbar_init(&sh->drain, 1);
     sh->abort = 0;
     fence_mbar_init();
@@ -992,18 +1021,17 @@ __global__ void __launch_bounds__(kThreadsC, 1)
   __syncthreads();
   tc_after();
   pdl_wait();
-  const int n_pieces = __ldcg(plan.head + kPlanPieces);
   if (warp < kWarpMma) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-    chunk_softmax<T, DP>(P, plan, n_pieces, tok1, warp >> 2, sh);
+    chunk_softmax<T, DP>(P, tok1, warp >> 2, sh);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
     if (warp == kWarpMma)
-      chunk_mma<T, DP>(P, plan, n_pieces, tok1, sh);
+      chunk_mma<T, DP>(P, tok1, sh);
     else if (warp == kWarpLoad)
-      chunk_load<DP>(P, M, plan, n_pieces, tok1, sh);
+      chunk_load<DP>(P, M, plan, tok1, sh);
     else if (warp == kWarpFix)
-      chunk_fix<DP>(P, plan, n_pieces, tok1, sh);
+      chunk_fix<DP>(P, tok1, sh);
   }
   tc_before();
   __syncthreads();
