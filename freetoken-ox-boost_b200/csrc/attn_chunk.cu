@@ -451,16 +451,18 @@ __device__ __forceinline__ float max3v(float a, float b, float c) {
 // ---- the kernel --------------------------------------------------------------------------------
 
 constexpr int kPieceRing = 4, kPieceReaders = 8 + 2;  // softmax warps, MMA, fixer
-constexpr int chunk_stages(int DP) { return DP == 128 ? 5 : 8; }
+// Three Q buffers for the two tiles: the next item's A comes in while this one is still in use.
+constexpr int kQBufs = 3;
+constexpr int chunk_stages(int DP) { return DP == 128 ? 4 : 8; }
 template <int DP>
 struct ChunkSmem {
   static constexpr int kStages = chunk_stages(DP);
   static constexpr int kTileBytes = kTileK * DP * 2;
-  alignas(1024) uint8_t q[2][kTileBytes];          // [half][row][64]
+  alignas(1024) uint8_t q[kQBufs][kTileBytes];      // [half][row][64]
   alignas(1024) uint8_t ring[kStages][kTileBytes];  // [half][key][64]
   uint64_t full[kStages], empty[kStages];
   uint64_t land[kStages];  // a V tile that the fixer completes has landed
-  uint64_t q_full[2], q_empty[2];
+  uint64_t q_full[kQBufs], q_empty[kQBufs];
   uint64_t s_full[2], p_ready[2][2], o_full[2];  // p_ready: by halves of the keys
   Piece piece[kPieceRing];
   uint64_t piece_full[kPieceRing], piece_empty[kPieceRing];
@@ -545,7 +547,8 @@ __device__ void chunk_load(const AttnParams& P, const AttnMaps& M, const Plan& p
   const uint32_t box_bytes = (uint32_t)r * 128 * kH;
   const uint32_t q_bytes = (uint32_t)(tok1 * P.G) * 128 * kH;
   int stage = 0;
-  uint32_t parity = 1, q_par[2] = {1, 1};
+  int qb = 0;  // next Q buffer
+  uint32_t parity = 1, q_par = 1;
   // for the exit after a timeout: stages whose last copy signals land[], a bit each
   uint32_t on_land = 0, land_par = 0;  // parity of a stage's next phase on land[]
   bool ok = true, first_round = true;
@@ -567,7 +570,22 @@ __device__ void chunk_load(const AttnParams& P, const AttnMaps& M, const Plan& p
     const RowTile ra = row_tile(P, p, 0, tok1), rb = row_tile(P, p, 1, tok1);
     const int n = max(ra.n, rb.n);
     const int32_t* table = P.block_table + (int64_t)p.seq * P.table_stride;
-    for (int j = 0; j < 2 * n && ok; ++j) {  // K0 V0 K1 V1 ...
+    auto load_q = [&](const RowTile& rt) {
+      if (!sy.wait_warp(&sh->q_empty[qb], q_par)) return false;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&sh->q_full[qb], q_bytes);
+#pragma unroll
+        for (int h = 0; h < kH; ++h)
+          tma_4d(smem_u32(sh->q[qb]) + h * kTileM * 128, &M.q, h * 64, 0, p.head,
+                 p.q_tok + rt.tok0, &sh->q_full[qb]);
+      }
+      __syncwarp();
+      if (++qb == kQBufs) qb = 0, q_par ^= 1u;
+      return true;
+    };
+    // Q of A, K0, Q of B (whose buffer comes free last), V0, K1, V1, ...
+    if (ra.n > 0) ok = load_q(ra);
+    for (int j = 0; j < 2 * n && ok; ++j) {
       const bool v = j & 1;
       const int key0 = (p.t0 + (j >> 1)) * kTileK;
       const int b0 = p.lo > key0 ? (p.lo - key0) / r : 0;
@@ -598,24 +616,7 @@ __device__ void chunk_load(const AttnParams& P, const AttnMaps& M, const Plan& p
           tma_5d(dst + h * kTileK * 128, v ? &M.v : &M.k, h * 64, row, p.head, id, 0, bar);
       }
       if (++stage == kStages) stage = 0, parity ^= 1u, first_round = false;
-      if (j == 0) {  // Q after the first K: its buffers come free last
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const RowTile& rt = x ? rb : ra;
-          if (rt.n == 0 || !ok) continue;
-          ok = sy.wait_warp(&sh->q_empty[x], q_par[x]);
-          if (!ok) break;
-          q_par[x] ^= 1u;
-          if (lane == 0) {
-            mbar_arrive_expect_tx(&sh->q_full[x], q_bytes);
-#pragma unroll
-            for (int h = 0; h < kH; ++h)
-              tma_4d(smem_u32(sh->q[x]) + h * kTileM * 128, &M.q, h * 64, 0, p.head,
-                     p.q_tok + rt.tok0, &sh->q_full[x]);
-          }
-          __syncwarp();
-        }
-      }
+      if (j == 0 && rb.n > 0) ok = load_q(rb);
     }
     if (!ok) break;
     // (taken only now: a block that took its next piece early could hold it while others idle)
@@ -636,9 +637,9 @@ __device__ void chunk_load(const AttnParams& P, const AttnMaps& M, const Plan& p
       for (uint32_t k = 0; k < kSpinLimit; ++k)
         if (mbar_try_wait(land ? &sh->land[i] : &sh->full[i], par)) break;
     }
-    for (int x = 0; x < 2; ++x)
-      for (uint32_t k = 0; k < kSpinLimit; ++k)  // (before its first copy: passes at once)
-        if (mbar_try_wait(&sh->q_full[x], q_par[x])) break;
+    for (int i = 0; i < kQBufs; ++i)  // (before a buffer's first copy: passes at once)
+      for (uint32_t k = 0; k < kSpinLimit; ++k)
+        if (mbar_try_wait(&sh->q_full[i], i < qb ? q_par ^ 1u : q_par)) break;
   }
 }
 
@@ -688,7 +689,8 @@ __device__ void chunk_mma(const AttnParams& P, int tok1, ChunkSmem<DP>* sh) {
   const uint32_t vd = desc_low(smem_u32(sh->ring[0]), kTileK * 128);
   constexpr uint32_t kIdS = idesc<T>(kTileK, false), kIdO = idesc<T>(DP, true);
   int stage = 0;
-  uint32_t parity = 0, q_par[2] = {0, 0}, p_par[2] = {0, 0};
+  int qb = 0, q_of[2] = {0, 0};  // next Q buffer; the tiles' buffers
+  uint32_t parity = 0, q_par = 0, p_par[2] = {0, 0};
   // tile x's P V of the last step: not issued yet; whether it adds to O, ends its row tile
   bool pend[2] = {false, false}, acc[2] = {false, false}, last[2] = {false, false};
   int v_stage = -1;
@@ -734,12 +736,13 @@ __device__ void chunk_mma(const AttnParams& P, int tok1, ChunkSmem<DP>* sh) {
         if (!ok) break;
         if (j >= nx[x]) continue;
         if (j == 0) {
-          ok = sy.wait_warp(&sh->q_full[x], q_par[x]);
+          ok = sy.wait_warp(&sh->q_full[qb], q_par);
           if (!ok) break;
-          q_par[x] ^= 1u;
+          q_of[x] = qb;
+          if (++qb == kQBufs) qb = 0, q_par ^= 1u;
         }
         tc_after();
-        const uint32_t a = qd + (uint32_t)((x * kTileBytes) >> 4);
+        const uint32_t a = qd + (uint32_t)((q_of[x] * kTileBytes) >> 4);
         const uint32_t b = kd + (uint32_t)((stage * kTileBytes) >> 4);
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k) {
@@ -747,7 +750,6 @@ __device__ void chunk_mma(const AttnParams& P, int tok1, ChunkSmem<DP>* sh) {
           mma_ss(tb + kTmemS + x * 128, a + o, b + o, kIdS, k > 0 ? 1u : 0u);
         }
         mma_commit1(&sh->s_full[x]);
-        if (j == nx[x] - 1) mma_commit1(&sh->q_empty[x]);
         pend[x] = true, acc[x] = j > 0, last[x] = j == nx[x] - 1;
       }
       if (!ok) break;
@@ -786,12 +788,18 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
   // becomes one that is small enough to be flat and keeps a masked -inf at -inf.
   const bool flip = P.scale_log2 < 0.f;
   const float sc = fmaxf(fabsf(P.scale_log2), 1e-30f);
-  const bool sectors = P.D % 16 == 0 && (reinterpret_cast<uintptr_t>(P.out) & 31) == 0;
+  int q_next = 0;
   uint32_t s_par = 0, o_par = 0;
   constexpr int kSlot = 2 * kTileM * (DP + 2);
   PieceReader<DP> pieces;
   for (Piece p; pieces.next(sy, p);) {
     const RowTile rt = row_tile(P, p, x, tok1);
+    // Q buffers are taken in order: A's, B's, the next item's A's, ...
+    const int n_other = row_tile(P, p, x ^ 1, tok1).n;
+    int q_mine = q_next;
+    if (rt.n > 0 && x == 1 && n_other > 0) q_mine = q_mine + 1 == kQBufs ? 0 : q_mine + 1;
+    q_next += (rt.n > 0) + (n_other > 0);
+    if (q_next >= kQBufs) q_next -= kQBufs;
     if (rt.toks == 0) continue;
     const bool live = tok < rt.toks;
     // keys this row sees: [kmin, kmax); the tile's rows all see [tile_min, tile_max)
@@ -837,13 +845,13 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
         }
       };
       auto highest = [&] {
-        float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
+        float m0 = -INFINITY, m1 = m0, m2 = m0, m3 = m0;
 #pragma unroll
-        for (int c = 4; c < kTileK; c += 4) {
-          m0 = fmaxf(m0, s[c]), m1 = fmaxf(m1, s[c + 1]);
-          m2 = fmaxf(m2, s[c + 2]), m3 = fmaxf(m3, s[c + 3]);
+        for (int c = 0; c < kTileK; c += 8) {
+          m0 = max3v(m0, s[c], s[c + 1]), m1 = max3v(m1, s[c + 2], s[c + 3]);
+          m2 = max3v(m2, s[c + 4], s[c + 5]), m3 = max3v(m3, s[c + 6], s[c + 7]);
         }
-        return fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+        return fmaxf(max3v(m0, m1, m2), m3);
       };
       load();
       // The maximum is rarely news after the first tile. It is taken beside the exponentials with
@@ -851,10 +859,15 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
       // masked ones take it beforehand.
       bool known = j > 0 && !masked;
       if (!known) {
-        if (masked) {
-          const int a = kmin - key0, b = kmax - key0;
+        if (masked) {  // a bit per key: one test and one select per score
 #pragma unroll
-          for (int c = 0; c < kTileK; ++c) s[c] = c >= a && c < b ? s[c] : -INFINITY;
+          for (int c0 = 0; c0 < kTileK; c0 += 32) {
+            const int a = kmin - key0 - c0, b = kmax - key0 - c0;
+            const uint32_t below = a <= 0 ? 0u : a >= 32 ? ~0u : (1u << a) - 1u;
+            const uint32_t seen = b <= 0 ? 0u : (b >= 32 ? ~0u : (1u << b) - 1u) & ~below;
+#pragma unroll
+            for (int c = 0; c < 32; ++c) s[c0 + c] = seen & (1u << c) ? s[c0 + c] : -INFINITY;
+          }
         }
         move_to(highest());
       }
@@ -874,7 +887,8 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
         l0 = l1 = 0;
         auto scaled = [&](int i, float& m) {
           unpair(fma2v(pair(s[2 * i], s[2 * i + 1]), sc2, off2), s[2 * i], s[2 * i + 1]);
-          m = max3v(m, s[2 * i], s[2 * i + 1]);
+          // (two pairs behind: a warp issues in order, and would wait for the product)
+          if (i >= 2) m = max3v(m, s[2 * i - 4], s[2 * i - 3]);
         };
         auto done = [&](int d) {
           pk[d % (kPairs / 2)] = pack2v<T>(s[2 * d], s[2 * d + 1]);
@@ -890,13 +904,17 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
           if (lane == 0) mbar_arrive(&sh->p_ready[x][half]);
         };
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) scaled(i, m0);
+        for (int i = 0; i < kAhead; ++i) scaled(i, i & 1 ? m1 : m0);
 #pragma unroll
         for (int i = 0; i < kPairs / 2; ++i) {
           s[2 * i] = ex2v(s[2 * i]);
           if (kAhead + 2 * i < kPairs) scaled(kAhead + 2 * i, m0);
           s[2 * i + 1] = ex2v(s[2 * i + 1]);
           if (kAhead + 2 * i + 1 < kPairs) scaled(kAhead + 2 * i + 1, m1);
+          if (kAhead + 2 * i == kPairs) {  // the last two pairs, before they are exponentials
+            m0 = max3v(m0, s[kTileK - 4], s[kTileK - 3]);
+            m1 = max3v(m1, s[kTileK - 2], s[kTileK - 1]);
+          }
           if (i >= kAhead) done(i - kAhead);
         }
         if (known && __any_sync(0xffffffffu, fmaxf(m0, m1) > kLazy)) {
@@ -944,34 +962,49 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
         }
       }
     } else {
+      // Through the tile's Q buffer (its last S is done), each warp its own rows, so that the
+      // stores are whole lines: a lane's row would take a line per 32 bytes. 16-byte units are
+      // placed at unit ^ (row % 8), which spreads both the columns and the rows over the banks.
+      constexpr int kUnits = DP / 8;  // 16-byte units of a row
       const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-      for (int c = 0; c < DP; c += 32) {
-        float o[32];
-        if (rt.n > 0) {
+      uint8_t* stage = sh->q[q_mine] + (row & ~31) * DP * 2;
+      if (rt.n > 0) {
+#pragma unroll 1
+        for (int c = 0; c < DP; c += 32) {
+          float o[32];
           tm_ld32(to + c, o);
           tm_ld_wait();
-        }
-        if (live) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 16) {  // a sector at a time where rows are whole sectors
-            uint32_t w[8];
+          for (int i = 0; i < 32; i += 8) {
+            uint32_t w[4];
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              w[k] = l == 0.f ? 0u : pack2<T>(o[i + 2 * k] * inv, o[i + 2 * k + 1] * inv);
-            uint16_t* op = P.out + out_row * P.D + c + i;
-            if (sectors) {
-              if (c + i < P.D) st_sector(op, w);
-            } else {
-              if (c + i < P.D) *reinterpret_cast<uint4*>(op) = make_uint4(w[0], w[1], w[2], w[3]);
-              if (c + i + 8 < P.D)
-                *reinterpret_cast<uint4*>(op + 8) = make_uint4(w[4], w[5], w[6], w[7]);
-            }
+            for (int k = 0; k < 4; ++k)
+              w[k] = pack2<T>(o[i + 2 * k] * inv, o[i + 2 * k + 1] * inv);
+            // (a row without keys has O = 0, or never had one: both are 0 by its l)
+            *reinterpret_cast<uint4*>(stage + lane * DP * 2 + (((c + i) / 8 ^ (lane & 7)) << 4)) =
+                l == 0.f ? make_uint4(0, 0, 0, 0) : make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
+        __syncwarp();
+      }
+      constexpr int kRowsAt = 32 / kUnits;  // rows per store of the warp
+      const int unit = lane % kUnits;
+#pragma unroll 1
+      for (int r = lane / kUnits; r < 32; r += kRowsAt) {
+        const int64_t dst = __shfl_sync(0xffffffffu, out_row, r);
+        const bool is = __shfl_sync(0xffffffffu, live, r);
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (rt.n > 0) v = *reinterpret_cast<const uint4*>(stage + r * DP * 2 + ((unit ^ (r & 7)) << 4));
+        if (is && unit * 8 < P.D) *reinterpret_cast<uint4*>(P.out + dst * P.D + unit * 8) = v;
       }
       if (live && P.lse)
         P.lse[out_row] =
             l == 0.f ? -INFINITY : (ref * sc + log2f(l)) * 0.69314718055994531f;
+    }
+    if (rt.n > 0) {  // the Q buffer goes back to the copies
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->q_empty[q_mine]);
     }
     tc_before();  // O has been read before the next item's P is announced
   }
@@ -992,9 +1025,11 @@ __global__ void __launch_bounds__(kThreadsC, 1)
       mbar_init(&sh->empty[i], 1);
       mbar_init(&sh->land[i], 1);
     }
+    for (int i = 0; i < kQBufs; ++i) {
+      mbar_init(&sh->q_full[i], 1);
+      mbar_init(&sh->q_empty[i], 4);  // the tile's softmax warps
+    }
     for (int x = 0; x < 2; ++x) {
-      mbar_init(&sh->q_full[x], 1);
-      mbar_init(&sh->q_empty[x], 1);
       mbar_init(&sh->s_full[x], 1);
       mbar_init(&sh->p_ready[x][0], 4);
       mbar_init(&sh->p_ready[x][1], 4);
