@@ -938,7 +938,6 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
       l += la + lb;
     }
     // output of the row tile
-    const int64_t out_row = (int64_t)(p.q_tok + rt.tok0 + tok) * P.Hq + p.head * P.G + g;
     if (rt.n > 0) {
       if (!sy.wait_warp(&sh->o_full[x], o_par)) return;
       o_par ^= 1u;
@@ -950,13 +949,14 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
         part[kTileM * DP + row] = ref == -INFINITY ? -INFINITY : ref * sc;
         part[kTileM * DP + kTileM + row] = l;
       }
-      for (int c = 0; c < DP && rt.n > 0; c += 32) {
-        float o[32];
-        tm_ld32(to + c, o);
+#pragma unroll 1
+      for (int c = 0; c < DP && rt.n > 0; c += 16) {
+        float o[16];
+        tm_ld16(to + c, o);
         tm_ld_wait();
         if (live) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 4)
+          for (int i = 0; i < 16; i += 4)
             *reinterpret_cast<float4*>(part + ((c + i) / 4 * kTileM + row) * 4) =
                 make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
         }
@@ -968,37 +968,38 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
       constexpr int kUnits = DP / 8;  // 16-byte units of a row
       const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
       uint8_t* stage = sh->q[q_mine] + (row & ~31) * DP * 2;
+      // (short loops: code that runs once per item is fetched as it runs)
       if (rt.n > 0) {
 #pragma unroll 1
-        for (int c = 0; c < DP; c += 32) {
-          float o[32];
-          tm_ld32(to + c, o);
+        for (int c = 0; c < DP; c += 16) {
+          float o[16];
+          tm_ld16(to + c, o);
           tm_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 32; i += 8) {
+          for (int i = 0; i < 16; i += 8) {
             uint32_t w[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              w[k] = pack2<T>(o[i + 2 * k] * inv, o[i + 2 * k + 1] * inv);
-            // (a row without keys has O = 0, or never had one: both are 0 by its l)
+            for (int k = 0; k < 4; ++k) w[k] = pack2<T>(o[i + 2 * k] * inv, o[i + 2 * k + 1] * inv);
+            // (inv is 0 for a row without keys, whose O is 0 too)
             *reinterpret_cast<uint4*>(stage + lane * DP * 2 + (((c + i) / 8 ^ (lane & 7)) << 4)) =
-                l == 0.f ? make_uint4(0, 0, 0, 0) : make_uint4(w[0], w[1], w[2], w[3]);
+                make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
         __syncwarp();
       }
       constexpr int kRowsAt = 32 / kUnits;  // rows per store of the warp
       const int unit = lane % kUnits;
-#pragma unroll 1
+      uint16_t* out0 = P.out + ((int64_t)(p.q_tok + rt.tok0) * P.Hq + p.head * P.G) * P.D + unit * 8;
+      const int to_row = live ? tok * P.Hq + g : -1;
+#pragma unroll 2
       for (int r = lane / kUnits; r < 32; r += kRowsAt) {
-        const int64_t dst = __shfl_sync(0xffffffffu, out_row, r);
-        const bool is = __shfl_sync(0xffffffffu, live, r);
+        const int dst = __shfl_sync(0xffffffffu, to_row, r);
         uint4 v = make_uint4(0, 0, 0, 0);
         if (rt.n > 0) v = *reinterpret_cast<const uint4*>(stage + r * DP * 2 + ((unit ^ (r & 7)) << 4));
-        if (is && unit * 8 < P.D) *reinterpret_cast<uint4*>(P.out + dst * P.D + unit * 8) = v;
+        if (dst >= 0 && unit * 8 < P.D) *reinterpret_cast<uint4*>(out0 + (int64_t)dst * P.D) = v;
       }
       if (live && P.lse)
-        P.lse[out_row] =
+        P.lse[(int64_t)(p.q_tok + rt.tok0 + tok) * P.Hq + p.head * P.G + g] =
             l == 0.f ? -INFINITY : (ref * sc + log2f(l)) * 0.69314718055994531f;
     }
     if (rt.n > 0) {  // the Q buffer goes back to the copies
