@@ -40,7 +40,7 @@ constexpr float kLazy = 8.f;             // log2 of what a score may exceed the 
 
 // ---- plan --------------------------------------------------------------------------------------
 
-struct Piece {
+struct alignas(16) Piece {
   int q_tok;    // row of q of the first token
   int n_tok;    // tokens
   int seq, head;
@@ -53,17 +53,24 @@ struct Piece {
 };
 static_assert(sizeof(Piece) == 48, "three 16-byte loads");
 
-struct Join {
+struct alignas(16) Join {
   int q_tok, n_tok, head, slot, parts;
   int pad[3];
 };
 static_assert(sizeof(Join) == 32, "two 16-byte loads");
 
+// A sequence's tokens of two row tiles, as the plan keeps it.
+struct PlanGroup {
+  int seq, q_tok, n_tok, pos, len, lo, hi;  // as in Piece
+  int t0, tiles;
+  int place, part0;  // among its size class, and of its first part
+};
+
 struct Plan {
   int* head;        // kPlan* counts
   Piece* pieces;
   Join* joins;
-  int* scratch;     // 3 ints per group, where they do not fit the plan block's shared memory
+  int* scratch;     // a PlanGroup per group, where they do not fit the plan block's shared memory
   int max_pieces, max_parts, max_joins, max_groups;
 };
 enum { kPlanPieces = 0, kPlanJoins = 1, kPlanNext = 2, kPlanInts = 64 };
@@ -90,7 +97,7 @@ Plan carve_plan(char* base, int64_t groups, int Hkv, size_t* bytes) {
   p.head = reinterpret_cast<int*>(take(kPlanInts * 4));
   p.pieces = reinterpret_cast<Piece*>(take((size_t)p.max_pieces * sizeof(Piece)));
   p.joins = reinterpret_cast<Join*>(take((size_t)p.max_joins * sizeof(Join)));
-  p.scratch = reinterpret_cast<int*>(take((size_t)groups * 12));
+  p.scratch = reinterpret_cast<int*>(take((size_t)groups * sizeof(PlanGroup)));
   *bytes = off;
   return p;
 }
@@ -176,20 +183,10 @@ __global__ void __launch_bounds__(kPlanThreads)
   groups = min(groups, plan.max_groups);
   if (tid == 0) first_group[P.batch] = groups;
   __syncthreads();
-  // per group: sequence, place among its size class, number of its first part
-  int* seq_of = dyn + P.batch + 1;
-  if ((size_t)(P.batch + 1 + 3 * groups) * 4 > kPlanSmem) seq_of = plan.scratch;
-  int* pos = seq_of + groups;
-  int* part0 = pos + groups;
-  auto key_tiles = [&](const AttnSeq& s, int i0, KeyRange& r) {
-    const int i1 = min(i0 + tok, s.n);
-    r = attn_range(P, s, i0, i1 - 1);
-    int2 t = make_int2(0, 0);
-    if (r.lo < r.hi) t = make_int2(r.lo / kTileK, (r.hi + kTileK - 1) / kTileK);
-    return t;
-  };
-  unsigned long long mine = 0;
-  int big = 0;
+  PlanGroup* group = reinterpret_cast<PlanGroup*>(dyn + P.batch + 1);
+  if ((size_t)(P.batch + 1) * 4 + (size_t)groups * sizeof(PlanGroup) > (size_t)kPlanSmem)
+    group = reinterpret_cast<PlanGroup*>(plan.scratch);
+  int tiles_mine = 0, big = 0;
   for (int g = tid; g < groups; g += kPlanThreads) {
     int a = 0, z = P.batch;  // the sequence with first_group[a] <= g < first_group[a + 1]
     while (z - a > 1) {
@@ -199,15 +196,21 @@ __global__ void __launch_bounds__(kPlanThreads)
       else
         z = mid;
     }
-    seq_of[g] = a;
-    KeyRange r;
-    const int2 t = key_tiles(attn_seq(P, a), (g - first_group[a]) * tok, r);
-    pos[g] = t.y - t.x;  // for now
-    mine += t.y - t.x;
-    big = max(big, t.y - t.x);
+    const AttnSeq s = attn_seq(P, a);
+    const int i0 = (g - first_group[a]) * tok, n = min(tok, s.n - i0);
+    const KeyRange r = attn_range(P, s, i0, i0 + n - 1);
+    const bool any = r.lo < r.hi;
+    const int t0 = any ? r.lo / kTileK : 0, t1 = any ? (r.hi + kTileK - 1) / kTileK : 0;
+    group[g] = PlanGroup{a, s.q0 + i0, n, s.len - s.n + i0, s.len, r.lo, r.hi, t0, t1 - t0, 0, 0};
+    tiles_mine += t1 - t0;
+    big = max(big, t1 - t0);
   }
-  if (mine) atomicAdd(&sum_tiles, mine);
-  if (big) atomicMax(&biggest, big);
+  tiles_mine = __reduce_add_sync(0xffffffffu, tiles_mine);
+  big = __reduce_max_sync(0xffffffffu, big);
+  if (lane == 0 && big > 0) {
+    atomicAdd(&sum_tiles, (unsigned long long)tiles_mine);
+    atomicMax(&biggest, big);
+  }
   __syncthreads();
   // The longest piece: the longest item cut into 1, 2, ... parts (lane by lane), whichever ends
   // first by an estimate: rounds of pieces of the mean size, kPieceTiles for the start and end of
@@ -218,7 +221,7 @@ __global__ void __launch_bounds__(kPlanThreads)
   const int most = max((top + ways - 1) / ways, kFewest);
   int n_mine = 0;
   for (int g = warp; g < groups; g += kPlanThreads / 32)
-    n_mine += cut_group(pos[g], most).parts;
+    n_mine += cut_group(group[g].tiles, most).parts;
   if (n_mine) atomicAdd(&parts_of[lane], n_mine);
   __syncthreads();
   if (warp == 0) {
@@ -247,7 +250,7 @@ __global__ void __launch_bounds__(kPlanThreads)
     int v[kClasses + 1] = {}, total[kClasses + 1];
     int k = 0, parts = 0;
     if (g < groups) {
-      const Cut c = cut_group(pos[g], limit);
+      const Cut c = cut_group(group[g].tiles, limit);
       k = min(kClasses - 1, (limit - c.size) * kClasses / limit);
       parts = c.parts;
 #pragma unroll
@@ -260,8 +263,8 @@ __global__ void __launch_bounds__(kPlanThreads)
 #pragma unroll
       for (int i = 0; i < kClasses; ++i)
         if (i == k) at = run[i] + v[i] - parts;
-      pos[g] = at;
-      part0[g] = run[kClasses] + v[kClasses] - (parts > 1 ? parts : 0);
+      group[g].place = at;
+      group[g].part0 = run[kClasses] + v[kClasses] - (parts > 1 ? parts : 0);
     }
 #pragma unroll
     for (int i = 0; i <= kClasses; ++i) run[i] += total[i];
@@ -270,11 +273,8 @@ __global__ void __launch_bounds__(kPlanThreads)
   // emission: a warp per group, a lane per piece; in a class one kv head after another, so that
   // blocks that run at the same time share keys
   for (int g = warp; g < groups; g += kPlanThreads / 32) {
-    const int seq = seq_of[g], i0 = (g - first_group[seq]) * tok;
-    const AttnSeq s = attn_seq(P, seq);
-    KeyRange r;
-    const int2 t = key_tiles(s, i0, r);
-    const Cut c = cut_group(t.y - t.x, limit);
+    const PlanGroup u = group[g];
+    const Cut c = cut_group(u.tiles, limit);
     const int k = min(kClasses - 1, (limit - c.size) * kClasses / limit);
     int start = 0, per_head = 0;
 #pragma unroll
@@ -282,16 +282,14 @@ __global__ void __launch_bounds__(kPlanThreads)
       if (i < k) start += run[i] * P.Hkv;
       if (i == k) per_head = run[i];
     }
-    Piece p;
-    p.q_tok = s.q0 + i0, p.n_tok = min(tok, s.n - i0), p.seq = seq;
-    p.pos = s.len - s.n + i0, p.len = s.len, p.lo = r.lo, p.hi = r.hi, p.pad = 0;
     for (int i = lane; i < c.parts * P.Hkv; i += 32) {
-      const int head = i / c.parts, part = i - head * c.parts;
-      p.head = head;
-      p.t0 = t.x + part * c.size;
-      p.t1 = min(p.t0 + c.size, t.y);
-      p.slot = c.parts > 1 ? part0[g] * P.Hkv + i : -1;
-      plan.pieces[start + head * per_head + pos[g] + part] = p;
+      const int head = i / c.parts, part = i - head * c.parts, t0 = u.t0 + part * c.size;
+      Piece p{u.q_tok, u.n_tok, u.seq, head, u.pos, u.len, u.lo, u.hi, t0,
+              min(t0 + c.size, u.t0 + u.tiles), c.parts > 1 ? u.part0 * P.Hkv + i : -1, 0};
+      int4* to = reinterpret_cast<int4*>(plan.pieces + start + head * per_head + u.place + part);
+      to[0] = make_int4(p.q_tok, p.n_tok, p.seq, p.head);
+      to[1] = make_int4(p.pos, p.len, p.lo, p.hi);
+      to[2] = make_int4(p.t0, p.t1, p.slot, 0);
       if (c.parts > 1 && part == 0) {
         Join o{};
         o.q_tok = p.q_tok, o.n_tok = p.n_tok, o.head = head, o.slot = p.slot, o.parts = c.parts;
@@ -1176,7 +1174,7 @@ int run_chunk(const AttnMaps& M, const AttnParams& P, const Plan& plan, int tok1
   if (err != cudaSuccess) return cuda_status(err);
   const int sms = sm_count();
   // the plan's arrays by sequence and by group, the latter in the workspace where they are too many
-  size_t plan_smem = ((size_t)P.batch + 1 + 3 * (size_t)groups) * sizeof(int);
+  size_t plan_smem = ((size_t)P.batch + 1) * sizeof(int) + (size_t)groups * sizeof(PlanGroup);
   if (plan_smem > (size_t)kPlanSmem) plan_smem = kPlanSmem;
   err = launch_pdl(k_attn_plan, dim3(1), dim3(kPlanThreads), plan_smem, stream, P, plan, 2 * tok1,
                    sms);
