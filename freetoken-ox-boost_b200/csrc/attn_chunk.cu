@@ -75,7 +75,7 @@ struct Plan {
 };
 enum { kPlanPieces = 0, kPlanJoins = 1, kPlanNext = 2, kPlanInts = 64 };
 constexpr int kClasses = 4;
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 512;
 constexpr int kPartsPerSm = 8;
 constexpr int kPlanSmem = 200 * 1024, kMaxBatch = kPlanSmem / 8;
 
@@ -120,7 +120,7 @@ __device__ __forceinline__ void block_scan(int (&v)[N], int (&total)[N], int (*r
   __syncthreads();
   int w[N];
 #pragma unroll
-  for (int k = 0; k < N; ++k) w[k] = red[k][lane];
+  for (int k = 0; k < N; ++k) w[k] = lane < kPlanThreads / 32 ? red[k][lane] : 0;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1)
 #pragma unroll
@@ -225,12 +225,12 @@ __global__ void __launch_bounds__(kPlanThreads)
   if (n_mine) atomicAdd(&parts_of[lane], n_mine);
   __syncthreads();
   if (warp == 0) {
-    const int64_t n = (int64_t)parts_of[lane] * P.Hkv;
-    const int64_t rounds = (n + blocks - 1) / blocks;
-    const float mean = n ? (float)(sum_tiles * P.Hkv) / (float)n : 0.f;
+    const float n = (float)parts_of[lane] * P.Hkv, items = (float)groups * P.Hkv;
+    const float rounds = ceilf(n / (float)blocks);
+    const float mean = n > 0.f ? (float)(sum_tiles * P.Hkv) / n : 0.f;
     float cost = fmaxf((float)most, mean * rounds) + kPieceTiles * rounds;
-    if (n > (int64_t)groups * P.Hkv) cost += kJoinTiles * rounds;
-    if (n - (int64_t)groups * P.Hkv > plan.max_parts / 2) cost = INFINITY;  // parts <= 2 (n - items)
+    if (n > items) cost += kJoinTiles * rounds;
+    if (n - items > (float)(plan.max_parts / 2)) cost = INFINITY;  // parts <= 2 (n - items)
     int best = lane;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
