@@ -69,12 +69,13 @@ __device__ __forceinline__ void store_bits(uint16_t* p, const uint16_t (&v)[VEC]
 }
 
 // Block (cols, heads per sweep), one per token: column threadIdx.x of 2 VEC elements of heads
-// threadIdx.y, + blockDim.y, ... A batch of kBatch heads is loaded before the token's cos and sin
-// (which every head shares) have come through shared memory, so the two latencies overlap.
-constexpr int kBatch = 2;  // 8190 tokens of 32 + 8 + 8 heads of 128: 38.2 us (5.4 TB/s), 48.6 with 4 (registers)
-
+// threadIdx.y, + blockDim.y, ... The first heads are loaded before the token's cos and sin (which
+// every head shares) have come through shared memory, so the two latencies overlap; beyond that,
+// many resident warps hide more than loads ahead, which cost registers (8190 tokens of 32 + 8 + 8
+// heads of 128 with 1 / 2 / 4 heads ahead, us: 38.4 / 38.2 / 48.6, 5.4 TB/s; with random positions
+// 39.4 / 43.1 / 55.4).
 template <typename T, int VEC>
-__global__ void k_rope(const __grid_constant__ RopeParams P) {
+__global__ void __launch_bounds__(256, 8) k_rope(const __grid_constant__ RopeParams P) {
   __shared__ float table[2 * kMaxPairs];  // cos, then sin
   pdl_launch_dependents();
   const int col = threadIdx.x;
@@ -95,20 +96,15 @@ __global__ void k_rope(const __grid_constant__ RopeParams P) {
   const int c0 = col * 2 * VEC;
   const int64_t tok = blockIdx.x;
   const int heads = P.Hq + 2 * P.Hkv;
-  uint16_t a[kBatch][VEC], b[kBatch][VEC];
-  auto load = [&](int h0) {
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const int hh = h0 + i * blockDim.y;
-      if (hh >= heads) continue;
-      const bool is_v = hh >= P.Hq + P.Hkv;
-      if (is_v && !P.v_dst) continue;
-      const uint16_t* src = hh < P.Hq ? P.q + tok * P.q_st + hh * P.q_sh
-                            : is_v    ? P.v + tok * P.v_st + (hh - P.Hq - P.Hkv) * P.v_sh
-                                      : P.k + tok * P.k_st + (hh - P.Hq) * P.k_sh;
-      load_bits<VEC>(src + (is_v ? c0 : e0), a[i]);
-      load_bits<VEC>(src + (is_v ? c0 + VEC : e1), b[i]);
-    }
+  uint16_t a[VEC], b[VEC];
+  auto load = [&](int hh) {
+    const bool is_v = hh >= P.Hq + P.Hkv;
+    if (hh >= heads || (is_v && !P.v_dst)) return;
+    const uint16_t* src = hh < P.Hq ? P.q + tok * P.q_st + hh * P.q_sh
+                          : is_v    ? P.v + tok * P.v_st + (hh - P.Hq - P.Hkv) * P.v_sh
+                                    : P.k + tok * P.k_st + (hh - P.Hq) * P.k_sh;
+    load_bits<VEC>(src + (is_v ? c0 : e0), a);
+    load_bits<VEC>(src + (is_v ? c0 + VEC : e1), b);
   };
   pdl_wait();
   load(threadIdx.y);
@@ -137,44 +133,38 @@ __global__ void k_rope(const __grid_constant__ RopeParams P) {
     cs[j] = turns ? table[col * VEC + j] : 1.f;
     sn[j] = turns ? table[half + col * VEC + j] : 0.f;
   }
-  for (int h0 = threadIdx.y; h0 < heads; h0 += kBatch * blockDim.y) {
-    if (h0 != threadIdx.y) load(h0);
+  for (int hh = threadIdx.y; hh < heads; hh += blockDim.y) {
+    if (hh != threadIdx.y) load(hh);
+    const bool is_q = hh < P.Hq, is_v = hh >= P.Hq + P.Hkv;
+    if (!is_q && (!keep || (is_v && !P.v_dst))) continue;
+    uint16_t* dst =
+        is_q ? P.q_out + (tok * P.Hq + hh) * P.D
+        : is_v ? P.v_dst + page * P.vc_page + slot * P.vc_tok + (hh - P.Hq - P.Hkv) * P.vc_head
+               : P.k_dst + page * P.kc_page + slot * P.kc_tok + (hh - P.Hq) * P.kc_head;
+    if (turns && !is_v) {
+      if (P.adjacent) {
+        uint16_t w[2 * VEC];
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const int hh = h0 + i * blockDim.y;
-      if (hh >= heads) continue;
-      const bool is_q = hh < P.Hq, is_v = hh >= P.Hq + P.Hkv;
-      if (!is_q && (!keep || (is_v && !P.v_dst))) continue;
-      uint16_t* dst =
-          is_q ? P.q_out + (tok * P.Hq + hh) * P.D
-          : is_v
-              ? P.v_dst + page * P.vc_page + slot * P.vc_tok + (hh - P.Hq - P.Hkv) * P.vc_head
-              : P.k_dst + page * P.kc_page + slot * P.kc_tok + (hh - P.Hq) * P.kc_head;
-      if (turns && !is_v) {
-        if (P.adjacent) {
-          uint16_t w[2 * VEC];
+        for (int j = 0; j < VEC; ++j) w[j] = a[j], w[VEC + j] = b[j];
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) w[j] = a[i][j], w[VEC + j] = b[i][j];
+        for (int j = 0; j < VEC; ++j) {
+          const float u = elem_f32<T>(w[2 * j]), v = elem_f32<T>(w[2 * j + 1]);
+          w[2 * j] = elem_bits<T>(u * cs[j] - v * sn[j]);
+          w[2 * j + 1] = elem_bits<T>(v * cs[j] + u * sn[j]);
+        }
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const float u = elem_f32<T>(w[2 * j]), v = elem_f32<T>(w[2 * j + 1]);
-            w[2 * j] = elem_bits<T>(u * cs[j] - v * sn[j]);
-            w[2 * j + 1] = elem_bits<T>(v * cs[j] + u * sn[j]);
-          }
+        for (int j = 0; j < VEC; ++j) a[j] = w[j], b[j] = w[VEC + j];
+      } else {
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) a[i][j] = w[j], b[i][j] = w[VEC + j];
-        } else {
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const float u = elem_f32<T>(a[i][j]), v = elem_f32<T>(b[i][j]);
-            a[i][j] = elem_bits<T>(u * cs[j] - v * sn[j]);
-            b[i][j] = elem_bits<T>(v * cs[j] + u * sn[j]);
-          }
+        for (int j = 0; j < VEC; ++j) {
+          const float u = elem_f32<T>(a[j]), v = elem_f32<T>(b[j]);
+          a[j] = elem_bits<T>(u * cs[j] - v * sn[j]);
+          b[j] = elem_bits<T>(v * cs[j] + u * sn[j]);
         }
       }
-      store_bits<VEC>(dst + (is_v ? c0 : e0), a[i]);
-      store_bits<VEC>(dst + (is_v ? c0 + VEC : e1), b[i]);
     }
+    store_bits<VEC>(dst + (is_v ? c0 : e0), a);
+    store_bits<VEC>(dst + (is_v ? c0 + VEC : e1), b);
   }
 }
 
