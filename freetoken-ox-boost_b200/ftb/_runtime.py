@@ -39,26 +39,17 @@ def require(t: torch.Tensor, name: str, dtype=None, shape=None, contiguous=True)
         raise ValueError(f"{name} must be contiguous")
 
 
-def signature(*tensors) -> tuple:
-    """What the argument checks of a call look at: shape, strides, dtype and device of each tensor
-    (or the None in its place)."""
-    return tuple([None if t is None else (t.shape, t.stride(), t.dtype, t.device)
-                  for t in tensors])
-
-
+# Argument blocks of calls, all but their pointers, as they were when a call of that key was first
+# checked: the checks cost more than the launch. A key holds what the checks look at: shape,
+# strides, dtype and device of each tensor (or the None in its place) and the options.
 _ARGS: dict = {}
 
 
-def checked_args(key: tuple, make):
-    """A copy of the argument block that ``make()`` built, all but its pointers, when a call of this
-    ``key`` (its signature and options) was first checked. The checks cost more than the launch."""
-    a = _ARGS.get(key)
-    if a is None:
-        a = make()
-        if len(_ARGS) >= 4096:
-            _ARGS.clear()
-        _ARGS[key] = a
-    return type(a).from_buffer_copy(a)
+def remember(key: tuple, args):
+    if len(_ARGS) >= 4096:
+        _ARGS.clear()
+    _ARGS[key] = args
+    return args
 
 
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor:

@@ -6,7 +6,7 @@ import ctypes
 import torch
 
 from . import _lib
-from ._runtime import (checked_args, read_status, require_cuda, signature, stream_handle,
+from ._runtime import (_ARGS, read_status, remember, require_cuda, stream_handle,
                        zeroed_workspace)
 from .block import _TYPE, _new
 
@@ -72,10 +72,15 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     Returns out [total, q heads, D], with ``return_lse`` also the natural log of the sum of the
     exponentials, float32 [total, q heads]. ``check_status`` reads the device status word
     (synchronises) and raises on page ids, lengths or starts outside the tensors."""
-    a = checked_args(
-        ("attention", signature(q, k_cache, v_cache, block_table, kv_len, cu_q), max_q, scale,
-         causal, window),
-        lambda: _args(q, k_cache, v_cache, block_table, kv_len, cu_q, max_q, scale, causal, window))
+    key = (q.shape, q.stride(), q.dtype, q.device, k_cache.shape, k_cache.stride(), k_cache.dtype,
+           k_cache.device, v_cache.shape, v_cache.stride(), v_cache.dtype, v_cache.device,
+           block_table.shape, block_table.stride(), block_table.dtype, block_table.device,
+           kv_len.shape, kv_len.stride(), kv_len.dtype, kv_len.device,
+           None if cu_q is None else (cu_q.shape, cu_q.stride(), cu_q.dtype, cu_q.device), max_q,
+           scale, causal, window)
+    a = _ARGS.get(key) or remember(key, _args(q, k_cache, v_cache, block_table, kv_len, cu_q, max_q,
+                                              scale, causal, window))
+    a = _lib.AttnArgsStruct.from_buffer_copy(a)
     dev = q.device
     if out is None:
         out = _new(q, q.dtype)

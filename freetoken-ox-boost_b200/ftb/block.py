@@ -14,7 +14,7 @@ import ctypes
 import torch
 
 from . import _lib
-from ._runtime import checked_args, require, require_cuda, signature, stream_handle
+from ._runtime import _ARGS, remember, require, require_cuda, stream_handle
 
 _TYPE = {torch.bfloat16: _lib.FTB_TYPE_BF16, torch.float16: _lib.FTB_TYPE_F16}
 _GATE_ACTS = {None: _lib.FTB_GATE_LINEAR, "sigmoid": _lib.FTB_GATE_SIGMOID}
@@ -84,7 +84,12 @@ def _norm_args(x, y, gate, post, pre, scale, eps, gate_act, dtype):
     return a
 
 
+def _kind(t):
+    return t.shape, t.stride(), t.dtype, t.device
+
+
 def _launch_norm(a, x, y, gate, post, pre, r, h):
+    a = _lib.NormArgsStruct.from_buffer_copy(a)
     a.x = x.data_ptr()
     if y is not None:
         a.y, a.r = y.data_ptr(), r.data_ptr()
@@ -125,9 +130,12 @@ def block_norm(x: torch.Tensor, y: torch.Tensor, *, post_weight: torch.Tensor | 
 
     ``gate``: [H], [..., 1] or [..., H], through a sigmoid with ``gate_act="sigmoid"``.
     ``residual_out`` may be ``x`` and ``out`` may be ``y``."""
-    a = checked_args(
-        ("norm", signature(x, y, gate, post_weight, pre_weight), scale, eps, gate_act),
-        lambda: _norm_args(x, y, gate, post_weight, pre_weight, scale, eps, gate_act, y.dtype))
+    key = (x.shape, x.stride(), x.dtype, x.device, y.shape, y.stride(), y.dtype, y.device,
+           None if gate is None else (gate.shape, gate.stride(), gate.dtype, gate.device),
+           None if post_weight is None else _kind(post_weight),
+           None if pre_weight is None else _kind(pre_weight), scale, eps, gate_act)
+    a = _ARGS.get(key) or remember(key, _norm_args(x, y, gate, post_weight, pre_weight, scale, eps,
+                                                   gate_act, y.dtype))
     r = _new(x, x.dtype) if residual_out is None else _given(residual_out, "residual_out", x, x.dtype)
     h = None
     if pre_weight is not None:
@@ -141,9 +149,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     """``x * rsqrt(mean(x^2) + eps) * weight`` over the last dimension, in ``out_dtype`` (``x``'s
     own, or bfloat16 for a float32 ``x``)."""
     dtype = out_dtype or (torch.bfloat16 if x.dtype == torch.float32 else x.dtype)
-    a = checked_args(
-        ("rms", signature(x, weight), eps, dtype),
-        lambda: _norm_args(x, None, None, None, weight, 1.0, eps, None, dtype))
+    key = ("rms", x.shape, x.stride(), x.dtype, x.device, _kind(weight), eps, dtype)
+    a = _ARGS.get(key) or remember(key, _norm_args(x, None, None, None, weight, 1.0, eps, None, dtype))
     h = _new(x, dtype)
     _launch_norm(a, x, None, None, None, weight, None, h)
     return h
@@ -233,9 +240,16 @@ def _rope_args(q, k, v, positions, table, k_dst, v_dst, slots, sections, order, 
 def _rope(q, k, v, positions, table, k_dst, v_dst, slots, sections, order, pairs, q_out):
     if sections is not None:
         sections = tuple(sections)
-    a = checked_args(
-        ("rope", signature(q, k, v, positions, table, k_dst, v_dst, slots), sections, order, pairs),
-        lambda: _rope_args(q, k, v, positions, table, k_dst, v_dst, slots, sections, order, pairs))
+    key = (q.shape, q.stride(), q.dtype, q.device, k.shape, k.stride(), k.dtype, k.device,
+           positions.shape, positions.stride(), positions.dtype, positions.device, table.shape,
+           table.stride(), table.dtype, table.device, sections, order, pairs,
+           None if slots is None else (
+               v.shape, v.stride(), v.dtype, v.device, k_dst.shape, k_dst.stride(), k_dst.dtype,
+               k_dst.device, v_dst.shape, v_dst.stride(), v_dst.dtype, v_dst.device, slots.shape,
+               slots.stride(), slots.dtype, slots.device))
+    a = _ARGS.get(key) or remember(key, _rope_args(q, k, v, positions, table, k_dst, v_dst, slots,
+                                                   sections, order, pairs))
+    a = _lib.RopeArgsStruct.from_buffer_copy(a)
     out = _new(q, q.dtype) if q_out is None else _given(q_out, "q_out", q, q.dtype)
     a.q, a.k, a.q_out, a.k_dst = q.data_ptr(), k.data_ptr(), out.data_ptr(), k_dst.data_ptr()
     a.positions, a.table = positions.data_ptr(), table.data_ptr()
