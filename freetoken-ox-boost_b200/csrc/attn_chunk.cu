@@ -822,13 +822,38 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
 #pragma unroll
           for (int c = 0; c < kTileK; ++c) s[c] = -s[c];
         }
+        if (masked) {  // a bit per key: one test and one select per score
+#pragma unroll
+          for (int c0 = 0; c0 < kTileK; c0 += 32) {
+            const int a = kmin - key0 - c0, b = kmax - key0 - c0;
+            const uint32_t below = a <= 0 ? 0u : a >= 32 ? ~0u : (1u << a) - 1u;
+            const uint32_t seen = b <= 0 ? 0u : (b >= 32 ? ~0u : (1u << b) - 1u) & ~below;
+#pragma unroll
+            for (int c = 0; c < 32; ++c) s[c0 + c] = seen & (1u << c) ? s[c0 + c] : -INFINITY;
+          }
+        }
       };
-      // moves the reference of the rows that exceed it, and what was summed with the old one
-      auto move_to = [&](float mx) {
-        const bool move = (mx - ref) * sc > kLazy;  // from -inf always (NaN where both are)
-        if (!__any_sync(0xffffffffu, move)) return;
-        const float f = move ? ex2((ref - mx) * sc) : 1.f;
-        if (move) ref = mx;
+      auto highest = [&] {
+        float m0 = -INFINITY, m1 = m0, m2 = m0, m3 = m0;
+#pragma unroll
+        for (int c = 0; c < kTileK; c += 8) {
+          m0 = max3v(m0, s[c], s[c + 1]), m1 = max3v(m1, s[c + 2], s[c + 3]);
+          m2 = max3v(m2, s[c + 4], s[c + 5]), m3 = max3v(m3, s[c + 6], s[c + 7]);
+        }
+        return fmaxf(max3v(m0, m1, m2), m3);
+      };
+      // A row is off where a score exceeds the reference by more than 2^kLazy, or all fall as far
+      // short with nothing summed yet (`high` in powers of two above the reference).
+      auto is_off = [&](float high) {
+        return high > kLazy || (l == 0.f && high < -kLazy && high != -INFINITY);
+      };
+      // Makes this tile's maximum the reference of the rows that are off, and moves what was summed
+      // with the old one.
+      auto move = [&] {
+        const float mx = highest();
+        const bool off = is_off((mx - ref) * sc);
+        const float f = off && l > 0.f ? ex2((ref - mx) * sc) : 1.f;  // (nothing summed: O is 0)
+        if (off) ref = mx;
         l *= f;
         if (j == 0) return;
         // (P V of the tiles before has finished: S of this one came after it)
@@ -842,33 +867,12 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
           tm_st16(to + c, reinterpret_cast<uint32_t*>(o));
         }
       };
-      auto highest = [&] {
-        float m0 = -INFINITY, m1 = m0, m2 = m0, m3 = m0;
-#pragma unroll
-        for (int c = 0; c < kTileK; c += 8) {
-          m0 = max3v(m0, s[c], s[c + 1]), m1 = max3v(m1, s[c + 2], s[c + 3]);
-          m2 = max3v(m2, s[c + 4], s[c + 5]), m3 = max3v(m3, s[c + 6], s[c + 7]);
-        }
-        return fmaxf(max3v(m0, m1, m2), m3);
-      };
-      load();
-      // The maximum is rarely news after the first tile. It is taken beside the exponentials with
-      // the reference so far, and looked at before any of P is announced; only the first tile and
-      // masked ones take it beforehand.
-      bool known = j > 0 && !masked;
-      if (!known) {
-        if (masked) {  // a bit per key: one test and one select per score
-#pragma unroll
-          for (int c0 = 0; c0 < kTileK; c0 += 32) {
-            const int a = kmin - key0 - c0, b = kmax - key0 - c0;
-            const uint32_t below = a <= 0 ? 0u : a >= 32 ? ~0u : (1u << a) - 1u;
-            const uint32_t seen = b <= 0 ? 0u : (b >= 32 ? ~0u : (1u << b) - 1u) & ~below;
-#pragma unroll
-            for (int c = 0; c < 32; ++c) s[c0 + c] = seen & (1u << c) ? s[c0 + c] : -INFINITY;
-          }
-        }
-        move_to(highest());
-      }
+      // The reference starts at 0, where normalised queries and keys leave it, and the maximum is
+      // rarely news after the first tile. So it is taken beside the exponentials with the
+      // reference so far, and looked at before any of P is announced; where a row of the warp is
+      // off, the tile is begun again.
+      if (j == 0) ref = 0.f;
+      bool moved = false;
       // The instructions of other pairs are laid between the two exponentials of a pair, which keep
       // the special-function unit busy for 16 cycles: the products of pairs to come (all of them,
       // and so the maximum, within the first half), rounding and summing of one kAhead before. In
@@ -878,7 +882,9 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
       constexpr int kPairs = kTileK / 2, kAhead = 4;
       uint64_t l0, l1;
       for (;;) {
-        const float off = ref == -INFINITY ? 0.f : -ref * sc;
+        load();
+        if (moved) move();
+        const float off = -ref * sc;
         const uint64_t sc2 = pair(sc, sc), off2 = pair(off, off);
         uint32_t pk[kPairs / 2];
         float m0 = -INFINITY, m1 = -INFINITY;
@@ -915,10 +921,8 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
           }
           if (i >= kAhead) done(i - kAhead);
         }
-        if (known && __any_sync(0xffffffffu, fmaxf(m0, m1) > kLazy)) {
-          known = false;  // rare: from the scores again, with the new maximum
-          load();
-          move_to(highest());
+        if (!moved && __any_sync(0xffffffffu, is_off(fmaxf(m0, m1)))) {
+          moved = true;
           continue;
         }
 #pragma unroll
