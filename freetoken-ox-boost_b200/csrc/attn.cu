@@ -76,7 +76,7 @@ size_t ftb_attention_workspace_bytes(int64_t total_q, int batch, int max_q, int 
   if (total_q < 0 || batch < 0 || max_q < 0 || Hkv < 1 || Hq < Hkv || D < 8) return 0;
   const int G = Hq / Hkv;
   if (G > 128) return 0;
-  const int64_t rows = (int64_t)max_q * G;
+  const int64_t rows = std::min<int64_t>(max_q, total_q) * G;
   const size_t stream = attn_stream_partial_bytes(rows, D);
   if (rows <= kStreamRows) return FTB_ATTN_ZERO_BYTES + stream;
   // (more rows: either kernel, by the lengths)
@@ -84,8 +84,12 @@ size_t ftb_attention_workspace_bytes(int64_t total_q, int batch, int max_q, int 
          std::max(stream, attn_chunk_workspace_bytes(total_q, batch, Hkv, G, D));
 }
 
-int ftb_attention(const ftb_attn_args* a, ftb_stream_t stream) {
-  if (!a) return FTB_ERR_ARG;
+int ftb_attention(const ftb_attn_args* args, ftb_stream_t stream) {
+  if (!args) return FTB_ERR_ARG;
+  ftb_attn_args call = *args;
+  // (a caller's bound may be its model's; no sequence has more than all rows)
+  if (call.total_q >= 0) call.max_q = (int)std::min<int64_t>(call.max_q, call.total_q);
+  const ftb_attn_args* a = &call;
   if (a->type != FTB_TYPE_BF16 && a->type != FTB_TYPE_F16) return FTB_ERR_ARG;
   if (a->total_q < 0 || a->total_q > 0x7fffffff || a->batch < 0 || a->max_q < 0 || a->Hkv < 1 ||
       a->Hq < 1 || a->Hq % a->Hkv || a->Hq / a->Hkv > 128 || a->D < 8 || a->D > 128 || a->D % 8 ||

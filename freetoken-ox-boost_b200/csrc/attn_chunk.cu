@@ -8,15 +8,29 @@
 //   P = 2^(s - ref), l += sum P     one thread per row, all 128 scores in registers
 //   O += P V    tcgen05.mma M = 128, N = D, P from tensor memory (it takes S's place), V from
 //               shared memory (its rows are keys: the MN-major operand layout)
-// ref is the row's reference maximum. It moves only when a tile's maximum exceeds it by more than
-// 2^8 (the sums are fp32, and a P of up to 2^8 keeps its relative precision in bf16 and f16), so
-// O, in tensor memory, is rescaled rarely.
+// ref is the row's reference. It starts at 0 and moves to a tile's maximum only where that exceeds
+// it by more than 2^8, or falls as far short with nothing summed yet, so O, in tensor memory, is
+// rescaled rarely. The sums are fp32; P within 2^8 of 1 keeps its relative precision in bf16 and,
+// down to weights of 2^-6 of the row's largest at the lower end, in f16 (below that its error is
+// at most 2^-17 of the largest).
 //
 // Bound: the tensor cores, 4 D per visible (row, key), with the exponentials next: a 128 x 128
 // tile costs 1024 cycles of MMA at D = 128 and as many of the special-function unit. Two tiles
-// are in flight so that A's softmax runs beside B's MMAs.
+// are in flight so that A's softmax runs beside B's MMAs; a third would not fit tensor memory
+// (S and O of a tile take 256 of its 512 columns). A pair of tiles takes about 3100 cycles where
+// MMAs and exponentials alone would take 2048 each: with two in flight, a tile's chain (S, its
+// softmax of about 2000 cycles, P V) is not covered entirely.
 //
-// Warps: 0-3 softmax and output of tile A, 4-7 of tile B (one thread per row), 8 issues the MMAs,
+// On one B200, bf16, 32 query heads of 128 over 8: 4093 new tokens at 32771 keys 1.99 ms, 1.03
+// PFLOP/s, 62 % of a large matrix product's rate (at the 1000 W power limit, where the clock is
+// 1.5 to 1.75 GHz); 8 causal prompts of up to 2048 tokens (62 GFLOP) 108 us, most of the rest in
+// half-masked tiles and the SMs' uneven last pieces; 12 ragged chunks of up to 300 tokens, 24
+// heads of 64 over 8, window 1000 (4.1 GFLOP) 38 us, of which plan and joins about 9.
+// A chunk of 2048 tokens at 16384 keys keeps the tensor pipe and the special-function pipe each
+// active 60 % of the time, and reads 85 MB from DRAM (87 % of the loads hit L2).
+//
+// Warps: 0-3 softmax and output of tile A, 4-7 of tile B (one thread per row: no exchange of
+// maxima or sums; two threads per row spilt registers), 8 issues the MMAs of both tiles in turn,
 // 9 the TMA copies, 10 clears V rows that no token of the item may see (their weight is 0, but
 // 0 x NaN is not). K and V tiles share a ring in the order of their use: K0 V0 K1 V1 ...
 //
@@ -32,8 +46,8 @@ constexpr int kTileK = 128;   // keys per tile
 constexpr int kTileM = 128;   // rows per tile
 constexpr int kThreadsC = 384;
 constexpr int kWarpMma = 8, kWarpLoad = 9, kWarpFix = 10;
-// registers: softmax 2 x 128 threads x 208 + 128 x 88 = 64512 = 384 x 168 at launch
-constexpr int kRegsLaunch = 168, kRegsSoftmax = 208, kRegsOther = 88;
+// registers: softmax 2 x 128 threads x 216 + 128 x 72 = 64512 = 384 x 168 at launch
+constexpr int kRegsLaunch = 168, kRegsSoftmax = 216, kRegsOther = 72;
 static_assert(2 * 128 * kRegsSoftmax + 128 * kRegsOther <= kThreadsC * kRegsLaunch, "registers");
 constexpr int kTmemS = 0, kTmemO = 256;  // + 128 for tile B
 constexpr float kLazy = 8.f;             // log2 of what a score may exceed the reference by

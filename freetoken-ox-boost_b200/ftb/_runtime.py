@@ -65,12 +65,24 @@ def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     return t
 
 
+_REPLACED: list = []
+
+
 def zeroed_workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     """A cached buffer like :func:`workspace`, of its own and zero-filled when it is made: for
-    calls whose counters start at zero and are left at zero."""
+    calls whose counters start at zero and are left at zero.
+
+    A buffer that a larger one replaces stays allocated, since a captured graph may hold it (it
+    grows by half at least: the old ones together are no more than twice the new one). One that is
+    made under capture belongs to the graph alone: it is zeroed at each replay, not now."""
     key = (device.index, stream_handle(device), "zeroed")
     t = _WS.get(key)
     if t is None or t.numel() < nbytes:
+        if torch.cuda.is_current_stream_capturing():
+            return torch.zeros(int(nbytes), dtype=torch.uint8, device=device)
+        if t is not None:
+            _REPLACED.append(t)
+            nbytes = max(nbytes, t.numel() * 3 // 2)
         t = torch.zeros(int(nbytes), dtype=torch.uint8, device=device)
         _WS[key] = t
     return t

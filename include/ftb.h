@@ -470,13 +470,16 @@ FTB_API int ftb_rope(const ftb_rope_args* args, ftb_stream_t stream);
  * j > p - window when window > 0. Key j is row j % page of page block_table[b, j / page].
  *   out = sum_j softmax_j(scale q.k_j) v_j,   lse = log sum_j exp(scale q.k_j)   (natural log)
  * A token that sees no key gets out = 0 and lse = -inf. Cache rows at or past kv_len, or below
- * every token's window, are never used, whatever they hold.
+ * every token's window, are never used, whatever they hold. A V row that only some of a sequence's
+ * tokens in the call see must be finite: its weight for the others is 0, and 0 x NaN is NaN (a K
+ * row may hold anything for the tokens that do not see it).
  *   q [total_q, Hq, D] with token and head strides; out [total_q, Hq, D] contiguous; lse
  *   [total_q, Hq] fp32 or NULL; caches [num_pages, page, Hkv, D] by strides {page, row, head}
  *   (any order of page rows and heads). Query head h reads kv head h / (Hq / Hkv).
  *   block_table int32 [batch, table_width] (table_stride apart), kv_len int32 [batch], cu_q int32
  *   [batch + 1].
- *   max_q: no sequence has more new tokens (tokens past it are not computed, status bit 1).
+ *   max_q: no sequence has more new tokens (tokens past it are not computed, status bit 1). Rows
+ *   of q that belong to no sequence (a padded batch) are not computed either.
  * D % 8 == 0, D <= 128; Hq / Hkv <= 128; page a power of two, >= 8; strides multiples of 8
  * elements, pointers 16-byte aligned; type BF16 or F16. Softmax, sums and accumulators are fp32;
  * the probabilities are rounded to `type` as the tensor cores' operand.
@@ -485,7 +488,10 @@ FTB_API int ftb_rope(const ftb_rope_args* args, ftb_stream_t stream);
  * memset), and every call leaves the counters there zero again. Bytes [0, 4) are the
  * status word, sticky until the caller clears it: bit 0 = a page id outside [0, num_pages) or a
  * kv_len outside [0, table_width * page] (read as zero keys, or clamped), bit 1 = more new tokens
- * than max_q, or cu_q outside [0, total_q]; bit 2 = a bounded device-side wait gave up.
+ * than max_q, or cu_q outside [0, total_q]; bit 2 = a bounded device-side wait gave up
+ * (the counters may then hold anything: zero all FTB_ATTN_ZERO_BYTES before the next call).
+ * Its size does not grow with the cache: split parts are bounded by the SM count (158 MB on 148
+ * SMs for calls of many rows, 5 MB for decode, D = 128).
  */
 #define FTB_ATTN_ZERO_BYTES 65536
 typedef struct ftb_attn_args {

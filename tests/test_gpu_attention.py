@@ -223,6 +223,48 @@ def test_another_stream_and_a_graph():
     assert torch.equal(out, again) and not torch.equal(out, want)
 
 
+def attend(c, **kw):
+    return ftb.paged_attention(**{**c.t, **kw})
+
+
+def test_a_graph_without_an_eager_call_and_a_grown_workspace():
+    """The capture makes its own workspace, zeroed at each replay; a workspace that a graph holds
+    stays when a larger call replaces it."""
+    small = AttnCase([(1, 3000), (1, 50)], cu=False)
+    large = AttnCase([(300, 700), (90, 90), (2, 3000)])
+    build(small), build(large)
+    want, want_large = attend(small).clone(), attend(large).clone()
+    for eager_first in (False, True):
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        graph, out = torch.cuda.CUDAGraph(), torch.empty_like(want)
+        with torch.cuda.stream(s):
+            if eager_first:
+                ftb.paged_attention(**small.t, out=out)
+                s.synchronize()
+            with torch.cuda.graph(graph, stream=s):
+                ftb.paged_attention(**small.t, out=out)
+            for _ in range(2):
+                assert torch.equal(ftb.paged_attention(**large.t), want_large)
+                out.zero_()
+                graph.replay()
+                s.synchronize()
+                assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("pairs", [[(5, 70), (0, 9), (3, 3)], [(400, 900), (0, 9), (129, 129)]])
+def test_a_loose_max_q_and_rows_of_no_sequence(pairs):
+    """max_q may be any bound (a model's longest), and rows behind the last sequence stay."""
+    c = AttnCase(pairs)
+    build(c)
+    want = attend(c)
+    assert torch.equal(attend(c, max_q=1 << 20), want)
+    q = torch.cat([c.t["q"], torch.full_like(c.t["q"][:7], math.nan)])
+    out = torch.full_like(q, 3.0)
+    attend(c, q=q, out=out)
+    assert torch.equal(out[:-7], want) and (out[-7:] == 3.0).all()
+
+
 def test_refusals():
     c = AttnCase([(1, 50), (1, 60)], cu=False)
     build(c)
