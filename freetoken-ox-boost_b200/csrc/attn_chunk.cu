@@ -170,12 +170,12 @@ __global__ void __launch_bounds__(kPlanThreads)
                 int blocks) {
   extern __shared__ int dyn[];
   __shared__ int red[kClasses + 1][32];
-  __shared__ unsigned long long sum_tiles;
-  __shared__ int biggest, n_joins, most_best, parts_of[32];
+  __shared__ unsigned long long sum_tiles, cheapest;
+  __shared__ int biggest, n_joins, most_best, tail_best, fine_best, parts_of[32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int* first_group = dyn;  // [batch + 1]
   pdl_launch_dependents();
-  if (tid == 0) sum_tiles = 0, biggest = 0, n_joins = 0;
+  if (tid == 0) sum_tiles = 0, cheapest = ~0ull, biggest = 0, n_joins = 0;
   if (tid < 32) parts_of[tid] = 0;
   pdl_wait();
   int groups = 0;
@@ -226,10 +226,12 @@ __global__ void __launch_bounds__(kPlanThreads)
     atomicMax(&biggest, big);
   }
   __syncthreads();
-  // The longest piece: the longest item cut into 1, 2, ... parts (lane by lane), whichever ends
-  // first by an estimate: rounds of pieces of the mean size, kPieceTiles for the start and end of
-  // a piece, kJoinTiles more for a part that has to be joined.
-  constexpr int kPieceTiles = 2, kJoinTiles = 1, kFewest = 2;
+  // The longest piece: the longest item cut into 1, 2, ... parts (lane by lane). These fill some
+  // whole rounds of the blocks; what is left for the last one may be cut 1..8 times finer (warp by
+  // warp), so that all blocks share it. Whichever ends first by an estimate: pieces of the mean
+  // size (less is lost to whole rounds where sizes differ: the small ones, last, fill the gaps),
+  // kPieceTiles for the start and end of a piece, kJoinTiles more for a part that has to be joined.
+  constexpr int kPieceTiles = 2, kJoinTiles = 3, kFewest = 2, kFiner = 8;
   const int top = max(biggest, 1);
   const int ways = lane < 16 ? lane + 1 : (lane - 13) * (lane - 13) / 2 + 12;  // 1..16, 16.., 174
   const int most = max((top + ways - 1) / ways, kFewest);
@@ -238,57 +240,76 @@ __global__ void __launch_bounds__(kPlanThreads)
     n_mine += cut_group(group[g].tiles, most).parts;
   if (n_mine) atomicAdd(&parts_of[lane], n_mine);
   __syncthreads();
-  if (warp == 0) {
+  if (warp < kFiner) {
     const float n = (float)parts_of[lane] * P.Hkv, items = (float)groups * P.Hkv;
-    const float rounds = ceilf(n / (float)blocks);
-    const float mean = n > 0.f ? (float)(sum_tiles * P.Hkv) / n : 0.f;
-    float cost = fmaxf((float)most, mean * rounds) + kPieceTiles * rounds;
-    if (n > items) cost += kJoinTiles * rounds;
-    if (n - items > (float)(plan.max_parts / 2)) cost = INFINITY;  // parts <= 2 (n - items)
-    int best = lane;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float c = __shfl_xor_sync(0xffffffffu, cost, o);
-      const int b = __shfl_xor_sync(0xffffffffu, best, o);
-      if (c < cost || (c == cost && b < best)) cost = c, best = b;
-    }
-    const int m = __shfl_sync(0xffffffffu, most, best);
-    if (lane == 0) most_best = m;
+    const float k = (float)(warp + 1), per_block = 1.f / (float)blocks;
+    const float tiles = (float)sum_tiles * P.Hkv, mean = n > 0.f ? tiles / n : 0.f;
+    const float rounds = floorf((n + 0.5f) * per_block), left = n - rounds * (float)blocks;
+    const float last = ceilf((left * k - 0.5f) * per_block);  // rounds of the finer pieces
+    const float even = tiles * per_block, gap = mean * (rounds + last / k) - even;
+    const float alike = fmaxf(0.f, 2.f * mean / (float)most - 1.f);  // 1: all of the longest's size
+    const float joined = n > items ? n + left * (k - 1.f) : warp ? left * k : 0.f;
+    float cost = fmaxf((float)most, even + gap * alike) + kPieceTiles * (rounds + last) +
+                 kJoinTiles * joined * per_block;
+    // (parts <= 2 (pieces - items))
+    if ((warp && mean < k * kFewest) ||
+        n - items + left * (k - 1.f) > (float)(plan.max_parts / 2))
+      cost = INFINITY;
+    const unsigned long long key = (unsigned long long)__float_as_uint(cost) << 32 |
+                                   (uint32_t)(warp << 5 | lane);  // (costs are not negative)
+    atomicMin(&cheapest, key);
   }
   __syncthreads();
-  const int limit = min(most_best, top);
+  if (tid == (int)(cheapest & 0xffffffffu)) {
+    most_best = most;
+    const float n = (float)parts_of[lane];
+    const int left = (int)((long long)parts_of[lane] * P.Hkv % blocks);
+    tail_best = warp ? (int)ceilf((float)left * (float)groups / (n * P.Hkv)) : 0;
+    fine_best = (most + warp) / (warp + 1);
+  }
+  __syncthreads();
+  const int limit = min(most_best, top), fine = min(fine_best, limit);
+  int tail = min(tail_best, groups);  // groups 0..tail-1 are cut finer
   // places: largest pieces first, by class
-  int run[kClasses + 1] = {};
-  for (int g0 = 0; g0 < groups; g0 += kPlanThreads) {
-    const int g = g0 + tid;
-    int v[kClasses + 1] = {}, total[kClasses + 1];
-    int k = 0, parts = 0;
-    if (g < groups) {
-      const Cut c = cut_group(group[g].tiles, limit);
-      k = min(kClasses - 1, (limit - c.size) * kClasses / limit);
-      parts = c.parts;
+  int run[kClasses + 1];
+  for (;;) {
 #pragma unroll
-      for (int i = 0; i < kClasses; ++i) v[i] = i == k ? parts : 0;
-      v[kClasses] = parts > 1 ? parts : 0;
+    for (int i = 0; i <= kClasses; ++i) run[i] = 0;
+    for (int g0 = 0; g0 < groups; g0 += kPlanThreads) {
+      const int g = g0 + tid;
+      int v[kClasses + 1] = {}, total[kClasses + 1];
+      int k = 0, parts = 0;
+      if (g < groups) {
+        const Cut c = cut_group(group[g].tiles, g < tail ? fine : limit);
+        k = min(kClasses - 1, (limit - c.size) * kClasses / limit);
+        parts = c.parts;
+#pragma unroll
+        for (int i = 0; i < kClasses; ++i) v[i] = i == k ? parts : 0;
+        v[kClasses] = parts > 1 ? parts : 0;
+      }
+      block_scan<kClasses + 1>(v, total, red);
+      if (g < groups) {
+        int at = 0;
+#pragma unroll
+        for (int i = 0; i < kClasses; ++i)
+          if (i == k) at = run[i] + v[i] - parts;
+        group[g].place = at;
+        group[g].part0 = run[kClasses] + v[kClasses] - (parts > 1 ? parts : 0);
+      }
+#pragma unroll
+      for (int i = 0; i <= kClasses; ++i) run[i] += total[i];
     }
-    block_scan<kClasses + 1>(v, total, red);
-    if (g < groups) {
-      int at = 0;
-#pragma unroll
-      for (int i = 0; i < kClasses; ++i)
-        if (i == k) at = run[i] + v[i] - parts;
-      group[g].place = at;
-      group[g].part0 = run[kClasses] + v[kClasses] - (parts > 1 ? parts : 0);
-    }
-#pragma unroll
-    for (int i = 0; i <= kClasses; ++i) run[i] += total[i];
+    // (the estimate counts pieces of the mean size: where the finer cut makes more parts than there
+    // is room for, it is left out)
+    if (tail == 0 || run[kClasses] * P.Hkv <= plan.max_parts) break;
+    tail = 0;
   }
   __syncthreads();
   // emission: a warp per group, a lane per piece; in a class one kv head after another, so that
   // blocks that run at the same time share keys
   for (int g = warp; g < groups; g += kPlanThreads / 32) {
     const PlanGroup u = group[g];
-    const Cut c = cut_group(u.tiles, limit);
+    const Cut c = cut_group(u.tiles, g < tail ? fine : limit);
     const int k = min(kClasses - 1, (limit - c.size) * kClasses / limit);
     int start = 0, per_head = 0;
 #pragma unroll

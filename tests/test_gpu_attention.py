@@ -223,6 +223,15 @@ def test_another_stream_and_a_graph():
     assert torch.equal(out, again) and not torch.equal(out, want)
 
 
+@pytest.mark.parametrize("c", [
+    AttnCase([(700, 1700)], q_heads=64, kv_heads=1, head=64),  # 175 items, a few more than blocks
+    AttnCase([(700, 1700)], q_heads=64, kv_heads=1, head=64, window=1100),
+    AttnCase([(256, 2300)], q_heads=160, kv_heads=160, head=8),  # more heads than parts' room
+], ids=["left", "left-window", "heads"])
+def test_items_left_over_after_whole_rounds(c):
+    check(c)
+
+
 def attend(c, **kw):
     return ftb.paged_attention(**{**c.t, **kw})
 
