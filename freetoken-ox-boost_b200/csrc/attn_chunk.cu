@@ -21,11 +21,11 @@
 // MMAs and exponentials alone would take 2048 each: with two in flight, a tile's chain (S, its
 // softmax of about 2000 cycles, P V) is not covered entirely.
 //
-// On one B200, bf16, 32 query heads of 128 over 8: 4093 new tokens at 32771 keys 1.99 ms, 1.03
-// PFLOP/s, 62 % of a large matrix product's rate (at the 1000 W power limit, where the clock is
+// On one B200, bf16, 32 query heads of 128 over 8: 4093 new tokens at 32771 keys 1.94 ms, 1.06
+// PFLOP/s, 64 % of a large matrix product's rate (at the 1000 W power limit, where the clock is
 // 1.5 to 1.75 GHz); 8 causal prompts of up to 2048 tokens (62 GFLOP) 108 us, most of the rest in
-// half-masked tiles and the SMs' uneven last pieces; 12 ragged chunks of up to 300 tokens, 24
-// heads of 64 over 8, window 1000 (4.1 GFLOP) 38 us, of which plan and joins about 9.
+// half-masked tiles and the starts and ends of short items; 12 ragged chunks of up to 300 tokens,
+// 24 heads of 64 over 8, window 1000 (4.1 GFLOP) 37 us, of which the plan about 5.
 // A chunk of 2048 tokens at 16384 keys keeps the tensor pipe and the special-function pipe each
 // active 60 % of the time, and reads 85 MB from DRAM (87 % of the loads hit L2).
 //
@@ -230,7 +230,10 @@ __global__ void __launch_bounds__(kPlanThreads)
   // whole rounds of the blocks; what is left for the last one may be cut 1..8 times finer (warp by
   // warp), so that all blocks share it. Whichever ends first by an estimate: pieces of the mean
   // size (less is lost to whole rounds where sizes differ: the small ones, last, fill the gaps),
-  // kPieceTiles for the start and end of a piece, kJoinTiles more for a part that has to be joined.
+  // kPieceTiles for the start and end of a piece, kJoinTiles more for a part that has to be joined
+  // (its 133 KB per row tile are written and read again). Against equal cuts of every item: 2048
+  // tokens at 16384 keys, 256 items, 505 -> 465 us; 700 tokens of 64 heads over one, 175 items, 187
+  // -> 137 us; 512 tokens at 65536 keys, 64 long items, 504 -> 510 us.
   constexpr int kPieceTiles = 2, kJoinTiles = 3, kFewest = 2, kFiner = 8;
   const int top = max(biggest, 1);
   const int ways = lane < 16 ? lane + 1 : (lane - 13) * (lane - 13) / 2 + 12;  // 1..16, 16.., 174

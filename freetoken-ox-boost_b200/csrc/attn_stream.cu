@@ -6,8 +6,8 @@
 //   S = Q K^T (fp32),  m, l = running maximum and sum per row,  O = O 2^(m_old - m) + P V.
 // Bound: DRAM, 2 * D * 2 bytes per key and kv head. On one B200, bf16, 32 heads of 128 over 8: 61
 // tokens at up to 8192 keys (850 MB) 146 us, 5.8 TB/s, 0.89 of the measured copy rate; 3 at up to
-// 131072 keys (754 MB) 128 us, 5.9 TB/s; one at 777 keys 11 us, latency of the chain of loads, join
-// and launch. DRAM traffic is 1.04 of the algorithmic bytes; what is left is mostly the spread
+// 131072 keys (754 MB) 128 us, 5.9 TB/s; one at 777 keys 10.6 us, latency of the chain of
+// loads, join and launch. DRAM traffic is 1.04 of the algorithmic bytes; what is left is mostly the spread
 // between SMs (241K cycles on average, 276K the slowest: equal shares, unequal distances to the
 // memory). Four shares taken in turn per block instead of one cost more in restarts and joins than
 // they evened out (146 -> 157 us, 128 -> 194).
@@ -428,29 +428,61 @@ __device__ void stream_consumer(const AttnParams& P, StreamSmem<DP>* sh, Walk w,
         // part 0 is slot 1 of its block (it began the pair), the others slot 0 of theirs
         const float* p0 = P.partial + (2 * blk0 + 1) * kSlot;
         const float* p1 = P.partial + 2 * (blk0 + 1) * kSlot;
-        if (orow < rows) {
-          float mm = -INFINITY;
-          for (int i = 0; i < parts; ++i) {
+        // Where there are few rows, the threads of the others take their share of the parts: part i
+        // goes to way i % ways of its row (one token at 777 keys 11.2 -> 10.6 us, at 4096 16.0 -> 14.9).
+        const int lg = rows > 1 ? 32 - __clz(rows - 1) : 0, ways = kRows >> lg;
+        const int jrow = orow & ((1 << lg) - 1), way = orow >> lg;
+        const bool mine = jrow < rows;
+        float mm = -INFINITY, ll = 0.f;
+        float4 acc[DP / kMergeCols];
+#pragma unroll
+        for (int c = 0; c < DP / kMergeCols; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+        auto add = [&](float f, const float4& b, int c) {
+          acc[c].x += f * b.x, acc[c].y += f * b.y, acc[c].z += f * b.z, acc[c].w += f * b.w;
+        };
+        if (mine) {
+          for (int i = way; i < parts; i += ways) {
             const float* p = i == 0 ? p0 : p1 + (int64_t)(i - 1) * 2 * kSlot;
-            mm = fmaxf(mm, __ldcg(p + kRows * DP + orow));
+            mm = fmaxf(mm, __ldcg(p + kRows * DP + jrow));
           }
           const float ref = mm == -INFINITY ? 0.f : mm;
-          float ll = 0.f;
-          float4 acc[DP / kMergeCols];
-#pragma unroll
-          for (int c = 0; c < DP / kMergeCols; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int i = 0; i < parts; ++i) {
+          for (int i = way; i < parts; i += ways) {
             const float* p = i == 0 ? p0 : p1 + (int64_t)(i - 1) * 2 * kSlot;
-            const float f = ex2(__ldcg(p + kRows * DP + orow) - ref);
-            ll += f * __ldcg(p + kRows * DP + kRows + orow);
+            const float f = ex2(__ldcg(p + kRows * DP + jrow) - ref);
+            ll += f * __ldcg(p + kRows * DP + kRows + jrow);
 #pragma unroll
-            for (int c = 0; c < DP / kMergeCols; ++c) {
-              const float4 b = __ldcg(reinterpret_cast<const float4*>(p + orow * DP + c * kMergeCols + oc));
-              acc[c].x += f * b.x, acc[c].y += f * b.y, acc[c].z += f * b.z, acc[c].w += f * b.w;
+            for (int c = 0; c < DP / kMergeCols; ++c)
+              add(f, __ldcg(reinterpret_cast<const float4*>(p + jrow * DP + c * kMergeCols + oc)), c);
+          }
+        }
+        if (ways > 1) {
+          static_assert(kConsumers * kMergePitch >= DP, "the ways' sums fit the merge buffer");
+          float* all = &sh->merge[0][0][0];
+#pragma unroll
+          for (int c = 0; c < DP / kMergeCols; ++c)
+            *reinterpret_cast<float4*>(all + orow * DP + c * kMergeCols + oc) = acc[c];
+          if (oc == 0) sh->ml[0][orow][0] = mm, sh->ml[0][orow][1] = ll;
+          named_bar(1, kConsumers * kWarp);
+          if (mine && way == 0) {
+            for (int i = 1; i < ways; ++i) mm = fmaxf(mm, sh->ml[0][jrow + (i << lg)][0]);
+            const float ref = mm == -INFINITY ? 0.f : mm;
+            ll = 0.f;
+#pragma unroll
+            for (int c = 0; c < DP / kMergeCols; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int i = 0; i < ways; ++i) {
+              const int at = jrow + (i << lg);
+              const float f = ex2(sh->ml[0][at][0] - ref);
+              ll += f * sh->ml[0][at][1];
+#pragma unroll
+              for (int c = 0; c < DP / kMergeCols; ++c)
+                add(f, *reinterpret_cast<const float4*>(all + at * DP + c * kMergeCols + oc), c);
             }
           }
+          named_bar(1, kConsumers * kWarp);  // (the next pair writes the merge buffer)
+        }
+        if (mine && way == 0) {
           const float inv = ll > 0.f || ll != ll ? 1.f / ll : 0.f;
-          const int row = row0 + orow;
+          const int row = row0 + jrow;
           const int64_t at = (int64_t)(s.q0 + row / P.G) * P.Hq + w.head * P.G + row % P.G;
 #pragma unroll
           for (int c = 0; c < DP / kMergeCols; ++c) {

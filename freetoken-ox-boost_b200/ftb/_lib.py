@@ -210,6 +210,33 @@ def load(path: str = LIB_PATH):
         return lib
 
 
+_entries: dict = {}
+
+
+def entry(name: str) -> int:
+    """The address of a C entry point."""
+    at = _entries.get(name)
+    if at is None:
+        at = _entries[name] = ctypes.cast(getattr(load(), name), ctypes.c_void_p).value
+    return at
+
+
+def offsets(struct, *names: str) -> tuple:
+    """Where the fields are in an argument struct."""
+    return tuple(getattr(struct, n).offset for n in names)
+
+
+class _NotBuilt:
+    """Stands for the compiled module where it is missing: its first use raises."""
+
+    def __init__(self, why):
+        self.why = why
+
+    def __getattr__(self, name):
+        raise FtbLibraryError(f"ftb/_pycall.so is not built ({self.why}); build it with `make -C "
+                              "freetoken-ox-boost_b200/csrc`")
+
+
 def status_string(status: int) -> str:
     try:
         return load().ftb_status_string(int(status)).decode()

@@ -7,6 +7,11 @@ import torch
 
 from . import _lib
 
+try:
+    from . import _pycall
+except ImportError as _e:
+    _pycall = _lib._NotBuilt(_e)
+
 _WS: dict = {}
 
 
@@ -41,15 +46,17 @@ def require(t: torch.Tensor, name: str, dtype=None, shape=None, contiguous=True)
 
 # Argument blocks of calls, all but their pointers, as they were when a call of that key was first
 # checked: the checks cost more than the launch. A key holds what the checks look at: shape,
-# strides, dtype and device of each tensor (or the None in its place) and the options.
+# strides, dtype and device of each tensor (_pycall.key, or the mark of a None in its place) and
+# the options.
 _ARGS: dict = {}
 
 
-def remember(key: tuple, args):
+def remember(key: tuple, args, *extra):
+    """Keeps (and returns) the argument struct's bytes and what else the call needs to know."""
     if len(_ARGS) >= 4096:
         _ARGS.clear()
-    _ARGS[key] = args
-    return args
+    known = _ARGS[key] = (bytes(args), *extra)
+    return known
 
 
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor:

@@ -1,14 +1,15 @@
 """Attention of new tokens over a paged cache, on libftb (``ftb_attention`` in ``include/ftb.h``)."""
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
-from ._runtime import (_ARGS, read_status, remember, require_cuda, stream_handle,
+from ._runtime import (_ARGS, _pycall, read_status, remember, require_cuda, stream_handle,
                        zeroed_workspace)
-from .block import _TYPE, _new
+from .block import _TYPE
+
+_POINTERS = _lib.offsets(_lib.AttnArgsStruct, "q", "k_cache", "v_cache", "block_table", "kv_len",
+                         "cu_q", "out", "lse", "workspace")
 
 
 def _int32(t, name, shape, dev):
@@ -72,30 +73,20 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     Returns out [total, q heads, D], with ``return_lse`` also the natural log of the sum of the
     exponentials, float32 [total, q heads]. ``check_status`` reads the device status word
     (synchronises) and raises on page ids, lengths or starts outside the tensors."""
-    key = (q.shape, q.stride(), q.dtype, q.device, k_cache.shape, k_cache.stride(), k_cache.dtype,
-           k_cache.device, v_cache.shape, v_cache.stride(), v_cache.dtype, v_cache.device,
-           block_table.shape, block_table.stride(), block_table.dtype, block_table.device,
-           kv_len.shape, kv_len.stride(), kv_len.dtype, kv_len.device,
-           None if cu_q is None else (cu_q.shape, cu_q.stride(), cu_q.dtype, cu_q.device), max_q,
-           scale, causal, window)
-    a = _ARGS.get(key) or remember(key, _args(q, k_cache, v_cache, block_table, kv_len, cu_q, max_q,
-                                              scale, causal, window))
-    a = _lib.AttnArgsStruct.from_buffer_copy(a)
+    key = (_pycall.key(q, k_cache, v_cache, block_table, kv_len, cu_q), max_q, scale, causal, window)
+    known = _ARGS.get(key)
+    if known is None:
+        a = _args(q, k_cache, v_cache, block_table, kv_len, cu_q, max_q, scale, causal, window)
+        known = remember(key, a, a.workspace_bytes)
     dev = q.device
     if out is None:
-        out = _new(q, q.dtype)
+        out = _pycall.empty(q, q)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
         raise ValueError("out must be contiguous, of q's shape and dtype")
     lse = q.new_empty(q.shape[:2], dtype=torch.float32) if return_lse else None
-    ws = zeroed_workspace(a.workspace_bytes, dev)
-    a.q, a.k_cache, a.v_cache = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
-    a.block_table, a.kv_len, a.out = block_table.data_ptr(), kv_len.data_ptr(), out.data_ptr()
-    a.workspace = ws.data_ptr()
-    if cu_q is not None:
-        a.cu_q = cu_q.data_ptr()
-    if lse is not None:
-        a.lse = lse.data_ptr()
-    st = _lib.load().ftb_attention(ctypes.byref(a), stream_handle(dev))
+    ws = zeroed_workspace(known[1], dev)
+    st = _pycall.call(_lib.entry("ftb_attention"), known[0], _POINTERS, stream_handle(dev), q, k_cache,
+                      v_cache, block_table, kv_len, cu_q, out, lse, ws)
     if st:
         _lib.check("ftb_attention", st)
     if check_status:

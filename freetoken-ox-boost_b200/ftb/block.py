@@ -9,17 +9,18 @@ Shapes, types and strides are those of ``ftb_block_norm`` and ``ftb_rope`` in ``
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
-from ._runtime import _ARGS, remember, require, require_cuda, stream_handle
+from ._runtime import _ARGS, _pycall, remember, require, require_cuda, stream_handle
 
 _TYPE = {torch.bfloat16: _lib.FTB_TYPE_BF16, torch.float16: _lib.FTB_TYPE_F16}
 _GATE_ACTS = {None: _lib.FTB_GATE_LINEAR, "sigmoid": _lib.FTB_GATE_SIGMOID}
 _PAIRS = {"half": _lib.FTB_PAIRS_HALF, "adjacent": _lib.FTB_PAIRS_ADJACENT}
 _ORDERS = {"blocks": _lib.FTB_AXES_BLOCKS, "cyclic": _lib.FTB_AXES_CYCLIC}
+_NORM_POINTERS = _lib.offsets(_lib.NormArgsStruct, "x", "y", "gate", "post", "pre", "r", "h")
+_ROPE_POINTERS = _lib.offsets(_lib.RopeArgsStruct, "q", "k", "v", "q_out", "k_dst", "v_dst",
+                              "positions", "table", "slots")
 
 
 def _row_stride(t: torch.Tensor, name: str) -> int:
@@ -32,9 +33,9 @@ def _row_stride(t: torch.Tensor, name: str) -> int:
 
 
 def _new(like: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-    if like.is_contiguous():
-        return torch.empty_like(like) if like.dtype == dtype else torch.empty_like(like, dtype=dtype)
-    return like.new_empty(like.shape, dtype=dtype)
+    if like.dtype == dtype:
+        return _pycall.empty(like, like)
+    return torch.empty(like.shape, dtype=dtype, device=like.device)
 
 
 def _given(t: torch.Tensor, name: str, like: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
@@ -84,22 +85,9 @@ def _norm_args(x, y, gate, post, pre, scale, eps, gate_act, dtype):
     return a
 
 
-def _kind(t):
-    return t.shape, t.stride(), t.dtype, t.device
-
-
-def _launch_norm(a, x, y, gate, post, pre, r, h):
-    a = _lib.NormArgsStruct.from_buffer_copy(a)
-    a.x = x.data_ptr()
-    if y is not None:
-        a.y, a.r = y.data_ptr(), r.data_ptr()
-    if gate is not None:
-        a.gate = gate.data_ptr()
-    if post is not None:
-        a.post = post.data_ptr()
-    if pre is not None:
-        a.pre, a.h = pre.data_ptr(), h.data_ptr()
-    st = _lib.load().ftb_block_norm(ctypes.byref(a), stream_handle(x.device))
+def _launch_norm(args, x, y, gate, post, pre, r, h):
+    st = _pycall.call(_lib.entry("ftb_block_norm"), args, _NORM_POINTERS, stream_handle(x.device), x,
+                      y, gate, post, pre, r, h)
     if st:
         _lib.check("ftb_block_norm", st)
 
@@ -130,17 +118,14 @@ def block_norm(x: torch.Tensor, y: torch.Tensor, *, post_weight: torch.Tensor | 
 
     ``gate``: [H], [..., 1] or [..., H], through a sigmoid with ``gate_act="sigmoid"``.
     ``residual_out`` may be ``x`` and ``out`` may be ``y``."""
-    key = (x.shape, x.stride(), x.dtype, x.device, y.shape, y.stride(), y.dtype, y.device,
-           None if gate is None else (gate.shape, gate.stride(), gate.dtype, gate.device),
-           None if post_weight is None else _kind(post_weight),
-           None if pre_weight is None else _kind(pre_weight), scale, eps, gate_act)
-    a = _ARGS.get(key) or remember(key, _norm_args(x, y, gate, post_weight, pre_weight, scale, eps,
-                                                   gate_act, y.dtype))
-    r = _new(x, x.dtype) if residual_out is None else _given(residual_out, "residual_out", x, x.dtype)
+    key = (_pycall.key(x, y, gate, post_weight, pre_weight), scale, eps, gate_act)
+    known = _ARGS.get(key) or remember(key, _norm_args(x, y, gate, post_weight, pre_weight, scale,
+                                                       eps, gate_act, y.dtype))
+    r = _pycall.empty(x, x) if residual_out is None else _given(residual_out, "residual_out", x, x.dtype)
     h = None
     if pre_weight is not None:
-        h = _new(x, y.dtype) if out is None else _given(out, "out", x, y.dtype)
-    _launch_norm(a, x, y, gate, post_weight, pre_weight, r, h)
+        h = _pycall.empty(x, y) if out is None else _given(out, "out", x, y.dtype)
+    _launch_norm(known[0], x, y, gate, post_weight, pre_weight, None if y is None else r, h)
     return r, h
 
 
@@ -149,10 +134,11 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     """``x * rsqrt(mean(x^2) + eps) * weight`` over the last dimension, in ``out_dtype`` (``x``'s
     own, or bfloat16 for a float32 ``x``)."""
     dtype = out_dtype or (torch.bfloat16 if x.dtype == torch.float32 else x.dtype)
-    key = ("rms", x.shape, x.stride(), x.dtype, x.device, _kind(weight), eps, dtype)
-    a = _ARGS.get(key) or remember(key, _norm_args(x, None, None, None, weight, 1.0, eps, None, dtype))
+    key = (_pycall.key(x, weight), eps, dtype)
+    known = _ARGS.get(key) or remember(key, _norm_args(x, None, None, None, weight, 1.0, eps, None,
+                                                       dtype))
     h = _new(x, dtype)
-    _launch_norm(a, x, None, None, None, weight, None, h)
+    _launch_norm(known[0], x, None, None, None, weight, None, h)
     return h
 
 
@@ -240,23 +226,14 @@ def _rope_args(q, k, v, positions, table, k_dst, v_dst, slots, sections, order, 
 def _rope(q, k, v, positions, table, k_dst, v_dst, slots, sections, order, pairs, q_out):
     if sections is not None:
         sections = tuple(sections)
-    key = (q.shape, q.stride(), q.dtype, q.device, k.shape, k.stride(), k.dtype, k.device,
-           positions.shape, positions.stride(), positions.dtype, positions.device, table.shape,
-           table.stride(), table.dtype, table.device, sections, order, pairs,
-           None if slots is None else (
-               v.shape, v.stride(), v.dtype, v.device, k_dst.shape, k_dst.stride(), k_dst.dtype,
-               k_dst.device, v_dst.shape, v_dst.stride(), v_dst.dtype, v_dst.device, slots.shape,
-               slots.stride(), slots.dtype, slots.device))
-    a = _ARGS.get(key) or remember(key, _rope_args(q, k, v, positions, table, k_dst, v_dst, slots,
-                                                   sections, order, pairs))
-    a = _lib.RopeArgsStruct.from_buffer_copy(a)
-    out = _new(q, q.dtype) if q_out is None else _given(q_out, "q_out", q, q.dtype)
-    a.q, a.k, a.q_out, a.k_dst = q.data_ptr(), k.data_ptr(), out.data_ptr(), k_dst.data_ptr()
-    a.positions, a.table = positions.data_ptr(), table.data_ptr()
-    if slots is not None:
-        a.v, a.v_dst, a.slots = v.data_ptr(), v_dst.data_ptr(), slots.data_ptr()
-    if a.tokens:
-        st = _lib.load().ftb_rope(ctypes.byref(a), stream_handle(q.device))
+    key = (_pycall.key(q, k, positions, table) if slots is None else
+           _pycall.key(q, k, positions, table, v, k_dst, v_dst, slots), sections, order, pairs)
+    known = _ARGS.get(key) or remember(key, _rope_args(q, k, v, positions, table, k_dst, v_dst, slots,
+                                                       sections, order, pairs))
+    out = _pycall.empty(q, q) if q_out is None else _given(q_out, "q_out", q, q.dtype)
+    if q.shape[0]:
+        st = _pycall.call(_lib.entry("ftb_rope"), known[0], _ROPE_POINTERS, stream_handle(q.device),
+                          q, k, v, out, k_dst, v_dst, positions, table, slots)
         if st:
             _lib.check("ftb_rope", st)
     return out
