@@ -5,12 +5,17 @@
 // is read once from DRAM and used by all rows:
 //   S = Q K^T (fp32),  m, l = running maximum and sum per row,  O = O 2^(m_old - m) + P V.
 // Bound: DRAM, 2 * D * 2 bytes per key and kv head. On one B200, bf16, 32 heads of 128 over 8: 61
-// tokens at up to 8192 keys (850 MB) 146 us, 5.8 TB/s, 0.89 of the measured copy rate; 3 at up to
-// 131072 keys (754 MB) 128 us, 5.9 TB/s; one at 777 keys 10.6 us, latency of the chain of
-// loads, join and launch. DRAM traffic is 1.04 of the algorithmic bytes; what is left is mostly the spread
+// tokens at up to 8192 keys (850 MB) 149 us, 5.7 TB/s, 0.87 of the measured copy rate; 3 at up to
+// 131072 keys (754 MB) 128 us, 5.9 TB/s; one at 777 keys 10.8 us, latency of the chain of loads,
+// join and launch. DRAM traffic is 1.04 of the algorithmic bytes; what is left is mostly the spread
 // between SMs (241K cycles on average, 276K the slowest: equal shares, unequal distances to the
 // memory). Four shares taken in turn per block instead of one cost more in restarts and joins than
 // they evened out (146 -> 157 us, 128 -> 194).
+//
+// P is two operands, its rounding to the tensors' type and what that left, each with its own MMAs: the
+// output's error is then its own rounding alone, where P rounded once adds as much again (few
+// outputs, as a single token has, may show more than that on average). It costs little beside the
+// loads: 147 -> 150 us and nothing on the two others above.
 //
 // Split: the work of all (sequence, kv head) pairs, in tiles of 64 keys, is one line cut into
 // gridDim.x equal shares, whatever the lengths; a block finds its share by a scan over the batch
@@ -290,7 +295,7 @@ __device__ void stream_consumer(const AttnParams& P, StreamSmem<DP>* sh, Walk w,
           const bool seen = clean || (key >= kmin[i >> 1] && key < kmax[i >> 1]);
           sc[h][i] = seen ? sc[h][i] * P.scale_log2 : -INFINITY;
         }
-      uint32_t pa[4];
+      uint32_t pa[4], pr[4];  // P rounded to the operand's type, and what the rounding left
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         float mx = fmaxf(fmaxf(sc[0][2 * e], sc[0][2 * e + 1]), fmaxf(sc[1][2 * e], sc[1][2 * e + 1]));
@@ -305,6 +310,9 @@ __device__ void stream_consumer(const AttnParams& P, StreamSmem<DP>* sh, Walk w,
         l[e] = l[e] * f + ((p0 + p1) + (p2 + p3));
         pa[e] = pack2<T>(p0, p1);
         pa[2 + e] = pack2<T>(p2, p3);
+        const float2 a = unpack2<T>(pa[e]), b = unpack2<T>(pa[2 + e]);
+        pr[e] = pack2<T>(p0 - a.x, p1 - a.y);
+        pr[2 + e] = pack2<T>(p2 - b.x, p3 - b.y);
         if (__any_sync(0xffffffffu, f != 1.f)) {
 #pragma unroll
           for (int jj = 0; jj < DP / 8; ++jj) o[jj][2 * e] *= f, o[jj][2 * e + 1] *= f;
@@ -329,6 +337,8 @@ __device__ void stream_consumer(const AttnParams& P, StreamSmem<DP>* sh, Walk w,
         if (!inside) b[0] &= mk[0], b[1] &= mk[1], b[2] &= mk[0], b[3] &= mk[1];
         mma16816<T>(o[2 * c], pa, b[0], b[1]);
         mma16816<T>(o[2 * c + 1], pa, b[2], b[3]);
+        mma16816<T>(o[2 * c], pr, b[0], b[1]);
+        mma16816<T>(o[2 * c + 1], pr, b[2], b[3]);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->empty[stage]);
