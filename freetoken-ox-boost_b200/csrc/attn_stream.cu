@@ -5,17 +5,17 @@
 // is read once from DRAM and used by all rows:
 //   S = Q K^T (fp32),  m, l = running maximum and sum per row,  O = O 2^(m_old - m) + P V.
 // Bound: DRAM, 2 * D * 2 bytes per key and kv head. On one B200, bf16, 32 heads of 128 over 8: 61
-// tokens at up to 8192 keys (850 MB) 149 us, 5.7 TB/s, 0.87 of the measured copy rate; 3 at up to
+// tokens at up to 8192 keys (850 MB) 151 us, 5.6 TB/s, 0.86 of the measured copy rate; 3 at up to
 // 131072 keys (754 MB) 128 us, 5.9 TB/s; one at 777 keys 10.8 us, latency of the chain of loads,
 // join and launch. DRAM traffic is 1.04 of the algorithmic bytes; what is left is mostly the spread
 // between SMs (241K cycles on average, 276K the slowest: equal shares, unequal distances to the
 // memory). Four shares taken in turn per block instead of one cost more in restarts and joins than
-// they evened out (146 -> 157 us, 128 -> 194).
+// they evened out (146 -> 157 us, 128 -> 194, before P was two operands).
 //
 // P is two operands, its rounding to the tensors' type and what that left, each with its own MMAs: the
 // output's error is then its own rounding alone, where P rounded once adds as much again (few
 // outputs, as a single token has, may show more than that on average). It costs little beside the
-// loads: 147 -> 150 us and nothing on the two others above.
+// loads: 147 -> 151 us, 10.6 -> 10.8 and nothing on the longest.
 //
 // Split: the work of all (sequence, kv head) pairs, in tiles of 64 keys, is one line cut into
 // gridDim.x equal shares, whatever the lengths; a block finds its share by a scan over the batch
