@@ -472,7 +472,8 @@ FTB_API int ftb_rope(const ftb_rope_args* args, ftb_stream_t stream);
  * A token that sees no key gets out = 0 and lse = -inf. Cache rows at or past kv_len, or below
  * every token's window, are never used, whatever they hold. A V row that only some of a sequence's
  * tokens in the call see must be finite: its weight for the others is 0, and 0 x NaN is NaN (a K
- * row may hold anything for the tokens that do not see it).
+ * row may hold anything for the tokens that do not see it). Where a token sees a non-finite V, its
+ * output is infinite or NaN.
  *   q [total_q, Hq, D] with token and head strides; out [total_q, Hq, D] contiguous; lse
  *   [total_q, Hq] fp32 or NULL; caches [num_pages, page, Hkv, D] by strides {page, row, head}
  *   (any order of page rows and heads). Query head h reads kv head h / (Hq / Hkv).
