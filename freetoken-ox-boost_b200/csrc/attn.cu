@@ -19,12 +19,12 @@ CUtensorMapDataType attn_dtype(int type) {
 
 // Which kernel: the streaming one for up to 16 query rows per kv head (one mma.sync row tile, bound
 // by DRAM), and for small work, where the tensor-core kernel's plan and join cost more than its
-// rate gives: at most 2 GFLOP by the bound that the host knows (every token against the whole
-// table, or its window). On one B200, us (streaming / tensor cores), 32 heads over 8 of 128: 64 new
-// tokens of a prompt 7.4 / 19.3, 256 18.2 / 21.9, 512 49 / 25; 16 tokens at 2048 keys 14.1 / 20.3, 64
-// 28.9 / 24.9.
+// rate gives: at most 1.1 GFLOP by the bound that the host knows (every token against the whole
+// table, or its window). On one B200, us (streaming / tensor cores), 32 heads over 8 of 128: prompts
+// of 64 tokens 7.6 / 18.0, 256 (1.1 GFLOP) 19.3 / 20.2, 384 37.7 / 22.8, 512 53.7 / 22.5; 16 tokens at
+// 2048 keys (0.5 GFLOP) 17.4 / 20.6, 64 32.0 / 24.3.
 constexpr int kStreamRows = 16;
-constexpr double kStreamFlops = 2e9;
+constexpr double kStreamFlops = 1.1e9;
 bool streams(int64_t total_q, int max_q, int Hq, int Hkv, int D, int64_t keys) {
   return (int64_t)max_q * (Hq / Hkv) <= kStreamRows ||
          4.0 * D * Hq * (double)total_q * (double)keys <= kStreamFlops;
