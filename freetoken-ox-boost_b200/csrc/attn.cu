@@ -21,8 +21,8 @@ CUtensorMapDataType attn_dtype(int type) {
 // by DRAM), and for small work, where the tensor-core kernel's plan and join cost more than its
 // rate gives: at most 1.1 GFLOP by the bound that the host knows (every token against the whole
 // table, or its window). On one B200, us (streaming / tensor cores), 32 heads over 8 of 128: prompts
-// of 64 tokens 7.6 / 18.0, 256 (1.1 GFLOP) 19.3 / 20.2, 384 37.7 / 22.8, 512 53.7 / 22.5; 16 tokens at
-// 2048 keys (0.5 GFLOP) 17.4 / 20.6, 64 32.0 / 24.3.
+// of 64 tokens 7.6 / 18.0, 256 (1.1 GFLOP) 19.3 / 20.2, 300 35.2 / 21.6, 384 37.7 / 22.8, 512 53.7 /
+// 22.5; 16 tokens at 2048 keys (0.5 GFLOP) 17.4 / 20.6, 64 32.0 / 24.3.
 constexpr int kStreamRows = 16;
 constexpr double kStreamFlops = 1.1e9;
 bool streams(int64_t total_q, int max_q, int Hq, int Hkv, int D, int64_t keys) {
