@@ -986,7 +986,9 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
     if (p.slot >= 0) {
       float* part = P.partial + (int64_t)p.slot * kSlot + (int64_t)x * kTileM * (DP + 2);
       if (live) {
-        part[kTileM * DP + row] = ref == -INFINITY ? -INFINITY : ref * sc;
+        // (a row that summed nothing here has no reference: the one it started from, 0, may lie so
+        // far above those of the other parts that the join would weigh them as nothing)
+        part[kTileM * DP + row] = l == 0.f ? -INFINITY : ref * sc;
         part[kTileM * DP + kTileM + row] = l;
       }
 #pragma unroll 1
@@ -1166,7 +1168,7 @@ __global__ void __launch_bounds__(256) k_attn_join(const __grid_constant__ AttnP
       for (int c = 0; c < kCols; ++c) o[c] *= keep;
 #pragma unroll
       for (int k = 0; k < kTogether; ++k) {
-        if (mk[k] == -INFINITY) continue;  // a part without keys of this row left no O
+        if (mk[k] == -INFINITY) continue;  // a part that summed nothing of this row left no O
         const float f = ex2(mk[k] - mx);
         l += f * lk[k];
 #pragma unroll
