@@ -9,10 +9,14 @@
 //   O += P V    tcgen05.mma M = 128, N = D, P from tensor memory (it takes S's place), V from
 //               shared memory (its rows are keys: the MN-major operand layout)
 // ref is the row's reference. It starts at 0 and moves to a tile's maximum only where that exceeds
-// it by more than 2^8, or falls as far short with nothing summed yet, so O, in tensor memory, is
-// rescaled rarely. The sums are fp32; P within 2^8 of 1 keeps its relative precision in bf16 and,
-// down to weights of 2^-6 of the row's largest at the lower end, in f16 (below that its error is
-// at most 2^-17 of the largest).
+// it by more than 2^8, or falls short of it with nothing summed yet (by more than 2^8 in bf16, at
+// all in f16), so O, in tensor memory, is rescaled rarely. The sums are fp32. P is rounded to the
+// tensors' type: in bf16, with fp32's exponents, to 2^-9 of itself wherever ref lies; in f16, where
+// ref is never above the row's maximum, to 2^-12 of itself down to weights of 2^-14 of the largest,
+// and to at most 2^-25 of the largest below that. The rest of the rounding is dropped by choice: as
+// a second operand, which the streaming kernel can afford, it would make half as many MMAs again,
+// and they are the bound here. It adds about as much error as the output's own rounding (1.4 times
+// in all).
 //
 // Bound: the tensor cores, 4 D per visible (row, key), with the exponentials next: a 128 x 128
 // tile costs 1024 cycles of MMA at D = 128 and as many of the special-function unit. Two tiles
@@ -51,6 +55,11 @@ constexpr int kRegsLaunch = 168, kRegsSoftmax = 216, kRegsOther = 72;
 static_assert(2 * 128 * kRegsSoftmax + 128 * kRegsOther <= kThreadsC * kRegsLaunch, "registers");
 constexpr int kTmemS = 0, kTmemO = 256;  // + 128 for tile B
 constexpr float kLazy = 8.f;             // log2 of what a score may exceed the reference by
+// log2 of what a row's maximum may fall short of it. f16 has no exponents to spare: 2^8 above the
+// maximum, weights of 2^-17 of the largest would be rounded away, and many of those can hold much
+// of the sum.
+template <typename T>
+constexpr float kShort = std::is_same<T, __half>::value ? 0.f : kLazy;
 
 // ---- plan --------------------------------------------------------------------------------------
 
@@ -880,10 +889,10 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
         }
         return fmaxf(max3v(m0, m1, m2), m3);
       };
-      // A row is off where a score exceeds the reference by more than 2^kLazy, or all fall as far
-      // short with nothing summed yet (`high` in powers of two above the reference).
+      // A row is off where a score exceeds the reference by more than 2^kLazy, or all fall short of
+      // it by more than 2^kShort with nothing summed yet (`high` in powers of two above it).
       auto is_off = [&](float high) {
-        return high > kLazy || (l == 0.f && high < -kLazy && high != -INFINITY);
+        return high > kLazy || (l == 0.f && high < -kShort<T> && high != -INFINITY);
       };
       // Makes this tile's maximum the reference of the rows that are off, and moves what was summed
       // with the old one.

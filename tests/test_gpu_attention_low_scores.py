@@ -5,11 +5,13 @@ Bounds, beside those of tests/attn_cases.py: the shift is one product of about 2
 scale of 2^-3.5, so each of the up to 128 products of a score may be cut to that sum's last place,
 2^-12: 2^-5 in all, 2^-8.5 after the scale. A weight is off by that on both sides of the division:
 2^-7.5 < 2^-7 of A. lse: 2^-8.5, and the rounding of its own 2^8 many times smaller: 2^-8."""
+import math
+
 import pytest
 import torch
 
 import ftb
-from tests.attn_cases import AttnCase, build, reference
+from tests.attn_cases import U, AttnCase, build, reference
 
 pytestmark = pytest.mark.gpu
 BF, F16 = torch.bfloat16, torch.float16
@@ -65,3 +67,30 @@ def test_low_scores(c, dtype, by):
     """Cut items have parts in which some rows see no key."""
     check(AttnCase(**c, dtype=dtype), by)
 
+
+
+def test_f16_weights_under_a_low_maximum():
+    """One key at a score of -5 and 16383 12.5 below it, which hold 6 % of the sum together: in
+    f16 a weight is good to 2^-25 of the largest where the reference is not above it, so 2^-25
+    times the number of keys over the sum comes to the bounds of tests/attn_cases.py, which are
+    without their 2^-17 here. Scores are one product each, and exact."""
+    heads = torch.cuda.get_device_properties(0).multi_processor_count  # an item per SM, uncut
+    c = AttnCase([(17, 16384)], q_heads=heads, kv_heads=heads, head=8, page=64, dtype=F16,
+                 causal=False, scale=1.0)
+    _, keys = build(c)
+    x = torch.zeros_like(keys[0])
+    x[:, 0, :, 0] = -17.5
+    x[:, 1] = 1.0
+    x[7, 0, :, 0], x[7, 1] = -5.0, -1.0
+    rewrite_keys(c, [x])
+    c.t["v_cache"].fill_(1.0)
+    page = int(c.t["block_table"][0, 0])
+    c.t["v_cache"][page, 7] = -1.0
+    c.t["q"].zero_()
+    c.t["q"][..., 0] = 1.0
+    out, lse = ftb.paged_attention(**c.t, causal=False, scale=1.0, return_lse=True)
+    few = 16383 * math.exp(-12.5)
+    want, u = (few - 1.0) / (few + 1.0), U[F16]
+    bound = u * (abs(want) + 1.0) + 2.0 ** -13 + 2.0 ** -25 * 16384 / (few + 1.0)
+    assert (out.double().cpu() - want).abs().max() <= bound
+    assert (lse.double().cpu() - (-5.0 + math.log1p(few))).abs().max() <= 2.0 ** -14
