@@ -594,7 +594,7 @@ __device__ void chunk_load(const AttnParams& P, const AttnMaps& M, const Plan& p
   int stage = 0;
   int qb = 0;  // next Q buffer
   uint32_t parity = 1, q_par = 1;
-  // for the exit after a timeout: stages whose last copy signals land[], a bit each
+  // for the exit: stages whose last copy signals land[], a bit each
   uint32_t on_land = 0, land_par = 0;  // parity of a stage's next phase on land[]
   bool ok = true, first_round = true;
   // (the first piece is loaded before the length of the list is known: there is one at least)
@@ -673,19 +673,19 @@ __device__ void chunk_load(const AttnParams& P, const AttnMaps& M, const Plan& p
     else
       p.seq = -1;
   }
-  if (!ok) {  // a wait gave up: stay until the copies in flight have landed (again bounded)
-    for (int i = 0; i < kStages; ++i) {
-      // the last use of stage i: this round of the ring before `stage`, the one before after it
-      const bool land = on_land >> i & 1u;
-      const uint32_t par = land ? (land_par >> i & 1u) ^ 1u : i < stage ? parity ^ 1u : parity;
-      if (!land && i >= stage && first_round) continue;  // never used
-      for (uint32_t k = 0; k < kSpinLimit; ++k)
-        if (mbar_try_wait(land ? &sh->land[i] : &sh->full[i], par)) break;
-    }
-    for (int i = 0; i < kQBufs; ++i)  // (before a buffer's first copy: passes at once)
-      for (uint32_t k = 0; k < kSpinLimit; ++k)
-        if (mbar_try_wait(&sh->q_full[i], i < qb ? q_par ^ 1u : q_par)) break;
+  // Stay until the last copies have landed, again with a limit: a warp that gave up leaves without
+  // them.
+  for (int i = 0; i < kStages; ++i) {
+    // the last use of stage i: this round of the ring before `stage`, the one before after it
+    const bool land = on_land >> i & 1u;
+    const uint32_t par = land ? (land_par >> i & 1u) ^ 1u : i < stage ? parity ^ 1u : parity;
+    if (!land && i >= stage && first_round) continue;  // never used
+    for (uint32_t k = 0; k < kSpinLimit; ++k)
+      if (mbar_try_wait(land ? &sh->land[i] : &sh->full[i], par)) break;
   }
+  for (int i = 0; i < kQBufs; ++i)  // (before a buffer's first copy: passes at once)
+    for (uint32_t k = 0; k < kSpinLimit; ++k)
+      if (mbar_try_wait(&sh->q_full[i], i < qb ? q_par ^ 1u : q_par)) break;
 }
 
 // Clears the rows of V tiles that no token of the piece's item sees.

@@ -26,6 +26,10 @@
 // A block is one producer warp and four consumer warps. The producer copies a tile's K and V
 // pages with TMA into a ring (mbarriers, bounded waits); warp w takes keys 16w..16w+15 of each
 // tile with its own m, l and O, and the four are joined in shared memory at the end of a pair.
+//
+// The consumers share barriers without a limit, so a warp whose wait gives up passes them all the
+// same: it takes no more tiles, makes its rows' sums NaN, and walks on through its share's joins
+// and counts. Every block so ends, and the counters return to zero.
 #include "attn.cuh"
 
 namespace ftb {
@@ -213,11 +217,11 @@ __device__ void stream_producer(const AttnParams& P, const AttnMaps& M, StreamSm
     }
     w.next(P, row0, n);
   }
-  if (!ok) {  // a wait gave up: stay until the copies in flight have landed (again bounded)
-    for (uint32_t u = issued > kStages ? issued - kStages : 0; u < issued; ++u)
-      for (uint32_t i = 0; i < kSpinLimit; ++i)
-        if (mbar_try_wait(&sh->full[u % kStages], (u / kStages) & 1u)) break;
-  }
+  // Stay until the last copies have landed, again with a limit: a consumer that gave up leaves
+  // without them.
+  for (uint32_t u = issued > kStages ? issued - kStages : 0; u < issued; ++u)
+    for (uint32_t i = 0; i < kSpinLimit; ++i)
+      if (mbar_try_wait(&sh->full[u % kStages], (u / kStages) & 1u)) break;
 }
 
 template <typename T, int DP>
@@ -238,7 +242,8 @@ __device__ void stream_consumer(const AttnParams& P, StreamSmem<DP>* sh, Walk w,
   const int v_off = (kv / r) * box_bytes + (kv % r) * 128, v_sw = (kv % r) & 7;
   const int kc = mi & 1, vc = mi >> 1;
   int stage = 0;
-  uint32_t parity = 0;
+  uint32_t parity = 0;  // + kGaveUp once a wait did (one register for both)
+  constexpr uint32_t kGaveUp = 2;
   while (w.left > 0) {
     const int n = w.take();
     const AttnSeq s = w.s;
@@ -271,9 +276,12 @@ __device__ void stream_consumer(const AttnParams& P, StreamSmem<DP>* sh, Walk w,
     for (int j = 0; j < DP / 8; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[j][i] = 0.f;
-    for (int j = 0; j < n; ++j) {
+    for (int j = 0; j < n && parity < kGaveUp; ++j) {
       const int key0 = (w.tile + j) * kTile + warp * 16;
-      if (!__all_sync(0xffffffffu, sy.wait(&sh->full[stage], parity))) return;
+      if (!__all_sync(0xffffffffu, sy.wait(&sh->full[stage], parity))) {
+        parity = kGaveUp;
+        break;
+      }
       const uint32_t kb = smem_u32(sh->ring[stage][0]), vb = smem_u32(sh->ring[stage][1]);
       float sc[2][4] = {};
 #pragma unroll
@@ -344,6 +352,7 @@ __device__ void stream_consumer(const AttnParams& P, StreamSmem<DP>* sh, Walk w,
       if (lane == 0) mbar_arrive(&sh->empty[stage]);
       if (++stage == kStages) stage = 0, parity ^= 1u;
     }
+    if (parity >= kGaveUp) l[0] = l[1] = NAN;
     // join the four warps' parts of the rows
 #pragma unroll
     for (int e = 0; e < 2; ++e) {

@@ -92,7 +92,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if check_status:
         status = read_status(ws)
         if status:
-            ws[:_lib.FTB_ATTN_ZERO_BYTES].zero_()  # (a timeout leaves counters behind)
+            ws[:4].zero_()
             raise ValueError(f"paged_attention: device status {status} (1: page id or kv_len "
                              "outside the cache, 2: cu_q outside q or above max_q, 4: timeout)")
     return (out, lse) if return_lse else out

@@ -489,8 +489,8 @@ FTB_API int ftb_rope(const ftb_rope_args* args, ftb_stream_t stream);
  * memset), and every call leaves the counters there zero again. Bytes [0, 4) are the
  * status word, sticky until the caller clears it: bit 0 = a page id outside [0, num_pages) or a
  * kv_len outside [0, table_width * page] (read as zero keys, or clamped), bit 1 = more new tokens
- * than max_q, or cu_q outside [0, total_q]; bit 2 = a bounded device-side wait gave up
- * (the counters may then hold anything: zero all FTB_ATTN_ZERO_BYTES before the next call).
+ * than max_q, or cu_q outside [0, total_q]; bit 2 = a bounded device-side wait gave up (out and lse
+ * are then not valid; the counters are zero again all the same).
  * Its size does not grow with the cache: split parts are bounded by the SM count (158 MB on 148
  * SMs for calls of many rows, 5 MB for decode, D = 128).
  */
