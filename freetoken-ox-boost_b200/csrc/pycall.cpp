@@ -5,7 +5,9 @@
 //   key(a, b, ...)    these properties of all arguments in one bytes object (None has its mark)
 //   call(fn, template, offsets, stream, a, b, ...)
 //                     copies an argument struct, writes the tensors' data pointers at the given
-//                     offsets and calls int fn(const void* args, void* stream)
+//                     offsets and calls int fn(const void* args, void* stream), without the
+//                     interpreter's lock; calls of one stream take turns, since one may be several
+//                     launches over the stream's workspace
 //   empty(a, b)       the output: a's shape and device, b's dtype, contiguous
 // On one host, per call: 2.5 -> 0.3 us for the key and its look-up, 1.7 -> 0.2 us for the struct and
 // the call, 1.4 to 2.7 -> 0.6 to 1.2 us for an output. A norm of one row went from 10.5 to 6.2 us, the
@@ -18,10 +20,19 @@
 #include <cstdint>
 #include <cstring>
 #include <exception>
+#include <functional>
+#include <mutex>
 
 namespace {
 
 constexpr size_t kMaxArgs = 1024;  // bytes of an argument struct
+
+// The lock of a stream's calls (streams may share one). Taken without the interpreter's lock, which
+// is taken again only after it is given back.
+std::mutex& lock_of(void* stream) {
+  static std::mutex locks[61];
+  return locks[std::hash<void*>()(stream) % 61];
+}
 
 PyObject* key(PyObject*, PyObject* const* args, Py_ssize_t n) {
   int64_t buf[256];
@@ -94,7 +105,10 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
   int st;
   Py_BEGIN_ALLOW_THREADS;
-  st = reinterpret_cast<int (*)(const void*, void*)>(fn)(buf, stream);
+  {
+    const std::lock_guard<std::mutex> turn(lock_of(stream));
+    st = reinterpret_cast<int (*)(const void*, void*)>(fn)(buf, stream);
+  }
   Py_END_ALLOW_THREADS;
   return PyLong_FromLong(st);
 }

@@ -1,0 +1,43 @@
+"""ftb._pycall.call from several threads: a call may be several launches over its stream's
+workspace, so calls of one stream must not interleave."""
+import ctypes
+import threading
+import time
+
+import ftb  # noqa: F401
+from ftb import _pycall
+
+
+def overlaps(streams):
+    """How often a call of a stream began while another of the same stream was under way."""
+    inside, found = {}, []
+
+    @ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p)
+    def entry(args, stream):
+        inside[stream] = inside.get(stream, 0) + 1
+        found.append(inside[stream] > 1)
+        time.sleep(0.005)  # (lets other threads in)
+        inside[stream] -= 1
+        return 0
+
+    fn = ctypes.cast(entry, ctypes.c_void_p).value
+    start = threading.Barrier(len(streams))
+
+    def work(stream):
+        start.wait()
+        for _ in range(8):
+            assert _pycall.call(fn, bytes(8), (), stream) == 0
+
+    threads = [threading.Thread(target=work, args=(s,)) for s in streams]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+        assert not t.is_alive()
+    assert len(found) == 8 * len(streams)
+    return sum(found)
+
+
+def test_calls_of_one_stream_take_turns():
+    assert overlaps([64] * 4) == 0
+    assert overlaps([64, 64, 4096, 4096]) == 0
