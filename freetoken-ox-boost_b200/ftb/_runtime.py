@@ -25,6 +25,31 @@ def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def launch(name: str, device: torch.device, *args) -> None:
+    """Calls entry point ``name`` with ``args`` and ``device``'s current stream, and raises its
+    errors. A launch goes to the current device, whatever its pointers: ``device`` is made that."""
+    if _current_device() != device.index:
+        with torch.cuda.device(device):
+            return launch(name, device, *args)
+    st = getattr(_lib.load(), name)(*args, stream_handle(device))
+    if st:
+        _lib.check(name, st)
+
+
+def caller(device: torch.device):
+    """``_pycall.call``, with ``device`` current as in :func:`launch`."""
+    if _current_device() == device.index:
+        return _pycall.call
+
+    def call(*args):
+        with torch.cuda.device(device):
+            return _pycall.call(*args)
+    return call
+
+
 def require_cuda(*tensors: torch.Tensor) -> torch.device:
     dev = tensors[0].device
     if dev.type != "cuda":

@@ -4,7 +4,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._runtime import (_ARGS, _pycall, read_status, remember, require_cuda, stream_handle,
+from ._runtime import (_ARGS, _pycall, caller, read_status, remember, require_cuda, stream_handle,
                        zeroed_workspace)
 from .block import _TYPE
 
@@ -85,8 +85,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         raise ValueError("out must be contiguous, of q's shape and dtype")
     lse = q.new_empty(q.shape[:2], dtype=torch.float32) if return_lse else None
     ws = zeroed_workspace(known[1], dev)
-    st = _pycall.call(_lib.entry("ftb_attention"), known[0], _POINTERS, stream_handle(dev), q, k_cache,
-                      v_cache, block_table, kv_len, cu_q, out, lse, ws)
+    st = caller(dev)(_lib.entry("ftb_attention"), known[0], _POINTERS, stream_handle(dev), q, k_cache,
+                     v_cache, block_table, kv_len, cu_q, out, lse, ws)
     if st:
         _lib.check("ftb_attention", st)
     if check_status:

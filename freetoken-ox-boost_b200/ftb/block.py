@@ -12,7 +12,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._runtime import _ARGS, _pycall, remember, require, require_cuda, stream_handle
+from ._runtime import _ARGS, _pycall, caller, remember, require, require_cuda, stream_handle
 
 _TYPE = {torch.bfloat16: _lib.FTB_TYPE_BF16, torch.float16: _lib.FTB_TYPE_F16}
 _GATE_ACTS = {None: _lib.FTB_GATE_LINEAR, "sigmoid": _lib.FTB_GATE_SIGMOID}
@@ -86,8 +86,9 @@ def _norm_args(x, y, gate, post, pre, scale, eps, gate_act, dtype):
 
 
 def _launch_norm(args, x, y, gate, post, pre, r, h):
-    st = _pycall.call(_lib.entry("ftb_block_norm"), args, _NORM_POINTERS, stream_handle(x.device), x,
-                      y, gate, post, pre, r, h)
+    dev = x.device
+    st = caller(dev)(_lib.entry("ftb_block_norm"), args, _NORM_POINTERS, stream_handle(dev), x, y, gate,
+                     post, pre, r, h)
     if st:
         _lib.check("ftb_block_norm", st)
 
@@ -232,8 +233,9 @@ def _rope(q, k, v, positions, table, k_dst, v_dst, slots, sections, order, pairs
                                                        sections, order, pairs))
     out = _pycall.empty(q, q) if q_out is None else _given(q_out, "q_out", q, q.dtype)
     if q.shape[0]:
-        st = _pycall.call(_lib.entry("ftb_rope"), known[0], _ROPE_POINTERS, stream_handle(q.device),
-                          q, k, v, out, k_dst, v_dst, positions, table, slots)
+        dev = q.device
+        st = caller(dev)(_lib.entry("ftb_rope"), known[0], _ROPE_POINTERS, stream_handle(dev), q, k, v,
+                         out, k_dst, v_dst, positions, table, slots)
         if st:
             _lib.check("ftb_rope", st)
     return out

@@ -36,7 +36,7 @@ import torch
 import torch.distributed as dist
 
 from . import _lib
-from ._runtime import ptr, require, require_cuda, stream_handle
+from ._runtime import launch, ptr, require, require_cuda, stream_handle
 from .banks import Nvfp4Bank
 
 
@@ -135,13 +135,9 @@ class EpGroup:
         kind, alpha, limit = _act_spec(activation, act_alpha, act_limit)
         b = bank.struct()
         s = shared.struct() if shared is not None else None
-        st = _lib.load().ftb_ep_forward_tokens(self._h, n, ptr(x), ptr(topk_weights),
-                                               ptr(topk_ids), ctypes.byref(b),
-                                               ctypes.byref(s) if s is not None else None, kind,
-                                               alpha, limit,
-                                               1 if apply_router_weight_on_input else 0,
-                                               ptr(out), stream_handle(dev))
-        _lib.check("ftb_ep_forward_tokens", st)
+        launch("ftb_ep_forward_tokens", dev, self._h, n, ptr(x), ptr(topk_weights), ptr(topk_ids),
+               ctypes.byref(b), ctypes.byref(s) if s is not None else None, kind, alpha, limit,
+               1 if apply_router_weight_on_input else 0, ptr(out))
         return out
 
     def set_trace(self, trace: torch.Tensor | None):
@@ -159,7 +155,8 @@ class EpGroup:
 
     def status(self, clear: bool = True) -> int:
         """The sticky device status word (synchronises the current stream)."""
-        v = _lib.load().ftb_ep_status(self._h, 1 if clear else 0, stream_handle(self.device))
+        with torch.cuda.device(self.device):
+            v = _lib.load().ftb_ep_status(self._h, 1 if clear else 0, stream_handle(self.device))
         if v < 0:
             _lib.check("ftb_ep_status", -v)
         return v

@@ -26,7 +26,7 @@ import ctypes
 import torch
 
 from . import _lib
-from ._runtime import ptr, read_status, require, require_cuda, stream_handle, workspace
+from ._runtime import launch, ptr, read_status, require, require_cuda, workspace
 from .banks import Nvfp4Bank
 
 _ACTS = {"silu": _lib.FTB_ACT_SILU, "swiglu_clamp": _lib.FTB_ACT_SWIGLU_CLAMP,
@@ -142,9 +142,8 @@ def quant_nvfp4(x: torch.Tensor):
     q = torch.empty(rows, K // 2, dtype=torch.uint8, device=dev)
     sf = torch.empty(rows, K // 16, dtype=torch.uint8, device=dev)
     g = torch.empty(rows, dtype=torch.float32, device=dev)
-    st = _lib.load().ftb_quant_nvfp4(ptr(x), 1 if x.dtype == torch.bfloat16 else 0, rows, K,
-                                     ptr(q), ptr(sf), ptr(g), stream_handle(dev))
-    _lib.check("ftb_quant_nvfp4", st)
+    launch("ftb_quant_nvfp4", dev, ptr(x), 1 if x.dtype == torch.bfloat16 else 0, rows, K, ptr(q),
+           ptr(sf), ptr(g))
     return q, sf, g
 
 
@@ -195,8 +194,7 @@ def _layer(path: int, x, bank, topk_weights, topk_ids, activation, act_alpha, ac
                          shared_out=torch.zeros(T, H, dtype=bf, device=dev))
         for name, t in inter.items():
             setattr(a, name, t.data_ptr())
-    st = lib.ftb_moe_layer(ctypes.byref(a), stream_handle(dev))
-    _lib.check("ftb_moe_layer", st)
+    launch("ftb_moe_layer", dev, ctypes.byref(a))
     if check_status or debug:
         status = read_status(ws)
         if inter is not None:
@@ -343,9 +341,8 @@ def moe_sum_reduce(ic3: torch.Tensor, topk_ids: torch.Tensor, num_experts: int,
         out = torch.empty(T, H, dtype=torch.bfloat16, device=dev)
     if shared_out is not None:
         require(shared_out, "shared_out", torch.bfloat16, (T, H))
-    st = _lib.load().ftb_moe_combine(ptr(ic3), ptr(topk_ids), ptr(shared_out), T, H, K,
-                                     num_experts, ptr(out), stream_handle(dev))
-    _lib.check("ftb_moe_combine", st)
+    launch("ftb_moe_combine", dev, ptr(ic3), ptr(topk_ids), ptr(shared_out), T, H, K, num_experts,
+           ptr(out))
     return out
 
 
@@ -361,8 +358,6 @@ def moe_align_block_size(topk_ids: torch.Tensor, block_size: int, num_experts: i
     ntpp = torch.empty(1, dtype=torch.int32, device=dev)
     lib = _lib.load()
     ws = workspace(lib.ftb_moe_align_workspace_bytes(T, K, num_experts), dev)
-    st = lib.ftb_moe_align(ptr(topk_ids), T, K, num_experts, block_size, ptr(sorted_ids),
-                           ptr(expert_ids), ptr(ntpp), None, ptr(ws), ws.numel(),
-                           stream_handle(dev))
-    _lib.check("ftb_moe_align", st)
+    launch("ftb_moe_align", dev, ptr(topk_ids), T, K, num_experts, block_size, ptr(sorted_ids),
+           ptr(expert_ids), ptr(ntpp), None, ptr(ws), ws.numel())
     return sorted_ids, expert_ids, ntpp

@@ -16,7 +16,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._runtime import ptr, require, require_cuda, stream_handle
+from ._runtime import launch, ptr, require, require_cuda
 
 
 def _route(logits: torch.Tensor, top_k: int, mode: int, bias, scaling: float, renorm: bool):
@@ -30,9 +30,8 @@ def _route(logits: torch.Tensor, top_k: int, mode: int, bias, scaling: float, re
     b = None
     if bias is not None:
         b = bias.to(device=dev, dtype=torch.float32).contiguous()
-    st = _lib.load().ftb_route_topk(ptr(logits), T, E, top_k, mode, ptr(b), float(scaling),
-                                    1 if renorm else 0, ptr(w), ptr(ids), stream_handle(dev))
-    _lib.check("ftb_route_topk", st)
+    launch("ftb_route_topk", dev, ptr(logits), T, E, top_k, mode, ptr(b), float(scaling),
+           1 if renorm else 0, ptr(w), ptr(ids))
     return w, ids
 
 
@@ -77,10 +76,8 @@ def fused_route_ranked(logits: torch.Tensor, bias: torch.Tensor, top_k: int, ren
     rid = torch.empty(T, n_rank, dtype=torch.int32, device=dev)
     rsc = torch.empty(T, n_rank, dtype=torch.float32, device=dev)
     b = None if bias is None else bias.to(device=dev, dtype=torch.float32).contiguous()
-    st = _lib.load().ftb_route_ranked(ptr(logits), T, E, top_k, n_rank, ptr(b), float(scaling),
-                                      1 if renorm else 0, ptr(w), ptr(ids), ptr(rid), ptr(rsc),
-                                      stream_handle(dev))
-    _lib.check("ftb_route_ranked", st)
+    launch("ftb_route_ranked", dev, ptr(logits), T, E, top_k, n_rank, ptr(b), float(scaling),
+           1 if renorm else 0, ptr(w), ptr(ids), ptr(rid), ptr(rsc))
     return w, ids, rid, rsc
 
 
@@ -91,6 +88,5 @@ def router_logits(x: torch.Tensor, gate_weight: torch.Tensor) -> torch.Tensor:
     T, H = x.shape
     E = G.shape[0]
     out = torch.empty(T, E, dtype=torch.float32, device=dev)
-    st = _lib.load().ftb_router_gemv(ptr(x), ptr(G), T, H, E, ptr(out), stream_handle(dev))
-    _lib.check("ftb_router_gemv", st)
+    launch("ftb_router_gemv", dev, ptr(x), ptr(G), T, H, E, ptr(out))
     return out
