@@ -20,18 +20,19 @@
 #include <cstdint>
 #include <cstring>
 #include <exception>
-#include <functional>
+#include <map>
 #include <mutex>
+#include <utility>
 
 namespace {
 
 constexpr size_t kMaxArgs = 1024;  // bytes of an argument struct
 
-// The lock of a stream's calls (streams may share one). Taken without the interpreter's lock, which
-// is taken again only after it is given back.
-std::mutex& lock_of(void* stream) {
-  static std::mutex locks[61];
-  return locks[std::hash<void*>()(stream) % 61];
+// The lock of a stream's calls, found under the interpreter's lock and taken without it. One each:
+// a launch may wait for its stream, and that for a peer whose stream another thread has to feed.
+std::mutex& lock_of(int device, void* stream) {
+  static std::map<std::pair<int, void*>, std::mutex> locks;  // (nodes stay where they are)
+  return locks[{device, stream}];
 }
 
 PyObject* key(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -87,6 +88,8 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return nullptr;
   }
   std::memcpy(buf, PyBytes_AS_STRING(args[1]), size);
+  int device = -1;  // the tensors'
+  std::mutex* turn = nullptr;
   try {
     for (Py_ssize_t i = 4; i < n; ++i) {
       if (args[i] == Py_None) continue;
@@ -96,9 +99,12 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
         PyErr_SetString(PyExc_TypeError, "expected tensors, and offsets inside the struct");
         return nullptr;
       }
-      void* p = THPVariable_Unpack(args[i]).data_ptr();
+      const at::Tensor& t = THPVariable_Unpack(args[i]);
+      void* p = t.data_ptr();
       std::memcpy(buf + off, &p, sizeof(p));
+      device = t.device().index();
     }
+    turn = &lock_of(device, stream);
   } catch (const std::exception& e) {
     PyErr_SetString(PyExc_RuntimeError, e.what());
     return nullptr;
@@ -106,7 +112,7 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
   int st;
   Py_BEGIN_ALLOW_THREADS;
   {
-    const std::lock_guard<std::mutex> turn(lock_of(stream));
+    const std::lock_guard<std::mutex> held(*turn);
     st = reinterpret_cast<int (*)(const void*, void*)>(fn)(buf, stream);
   }
   Py_END_ALLOW_THREADS;

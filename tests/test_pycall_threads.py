@@ -1,5 +1,6 @@
-"""ftb._pycall.call from several threads: a call may be several launches over its stream's
-workspace, so calls of one stream must not interleave."""
+"""Entry points called from several threads: a call may be several launches over its stream's
+workspace, so calls of one stream must not interleave. Those of different streams may: a launch can
+wait for its stream, and that for a peer whose stream another thread has to feed."""
 import ctypes
 import threading
 import time
@@ -41,3 +42,20 @@ def overlaps(streams):
 def test_calls_of_one_stream_take_turns():
     assert overlaps([64] * 4) == 0
     assert overlaps([64, 64, 4096, 4096]) == 0
+
+
+def test_a_waiting_call_holds_up_its_own_stream_only():
+    free = threading.Event()
+
+    @ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p)
+    def entry(args, stream):
+        return 0 if stream != 16 or free.wait(60) else 1
+
+    fn = ctypes.cast(entry, ctypes.c_void_p).value
+    first = threading.Thread(target=lambda: _pycall.call(fn, bytes(8), (), 16))
+    first.start()
+    for stream in range(32, 32 + 16 * 200, 16):
+        assert _pycall.call(fn, bytes(8), (), stream) == 0
+    free.set()
+    first.join(60)
+    assert not first.is_alive()
