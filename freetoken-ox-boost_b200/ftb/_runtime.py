@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import ctypes
+import threading
 
 import torch
 
@@ -25,16 +26,22 @@ def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+_TURNS: dict = {}
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def launch(name: str, device: torch.device, *args) -> None:
     """Calls entry point ``name`` with ``args`` and ``device``'s current stream, and raises its
-    errors. A launch goes to the current device, whatever its pointers: ``device`` is made that."""
+    errors. A launch goes to the current device, whatever its pointers: ``device`` is made that.
+    Calls of one stream take turns between threads: one may be several launches over the stream's
+    workspace, and the interpreter's lock is not held around them."""
     if _current_device() != device.index:
         with torch.cuda.device(device):
             return launch(name, device, *args)
-    st = getattr(_lib.load(), name)(*args, stream_handle(device))
+    stream = stream_handle(device)
+    key = (device.index, stream)
+    with _TURNS.get(key) or _TURNS.setdefault(key, threading.Lock()):
+        st = getattr(_lib.load(), name)(*args, stream)
     if st:
         _lib.check(name, st)
 

@@ -4,9 +4,11 @@ wait for its stream, and that for a peer whose stream another thread has to feed
 import ctypes
 import threading
 import time
+import types
 
-import ftb  # noqa: F401
-from ftb import _pycall
+import torch
+
+from ftb import _lib, _pycall, _runtime
 
 
 def overlaps(streams):
@@ -59,3 +61,31 @@ def test_a_waiting_call_holds_up_its_own_stream_only():
     free.set()
     first.join(60)
     assert not first.is_alive()
+
+
+def test_launch_takes_turns_too(monkeypatch):
+    """_runtime.launch, the way of the entry points without an argument struct."""
+    current, inside, found = threading.local(), {}, []
+
+    def entry(arg, stream):
+        inside[stream] = inside.get(stream, 0) + 1
+        found.append(inside[stream] > 1)
+        time.sleep(0.005)
+        inside[stream] -= 1
+        return 0
+
+    monkeypatch.setattr(_runtime, "_current_device", lambda: 0)
+    monkeypatch.setattr(_runtime, "stream_handle", lambda d: current.stream)
+    monkeypatch.setattr(_lib, "load", lambda: types.SimpleNamespace(entry=entry))
+
+    def work(stream):
+        current.stream = stream
+        for _ in range(8):
+            _runtime.launch("entry", torch.device("cuda", 0), 1)
+
+    threads = [threading.Thread(target=work, args=(s,)) for s in (64, 64, 64, 4096)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert len(found) == 32 and sum(found) == 0
