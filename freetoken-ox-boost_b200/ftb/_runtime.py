@@ -107,23 +107,26 @@ def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
 _REPLACED: list = []
 
 
-def zeroed_workspace(nbytes: int, device: torch.device) -> torch.Tensor:
-    """A cached buffer like :func:`workspace`, of its own and zero-filled when it is made: for
-    calls whose counters start at zero and are left at zero.
+def zeroed_workspace(nbytes: int, zero_bytes: int, device: torch.device) -> torch.Tensor:
+    """A cached buffer like :func:`workspace`, of its own, whose first ``zero_bytes`` are zero when
+    it is made: for calls whose counters start at zero and are left at zero.
 
     A buffer that a larger one replaces stays allocated, since a captured graph may hold it (it
     grows by half at least: the old ones together are no more than twice the new one). One that is
-    made under capture belongs to the graph alone: it is zeroed at each replay, not now."""
+    made under capture belongs to the graph alone: its counters are zeroed at each replay, not
+    now."""
     key = (device.index, stream_handle(device), "zeroed")
     t = _WS.get(key)
     if t is None or t.numel() < nbytes:
-        if torch.cuda.is_current_stream_capturing():
-            return torch.zeros(int(nbytes), dtype=torch.uint8, device=device)
-        if t is not None:
+        with torch.cuda.device(device):
+            captured = torch.cuda.is_current_stream_capturing()
+        if t is not None and not captured:
             _REPLACED.append(t)
             nbytes = max(nbytes, t.numel() * 3 // 2)
-        t = torch.zeros(int(nbytes), dtype=torch.uint8, device=device)
-        _WS[key] = t
+        t = torch.empty(int(nbytes), dtype=torch.uint8, device=device)
+        t[:zero_bytes].zero_()
+        if not captured:
+            _WS[key] = t
     return t
 
 

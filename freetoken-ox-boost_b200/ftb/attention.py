@@ -84,7 +84,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
         raise ValueError("out must be contiguous, of q's shape and dtype")
     lse = q.new_empty(q.shape[:2], dtype=torch.float32) if return_lse else None
-    ws = zeroed_workspace(known[1], dev)
+    ws = zeroed_workspace(known[1], _lib.FTB_ATTN_ZERO_BYTES, dev)
     st = caller(dev)(_lib.entry("ftb_attention"), known[0], _POINTERS, stream_handle(dev), q, k_cache,
                      v_cache, block_table, kv_len, cu_q, out, lse, ws)
     if st:
