@@ -112,9 +112,10 @@ def zeroed_workspace(nbytes: int, zero_bytes: int, device: torch.device) -> torc
     it is made: for calls whose counters start at zero and are left at zero.
 
     A buffer that a larger one replaces stays allocated, since a captured graph may hold it (it
-    grows by half at least: the old ones together are no more than twice the new one). One that is
-    made under capture belongs to the graph alone: its counters are zeroed at each replay, not
-    now."""
+    grows by half at least: the old ones together are no more than twice the new one). Sizes are
+    rounded up to an eighth of their power of two, so that calls whose sizes hardly differ share a
+    buffer. One that is made under capture belongs to the graph alone: its counters are zeroed at
+    each replay, not now."""
     key = (device.index, stream_handle(device), "zeroed")
     t = _WS.get(key)
     if t is None or t.numel() < nbytes:
@@ -123,7 +124,9 @@ def zeroed_workspace(nbytes: int, zero_bytes: int, device: torch.device) -> torc
         if t is not None and not captured:
             _REPLACED.append(t)
             nbytes = max(nbytes, t.numel() * 3 // 2)
-        t = torch.empty(int(nbytes), dtype=torch.uint8, device=device)
+        step = 1 << max(16, int(nbytes).bit_length() - 4)
+        nbytes = -(-int(nbytes) // step) * step
+        t = torch.empty(nbytes, dtype=torch.uint8, device=device)
         t[:zero_bytes].zero_()
         if not captured:
             _WS[key] = t

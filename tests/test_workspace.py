@@ -4,7 +4,7 @@ import contextlib
 import pytest
 import torch
 
-from ftb import _runtime
+from ftb import _lib, _runtime
 
 CPU = torch.device("cpu")
 ZERO = 4096
@@ -48,3 +48,21 @@ def test_a_captured_workspace_is_not_kept(stream):
     assert _runtime.zeroed_workspace(10000, ZERO, CPU) is kept
     assert _runtime.zeroed_workspace(1 << 20, ZERO, CPU) is not larger
     assert any(t is kept for t in _runtime._REPLACED)
+
+
+def test_calls_whose_sizes_hardly_differ_share_a_buffer(stream):
+    """More tokens take a few bytes more of plan; the parts that fill the workspace do not grow."""
+    size = _lib.load().ftb_attention_workspace_bytes
+    first = None
+    for tokens in (300, 1000, 4093, 50000):
+        ws = _runtime.zeroed_workspace(size(tokens, 8, tokens, 32, 8, 128), ZERO, CPU)
+        first = ws if first is None else first
+        assert ws is first, tokens
+    assert first.numel() <= size(300, 8, 300, 32, 8, 128) * 9 // 8 and not _runtime._REPLACED
+
+
+def test_small_sizes_are_not_rounded_to_large_ones(stream):
+    for n in (1, 65536, 65537, 10 ** 6, 10 ** 7 + 1):
+        _runtime._WS.clear()
+        got = _runtime.zeroed_workspace(n, ZERO, CPU).numel()
+        assert n <= got <= max(65536, n * 9 // 8 + 65536)
