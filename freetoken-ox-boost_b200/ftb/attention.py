@@ -44,14 +44,16 @@ def _args(q, k_cache, v_cache, block_table, kv_len, cu_q, max_q, scale, causal, 
     elif batch != total or max_q != 1:
         raise ValueError(f"without cu_q q has one row per sequence (got {total} rows, batch {batch}, "
                          f"max_q {max_q})")
-    if window < 0:
-        raise ValueError(f"window={window}")
+    if window < 0 or max_q < 0:
+        raise ValueError(f"window={window}, max_q={max_q}")
+    # (bounds of any size: what lies past the rows and past every key says no more)
+    max_q, window = min(int(max_q), total), min(int(window), 2 ** 31 - 1)
     nbytes = _lib.load().ftb_attention_workspace_bytes(total, batch, max_q, Hq, Hkv, D)
     return _lib.AttnArgsStruct(
         workspace_bytes=nbytes, q_strides=q.stride()[:2], k_strides=k_cache.stride()[:3],
         v_strides=v_cache.stride()[:3], total_q=total, num_pages=pages,
-        table_stride=block_table.stride(0), batch=batch, max_q=int(max_q), table_width=width,
-        page=page, Hq=Hq, Hkv=Hkv, D=D, causal=int(causal), window=int(window),
+        table_stride=block_table.stride(0), batch=batch, max_q=max_q, table_width=width,
+        page=page, Hq=Hq, Hkv=Hkv, D=D, causal=int(causal), window=window,
         type=_TYPE[q.dtype], scale=D ** -0.5 if scale is None else scale)
 
 
