@@ -89,6 +89,9 @@ int ftb_attention(const ftb_attn_args* args, ftb_stream_t stream) {
   ftb_attn_args call = *args;
   // (a caller's bound may be its model's; no sequence has more than all rows)
   if (call.total_q >= 0) call.max_q = (int)std::min<int64_t>(call.max_q, call.total_q);
+  // (nor does a window that reaches every key hide any: j > p - window for all j and p < keys. As no
+  // window it also stays out of the kernels' 32-bit differences)
+  if (call.window >= (int64_t)call.table_width * call.page) call.window = std::min(call.window, 0);
   const ftb_attn_args* a = &call;
   if (a->type != FTB_TYPE_BF16 && a->type != FTB_TYPE_F16) return FTB_ERR_ARG;
   if (a->total_q < 0 || a->total_q > 0x7fffffff || a->batch < 0 || a->max_q < 0 || a->Hkv < 1 ||

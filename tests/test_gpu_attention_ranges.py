@@ -22,3 +22,14 @@ def test_bounds_past_32_bits(pairs):
         assert torch.equal(attend(c, window=window), want), window
     with pytest.raises(ValueError, match="max_q"):
         attend(c, max_q=-1)
+
+
+@pytest.mark.parametrize("pairs", [[(9, 4), (3, 70)], [(300, 200), (40, 1000)]])
+def test_a_window_that_reaches_every_key_is_no_window(pairs):
+    """Tokens before the first key too, which see every key where the mask is not causal."""
+    for causal in (True, False):
+        c = AttnCase(pairs, causal=causal)
+        build(c)
+        want = attend(c, causal=causal)
+        for window in (1300, 2 ** 31 - 1):
+            assert torch.equal(attend(c, causal=causal, window=window), want)
