@@ -22,12 +22,15 @@ CUtensorMapDataType attn_dtype(int type) {
 // rate gives: at most 1.1 GFLOP by the bound that the host knows (every token against the whole
 // table, or its window). On one B200, us (streaming / tensor cores), 32 heads over 8 of 128: prompts
 // of 64 tokens 7.6 / 18.0, 256 (1.1 GFLOP) 19.3 / 20.2, 300 35.2 / 21.6, 384 37.7 / 22.8, 512 53.7 /
-// 22.5; 16 tokens at 2048 keys (0.5 GFLOP) 17.4 / 20.6, 64 32.0 / 24.3.
+// 22.5; 16 tokens at 2048 keys (0.5 GFLOP) 17.4 / 20.6, 64 32.0 / 24.3. Its row tiles are a grid's
+// rows, so that many at most.
 constexpr int kStreamRows = 16;
 constexpr double kStreamFlops = 1.1e9;
 bool streams(int64_t total_q, int max_q, int Hq, int Hkv, int D, int64_t keys) {
-  return (int64_t)max_q * (Hq / Hkv) <= kStreamRows ||
-         4.0 * D * Hq * (double)total_q * (double)keys <= kStreamFlops;
+  const int64_t rows = (int64_t)max_q * (Hq / Hkv);
+  return rows <= kStreamRows ||
+         (rows <= (int64_t)kStreamRows * 65535 &&
+          4.0 * D * Hq * (double)total_q * (double)keys <= kStreamFlops);
 }
 int64_t keys_bound(const ftb_attn_args& a) {
   const int64_t all = (int64_t)a.table_width * a.page;

@@ -33,3 +33,23 @@ def test_a_window_that_reaches_every_key_is_no_window(pairs):
         want = attend(c, causal=causal)
         for window in (1300, 2 ** 31 - 1):
             assert torch.equal(attend(c, causal=causal, window=window), want)
+
+
+def test_more_row_tiles_than_a_grid_holds():
+    """128 heads over one, 8200 tokens by max_q (a loose bound): 65600 tiles of 16 rows of little
+    work each."""
+    c = AttnCase([(8, 8)] * 1025, q_heads=128, kv_heads=1, head=8, page=8)
+    build(c)
+    want = attend(c)
+    got = attend(c, max_q=8200)
+    # each way is within an output's and the weights' rounding of the definition: 2 * 2 * 2^-8 of
+    # values that reach 4, and a little for the scores
+    assert (got.float() - want.float()).abs().max() <= 2.0 ** -3
+    # a window of one key: each token gets its own V row (the first 7 see none), whose weight is
+    # rounded against a sum that is not: 2^-8 of it, and as much for the output
+    c = AttnCase([(8200, 8193)], q_heads=128, kv_heads=1, head=8, page=8)
+    _, keys = build(c)
+    out = attend(c, window=1).cpu()
+    v = keys[0][:, 1].float()
+    assert (out[:7] == 0).all()
+    assert ((out[7:].float() - v).abs() <= 2.0 ** -7 * 1.01 * v.abs()).all()
