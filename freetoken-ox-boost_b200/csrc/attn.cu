@@ -26,11 +26,13 @@ CUtensorMapDataType attn_dtype(int type) {
 // rows, so that many at most.
 constexpr int kStreamRows = 16;
 constexpr double kStreamFlops = 1.1e9;
-bool streams(int64_t total_q, int max_q, int Hq, int Hkv, int D, int64_t keys) {
-  const int64_t rows = (int64_t)max_q * (Hq / Hkv);
+// Of the two, a batch beyond the tensor-core kernel's plan goes to the streaming one.
+bool streams(const ftb_attn_args& a, int64_t keys) {
+  const int64_t rows = (int64_t)a.max_q * (a.Hq / a.Hkv);
   return rows <= kStreamRows ||
          (rows <= (int64_t)kStreamRows * 65535 &&
-          4.0 * D * Hq * (double)total_q * (double)keys <= kStreamFlops);
+          (4.0 * a.D * a.Hq * (double)a.total_q * (double)keys <= kStreamFlops ||
+           !attn_chunk_fits(a)));
 }
 int64_t keys_bound(const ftb_attn_args& a) {
   const int64_t all = (int64_t)a.table_width * a.page;
@@ -137,7 +139,7 @@ int ftb_attention(const ftb_attn_args* args, ftb_stream_t stream) {
   P.causal = a->causal != 0, P.window = a->window;
   P.keys_max = a->table_width * a->page;
   P.scale_log2 = a->scale * 1.44269504088896341f;
-  return streams(a->total_q, a->max_q, a->Hq, a->Hkv, a->D, keys_bound(*a))
+  return streams(*a, keys_bound(*a))
              ? launch_attn_stream(*a, P, (cudaStream_t)stream)
              : launch_attn_chunk(*a, P, (cudaStream_t)stream);
 }

@@ -46,6 +46,7 @@ int attn_q_map(CUtensorMap* m, const ftb_attn_args& a, uint32_t group, uint32_t 
 
 int launch_attn_stream(const ftb_attn_args& a, AttnParams P, cudaStream_t stream);
 size_t attn_stream_partial_bytes(int64_t rows_max, int D);
+bool attn_chunk_fits(const ftb_attn_args& a);  // its plan's batch and piece counts
 int launch_attn_chunk(const ftb_attn_args& a, AttnParams P, cudaStream_t stream);
 size_t attn_chunk_workspace_bytes(int64_t total_q, int batch, int Hkv, int G, int D);
 

@@ -1249,10 +1249,15 @@ size_t attn_chunk_workspace_bytes(int64_t total_q, int batch, int Hkv, int G, in
   return bytes + (size_t)plan_parts() * 2 * kTileM * (dp + 2) * sizeof(float);
 }
 
+bool attn_chunk_fits(const ftb_attn_args& a) {
+  return a.batch <= kMaxBatch &&
+         chunk_groups(a.total_q, a.batch, a.Hq / a.Hkv) * a.Hkv <= 0x3fffffff;
+}
+
 int launch_attn_chunk(const ftb_attn_args& a, AttnParams P, cudaStream_t stream) {
+  if (!attn_chunk_fits(a)) return FTB_ERR_SHAPE;
   const int tok1 = kTileM / P.G;
   const int64_t groups = chunk_groups(a.total_q, a.batch, P.G);
-  if (a.batch > kMaxBatch || groups * a.Hkv > 0x3fffffff) return FTB_ERR_SHAPE;
   AttnMaps M;
   const uint32_t r = a.page < kTileK ? a.page : kTileK;
   int st = attn_cache_map(&M.k, a.k_cache, a, a.k_strides, r, 1);

@@ -53,3 +53,19 @@ def test_more_row_tiles_than_a_grid_holds():
     v = keys[0][:, 1].float()
     assert (out[:7] == 0).all()
     assert ((out[7:].float() - v).abs() <= 2.0 ** -7 * 1.01 * v.abs()).all()
+
+
+def test_a_batch_beyond_the_plan():
+    """25700 sequences of 2 tokens of 16 heads over one: with half of them each, the other kernel."""
+    batch = 25700
+    c = AttnCase([(2, 9)] * batch, q_heads=32, kv_heads=2, head=64, page=8)
+    build(c)
+    got = attend(c)
+    half = batch // 2
+    for part in (slice(0, half), slice(half, batch)):
+        rows = slice(2 * part.start, 2 * part.stop)
+        cu = c.t["cu_q"][part.start:part.stop + 1] - 2 * part.start
+        want = attend(c, q=c.t["q"][rows], block_table=c.t["block_table"][part],
+                      kv_len=c.t["kv_len"][part], cu_q=cu)
+        # each within an output's and the weights' rounding of the definition, of values up to 5
+        assert (got[rows].float() - want.float()).abs().max() <= 4 * 5 * 2.0 ** -8
