@@ -106,7 +106,8 @@ int ftb_attention(const ftb_attn_args* args, ftb_stream_t stream) {
       (int64_t)a->table_width * a->page > 0x7fffff00)
     return FTB_ERR_SHAPE;
   if (a->total_q == 0 || a->batch == 0 || a->max_q == 0) return FTB_OK;
-  if (!a->q || !a->k_cache || !a->v_cache || !a->block_table || !a->kv_len || !a->out)
+  if (!a->q || !a->k_cache || !a->v_cache || (!a->block_table && a->table_width > 0) || !a->kv_len ||
+      !a->out)  // (a table without a column has no address: no sequence has a key)
     return FTB_ERR_ARG;
   if (!a->cu_q && a->total_q != a->batch) return FTB_ERR_SHAPE;
   if (!std::isfinite(a->scale)) return FTB_ERR_ARG;

@@ -69,3 +69,16 @@ def test_a_batch_beyond_the_plan():
                       kv_len=c.t["kv_len"][part], cu_q=cu)
         # each within an output's and the weights' rounding of the definition, of values up to 5
         assert (got[rows].float() - want.float()).abs().max() <= 4 * 5 * 2.0 ** -8
+
+
+def test_table_without_a_column():
+    """No sequence has a key: outputs 0, lse -inf."""
+    for n in (1, 40):
+        q = torch.randn(2 * n, 8, 64, device="cuda").bfloat16()
+        cache = torch.zeros(3, 16, 2, 64, dtype=torch.bfloat16, device="cuda")
+        table = torch.zeros(2, 0, dtype=torch.int32, device="cuda")
+        lens = torch.zeros(2, dtype=torch.int32, device="cuda")
+        cu = None if n == 1 else torch.tensor([0, n, 2 * n], dtype=torch.int32, device="cuda")
+        out, lse = ftb.paged_attention(q, cache, cache, table, lens, cu, n, return_lse=True,
+                                       check_status=True)
+        assert (out == 0).all() and torch.isneginf(lse).all()
