@@ -92,14 +92,13 @@ class DecoderLayer:
 
     def attention(self, hidden: torch.Tensor, step: AttnStep, cache: PagedKvCache) -> torch.Tensor:
         """The attention block's output of normed ``hidden`` [tokens, H]; fills the cache."""
-        tokens = hidden.shape[0]
-        qkv = (hidden @ self.qkv.t()).view(tokens, -1, self.head_dim)
+        qkv = (hidden @ self.qkv.t()).unflatten(1, (-1, self.head_dim))
         q, k, v = qkv.split([self.q_heads, self.kv_heads, self.kv_heads], 1)
         q = rope_append(q, k, v, step.positions, self.rope_table, cache.k, cache.v, step.slots,
                         **self.rope)
         out = paged_attention(q, cache.k, cache.v, step.block_table, step.kv_len, step.cu_q,
                               step.max_q, window=self.window)
-        return out.view(tokens, -1) @ self.o.t()
+        return out.flatten(1) @ self.o.t()
 
     def forward(self, residual: torch.Tensor, hidden: torch.Tensor | None, step: AttnStep,
                 cache: PagedKvCache, next_norm: torch.Tensor | None = None):
