@@ -15,6 +15,7 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <ATen/ops/empty.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdint>
@@ -65,8 +66,8 @@ PyObject* key(PyObject*, PyObject* const* args, Py_ssize_t n) {
       for (int64_t s : sizes) buf[at++] = s;
       for (int64_t s : strides) buf[at++] = s;
     }
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
+  } catch (const std::exception&) {  // (as torch raises it: out of memory is its own kind)
+    torch::translate_exception_to_python(std::current_exception());
     return nullptr;
   }
   return PyBytes_FromStringAndSize(reinterpret_cast<const char*>(buf), (Py_ssize_t)(at * 8));
@@ -105,8 +106,8 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
       device = t.device().index();
     }
     turn = &lock_of(device, stream);
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
+  } catch (const std::exception&) {  // (as torch raises it: out of memory is its own kind)
+    torch::translate_exception_to_python(std::current_exception());
     return nullptr;
   }
   int st;
@@ -129,8 +130,8 @@ PyObject* empty(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::Tensor& a = THPVariable_Unpack(args[0]);
     return THPVariable_Wrap(
         at::empty(a.sizes(), a.options().dtype(THPVariable_Unpack(args[1]).scalar_type())));
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
+  } catch (const std::exception&) {  // (as torch raises it: out of memory is its own kind)
+    torch::translate_exception_to_python(std::current_exception());
     return nullptr;
   }
 }
