@@ -119,6 +119,8 @@ def block_norm(x: torch.Tensor, y: torch.Tensor, *, post_weight: torch.Tensor | 
 
     ``gate``: [H], [..., 1] or [..., H], through a sigmoid with ``gate_act="sigmoid"``.
     ``residual_out`` may be ``x`` and ``out`` may be ``y``."""
+    if y is None:
+        raise ValueError("y is None: rms_norm(x, weight) is the norm alone")
     key = (_pycall.key(x, y, gate, post_weight, pre_weight), scale, eps, gate_act)
     known = _ARGS.get(key) or remember(key, _norm_args(x, y, gate, post_weight, pre_weight, scale,
                                                        eps, gate_act, y.dtype))
@@ -126,7 +128,7 @@ def block_norm(x: torch.Tensor, y: torch.Tensor, *, post_weight: torch.Tensor | 
     h = None
     if pre_weight is not None:
         h = _pycall.empty(x, y) if out is None else _given(out, "out", x, y.dtype)
-    _launch_norm(known[0], x, y, gate, post_weight, pre_weight, None if y is None else r, h)
+    _launch_norm(known[0], x, y, gate, post_weight, pre_weight, r, h)
     return r, h
 
 

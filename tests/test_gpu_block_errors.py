@@ -15,3 +15,9 @@ def test_an_output_that_does_not_fit_is_an_out_of_memory_error():
         ftb.rms_norm(x, w)
     with pytest.raises(torch.cuda.OutOfMemoryError):
         ftb.block_norm(x, x, pre_weight=w)
+
+
+def test_block_norm_without_a_block_output():
+    x = torch.zeros(4, 64, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="rms_norm"):
+        ftb.block_norm(x, None, pre_weight=x[0])
