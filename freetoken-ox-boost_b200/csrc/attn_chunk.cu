@@ -263,8 +263,10 @@ __global__ void __launch_bounds__(kPlanThreads)
     const float joined = n > items ? n + left * (k - 1.f) : warp ? left * k : 0.f;
     float cost = fmaxf((float)most, even + gap * alike) + kPieceTiles * (rounds + last) +
                  kJoinTiles * joined * per_block;
-    // (parts <= 2 (pieces - items))
-    if ((warp && mean < k * kFewest) ||
+    // (parts <= 2 (pieces - items): in whole numbers, since past 2^24 pieces the difference of two
+    // floats is off by more than the workspace allows. The finer cut is counted again below.)
+    const long long more = (long long)(parts_of[lane] - groups) * P.Hkv;
+    if ((warp && mean < k * kFewest) || more > plan.max_parts / 2 ||
         n - items + left * (k - 1.f) > (float)(plan.max_parts / 2))
       cost = INFINITY;
     const unsigned long long key = (unsigned long long)__float_as_uint(cost) << 32 |
