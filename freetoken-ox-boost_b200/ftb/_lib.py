@@ -226,15 +226,18 @@ def offsets(struct, *names: str) -> tuple:
     return tuple(getattr(struct, n).offset for n in names)
 
 
-class _NotBuilt:
-    """Stands for the compiled module where it is missing: its first use raises."""
-
-    def __init__(self, why):
-        self.why = why
+class Pycall:
+    """The compiled module ``ftb._pycall``, loaded at its first use: programs that make none of the
+    calls that go through it do not load it. Where it is missing, that use raises."""
 
     def __getattr__(self, name):
-        raise FtbLibraryError(f"ftb/_pycall.so is not built ({self.why}); build it with `make -C "
-                              "freetoken-ox-boost_b200/csrc`")
+        try:
+            from . import _pycall
+        except ImportError as e:
+            raise FtbLibraryError(f"ftb/_pycall.so is not built ({e}); build it with `make -C "
+                                  "freetoken-ox-boost_b200/csrc`") from None
+        self.key, self.call, self.empty = _pycall.key, _pycall.call, _pycall.empty
+        return getattr(_pycall, name)
 
 
 def status_string(status: int) -> str:

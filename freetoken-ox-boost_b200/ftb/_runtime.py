@@ -8,10 +8,7 @@ import torch
 
 from . import _lib
 
-try:
-    from . import _pycall
-except ImportError as _e:
-    _pycall = _lib._NotBuilt(_e)
+_pycall = _lib.Pycall()
 
 _WS: dict = {}
 
