@@ -17,6 +17,7 @@
 #include <ATen/ops/empty.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/version.h>
 
 #include <cstdint>
 #include <cstring>
@@ -149,4 +150,12 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_pycall", nullptr, -1, methods,
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__pycall() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__pycall() {
+  PyObject* m = PyModule_Create(&module);
+  // (its calls go into torch's libraries, whose C++ interface changes from version to version)
+  if (m && PyModule_AddStringConstant(m, "torch_version", TORCH_VERSION) < 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

@@ -228,11 +228,18 @@ def offsets(struct, *names: str) -> tuple:
 
 class Pycall:
     """The compiled module ``ftb._pycall``, loaded at its first use: programs that make none of the
-    calls that go through it do not load it. Where it is missing, that use raises."""
+    calls that go through it do not load it. Where it is missing, or built for another torch than
+    the one it would call into, that use raises."""
 
     def __getattr__(self, name):
+        import torch
+
         try:
             from . import _pycall
+
+            if not torch.__version__.startswith(_pycall.torch_version):
+                raise ImportError(f"built for torch {_pycall.torch_version}, this is "
+                                  f"{torch.__version__}")
         except ImportError as e:
             raise FtbLibraryError(f"ftb/_pycall.so is not built ({e}); build it with `make -C "
                                   "freetoken-ox-boost_b200/csrc`") from None
