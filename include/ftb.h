@@ -483,7 +483,9 @@ FTB_API int ftb_rope(const ftb_rope_args* args, ftb_stream_t stream);
  *   of q that belong to no sequence (a padded batch) are not computed either.
  * D % 8 == 0, D <= 128; Hq / Hkv <= 128; page a power of two, >= 8; strides multiples of 8
  * elements, pointers 16-byte aligned; type BF16 or F16. Softmax, sums and accumulators are fp32;
- * the probabilities are rounded to `type` as the tensor cores' operand.
+ * the probabilities are rounded to `type` as the tensor cores' operand. In calls of few rows (up to
+ * 16 per kv head, and little work) the rest of that rounding is a second operand; in the others it
+ * is dropped, and adds about as much error as the output's own rounding.
  * workspace: ftb_attention_workspace_bytes() bytes, 256-byte aligned, for calls of one stream
  * order. Its first FTB_ATTN_ZERO_BYTES bytes are zero before the first use (the caller's
  * memset), and every call leaves the counters there zero again. Bytes [0, 4) are the
