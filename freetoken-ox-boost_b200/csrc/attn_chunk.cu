@@ -11,8 +11,8 @@
 // ref is the row's reference. It starts at 0 and moves to a tile's maximum only where that exceeds
 // it by more than 2^8, or falls short of it with nothing summed yet (by more than 2^8 in bf16, at
 // all in f16), so O, in tensor memory, is rescaled rarely. The sums are fp32. P is rounded to the
-// tensors' type: in bf16, with fp32's exponents, to 2^-9 of itself wherever ref lies; in f16, where
-// ref is never above the row's maximum, to 2^-12 of itself down to weights of 2^-14 of the largest,
+// tensors' type: in bf16, with fp32's exponents, to 2^-8 of itself wherever ref lies; in f16, where
+// ref is never above the row's maximum, to 2^-11 of itself down to weights of 2^-14 of the largest,
 // and to at most 2^-25 of the largest below that. The rest of the rounding is dropped by choice: as
 // a second operand, which the streaming kernel can afford, it would make half as many MMAs again,
 // and they are the bound here. It adds about as much error as the output's own rounding (1.4 times
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(kPlanThreads)
   // warp), so that all blocks share it. Whichever ends first by an estimate: pieces of the mean
   // size (less is lost to whole rounds where sizes differ: the small ones, last, fill the gaps),
   // kPieceTiles for the start and end of a piece, kJoinTiles more for a part that has to be joined
-  // (its 133 KB per row tile are written and read again). Against equal cuts of every item: 2048
+  // (133 KB at D = 128, both row tiles, written and read again). Against equal cuts of every item: 2048
   // tokens at 16384 keys, 256 items, 505 -> 465 us; 700 tokens of 64 heads over one, 175 items, 187
   // -> 137 us; 512 tokens at 65536 keys, 64 long items, 504 -> 510 us.
   constexpr int kPieceTiles = 2, kJoinTiles = 3, kFewest = 2, kFiner = 8;
