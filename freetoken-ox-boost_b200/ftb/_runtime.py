@@ -76,7 +76,8 @@ def require(t: torch.Tensor, name: str, dtype=None, shape=None, contiguous=True)
 # Argument blocks of calls, all but their pointers, as they were when a call of that key was first
 # checked: the checks cost more than the launch. A key holds what the checks look at: shape,
 # strides, dtype and device of each tensor (_pycall.key, or the mark of a None in its place) and
-# the options.
+# the options, as Python's own numbers: a tensor among them would be found again by its identity,
+# whatever it holds by then.
 _ARGS: dict = {}
 
 

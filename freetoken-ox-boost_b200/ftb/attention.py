@@ -47,7 +47,7 @@ def _args(q, k_cache, v_cache, block_table, kv_len, cu_q, max_q, scale, causal, 
     if window < 0 or max_q < 0:
         raise ValueError(f"window={window}, max_q={max_q}")
     # (bounds of any size: what lies past the rows and past every key says no more)
-    max_q, window = min(int(max_q), total), min(int(window), 2 ** 31 - 1)
+    max_q, window = min(max_q, total), min(window, 2 ** 31 - 1)
     nbytes = _lib.load().ftb_attention_workspace_bytes(total, batch, max_q, Hq, Hkv, D)
     return _lib.AttnArgsStruct(
         workspace_bytes=nbytes, q_strides=q.stride()[:2], k_strides=k_cache.stride()[:3],
@@ -75,6 +75,10 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     Returns out [total, q heads, D], with ``return_lse`` also the natural log of the sum of the
     exponentials, float32 [total, q heads]. ``check_status`` reads the device status word
     (synchronises) and raises on page ids, lengths or starts outside the tensors."""
+    if type(max_q) is not int or type(window) is not int or type(causal) is not bool:
+        max_q, window, causal = int(max_q), int(window), bool(causal)
+    if scale is not None and type(scale) is not float:
+        scale = float(scale)
     key = (_pycall.key(q, k_cache, v_cache, block_table, kv_len, cu_q), max_q, scale, causal, window)
     known = _ARGS.get(key)
     if known is None:

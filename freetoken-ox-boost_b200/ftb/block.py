@@ -121,6 +121,8 @@ def block_norm(x: torch.Tensor, y: torch.Tensor, *, post_weight: torch.Tensor | 
     ``residual_out`` may be ``x`` and ``out`` may be ``y``."""
     if y is None:
         raise ValueError("y is None: rms_norm(x, weight) is the norm alone")
+    if type(scale) is not float or type(eps) is not float:
+        scale, eps = float(scale), float(eps)
     key = (_pycall.key(x, y, gate, post_weight, pre_weight), scale, eps, gate_act)
     known = _ARGS.get(key) or remember(key, _norm_args(x, y, gate, post_weight, pre_weight, scale,
                                                        eps, gate_act, y.dtype))
@@ -137,6 +139,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     """``x * rsqrt(mean(x^2) + eps) * weight`` over the last dimension, in ``out_dtype`` (``x``'s
     own, or bfloat16 for a float32 ``x``)."""
     dtype = out_dtype or (torch.bfloat16 if x.dtype == torch.float32 else x.dtype)
+    if type(eps) is not float:
+        eps = float(eps)
     key = (_pycall.key(x, weight), eps, dtype)
     known = _ARGS.get(key) or remember(key, _norm_args(x, None, None, None, weight, 1.0, eps, None,
                                                        dtype))
@@ -228,7 +232,7 @@ def _rope_args(q, k, v, positions, table, k_dst, v_dst, slots, sections, order, 
 
 def _rope(q, k, v, positions, table, k_dst, v_dst, slots, sections, order, pairs, q_out):
     if sections is not None:
-        sections = tuple(sections)
+        sections = tuple(map(int, sections))
     key = (_pycall.key(q, k, positions, table) if slots is None else
            _pycall.key(q, k, positions, table, v, k_dst, v_dst, slots), sections, order, pairs)
     known = _ARGS.get(key) or remember(key, _rope_args(q, k, v, positions, table, k_dst, v_dst, slots,
