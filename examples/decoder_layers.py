@@ -19,7 +19,7 @@ from ftb import synth  # noqa: E402
 
 
 def build_layer(seed: int, hidden=2048, inter=768, experts=64, top_k=8, q_heads=16, kv_heads=4,
-                head_dim=128, positions=8192):
+                head_dim=128, positions=1024):
     g = torch.Generator(device="cuda").manual_seed(seed)
 
     def weight(*shape, scale):
@@ -52,7 +52,7 @@ def main():
     ap.add_argument("--steps", type=int, default=16, help="decode steps after the prompts")
     args = ap.parse_args()
     page = 64
-    layers = [build_layer(i) for i in range(2)]
+    layers = [build_layer(i, positions=args.tokens + args.steps) for i in range(2)]
     prompts = [args.tokens, max(1, args.tokens // 3), max(1, args.tokens // 7), 1]
     need = [-(-(n + args.steps) // page) for n in prompts]
     ids = torch.randperm(sum(need)).tolist()
