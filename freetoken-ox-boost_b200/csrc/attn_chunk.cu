@@ -29,7 +29,7 @@
 // PFLOP/s, 64 % of a large matrix product's rate (at the 1000 W power limit, where the clock is
 // 1.5 to 1.75 GHz); 8 causal prompts of up to 2048 tokens (62 GFLOP) 108 us, most of the rest in
 // half-masked tiles and the starts and ends of short items; 12 ragged chunks of up to 300 tokens,
-// 24 heads of 64 over 8, window 1000 (4.1 GFLOP) 37 us, of which the plan about 5.
+// 24 heads of 64 over 8, window 1000 (4.1 GFLOP) 38 us, of which the plan about 5.
 // A chunk of 2048 tokens at 16384 keys keeps the tensor pipe and the special-function pipe each
 // active 60 % of the time, and reads 85 MB from DRAM (87 % of the loads hit L2).
 //

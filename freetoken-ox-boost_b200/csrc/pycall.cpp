@@ -11,7 +11,8 @@
 //   empty(a, b)       the output: a's shape and device, b's dtype, contiguous
 // On one host, per call: 2.5 -> 0.3 us for the key and its look-up, 1.7 -> 0.2 us for the struct and
 // the call, 1.4 to 2.7 -> 0.6 to 1.2 us for an output. A norm of one row went from 10.5 to 6.2 us, the
-// rotary positions of 64 tokens from 11.9 to 5.4.
+// rotary positions of 64 tokens from 11.9 to 5.4 (0.3 more for the turns of a stream's calls and the
+// look at the current device).
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <ATen/ops/empty.h>

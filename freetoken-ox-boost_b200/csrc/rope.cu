@@ -73,7 +73,8 @@ __device__ __forceinline__ void store_bits(uint16_t* p, const uint16_t (&v)[VEC]
 // every head shares) have come through shared memory, so the two latencies overlap; beyond that,
 // many resident warps hide more than loads ahead, which cost registers (8190 tokens of 32 + 8 + 8
 // heads of 128 with 1 / 2 / 4 heads ahead, us: 38.4 / 38.2 / 48.6, 5.4 TB/s; with random positions
-// 39.4 / 43.1 / 55.4).
+// 39.4 / 43.1 / 55.4). Eight blocks leave 32 registers: the widest variant spills (56 bytes stored, 88
+// loaded per thread in bf16; 28 and 52 in f16).
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256, 8) k_rope(const __grid_constant__ RopeParams P) {
   __shared__ float table[2 * kMaxPairs];  // cos, then sin

@@ -73,8 +73,10 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     Token i of n sees the keys up to its own position ``kv_len - n + i`` (``causal``), and no more
     than the last ``window`` of them (0: all). A token that sees none gets 0 (lse -inf).
     Returns out [total, q heads, D], with ``return_lse`` also the natural log of the sum of the
-    exponentials, float32 [total, q heads]. ``check_status`` reads the device status word
-    (synchronises) and raises on page ids, lengths or starts outside the tensors."""
+    exponentials, float32 [total, q heads]. ``check_status`` reads the stream's status word
+    (synchronises) and raises on page ids, lengths or starts outside the tensors, of this call or of
+    one before it that did not look. ``max_q`` and the table's width pick the kernel: pass no more
+    than the batch needs where that is known on the host."""
     if type(max_q) is not int or type(window) is not int or type(causal) is not bool:
         max_q, window, causal = int(max_q), int(window), bool(causal)
     if scale is not None and type(scale) is not float:
