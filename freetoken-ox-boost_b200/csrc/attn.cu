@@ -57,6 +57,22 @@ int attn_cache_map(CUtensorMap* m, const void* base, const ftb_attn_args& a,
   return r == CUDA_SUCCESS ? FTB_OK : FTB_ERR_CUDA;
 }
 
+int attn_cache_map8(CUtensorMap* m, const void* base, const ftb_attn_args& a,
+                    const int64_t (&strides)[3], uint32_t box_rows) {
+  PFN_cuTensorMapEncodeTiled fn = encode_fn();
+  if (!fn) return FTB_ERR_CUDA;
+  const cuuint64_t dims[5] = {(cuuint64_t)a.D, (cuuint64_t)a.page, (cuuint64_t)a.Hkv,
+                              (cuuint64_t)a.num_pages, 1};
+  const cuuint64_t st[4] = {(cuuint64_t)strides[1], (cuuint64_t)strides[2], (cuuint64_t)strides[0],
+                            128};
+  const cuuint32_t box[5] = {128, box_rows, 1, 1, 1};
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, const_cast<void*>(base), dims, st, box,
+                        estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? FTB_OK : FTB_ERR_CUDA;
+}
+
 int attn_q_map(CUtensorMap* m, const ftb_attn_args& a, uint32_t group, uint32_t tokens) {
   PFN_cuTensorMapEncodeTiled fn = encode_fn();
   if (!fn) return FTB_ERR_CUDA;
@@ -89,8 +105,7 @@ size_t ftb_attention_workspace_bytes(int64_t total_q, int batch, int max_q, int 
          std::max(stream, attn_chunk_workspace_bytes(total_q, batch, Hkv, G, D));
 }
 
-int ftb_attention(const ftb_attn_args* args, ftb_stream_t stream) {
-  if (!args) return FTB_ERR_ARG;
+static int attention(const ftb_attn_args* args, const ftb_attn_fp8_args* fp8, ftb_stream_t stream) {
   ftb_attn_args call = *args;
   // (a caller's bound may be its model's; no sequence has more than all rows)
   if (call.total_q >= 0) call.max_q = (int)std::min<int64_t>(call.max_q, call.total_q);
@@ -105,16 +120,23 @@ int ftb_attention(const ftb_attn_args* args, ftb_stream_t stream) {
       a->num_pages > 0x7fffffff - 1 || a->table_width < 0 || a->window < 0 ||
       (int64_t)a->table_width * a->page > 0x7fffff00)
     return FTB_ERR_SHAPE;
+  if (fp8) {
+    const int size = fp8->scale_block;
+    if (a->D % 16 || size < 16 || size > 128 || (size & (size - 1)) || size > a->page)
+      return FTB_ERR_SHAPE;
+  }
   if (a->total_q == 0 || a->batch == 0 || a->max_q == 0) return FTB_OK;
   if (!a->q || !a->k_cache || !a->v_cache || (!a->block_table && a->table_width > 0) || !a->kv_len ||
       !a->out)  // (a table without a column has no address: no sequence has a key)
     return FTB_ERR_ARG;
+  if (fp8 && (!fp8->k_scale || !fp8->v_scale)) return FTB_ERR_ARG;
   if (!a->cu_q && a->total_q != a->batch) return FTB_ERR_SHAPE;
   if (!std::isfinite(a->scale)) return FTB_ERR_ARG;
   if (!aligned16(a->q) || !aligned16(a->k_cache) || !aligned16(a->v_cache) || !aligned16(a->out))
     return FTB_ERR_ALIGN;
   for (int i = 0; i < 3; ++i)
-    if (a->k_strides[i] % 8 || a->v_strides[i] % 8 || a->k_strides[i] < 0 || a->v_strides[i] < 0)
+    if (a->k_strides[i] % (fp8 ? 16 : 8) || a->v_strides[i] % (fp8 ? 16 : 8) || a->k_strides[i] < 0 ||
+        a->v_strides[i] < 0)
       return FTB_ERR_ALIGN;
   for (int i = 0; i < 2; ++i)
     if (a->q_strides[i] % 8 || a->q_strides[i] < 0) return FTB_ERR_ALIGN;
@@ -140,9 +162,24 @@ int ftb_attention(const ftb_attn_args* args, ftb_stream_t stream) {
   P.causal = a->causal != 0, P.window = a->window;
   P.keys_max = a->table_width * a->page;
   P.scale_log2 = a->scale * 1.44269504088896341f;
+  if (fp8) {
+    P.k_scale = fp8->k_scale, P.v_scale = fp8->v_scale;
+    for (int i = 0; i < 3; ++i)
+      P.ks_st[i] = fp8->k_scale_strides[i], P.vs_st[i] = fp8->v_scale_strides[i];
+    while ((1 << P.block_log2) < fp8->scale_block) ++P.block_log2;
+    return launch_attn_stream(*a, P, true, (cudaStream_t)stream);
+  }
   return streams(*a, keys_bound(*a))
-             ? launch_attn_stream(*a, P, (cudaStream_t)stream)
+             ? launch_attn_stream(*a, P, false, (cudaStream_t)stream)
              : launch_attn_chunk(*a, P, (cudaStream_t)stream);
+}
+
+int ftb_attention(const ftb_attn_args* args, ftb_stream_t stream) {
+  return args ? attention(args, nullptr, stream) : FTB_ERR_ARG;
+}
+
+int ftb_attention_fp8(const ftb_attn_fp8_args* args, ftb_stream_t stream) {
+  return args ? attention(&args->attn, args, stream) : FTB_ERR_ARG;
 }
 
 }  // extern "C"

@@ -28,6 +28,10 @@ struct AttnParams {
   int Hq, Hkv, G, D;
   int causal, window, keys_max;  // keys_max = table_width * page
   float scale_log2;              // scale * log2(e): scores are kept as base-2 logarithms
+  // an 8-bit cache's scales, strides {page, block, head}
+  const float *k_scale, *v_scale;
+  int64_t ks_st[3], vs_st[3];
+  int block_log2;
 };
 
 // Tensor maps of the caches. A box is `r` = min(page, tile keys) key rows of one kv head by 64
@@ -41,10 +45,14 @@ struct AttnMaps {
 
 int attn_cache_map(CUtensorMap* m, const void* base, const ftb_attn_args& a,
                    const int64_t (&strides)[3], uint32_t box_rows, uint32_t halves);
+// The same for a cache of bytes: boxes of `box_rows` key rows by 128 bytes (D and zeros behind it).
+int attn_cache_map8(CUtensorMap* m, const void* base, const ftb_attn_args& a,
+                    const int64_t (&strides)[3], uint32_t box_rows);
 // Query rows of one kv head: boxes of `tokens` tokens x `group` heads x 64 elements.
 int attn_q_map(CUtensorMap* m, const ftb_attn_args& a, uint32_t group, uint32_t tokens);
 
-int launch_attn_stream(const ftb_attn_args& a, AttnParams P, cudaStream_t stream);
+// (fp8: the cache is one of bytes, with the scales in P)
+int launch_attn_stream(const ftb_attn_args& a, AttnParams P, bool fp8, cudaStream_t stream);
 size_t attn_stream_partial_bytes(int64_t rows_max, int D);
 bool attn_chunk_fits(const ftb_attn_args& a);  // its plan's batch and piece counts
 int launch_attn_chunk(const ftb_attn_args& a, AttnParams P, cudaStream_t stream);
@@ -87,6 +95,22 @@ __device__ __forceinline__ float2 unpack2(uint32_t v) {
     return __half22float2(*reinterpret_cast<const __half2*>(&v));
   else
     return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+
+// Scales of an 8-bit cache, kept within limits: what the kernels use of a block that holds garbage, and
+// what makes the softmax's exponents below safe.
+//   With t_j = log2(e) scale q.k_j + log2(vs_j), vs_j the scale of V: P'_j = 2^(t_j - M) is the weight of
+//   the code of v_j, so no scale is left outside, P' <= 1 for M the largest t, and
+//   out = sum P'_j c_j / l,  l = sum P'_j / vs_j,  lse = M + log2(l).
+//   P' and 1 / vs stay normal numbers wherever they matter: scales 2^80 apart at most.
+constexpr float kMaxScale = 0x1p40f, kMinScale = 0x1p-40f;
+struct BlockScale {
+  float k, v_log2, v_inv;  // scale of K; log2 and reciprocal of the scale of V
+};
+__device__ __forceinline__ BlockScale block_scale(float k, float v) {
+  k = fminf(fmaxf(k, kMinScale), kMaxScale);  // (NaN: the smallest)
+  v = fminf(fmaxf(v, kMinScale), kMaxScale);
+  return BlockScale{k, log2f(v), 1.f / v};
 }
 
 // One sequence as the kernels see it: clamped, so that no length or offset a caller passes can

@@ -41,11 +41,13 @@ constexpr int kRows = 16;
 constexpr int kMergeCols = 32, kMergePitch = kMergeCols + 8;  // pitch: 8 rows hit 32 banks
 constexpr int kCtasPerSm = 2;
 
-constexpr int stream_stages(int DP) { return DP == 128 ? 3 : 6; }
-template <int DP>
+constexpr int stream_stages(int DP, bool C8) { return DP == 128 && !C8 ? 3 : 6; }
+// C8: the cache is one of bytes. Its rows take 128 bytes whatever D is.
+template <int DP, bool C8>
 struct StreamSmem {
-  static constexpr int kStages = stream_stages(DP);
-  alignas(1024) uint8_t ring[kStages][2][kTile * DP * 2];
+  static constexpr int kStages = stream_stages(DP, C8);
+  alignas(1024) uint8_t ring[kStages][2][kTile * (C8 ? 128 : DP * 2)];
+  BlockScale scale[C8 ? kStages : 1][kConsumers];  // of each 16 keys of a tile
   alignas(16) float merge[kConsumers][kRows][kMergePitch];
   float ml[kConsumers][kRows][2];
   float fac[kConsumers][kRows];  // weight of each warp's part of a row
@@ -141,9 +143,9 @@ struct Walk {
   }
 };
 
-template <int DP>
+template <int DP, bool C8>
 struct StreamSync {
-  StreamSmem<DP>* sh;
+  StreamSmem<DP, C8>* sh;
   uint32_t* status;
   __device__ bool wait(uint64_t* bar, uint32_t parity) const {
     if (mbar_try_wait(bar, parity)) return true;
@@ -161,11 +163,11 @@ struct StreamSync {
 
 // One warp. Copies the tiles of the share into the ring.
 template <int DP>
-__device__ void stream_producer(const AttnParams& P, const AttnMaps& M, StreamSmem<DP>* sh,
+__device__ void stream_producer(const AttnParams& P, const AttnMaps& M, StreamSmem<DP, false>* sh,
                                 Walk w, int row0) {
-  constexpr int kStages = StreamSmem<DP>::kStages;
+  constexpr int kStages = StreamSmem<DP, false>::kStages;
   const int lane = threadIdx.x & 31;
-  const StreamSync<DP> sy{sh, P.status};
+  const StreamSync<DP, false> sy{sh, P.status};
   const int page = 1 << P.page_log2;
   const int r = page < kTile ? page : kTile;  // keys per box
   const int boxes = kTile / r;                // <= 8
@@ -224,13 +226,144 @@ __device__ void stream_producer(const AttnParams& P, const AttnMaps& M, StreamSm
       if (mbar_try_wait(&sh->full[u % kStages], (u / kStages) & 1u)) break;
 }
 
+// The same for a cache of bytes. Lanes 0..3 also bring the scales of the tile's 4 x 16 keys (a block of
+// tokens is 16 keys or more), while the tile's copies are on their way.
+template <int DP>
+__device__ void stream_producer8(const AttnParams& P, const AttnMaps& M, StreamSmem<DP, true>* sh,
+                                 Walk w, int row0) {
+  constexpr int kStages = StreamSmem<DP, true>::kStages;
+  const int lane = threadIdx.x & 31;
+  const StreamSync<DP, true> sy{sh, P.status};
+  const int page = 1 << P.page_log2;
+  const int r = page < kTile ? page : kTile;  // keys per box, >= 16
+  const int boxes = kTile / r;                // <= 4
+  int stage = 0;
+  uint32_t parity = 1, issued = 0;
+  bool ok = true;
+  while (w.left > 0 && ok) {
+    const int n = w.take();
+    for (int j = 0; j < n && ok; ++j) {
+      const int key0 = (w.tile + j) * kTile;
+      // boxes with a key in [lo, hi)
+      const int b0 = w.t.lo > key0 ? (w.t.lo - key0) / r : 0;
+      int b1 = (w.t.hi - key0 + r - 1) / r;
+      if (b1 > boxes) b1 = boxes;
+      int id = 0;  // page of keys 16 lane ..
+      const int key = key0 + lane * 16, box_of = lane * 16 / r;
+      const bool has = lane < kTile / 16 && box_of >= b0 && box_of < b1;
+      if (has) {
+        id = P.block_table[(int64_t)w.seq * P.table_stride + (key >> P.page_log2)];
+        if (id < 0 || id >= P.num_pages) {
+          atomicOr(P.status, kAttnBadPage);
+          id = (int)P.num_pages;  // outside the tensor: reads zeros
+        }
+      }
+      const int box_id = __shfl_sync(0xffffffffu, id, (lane * r >> 4) & 3);
+      ok = __all_sync(0xffffffffu, sy.wait(&sh->empty[stage], parity));
+      if (!ok) break;
+      ++issued;
+      if (lane >= b0 && lane < b1) {
+        const uint32_t at = lane * r * 128;
+        const int row = (key0 + lane * r) & (page - 1);
+        tma_5d(smem_u32(sh->ring[stage][0]) + at, &M.k, 0, row, w.head, box_id, 0, &sh->full[stage]);
+        tma_5d(smem_u32(sh->ring[stage][1]) + at, &M.v, 0, row, w.head, box_id, 0, &sh->full[stage]);
+      }
+      if (lane < kTile / 16) {
+        float ks = 1.f, vs = 1.f;
+        if (has && id < P.num_pages) {
+          const int block = (key & (page - 1)) >> P.block_log2;
+          ks = __ldg(P.k_scale + id * P.ks_st[0] + block * P.ks_st[1] + w.head * P.ks_st[2]);
+          vs = __ldg(P.v_scale + id * P.vs_st[0] + block * P.vs_st[1] + w.head * P.vs_st[2]);
+        }
+        sh->scale[stage][lane] = block_scale(ks, vs);
+      }
+      __syncwarp();
+      // (the phase stays open for this arrival, whatever has landed by now)
+      if (lane == 0)
+        mbar_arrive_expect_tx(&sh->full[stage], 2u * (uint32_t)(b1 - b0) * (uint32_t)r * 128u);
+      __syncwarp();
+      if (++stage == kStages) stage = 0, parity ^= 1u;
+    }
+    w.next(P, row0, n);
+  }
+  for (uint32_t u = issued > kStages ? issued - kStages : 0; u < issued; ++u)  // as above
+    for (uint32_t i = 0; i < kSpinLimit; ++i)
+      if (mbar_try_wait(&sh->full[u % kStages], (u / kStages) & 1u)) break;
+}
+
+// The key of column n of an 8-key group, by which rows of 128 swizzled bytes are read without bank
+// conflicts: K's 16-byte chunks 4 to a row (columns 2i and 2i + 1 in opposite halves of the banks) and
+// V's chunks 2 to a row (columns 0, 2, 4, 6, and 1, 3, 5, 7, in different quarters).
+__device__ __forceinline__ int key_of(int n) { return n & 1 ? (n - 1) ^ 5 : n; }
+
+// One row's part of a query head as A fragments of f16: this lane's elements are 16 (lane % 4) .. + 15
+// of each 64, as K's bytes lie in a lane. bf16 rows whose largest element f16 would not hold with all
+// its bits are taken times a power of two (returned: its inverse).
 template <typename T, int DP>
-__device__ void stream_consumer(const AttnParams& P, StreamSmem<DP>* sh, Walk w, int row0,
+__device__ __forceinline__ float load_q8(const uint16_t* qp, bool in, int D, int e,
+                                         uint32_t (&qa)[DP / 16][4]) {
+  const int tig = threadIdx.x & 3;
+  uint4 w[DP / 64][2];
+#pragma unroll
+  for (int h = 0; h < DP / 64; ++h)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int d = h * 64 + tig * 16 + i * 8;
+      w[h][i] = in && d < D ? __ldg(reinterpret_cast<const uint4*>(qp + d)) : make_uint4(0, 0, 0, 0);
+    }
+  float back = 1.f, by = 1.f;
+  if constexpr (!std::is_same<T, __half>::value) {
+    uint32_t top = 0;  // largest |x| as bf16 bits, in the upper half
+#pragma unroll
+    for (int h = 0; h < DP / 64; ++h)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t v[4] = {w[h][i].x, w[h][i].y, w[h][i].z, w[h][i].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          top = max(top, max(v[k] << 16 & 0x7fff0000u, v[k] & 0x7fff0000u));
+      }
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const int ex = (int)(top >> 23) - 127;
+    if (top && ex < 128 && (ex < -4 || ex > 14)) {  // (infinite and NaN rows stay so)
+      const int x = ex > 14 ? ex - 14 : max(ex, -126);  // (both factors are normal numbers)
+      by = __uint_as_float((uint32_t)(127 - x) << 23);
+      back = __uint_as_float((uint32_t)(127 + x) << 23);
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < DP / 64; ++h)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint32_t v[4] = {w[h][i].x, w[h][i].y, w[h][i].z, w[h][i].w};
+      if constexpr (!std::is_same<T, __half>::value) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 f = unpack2<T>(v[k]);
+          v[k] = pack2<__half>(f.x * by, f.y * by);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; k += 2) {
+        const int c = h * 4 + i * 2 + (k >> 1);
+        qa[c][e] = v[k], qa[c][2 + e] = v[k + 1];
+      }
+    }
+  return back;
+}
+
+template <typename T, int DP, bool C8>
+__device__ void stream_consumer(const AttnParams& P, StreamSmem<DP, C8>* sh, Walk w, int row0,
                                 int64_t share) {
-  constexpr int kStages = StreamSmem<DP>::kStages;
+  constexpr int kStages = StreamSmem<DP, C8>::kStages;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t2 = (lane & 3) * 2;
-  const StreamSync<DP> sy{sh, P.status};
+  const StreamSync<DP, C8> sy{sh, P.status};
+  // P's type: the tensors', or f16 beside V's codes, which are f16 numbers. The rounding's rest goes
+  // along where the output is as fine as P.
+  using TP = typename std::conditional<C8, __half, T>::type;
+  constexpr bool kRest = std::is_same<TP, T>::value;
   const int page = 1 << P.page_log2;
   const int r = page < kTile ? page : kTile;
   const int half_bytes = r * 128, box_bytes = half_bytes * (DP / 64);
@@ -252,6 +385,7 @@ __device__ void stream_consumer(const AttnParams& P, StreamSmem<DP>* sh, Walk w,
     // this lane's rows: limits on their keys, and Q fragments
     uint32_t qa[DP / 16][4];
     int kmin[2], kmax[2];  // keys kmin <= j < kmax
+    float q_back[2] = {1.f, 1.f};  // C8: what q was taken times, the inverse
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int row = row0 + g + 8 * e;
@@ -263,11 +397,15 @@ __device__ void stream_consumer(const AttnParams& P, StreamSmem<DP>* sh, Walk w,
         kmin[e] = k.lo, kmax[e] = k.hi;
       }
       const uint16_t* qp = P.q + (int64_t)(s.q0 + i) * P.q_st + (int64_t)hq * P.q_sh;
+      if constexpr (C8) {
+        q_back[e] = load_q8<T, DP>(qp, in, P.D, e, qa);
+      } else {
 #pragma unroll
-      for (int c = 0; c < DP / 16; ++c) {
-        const int d = c * 16 + t2;
-        qa[c][e] = in && d < P.D ? *reinterpret_cast<const uint32_t*>(qp + d) : 0u;
-        qa[c][2 + e] = in && d + 8 < P.D ? *reinterpret_cast<const uint32_t*>(qp + d + 8) : 0u;
+        for (int c = 0; c < DP / 16; ++c) {
+          const int d = c * 16 + t2;
+          qa[c][e] = in && d < P.D ? *reinterpret_cast<const uint32_t*>(qp + d) : 0u;
+          qa[c][2 + e] = in && d + 8 < P.D ? *reinterpret_cast<const uint32_t*>(qp + d + 8) : 0u;
+        }
       }
     }
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
@@ -284,13 +422,32 @@ __device__ void stream_consumer(const AttnParams& P, StreamSmem<DP>* sh, Walk w,
       }
       const uint32_t kb = smem_u32(sh->ring[stage][0]), vb = smem_u32(sh->ring[stage][1]);
       float sc[2][4] = {};
+      BlockScale bs{1.f, 0.f, 1.f};
+      if constexpr (C8) {
+        bs = sh->scale[stage][warp];
 #pragma unroll
-      for (int c = 0; c < DP / 16; ++c) {
-        uint32_t b[4];
-        const int chunk = (2 * c + kc) & 7;
-        ldsm4(kb + k_off + (c >> 2) * half_bytes + ((chunk ^ k_sw) << 4), b);
-        mma16816<T>(sc[0], qa[c], b[0], b[1]);
-        mma16816<T>(sc[1], qa[c], b[2], b[3]);
+        for (int h = 0; h < 2; ++h) {
+          const int kr = warp * 16 + h * 8 + key_of(g);
+#pragma unroll
+          for (int c = 0; c < DP / 64; ++c) {
+            const uint4 b = *reinterpret_cast<const uint4*>(
+                sh->ring[stage][0] + kr * 128 + (((4 * c + (lane & 3)) ^ (kr & 7)) << 4));
+            const uint32_t v[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              mma16816<__half>(sc[h], qa[4 * c + k], e4m3x2_to_f16x2((uint16_t)(v[k] & 0xffffu)),
+                               e4m3x2_to_f16x2((uint16_t)(v[k] >> 16)));
+          }
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) {
+          uint32_t b[4];
+          const int chunk = (2 * c + kc) & 7;
+          ldsm4(kb + k_off + (c >> 2) * half_bytes + ((chunk ^ k_sw) << 4), b);
+          mma16816<T>(sc[0], qa[c], b[0], b[1]);
+          mma16816<T>(sc[1], qa[c], b[2], b[3]);
+        }
       }
       // a warp's 16 keys, all seen by all of the tile's rows, need no mask
       const bool clean = key0 >= w.t.lo && key0 + 16 <= w.t.hi && (!P.causal || s.n == 1) &&
@@ -299,9 +456,12 @@ __device__ void stream_consumer(const AttnParams& P, StreamSmem<DP>* sh, Walk w,
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int key = key0 + h * 8 + t2 + (i & 1);
+          const int key = key0 + h * 8 + (C8 ? key_of(t2 + (i & 1)) : t2 + (i & 1));
           const bool seen = clean || (key >= kmin[i >> 1] && key < kmax[i >> 1]);
-          sc[h][i] = seen ? sc[h][i] * P.scale_log2 : -INFINITY;
+          const float score =
+              C8 ? fmaf(sc[h][i], bs.k * (P.scale_log2 * q_back[i >> 1]), bs.v_log2)
+                 : sc[h][i] * P.scale_log2;
+          sc[h][i] = seen ? score : -INFINITY;
         }
       uint32_t pa[4], pr[4];  // P rounded to the operand's type, and what the rounding left
 #pragma unroll
@@ -315,12 +475,15 @@ __device__ void stream_consumer(const AttnParams& P, StreamSmem<DP>* sh, Walk w,
         m[e] = mn;
         float p0 = ex2(sc[0][2 * e] - ref), p1 = ex2(sc[0][2 * e + 1] - ref);
         float p2 = ex2(sc[1][2 * e] - ref), p3 = ex2(sc[1][2 * e + 1] - ref);
-        l[e] = l[e] * f + ((p0 + p1) + (p2 + p3));
-        pa[e] = pack2<T>(p0, p1);
-        pa[2 + e] = pack2<T>(p2, p3);
-        const float2 a = unpack2<T>(pa[e]), b = unpack2<T>(pa[2 + e]);
-        pr[e] = pack2<T>(p0 - a.x, p1 - a.y);
-        pr[2 + e] = pack2<T>(p2 - b.x, p3 - b.y);
+        l[e] = C8 ? fmaf((p0 + p1) + (p2 + p3), bs.v_inv, l[e] * f)
+                  : l[e] * f + ((p0 + p1) + (p2 + p3));
+        pa[e] = pack2<TP>(p0, p1);
+        pa[2 + e] = pack2<TP>(p2, p3);
+        if constexpr (kRest) {
+          const float2 a = unpack2<TP>(pa[e]), b = unpack2<TP>(pa[2 + e]);
+          pr[e] = pack2<TP>(p0 - a.x, p1 - a.y);
+          pr[2 + e] = pack2<TP>(p2 - b.x, p3 - b.y);
+        }
         if (__any_sync(0xffffffffu, f != 1.f)) {
 #pragma unroll
           for (int jj = 0; jj < DP / 8; ++jj) o[jj][2 * e] *= f, o[jj][2 * e + 1] *= f;
@@ -328,25 +491,69 @@ __device__ void stream_consumer(const AttnParams& P, StreamSmem<DP>* sh, Walk w,
       }
       // V rows outside [lo, hi) have weight 0 but may hold NaN or infinity: made zero
       const bool inside = key0 >= w.t.lo && key0 + 16 <= w.t.hi;
-      uint32_t mk[2] = {0xffffffffu, 0xffffffffu};
-      if (!inside) {
+      if constexpr (C8) {
+        constexpr int VB = DP / 8;  // columns of O: VB (lane / 4) .. of V, VB n .. of the result
+        uint32_t v[2][2][VB / 4];   // [key group][column's parity][bytes]
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int key = key0 + h * 8 + t2;
-          mk[h] = (key >= w.t.lo && key < w.t.hi ? 0xffffu : 0u) |
-                  (key + 1 >= w.t.lo && key + 1 < w.t.hi ? 0xffff0000u : 0u);
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int kr = warp * 16 + h * 8 + key_of(t2 + e);
+            const int byte = g * VB;
+            const uint8_t* at = sh->ring[stage][1] + kr * 128 + (((byte >> 4) ^ (kr & 7)) << 4) + (byte & 15);
+            if constexpr (VB == 16) {
+              const uint4 b = *reinterpret_cast<const uint4*>(at);
+              v[h][e][0] = b.x, v[h][e][1] = b.y, v[h][e][2] = b.z, v[h][e][3] = b.w;
+            } else {
+              const uint2 b = *reinterpret_cast<const uint2*>(at);
+              v[h][e][0] = b.x, v[h][e][1] = b.y;
+            }
+            const int key = key0 - warp * 16 + kr;
+            if (!inside && (key < w.t.lo || key >= w.t.hi)) {
+#pragma unroll
+              for (int k = 0; k < VB / 4; ++k) v[h][e][k] = 0u;
+            }
+          }
+#pragma unroll
+        for (int k = 0; k < VB / 4; ++k) {
+          // bytes of two keys side by side, two columns to a word
+          uint32_t x[2][2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            x[h][0] = __byte_perm(v[h][0][k], v[h][1][k], 0x5140);
+            x[h][1] = __byte_perm(v[h][0][k], v[h][1][k], 0x7362);
+          }
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t b[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              b[h] = e4m3x2_to_f16x2((uint16_t)(c & 1 ? x[h][c >> 1] >> 16 : x[h][c >> 1] & 0xffffu));
+            mma16816<TP>(o[4 * k + c], pa, b[0], b[1]);
+            if constexpr (kRest) mma16816<TP>(o[4 * k + c], pr, b[0], b[1]);
+          }
         }
-      }
+      } else {
+        uint32_t mk[2] = {0xffffffffu, 0xffffffffu};
+        if (!inside) {
 #pragma unroll
-      for (int c = 0; c < DP / 16; ++c) {
-        uint32_t b[4];
-        const int chunk = (2 * c + vc) & 7;
-        ldsm4_t(vb + v_off + (c >> 2) * half_bytes + ((chunk ^ v_sw) << 4), b);
-        if (!inside) b[0] &= mk[0], b[1] &= mk[1], b[2] &= mk[0], b[3] &= mk[1];
-        mma16816<T>(o[2 * c], pa, b[0], b[1]);
-        mma16816<T>(o[2 * c + 1], pa, b[2], b[3]);
-        mma16816<T>(o[2 * c], pr, b[0], b[1]);
-        mma16816<T>(o[2 * c + 1], pr, b[2], b[3]);
+          for (int h = 0; h < 2; ++h) {
+            const int key = key0 + h * 8 + t2;
+            mk[h] = (key >= w.t.lo && key < w.t.hi ? 0xffffu : 0u) |
+                    (key + 1 >= w.t.lo && key + 1 < w.t.hi ? 0xffff0000u : 0u);
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) {
+          uint32_t b[4];
+          const int chunk = (2 * c + vc) & 7;
+          ldsm4_t(vb + v_off + (c >> 2) * half_bytes + ((chunk ^ v_sw) << 4), b);
+          if (!inside) b[0] &= mk[0], b[1] &= mk[1], b[2] &= mk[0], b[3] &= mk[1];
+          mma16816<T>(o[2 * c], pa, b[0], b[1]);
+          mma16816<T>(o[2 * c + 1], pa, b[2], b[3]);
+          mma16816<T>(o[2 * c], pr, b[0], b[1]);
+          mma16816<T>(o[2 * c + 1], pr, b[2], b[3]);
+        }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->empty[stage]);
@@ -387,13 +594,27 @@ __device__ void stream_consumer(const AttnParams& P, StreamSmem<DP>* sh, Walk w,
     float* slot = P.partial + (2 * blk + (begins ? 1 : 0)) * kSlot;
     const float f0 = sh->fac[warp][g], f1 = sh->fac[warp][g + 8];
     const int orow = threadIdx.x >> 3, oc = (threadIdx.x & 7) * 4;  // 16 rows x 8 threads x 4
+    // column of chunk c of 32 that this thread joins: C8's lanes hold DP / 8 columns in a row
+    auto col_of = [&](int c) { return C8 ? (int)(threadIdx.x & 7) * (DP / 8) + 4 * c : c * kMergeCols + oc; };
 #pragma unroll
     for (int c = 0; c < DP / kMergeCols; ++c) {
+      if constexpr (C8) {
 #pragma unroll
-      for (int jj = 0; jj < kMergeCols / 8; ++jj) {
-        const float(&v)[4] = o[c * (kMergeCols / 8) + jj];
-        *reinterpret_cast<float2*>(&sh->merge[warp][g][jj * 8 + t2]) = make_float2(v[0] * f0, v[1] * f0);
-        *reinterpret_cast<float2*>(&sh->merge[warp][g + 8][jj * 8 + t2]) = make_float2(v[2] * f1, v[3] * f1);
+        for (int e = 0; e < 2; ++e) {
+          const float(&v0)[4] = o[4 * c], (&v1)[4] = o[4 * c + 1], (&v2)[4] = o[4 * c + 2],
+                     (&v3)[4] = o[4 * c + 3];
+          *reinterpret_cast<float4*>(&sh->merge[warp][g][t2 * 4 + e * 4]) =
+              make_float4(v0[e] * f0, v1[e] * f0, v2[e] * f0, v3[e] * f0);
+          *reinterpret_cast<float4*>(&sh->merge[warp][g + 8][t2 * 4 + e * 4]) =
+              make_float4(v0[2 + e] * f1, v1[2 + e] * f1, v2[2 + e] * f1, v3[2 + e] * f1);
+        }
+      } else {
+#pragma unroll
+        for (int jj = 0; jj < kMergeCols / 8; ++jj) {
+          const float(&v)[4] = o[c * (kMergeCols / 8) + jj];
+          *reinterpret_cast<float2*>(&sh->merge[warp][g][jj * 8 + t2]) = make_float2(v[0] * f0, v[1] * f0);
+          *reinterpret_cast<float2*>(&sh->merge[warp][g + 8][jj * 8 + t2]) = make_float2(v[2] * f1, v[3] * f1);
+        }
       }
       named_bar(1, kConsumers * kWarp);
       float4 a = *reinterpret_cast<float4*>(&sh->merge[0][orow][oc]);
@@ -402,7 +623,7 @@ __device__ void stream_consumer(const AttnParams& P, StreamSmem<DP>* sh, Walk w,
         const float4 b = *reinterpret_cast<float4*>(&sh->merge[i][orow][oc]);
         a.x += b.x, a.y += b.y, a.z += b.z, a.w += b.w;
       }
-      const int d = c * kMergeCols + oc;
+      const int d = col_of(c);
       if (orow < rows) {
         if (!whole) {
           *reinterpret_cast<float4*>(slot + orow * DP + d) = a;
@@ -471,7 +692,7 @@ __device__ void stream_consumer(const AttnParams& P, StreamSmem<DP>* sh, Walk w,
             ll += f * __ldcg(p + kRows * DP + kRows + jrow);
 #pragma unroll
             for (int c = 0; c < DP / kMergeCols; ++c)
-              add(f, __ldcg(reinterpret_cast<const float4*>(p + jrow * DP + c * kMergeCols + oc)), c);
+              add(f, __ldcg(reinterpret_cast<const float4*>(p + jrow * DP + col_of(c))), c);
           }
         }
         if (ways > 1) {
@@ -479,7 +700,7 @@ __device__ void stream_consumer(const AttnParams& P, StreamSmem<DP>* sh, Walk w,
           float* all = &sh->merge[0][0][0];
 #pragma unroll
           for (int c = 0; c < DP / kMergeCols; ++c)
-            *reinterpret_cast<float4*>(all + orow * DP + c * kMergeCols + oc) = acc[c];
+            *reinterpret_cast<float4*>(all + orow * DP + col_of(c)) = acc[c];
           if (oc == 0) sh->ml[0][orow][0] = mm, sh->ml[0][orow][1] = ll;
           named_bar(1, kConsumers * kWarp);
           if (mine && way == 0) {
@@ -494,7 +715,7 @@ __device__ void stream_consumer(const AttnParams& P, StreamSmem<DP>* sh, Walk w,
               ll += f * sh->ml[0][at][1];
 #pragma unroll
               for (int c = 0; c < DP / kMergeCols; ++c)
-                add(f, *reinterpret_cast<const float4*>(all + at * DP + c * kMergeCols + oc), c);
+                add(f, *reinterpret_cast<const float4*>(all + at * DP + col_of(c)), c);
             }
           }
           named_bar(1, kConsumers * kWarp);  // (the next pair writes the merge buffer)
@@ -505,7 +726,7 @@ __device__ void stream_consumer(const AttnParams& P, StreamSmem<DP>* sh, Walk w,
           const int64_t at = (int64_t)(s.q0 + row / P.G) * P.Hq + w.head * P.G + row % P.G;
 #pragma unroll
           for (int c = 0; c < DP / kMergeCols; ++c) {
-            const int d = c * kMergeCols + oc;
+            const int d = col_of(c);
             if (d < P.D)
               *reinterpret_cast<uint2*>(P.out + at * P.D + d) = make_uint2(
                   pack2<T>(acc[c].x * inv, acc[c].y * inv), pack2<T>(acc[c].z * inv, acc[c].w * inv));
@@ -519,17 +740,17 @@ __device__ void stream_consumer(const AttnParams& P, StreamSmem<DP>* sh, Walk w,
   }
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool C8>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     k_attn_stream(const __grid_constant__ AttnMaps M, const __grid_constant__ AttnParams P) {
   extern __shared__ uint8_t smem_raw[];
-  StreamSmem<DP>* sh = reinterpret_cast<StreamSmem<DP>*>(
+  StreamSmem<DP, C8>* sh = reinterpret_cast<StreamSmem<DP, C8>*>(
       smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int row0 = blockIdx.y * kRows;
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
-    for (int i = 0; i < StreamSmem<DP>::kStages; ++i) {
+    for (int i = 0; i < StreamSmem<DP, C8>::kStages; ++i) {
       mbar_init(&sh->full[i], 1);
       mbar_init(&sh->empty[i], kConsumers);
     }
@@ -603,20 +824,24 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   const int64_t count = total - at < share ? total - at : share;
   Walk w;
   w.start(P, row0, sh->start_seq, sh->start_item, at, count);
-  if (warp == kConsumers)
-    stream_producer<DP>(P, M, sh, w, row0);
-  else
-    stream_consumer<T, DP>(P, sh, w, row0, share);
+  if (warp == kConsumers) {
+    if constexpr (C8)
+      stream_producer8<DP>(P, M, sh, w, row0);
+    else
+      stream_producer<DP>(P, M, sh, w, row0);
+  } else {
+    stream_consumer<T, DP, C8>(P, sh, w, row0, share);
+  }
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool C8>
 int run_stream(const AttnMaps& M, const AttnParams& P, dim3 grid, cudaStream_t stream) {
-  constexpr size_t smem = sizeof(StreamSmem<DP>) + 1024;
+  constexpr size_t smem = sizeof(StreamSmem<DP, C8>) + 1024;
   static_assert(smem <= 113 * 1024, "two blocks per SM");
   static std::atomic<uint64_t> done{0};
-  cudaError_t err = allow_smem(k_attn_stream<T, DP>, smem, done);
+  cudaError_t err = allow_smem(k_attn_stream<T, DP, C8>, smem, done);
   if (err != cudaSuccess) return cuda_status(err);
-  return cuda_status(launch_pdl(k_attn_stream<T, DP>, grid, dim3(kThreads), smem, stream, M, P));
+  return cuda_status(launch_pdl(k_attn_stream<T, DP, C8>, grid, dim3(kThreads), smem, stream, M, P));
 }
 
 // Blocks per row tile: two per SM over all row tiles, at least one.
@@ -636,24 +861,34 @@ size_t attn_stream_partial_bytes(int64_t rows_max, int D) {
   return (size_t)(tiles * w) * 2 * (kRows * dp + 2 * kRows) * sizeof(float);
 }
 
-int launch_attn_stream(const ftb_attn_args& a, AttnParams P, cudaStream_t stream) {
+template <bool C8>
+int pick_stream(const ftb_attn_args& a, const AttnMaps& M, const AttnParams& P, int dp, dim3 grid,
+                cudaStream_t stream) {
+  if (a.type == FTB_TYPE_BF16)
+    return dp == 64 ? run_stream<__nv_bfloat16, 64, C8>(M, P, grid, stream)
+                    : run_stream<__nv_bfloat16, 128, C8>(M, P, grid, stream);
+  return dp == 64 ? run_stream<__half, 64, C8>(M, P, grid, stream)
+                  : run_stream<__half, 128, C8>(M, P, grid, stream);
+}
+
+int launch_attn_stream(const ftb_attn_args& a, AttnParams P, bool fp8, cudaStream_t stream) {
   AttnMaps M;
   const uint32_t r = a.page < kTile ? a.page : kTile;
   const int dp = a.D <= 64 ? 64 : 128;
   const uint32_t halves = a.D == dp ? dp / 64 : 1;
-  int st = attn_cache_map(&M.k, a.k_cache, a, a.k_strides, r, halves);
-  if (!st) st = attn_cache_map(&M.v, a.v_cache, a, a.v_strides, r, halves);
+  int st = fp8 ? attn_cache_map8(&M.k, a.k_cache, a, a.k_strides, r)
+               : attn_cache_map(&M.k, a.k_cache, a, a.k_strides, r, halves);
+  if (!st)
+    st = fp8 ? attn_cache_map8(&M.v, a.v_cache, a, a.v_strides, r)
+             : attn_cache_map(&M.v, a.v_cache, a, a.v_strides, r, halves);
   if (st) return st;
   M.q = M.k;  // unused
   const int64_t tiles = ceil_div((int64_t)a.max_q * P.G, kRows);
   const int64_t w = stream_blocks(tiles);
   if (tiles > 65535 || (w > 1 && tiles * w > kAttnCounters)) return FTB_ERR_SHAPE;
   const dim3 grid((unsigned)w, (unsigned)tiles);
-  if (a.type == FTB_TYPE_BF16)
-    return dp == 64 ? run_stream<__nv_bfloat16, 64>(M, P, grid, stream)
-                    : run_stream<__nv_bfloat16, 128>(M, P, grid, stream);
-  return dp == 64 ? run_stream<__half, 64>(M, P, grid, stream)
-                  : run_stream<__half, 128>(M, P, grid, stream);
+  return fp8 ? pick_stream<true>(a, M, P, dp, grid, stream)
+             : pick_stream<false>(a, M, P, dp, grid, stream);
 }
 
 }  // namespace ftb

@@ -1,0 +1,129 @@
+// pages.cu - copies of whole pages of a set of caches that share their page ids (the keys, values and
+// scales of every layer), as forking a sequence and compacting a cache need them.
+//
+// Pair i copies page src[i] of every cache to page dst[i]; a pair with an id outside [0, num_pages),
+// or twice the same, copies nothing. One launch for all caches: a cache's pairs are cut into pieces of
+// kPiece bytes, or several small pages to a piece, and all caches' pieces are one line of thread
+// blocks. Every load of a piece is issued before its first store.
+//
+// Bound: DRAM, every byte read once and written once.
+#include "ftb_common.cuh"
+
+namespace ftb {
+namespace {
+
+constexpr int kThreads = 256, kLoads = 4;
+constexpr int kPiece = kThreads * kLoads * 16;
+
+struct PagesParams {
+  struct Cache {
+    char* base;
+    int64_t stride, bytes;  // of a page
+    int first;              // its first piece
+    int per_page;           // pieces per page; 0: several pages per piece
+    int pages;              // pages per piece
+    int vec;                // bytes per access
+  } cache[FTB_PAGES_MAX];
+  const void *src, *dst;
+  int64_t n, num_pages;
+  int caches, id64;
+};
+
+template <typename V>
+__device__ __forceinline__ void copy_piece(const PagesParams& P, const PagesParams::Cache& c,
+                                           int piece) {
+  const int64_t page_vecs = c.bytes / (int64_t)sizeof(V);
+  constexpr int kVecs = kPiece / sizeof(V);
+  auto id = [&](const void* ids, int64_t i) {
+    return P.id64 ? static_cast<const int64_t*>(ids)[i] : static_cast<const int32_t*>(ids)[i];
+  };
+  auto good = [&](int64_t s, int64_t d) {
+    return s >= 0 && s < P.num_pages && d >= 0 && d < P.num_pages && s != d;
+  };
+  if (c.per_page) {
+    const int64_t i = piece / c.per_page;
+    const int64_t s = id(P.src, i), d = id(P.dst, i);
+    if (!good(s, d)) return;
+    const int64_t v0 = (int64_t)(piece - i * c.per_page) * kVecs;
+    const int count = (int)(page_vecs - v0 < kVecs ? page_vecs - v0 : kVecs);
+    const V* from = reinterpret_cast<const V*>(c.base + s * c.stride) + v0;
+    V* to = reinterpret_cast<V*>(c.base + d * c.stride) + v0;
+    for (int v = threadIdx.x; v < count; v += kThreads * kLoads) {
+      V x[kLoads];
+#pragma unroll
+      for (int k = 0; k < kLoads; ++k)
+        if (v + k * kThreads < count) x[k] = from[v + k * kThreads];
+#pragma unroll
+      for (int k = 0; k < kLoads; ++k)
+        if (v + k * kThreads < count) to[v + k * kThreads] = x[k];
+    }
+    return;
+  }
+  const int64_t i0 = (int64_t)piece * c.pages;
+  const int pages = (int)(P.n - i0 < c.pages ? P.n - i0 : c.pages), vecs = (int)page_vecs;
+  for (int v = threadIdx.x; v < pages * vecs; v += kThreads) {
+    const int p = v / vecs;
+    const int64_t s = id(P.src, i0 + p), d = id(P.dst, i0 + p);
+    if (!good(s, d)) continue;
+    const int64_t at = (int64_t)(v - p * vecs) * sizeof(V);
+    *reinterpret_cast<V*>(c.base + d * c.stride + at) =
+        *reinterpret_cast<const V*>(c.base + s * c.stride + at);
+  }
+}
+
+__global__ void __launch_bounds__(kThreads) k_copy_pages(const __grid_constant__ PagesParams P) {
+  pdl_launch_dependents();
+  int a = 0;
+  while (a + 1 < P.caches && (int)blockIdx.x >= P.cache[a + 1].first) ++a;
+  const PagesParams::Cache& c = P.cache[a];
+  const int piece = (int)blockIdx.x - c.first;
+  pdl_wait();
+  if (c.vec == 16)
+    copy_piece<uint4>(P, c, piece);
+  else if (c.vec == 4)
+    copy_piece<uint32_t>(P, c, piece);
+  else
+    copy_piece<uint8_t>(P, c, piece);
+}
+
+}  // namespace
+}  // namespace ftb
+
+using namespace ftb;
+
+extern "C" int ftb_copy_pages(const ftb_pages_args* a, ftb_stream_t stream) {
+  if (!a) return FTB_ERR_ARG;
+  if (a->n < 0 || a->num_pages < 0 || a->n_caches < 0 || a->n_caches > FTB_PAGES_MAX)
+    return FTB_ERR_SHAPE;
+  if (a->n == 0 || a->n_caches == 0 || a->num_pages == 0) return FTB_OK;
+  if (!a->src || !a->dst) return FTB_ERR_ARG;
+  PagesParams P{};
+  P.src = a->src, P.dst = a->dst, P.n = a->n, P.num_pages = a->num_pages, P.id64 = a->id64;
+  int64_t pieces = 0;
+  for (int i = 0; i < a->n_caches; ++i) {
+    if (a->page_bytes[i] < 0 || a->page_strides[i] < 0) return FTB_ERR_SHAPE;
+    if (a->page_bytes[i] == 0) continue;
+    if (!a->caches[i]) return FTB_ERR_ARG;
+    // pages that overlap are no pages
+    if (a->num_pages > 1 && a->page_strides[i] < a->page_bytes[i]) return FTB_ERR_SHAPE;
+    PagesParams::Cache& c = P.cache[P.caches++];
+    c.base = static_cast<char*>(a->caches[i]);
+    c.stride = a->page_strides[i], c.bytes = a->page_bytes[i];
+    const uint64_t m = reinterpret_cast<uintptr_t>(c.base) | (uint64_t)c.stride | (uint64_t)c.bytes;
+    c.vec = m % 16 == 0 ? 16 : m % 4 == 0 ? 4 : 1;
+    c.first = (int)pieces;
+    if (c.bytes > kPiece / 2) {
+      const int64_t per = ceil_div(c.bytes, kPiece);
+      if (per > 0x7fffffff) return FTB_ERR_SHAPE;
+      c.per_page = (int)per;
+      pieces += a->n > 0x7fffffff / per ? (int64_t)0x7fffffff : a->n * per;
+    } else {
+      c.pages = (int)(kPiece / c.bytes);
+      pieces += ceil_div(a->n, c.pages);
+    }
+    if (pieces > 0x7ffffff0) return FTB_ERR_SHAPE;
+  }
+  if (P.caches == 0) return FTB_OK;
+  return cuda_status(launch_pdl(k_copy_pages, dim3((unsigned)pieces), dim3(kThreads), 0,
+                                (cudaStream_t)stream, P));
+}

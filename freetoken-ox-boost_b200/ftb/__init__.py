@@ -16,6 +16,7 @@ from .experts import B200Nvfp4Experts, Nvfp4MoELayer, select_nvfp4_backend
 from .fused_nvfp4 import (fused_experts_decode_nvfp4_marlin, fused_experts_decode_nvfp4_split,
                           fused_experts_nvfp4, moe_align_block_size, moe_decode, moe_prefill,
                           moe_prefill_fp4, quant_nvfp4)
+from .pages import PagePool, copy_pages
 from .fused_route import fused_route, fused_route_ranked, fused_topk, router_logits
 
 __all__ = [
@@ -26,5 +27,6 @@ __all__ = [
     "fused_route", "fused_route_ranked", "fused_topk", "router_logits",
     "bank_from_modelopt", "bank_to_modelopt", "moe_layers_in", "EpGroup", "ExpertParallelMoE",
     "AttnStep", "DecoderLayer", "PagedKvCache", "paged_attention", "block_norm", "rms_norm", "rope", "rope_append", "rope_table",
+    "PagePool", "copy_pages",
     "DsFp4Bank", "fused_experts_ds_fp4", "nvfp4_from_ds_fp4",
 ]

@@ -108,6 +108,27 @@ class RopeArgsStruct(ctypes.Structure):
     ]
 
 
+class RopeFp8ArgsStruct(ctypes.Structure):
+    """``ftb_rope_fp8_args``"""
+    _fields_ = [
+        ("rope", RopeArgsStruct), ("k_scale", _vp), ("v_scale", _vp), ("k_scale_strides", _i64 * 3),
+        ("v_scale_strides", _i64 * 3), ("workspace", _vp), ("workspace_bytes", _sz),
+        ("scale_block", _i32),
+    ]
+
+
+FTB_PAGES_MAX = 32
+
+
+class PagesArgsStruct(ctypes.Structure):
+    """``ftb_pages_args``"""
+    _fields_ = [
+        ("caches", _vp * FTB_PAGES_MAX), ("src", _vp), ("dst", _vp),
+        ("page_strides", _i64 * FTB_PAGES_MAX), ("page_bytes", _i64 * FTB_PAGES_MAX), ("n", _i64),
+        ("num_pages", _i64), ("n_caches", _i32), ("id64", _i32),
+    ]
+
+
 class AttnArgsStruct(ctypes.Structure):
     """``ftb_attn_args``"""
     _fields_ = [
@@ -117,6 +138,14 @@ class AttnArgsStruct(ctypes.Structure):
         ("total_q", _i64), ("num_pages", _i64), ("table_stride", _i64), ("batch", _i32),
         ("max_q", _i32), ("table_width", _i32), ("page", _i32), ("Hq", _i32), ("Hkv", _i32),
         ("D", _i32), ("causal", _i32), ("window", _i32), ("type", _i32), ("scale", _f32),
+    ]
+
+
+class AttnFp8ArgsStruct(ctypes.Structure):
+    """``ftb_attn_fp8_args``"""
+    _fields_ = [
+        ("attn", AttnArgsStruct), ("k_scale", _vp), ("v_scale", _vp), ("k_scale_strides", _i64 * 3),
+        ("v_scale_strides", _i64 * 3), ("scale_block", _i32),
     ]
 
 
@@ -167,6 +196,10 @@ SIGNATURES = {
     "ftb_rope": (_i32, [ctypes.POINTER(RopeArgsStruct), _vp]),
     "ftb_attention_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32, _i32, _i32]),
     "ftb_attention": (_i32, [ctypes.POINTER(AttnArgsStruct), _vp]),
+    "ftb_attention_fp8": (_i32, [ctypes.POINTER(AttnFp8ArgsStruct), _vp]),
+    "ftb_rope_fp8_workspace_bytes": (_sz, [_i64, _i64]),
+    "ftb_rope_fp8": (_i32, [ctypes.POINTER(RopeFp8ArgsStruct), _vp]),
+    "ftb_copy_pages": (_i32, [ctypes.POINTER(PagesArgsStruct), _vp]),
     "ftb_profile_begin": (_i32, []),
     "ftb_profile_end": (_i32, [_vp, _vp, _i32]),
 }

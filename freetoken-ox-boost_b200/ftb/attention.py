@@ -6,10 +6,12 @@ import torch
 from . import _lib
 from ._runtime import (_ARGS, _pycall, caller, read_status, remember, require_cuda, stream_handle,
                        zeroed_workspace)
-from .block import _TYPE
+from .block import _TYPE, FP8, scale_block
 
 _POINTERS = _lib.offsets(_lib.AttnArgsStruct, "q", "k_cache", "v_cache", "block_table", "kv_len",
                          "cu_q", "out", "lse", "workspace")
+# (the plain call's arguments are the first member)
+_FP8_POINTERS = _POINTERS + _lib.offsets(_lib.AttnFp8ArgsStruct, "k_scale", "v_scale")
 
 
 def _int32(t, name, shape, dev):
@@ -19,18 +21,21 @@ def _int32(t, name, shape, dev):
                          f"{shape} on {dev} with contiguous rows")
 
 
-def _args(q, k_cache, v_cache, block_table, kv_len, cu_q, max_q, scale, causal, window):
+def _args(q, k_cache, v_cache, block_table, kv_len, cu_q, max_q, scale, causal, window,
+          k_scale=None, v_scale=None):
     """The checks of a call, and its arguments without the pointers."""
     dev = require_cuda(q)
+    fp8 = k_scale is not None or v_scale is not None
+    cache_dtype = FP8 if fp8 else q.dtype
     if q.dim() != 3 or q.dtype not in _TYPE or q.stride(2) != 1:
         raise ValueError(f"q: {tuple(q.shape)} {q.dtype}, expected [total, heads, D] bf16 or f16 "
                          "with contiguous heads")
     total, Hq, D = q.shape
     for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if c.dim() != 4 or c.dtype != q.dtype or c.device != dev or c.shape[3] != D or (
+        if c.dim() != 4 or c.dtype != cache_dtype or c.device != dev or c.shape[3] != D or (
                 c.stride(3) != 1) or c.shape != k_cache.shape:
             raise ValueError(f"{name}: {tuple(c.shape)} {c.dtype} on {c.device}, expected [pages, "
-                             f"page, kv heads, {D}] {q.dtype} with contiguous heads on {dev}")
+                             f"page, kv heads, {D}] {cache_dtype} with contiguous heads on {dev}")
     pages, page, Hkv, _ = k_cache.shape
     if Hkv < 1 or Hq % Hkv:
         raise ValueError(f"{Hq} query heads do not divide into {Hkv} kv heads")
@@ -49,12 +54,17 @@ def _args(q, k_cache, v_cache, block_table, kv_len, cu_q, max_q, scale, causal, 
     # (bounds of any size: what lies past the rows and past every key says no more)
     max_q, window = min(max_q, total), min(window, 2 ** 31 - 1)
     nbytes = _lib.load().ftb_attention_workspace_bytes(total, batch, max_q, Hq, Hkv, D)
-    return _lib.AttnArgsStruct(
+    a = _lib.AttnArgsStruct(
         workspace_bytes=nbytes, q_strides=q.stride()[:2], k_strides=k_cache.stride()[:3],
         v_strides=v_cache.stride()[:3], total_q=total, num_pages=pages,
         table_stride=block_table.stride(0), batch=batch, max_q=max_q, table_width=width,
         page=page, Hq=Hq, Hkv=Hkv, D=D, causal=int(causal), window=window,
         type=_TYPE[q.dtype], scale=D ** -0.5 if scale is None else scale)
+    if not fp8:
+        return a
+    size = scale_block(k_cache, k_scale, v_scale, dev)
+    return _lib.AttnFp8ArgsStruct(attn=a, k_scale_strides=k_scale.stride(),
+                                  v_scale_strides=v_scale.stride(), scale_block=size)
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -62,7 +72,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     cu_q: torch.Tensor | None = None, max_q: int = 1, *,
                     scale: float | None = None, causal: bool = True, window: int = 0,
                     out: torch.Tensor | None = None, return_lse: bool = False,
-                    check_status: bool = False):
+                    check_status: bool = False, k_scale: torch.Tensor | None = None,
+                    v_scale: torch.Tensor | None = None):
     """Attention of the new tokens of a batch over their sequences' pages; their own keys and
     values are in the caches already (``rope_append``).
 
@@ -76,16 +87,23 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     exponentials, float32 [total, q heads]. ``check_status`` reads the stream's status word
     (synchronises) and raises on page ids, lengths or starts outside the tensors, of this call or of
     one before it that did not look. ``max_q`` and the table's width pick the kernel: pass no more
-    than the batch needs where that is known on the host."""
+    than the batch needs where that is known on the host.
+
+    With ``k_scale`` and ``v_scale``, float32 [pages, page / S, kv heads], the caches are
+    ``torch.float8_e4m3fn`` as :func:`rope_append` fills them: an element stands for its number times
+    the scale of its block of S tokens (16, 32, 64 or 128) and head. D is then a multiple of 16."""
     if type(max_q) is not int or type(window) is not int or type(causal) is not bool:
         max_q, window, causal = int(max_q), int(window), bool(causal)
     if scale is not None and type(scale) is not float:
         scale = float(scale)
-    key = (_pycall.key(q, k_cache, v_cache, block_table, kv_len, cu_q), max_q, scale, causal, window)
+    fp8 = k_scale is not None or v_scale is not None
+    key = (_pycall.key(q, k_cache, v_cache, block_table, kv_len, cu_q, k_scale, v_scale) if fp8 else
+           _pycall.key(q, k_cache, v_cache, block_table, kv_len, cu_q), max_q, scale, causal, window)
     known = _ARGS.get(key)
     if known is None:
-        a = _args(q, k_cache, v_cache, block_table, kv_len, cu_q, max_q, scale, causal, window)
-        known = remember(key, a, a.workspace_bytes)
+        a = _args(q, k_cache, v_cache, block_table, kv_len, cu_q, max_q, scale, causal, window, k_scale,
+                  v_scale)
+        known = remember(key, a, a.attn.workspace_bytes if fp8 else a.workspace_bytes)
     dev = q.device
     if out is None:
         out = _pycall.empty(q, q)
@@ -93,10 +111,14 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         raise ValueError("out must be contiguous, of q's shape and dtype")
     lse = q.new_empty(q.shape[:2], dtype=torch.float32) if return_lse else None
     ws = zeroed_workspace(known[1], _lib.FTB_ATTN_ZERO_BYTES, dev)
-    st = caller(dev)(_lib.entry("ftb_attention"), known[0], _POINTERS, stream_handle(dev), q, k_cache,
-                     v_cache, block_table, kv_len, cu_q, out, lse, ws)
+    if fp8:
+        st = caller(dev)(_lib.entry("ftb_attention_fp8"), known[0], _FP8_POINTERS, stream_handle(dev), q,
+                         k_cache, v_cache, block_table, kv_len, cu_q, out, lse, ws, k_scale, v_scale)
+    else:
+        st = caller(dev)(_lib.entry("ftb_attention"), known[0], _POINTERS, stream_handle(dev), q, k_cache,
+                         v_cache, block_table, kv_len, cu_q, out, lse, ws)
     if st:
-        _lib.check("ftb_attention", st)
+        _lib.check("ftb_attention_fp8" if fp8 else "ftb_attention", st)
     if check_status:
         status = read_status(ws)
         if status:

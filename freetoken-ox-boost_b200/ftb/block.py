@@ -12,7 +12,8 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._runtime import _ARGS, _pycall, caller, remember, require, require_cuda, stream_handle
+from ._runtime import (_ARGS, _pycall, caller, remember, require, require_cuda, stream_handle,
+                       zeroed_workspace)
 
 _TYPE = {torch.bfloat16: _lib.FTB_TYPE_BF16, torch.float16: _lib.FTB_TYPE_F16}
 _GATE_ACTS = {None: _lib.FTB_GATE_LINEAR, "sigmoid": _lib.FTB_GATE_SIGMOID}
@@ -21,6 +22,10 @@ _ORDERS = {"blocks": _lib.FTB_AXES_BLOCKS, "cyclic": _lib.FTB_AXES_CYCLIC}
 _NORM_POINTERS = _lib.offsets(_lib.NormArgsStruct, "x", "y", "gate", "post", "pre", "r", "h")
 _ROPE_POINTERS = _lib.offsets(_lib.RopeArgsStruct, "q", "k", "v", "q_out", "k_dst", "v_dst",
                               "positions", "table", "slots")
+# (the plain call's arguments are the first member)
+_ROPE_FP8_POINTERS = _ROPE_POINTERS + _lib.offsets(_lib.RopeFp8ArgsStruct, "k_scale", "v_scale",
+                                                   "workspace")
+FP8 = torch.float8_e4m3fn
 
 
 def _row_stride(t: torch.Tensor, name: str) -> int:
@@ -178,7 +183,26 @@ def _int_kind(t, name, dev):
     return t.dtype == torch.int64
 
 
-def _rope_args(q, k, v, positions, table, k_dst, v_dst, slots, sections, order, pairs):
+def scale_block(cache, k_scale, v_scale, dev) -> int:
+    """The tokens per scale of an 8-bit cache [pages, page, kv heads, D], after the scales' checks."""
+    pages, page, Hkv, _ = cache.shape
+    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if t is None:
+            raise ValueError(f"{name} is None: an 8-bit cache has both scales")
+        if t.dim() != 3 or t.dtype != torch.float32 or t.device != dev or t.shape != k_scale.shape or (
+                t.shape[0] != pages or t.shape[2] != Hkv):
+            raise ValueError(f"{name}: {tuple(t.shape)} {t.dtype} on {t.device}, expected float32 "
+                             f"[{pages}, page / tokens per scale, {Hkv}] on {dev}")
+    blocks = k_scale.shape[1]
+    size = page // blocks if blocks else 0
+    if size * blocks != page or size not in (16, 32, 64, 128):
+        raise ValueError(f"{blocks} scales for a page of {page} tokens: expected 16, 32, 64 or 128 "
+                         "tokens per scale")
+    return size
+
+
+def _rope_args(q, k, v, positions, table, k_dst, v_dst, slots, sections, order, pairs,
+               cache_dtype=None):
     """The checks of a rotary call, and its arguments without the pointers."""
     dev = require_cuda(q)
     dtype = q.dtype
@@ -214,11 +238,12 @@ def _rope_args(q, k, v, positions, table, k_dst, v_dst, slots, sections, order, 
         a.k_dst_strides = (0, Hkv * D, D)
         return a
     a.v_strides = _heads(v, "v", tokens, D, dtype, dev)
+    cache_dtype = cache_dtype or dtype
     for name, c in (("k_cache", k_dst), ("v_cache", v_dst)):
-        if c.dim() != 4 or c.shape != (*k_dst.shape[:2], Hkv, D) or c.dtype != dtype or (
+        if c.dim() != 4 or c.shape != (*k_dst.shape[:2], Hkv, D) or c.dtype != cache_dtype or (
                 c.device != dev or c.stride(3) != 1):
-            raise ValueError(f"{name}: {tuple(c.shape)} {c.dtype} on {c.device}, expected "
-                             f"[pages, page, {Hkv}, {D}] {dtype} with contiguous heads on {dev}")
+            raise ValueError(f"{name}: {tuple(c.shape)} {c.dtype} on {c.device}, expected [pages, "
+                             f"page, {Hkv}, {D}] {cache_dtype} with contiguous heads on {dev}")
     if v.shape[1] != Hkv:
         raise ValueError(f"v: shape {tuple(v.shape)}, expected {tuple(k.shape)}")
     a.slot64 = _int_kind(slots, "slots", dev)
@@ -247,6 +272,33 @@ def _rope(q, k, v, positions, table, k_dst, v_dst, slots, sections, order, pairs
     return out
 
 
+def _rope_fp8(q, k, v, positions, table, k_cache, v_cache, slots, sections, order, pairs, q_out,
+              k_scale, v_scale):
+    """The call into an 8-bit cache."""
+    if sections is not None:
+        sections = tuple(map(int, sections))
+    key = (_pycall.key(q, k, positions, table, v, k_cache, v_cache, slots, k_scale, v_scale), sections,
+           order, pairs)
+    known = _ARGS.get(key)
+    if known is None:
+        a = _rope_args(q, k, v, positions, table, k_cache, v_cache, slots, sections, order, pairs, FP8)
+        size = scale_block(k_cache, k_scale, v_scale, q.device)
+        nbytes = _lib.load().ftb_rope_fp8_workspace_bytes(a.tokens, a.n_slots)
+        b = _lib.RopeFp8ArgsStruct(rope=a, k_scale_strides=k_scale.stride(),
+                                   v_scale_strides=v_scale.stride(), workspace_bytes=nbytes,
+                                   scale_block=size)
+        known = remember(key, b, nbytes if nbytes > _lib.FTB_ATTN_ZERO_BYTES else 0)
+    out = _pycall.empty(q, q) if q_out is None else _given(q_out, "q_out", q, q.dtype)
+    if q.shape[0]:
+        dev = q.device
+        ws = zeroed_workspace(known[1], _lib.FTB_ATTN_ZERO_BYTES, dev) if known[1] else None
+        st = caller(dev)(_lib.entry("ftb_rope_fp8"), known[0], _ROPE_FP8_POINTERS, stream_handle(dev), q,
+                         k, v, out, k_cache, v_cache, positions, table, slots, k_scale, v_scale, ws)
+        if st:
+            _lib.check("ftb_rope_fp8", st)
+    return out
+
+
 def rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, *,
          sections=None, order: str = "blocks", pairs: str = "half"):
     """``(q, k)`` [tokens, heads, D] turned by their positions [tokens] or [axes, tokens]; the
@@ -259,7 +311,9 @@ def rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table: torch
 def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
                 table: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                 slots: torch.Tensor, *, sections=None, order: str = "blocks",
-                pairs: str = "half", q_out: torch.Tensor | None = None) -> torch.Tensor:
+                pairs: str = "half", q_out: torch.Tensor | None = None,
+                k_scale: torch.Tensor | None = None,
+                v_scale: torch.Tensor | None = None) -> torch.Tensor:
     """Turns q and k by their positions, writes the turned k and v into the caches [pages, page,
     kv heads, D] and returns the turned q (in ``q_out``, which may be a contiguous ``q``).
 
@@ -267,5 +321,14 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     ``positions`` [tokens], or [axes, tokens] with ``sections``, the number of frequencies of each
     axis: in ``order="blocks"`` one axis after another, in ``"cyclic"`` the axes in turn.
     ``pairs="half"`` turns (x[i], x[i + rot/2]), ``"adjacent"`` (x[2i], x[2i+1]), for the first
-    rot = table.shape[1] elements of a head; the rest is copied."""
+    rot = table.shape[1] elements of a head; the rest is copied.
+
+    With ``k_scale`` and ``v_scale``, float32 [pages, page / S, kv heads], the caches are
+    ``torch.float8_e4m3fn``, and an element stands for its number times the scale of its block of S
+    tokens (16, 32, 64 or 128) and head. Scales are powers of two; that of a block is set by the largest
+    element when its first row is written, and grows with what joins the block, whose older rows are
+    then rounded again (``ftb_rope_fp8`` in ``include/ftb.h`` has the rule)."""
+    if k_scale is not None or v_scale is not None:
+        return _rope_fp8(q, k, v, positions, table, k_cache, v_cache, slots, sections, order, pairs,
+                         q_out, k_scale, v_scale)
     return _rope(q, k, v, positions, table, k_cache, v_cache, slots, sections, order, pairs, q_out)

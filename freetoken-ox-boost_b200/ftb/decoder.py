@@ -12,18 +12,36 @@ from dataclasses import dataclass
 import torch
 
 from .attention import paged_attention
-from .block import block_norm, rms_norm, rope_append
+from .block import FP8, block_norm, rms_norm, rope_append
 
 
 class PagedKvCache:
-    """Keys and values of one layer in pages: ``k``, ``v`` [num_pages, page, kv heads, D]."""
+    """Keys and values of one layer in pages: ``k``, ``v`` [num_pages, page, kv heads, D]. With
+    ``dtype=torch.float8_e4m3fn`` in 8 bits, with ``k_scale``, ``v_scale`` float32 [num_pages,
+    page / scale_block, kv heads] (``scale_block`` tokens per scale: 16, 32, 64 or 128; by default the
+    page, 128 at most)."""
 
     def __init__(self, num_pages: int, page: int, kv_heads: int, head_dim: int,
-                 dtype=torch.bfloat16, device="cuda"):
+                 dtype=torch.bfloat16, device="cuda", scale_block: int | None = None):
         shape = (num_pages, page, kv_heads, head_dim)
         self.k = torch.zeros(shape, dtype=dtype, device=device)
         self.v = torch.zeros(shape, dtype=dtype, device=device)
         self.page = page
+        self.k_scale = self.v_scale = None
+        if dtype == FP8:
+            size = min(page, 128) if scale_block is None else scale_block
+            if size not in (16, 32, 64, 128) or page % size:
+                raise ValueError(f"{size} tokens per scale in pages of {page}: expected 16, 32, 64 or "
+                                 "128 that divide the page")
+            # (0: no scale yet)
+            self.k_scale, self.v_scale = (
+                torch.zeros(num_pages, page // size, kv_heads, device=device) for _ in "kv")
+        elif scale_block is not None:
+            raise ValueError(f"scale_block={scale_block}: a cache of {dtype} has no scales")
+
+    def tensors(self) -> list:
+        """What a page id names, as :func:`~ftb.copy_pages` takes it."""
+        return [self.k, self.v] + ([] if self.k_scale is None else [self.k_scale, self.v_scale])
 
 
 @dataclass
@@ -94,10 +112,13 @@ class DecoderLayer:
         """The attention block's output of normed ``hidden`` [tokens, H]; fills the cache."""
         qkv = (hidden @ self.qkv.t()).unflatten(1, (-1, self.head_dim))
         q, k, v = qkv.split([self.q_heads, self.kv_heads, self.kv_heads], 1)
+        scales = {}
+        if getattr(cache, "k_scale", None) is not None:
+            scales = dict(k_scale=cache.k_scale, v_scale=cache.v_scale)
         q = rope_append(q, k, v, step.positions, self.rope_table, cache.k, cache.v, step.slots,
-                        **self.rope)
+                        **scales, **self.rope)
         out = paged_attention(q, cache.k, cache.v, step.block_table, step.kv_len, step.cu_q,
-                              step.max_q, window=self.window)
+                              step.max_q, window=self.window, **scales)
         return out.flatten(1) @ self.o.t()
 
     def forward(self, residual: torch.Tensor, hidden: torch.Tensor | None, step: AttnStep,

@@ -521,6 +521,74 @@ FTB_API size_t ftb_attention_workspace_bytes(int64_t total_q, int batch, int max
 FTB_API int ftb_attention(const ftb_attn_args* args, ftb_stream_t stream);
 
 /*
+ * ---- The 8-bit cache ------------------------------------------------------------------------
+ * Keys and values in e4m3, [pages, page, Hkv, D] bytes by strides {page, row, head}, with one fp32
+ * scale for each block of scale_block tokens of a page and kv head, [pages, page / scale_block, Hkv] by
+ * strides {page, block, head} in floats: a byte c stands for c * scale. scale_block is a power of two,
+ * 16 <= scale_block <= 128, that divides the page. Scales are positive and finite; the calls below use
+ * 2^-40 for a smaller one (or NaN) and 2^40 for a larger one.
+ */
+
+/*
+ * ftb_rope() into an 8-bit cache: rope.k_dst and rope.v_dst are the caches (their strides in bytes),
+ * rope.slots is required, rope.n_slots = pages * page.
+ * For a block and head that the call writes to, with A the largest |x| that it writes there and 2^e the
+ * smallest power of two with A <= 448 * 2^e, -40 <= e <= 40: the scale becomes 2^e where the call
+ * writes the block's first row or the scale is no positive finite number, else the larger of 2^e and
+ * the scale so far (rounded up to a power of two). The rows written are x / scale, rounded to e4m3 from
+ * fp32 (infinite x to +-448, NaN stays); where the scale changed, the block's other rows below the last
+ * one written are rounded again. Rows past the last one written, and blocks without one, stay as they
+ * are. Tokens may come in any order; of two tokens with the same slot one is kept, whole.
+ * workspace: ftb_rope_fp8_workspace_bytes() bytes, 4-byte aligned, for calls of one stream order. It
+ * may be the one of ftb_attention(): its first FTB_ATTN_ZERO_BYTES bytes are not touched, and the rest
+ * may hold anything. Calls of up to 512 tokens take none (it may be NULL).
+ */
+typedef struct ftb_rope_fp8_args {
+  ftb_rope_args rope;
+  float* k_scale;
+  float* v_scale;
+  int64_t k_scale_strides[3], v_scale_strides[3];
+  void* workspace;
+  size_t workspace_bytes;
+  int scale_block;
+} ftb_rope_fp8_args;
+FTB_API size_t ftb_rope_fp8_workspace_bytes(int64_t tokens, int64_t n_slots);
+FTB_API int ftb_rope_fp8(const ftb_rope_fp8_args* args, ftb_stream_t stream);
+
+/*
+ * ftb_attention() over an 8-bit cache: attn.k_cache and attn.v_cache are the caches, attn.k_strides and
+ * attn.v_strides in bytes (multiples of 16), D % 16 == 0, page >= scale_block; all else as there, the
+ * workspace among it. Products are those of the codes with q in f16 (a bf16 row that f16 would not hold
+ * is taken times a power of two), the probabilities' operand is f16.
+ */
+typedef struct ftb_attn_fp8_args {
+  ftb_attn_args attn;
+  const float* k_scale;
+  const float* v_scale;
+  int64_t k_scale_strides[3], v_scale_strides[3];
+  int scale_block;
+} ftb_attn_fp8_args;
+FTB_API int ftb_attention_fp8(const ftb_attn_fp8_args* args, ftb_stream_t stream);
+
+/*
+ * Copies of whole pages of n_caches caches that share their page ids: page dst[i] of each becomes its
+ * page src[i], i < n. src and dst: int32 or int64 (id64) on the device. A pair with an id outside
+ * [0, num_pages), or with src[i] == dst[i], copies nothing (-1: padding). The copies have no order: no
+ * page of dst may be in src, or in dst twice. Page p of cache j is the page_bytes[j] bytes at
+ * caches[j] + p * page_strides[j] (in bytes; page_strides[j] >= page_bytes[j]).
+ */
+#define FTB_PAGES_MAX 32
+typedef struct ftb_pages_args {
+  void* caches[FTB_PAGES_MAX];
+  const void* src;
+  const void* dst;
+  int64_t page_strides[FTB_PAGES_MAX], page_bytes[FTB_PAGES_MAX];
+  int64_t n, num_pages;
+  int n_caches, id64;
+} ftb_pages_args;
+FTB_API int ftb_copy_pages(const ftb_pages_args* args, ftb_stream_t stream);
+
+/*
  * Measurement hooks (no counterpart in the reference): between ftb_profile_begin() and
  * ftb_profile_end() the library records a CUDA event pair on the launching stream around
  * each of its kernel launches (ids: FTB_KERNEL_*). ftb_profile_end() synchronises those
