@@ -167,11 +167,10 @@ static int attention(const ftb_attn_args* args, const ftb_attn_fp8_args* fp8, ft
     for (int i = 0; i < 3; ++i)
       P.ks_st[i] = fp8->k_scale_strides[i], P.vs_st[i] = fp8->v_scale_strides[i];
     while ((1 << P.block_log2) < fp8->scale_block) ++P.block_log2;
-    return launch_attn_stream(*a, P, true, (cudaStream_t)stream);
   }
   return streams(*a, keys_bound(*a))
-             ? launch_attn_stream(*a, P, false, (cudaStream_t)stream)
-             : launch_attn_chunk(*a, P, (cudaStream_t)stream);
+             ? launch_attn_stream(*a, P, fp8 != nullptr, (cudaStream_t)stream)
+             : launch_attn_chunk(*a, P, fp8 != nullptr, (cudaStream_t)stream);
 }
 
 int ftb_attention(const ftb_attn_args* args, ftb_stream_t stream) {

@@ -497,19 +497,27 @@ __device__ __forceinline__ float max3v(float a, float b, float c) {
 
 // ---- the kernel --------------------------------------------------------------------------------
 
-constexpr int kPieceRing = 4, kPieceReaders = 8 + 2;  // softmax warps, MMA, fixer
+constexpr int kPieceRing = 4, kPieceReaders = 8 + 2;  // softmax warps, MMA, fixer (C8: two)
 // Three Q buffers for the two tiles: the next item's A comes in while this one is still in use.
 constexpr int kQBufs = 3;
 constexpr int chunk_stages(int DP) { return DP == 128 ? 4 : 8; }
-template <int DP>
+// C8: the cache is one of bytes. A tile's rows of 128 bytes land in the last 16 KB of its stage and are
+// turned into f16 in place.
+constexpr int kScaleRing = 4;   // key tiles whose scales are kept
+constexpr int kGroup = 16;      // keys that share their scales for certain
+template <int DP, bool C8>
 struct ChunkSmem {
   static constexpr int kStages = chunk_stages(DP);
   static constexpr int kTileBytes = kTileK * DP * 2;
   alignas(1024) uint8_t q[kQBufs][kTileBytes];      // [half][row][64]
   alignas(1024) uint8_t ring[kStages][kTileBytes];  // [half][key][64]
+  // of each kGroup keys: the scale of K, log2 and reciprocal of V's, and (in the first) the lowest log2
+  float4 scale[C8 ? kScaleRing : 1][kTileK / kGroup];
+  int8_t q_log2[C8 ? kQBufs : 1][kTileM];  // what a row of q was divided by
   uint64_t full[kStages], empty[kStages];
-  uint64_t land[kStages];  // a V tile that the fixer completes has landed
-  uint64_t q_full[kQBufs], q_empty[kQBufs];
+  uint64_t land[kStages];  // a V tile that the fixer completes has landed (C8: any tile)
+  uint64_t q_full[kQBufs], q_empty[kQBufs], q_land[C8 ? kQBufs : 1];
+  uint64_t scale_full[C8 ? kScaleRing : 1];
   uint64_t s_full[2], p_ready[2][2], o_full[2];  // p_ready: by halves of the keys
   Piece piece[kPieceRing];
   uint64_t piece_full[kPieceRing], piece_empty[kPieceRing];
@@ -518,9 +526,9 @@ struct ChunkSmem {
   int abort;
 };
 
-template <int DP>
+template <int DP, bool C8>
 struct ChunkSync {
-  ChunkSmem<DP>* sh;
+  ChunkSmem<DP, C8>* sh;
   uint32_t* status;
   __device__ bool wait(uint64_t* bar, uint32_t parity) const {
     if (mbar_try_wait(bar, parity)) return true;
@@ -548,12 +556,12 @@ __device__ __forceinline__ Piece load_piece(const Piece* p) {
   d[0] = __ldcg(s), d[1] = __ldcg(s + 1), d[2] = __ldcg(s + 2);
   return r;
 }
-template <int DP>
+template <int DP, bool C8>
 struct PieceReader {
   int at = 0;
   uint32_t parity = 0;
   // the next piece; false at the end of the list or after a timeout
-  __device__ bool next(const ChunkSync<DP>& sy, Piece& p) {
+  __device__ bool next(const ChunkSync<DP, C8>& sy, Piece& p) {
     if (!sy.wait_warp(&sy.sh->piece_full[at], parity)) return false;
     p = sy.sh->piece[at];
     __syncwarp();
@@ -584,10 +592,10 @@ __device__ __forceinline__ RowTile row_tile(const AttnParams& P, const Piece& p,
 
 template <int DP>
 __device__ void chunk_load(const AttnParams& P, const AttnMaps& M, const Plan& plan, int tok1,
-                           ChunkSmem<DP>* sh) {
-  constexpr int kStages = ChunkSmem<DP>::kStages, kH = DP / 64;
+                           ChunkSmem<DP, false>* sh) {
+  constexpr int kStages = ChunkSmem<DP, false>::kStages, kH = DP / 64;
   const int lane = threadIdx.x & 31;
-  const ChunkSync<DP> sy{sh, P.status};
+  const ChunkSync<DP, false> sy{sh, P.status};
   const int page = 1 << P.page_log2;
   const int r = page < kTileK ? page : kTileK;
   const int boxes = kTileK / r;  // <= 16
@@ -692,13 +700,13 @@ __device__ void chunk_load(const AttnParams& P, const AttnMaps& M, const Plan& p
 
 // Clears the rows of V tiles that no token of the piece's item sees.
 template <int DP>
-__device__ void chunk_fix(const AttnParams& P, int tok1, ChunkSmem<DP>* sh) {
-  constexpr int kStages = ChunkSmem<DP>::kStages, kH = DP / 64;
+__device__ void chunk_fix(const AttnParams& P, int tok1, ChunkSmem<DP, false>* sh) {
+  constexpr int kStages = ChunkSmem<DP, false>::kStages, kH = DP / 64;
   const int lane = threadIdx.x & 31;
-  const ChunkSync<DP> sy{sh, P.status};
+  const ChunkSync<DP, false> sy{sh, P.status};
   int stage = 0;
   uint32_t land_par = 0;  // a bit per stage
-  PieceReader<DP> pieces;
+  PieceReader<DP, false> pieces;
   for (Piece p; pieces.next(sy, p);) {
     const RowTile ra = row_tile(P, p, 0, tok1), rb = row_tile(P, p, 1, tok1);
     const int n = max(ra.n, rb.n);
@@ -725,11 +733,253 @@ __device__ void chunk_fix(const AttnParams& P, int tok1, ChunkSmem<DP>* sh) {
   }
 }
 
+// Where in its stage a tile of bytes lands.
+constexpr int raw_at(int tile_bytes) { return tile_bytes - kTileK * 128; }
+
+// chunk_load for a cache of bytes. All tiles signal land[]; lanes 0..7 bring the scales of the tile's
+// groups of keys. A tile's scales take the place of those of four tiles before, which nobody reads any
+// more: its K stage came free after S of the tile two before, which came after P of the one before that.
 template <typename T, int DP>
-__device__ void chunk_mma(const AttnParams& P, int tok1, ChunkSmem<DP>* sh) {
-  constexpr int kStages = ChunkSmem<DP>::kStages;
-  constexpr int kTileBytes = ChunkSmem<DP>::kTileBytes;
-  const ChunkSync<DP> sy{sh, P.status};
+__device__ void chunk_load8(const AttnParams& P, const AttnMaps& M, const Plan& plan, int tok1,
+                            ChunkSmem<DP, true>* sh) {
+  using Smem = ChunkSmem<DP, true>;
+  constexpr int kStages = Smem::kStages, kH = DP / 64, kGroups = kTileK / kGroup;
+  constexpr bool kTurn = !std::is_same<T, __half>::value;  // q is turned into f16 too
+  const int lane = threadIdx.x & 31;
+  const ChunkSync<DP, true> sy{sh, P.status};
+  const int page = 1 << P.page_log2;
+  const int r = page < kTileK ? page : kTileK;  // >= kGroup
+  const int boxes = kTileK / r;                 // <= 8
+  const uint32_t q_bytes = (uint32_t)(tok1 * P.G) * 128 * kH;
+  int stage = 0, qb = 0, sc = 0;
+  uint32_t parity = 1, q_par = 1;
+  uint32_t land_next = 0;  // parity of a stage's next phase on land[], a bit each
+  uint32_t used = 0;       // stages that had a copy
+  bool ok = true;
+  Piece p = load_piece(plan.pieces + blockIdx.x);
+  const int n_pieces = __ldcg(plan.head + kPlanPieces);
+  if ((int)blockIdx.x >= n_pieces) p.seq = -1;
+  int slot = 0;
+  uint32_t slot_parity = 1;
+  for (;;) {
+    ok = sy.wait_warp(&sh->piece_empty[slot], slot_parity);
+    if (!ok) break;
+    if (lane == 0) {
+      sh->piece[slot] = p;
+      mbar_arrive(&sh->piece_full[slot]);
+    }
+    if (++slot == kPieceRing) slot = 0, slot_parity ^= 1u;
+    if (p.seq < 0) break;
+    const RowTile ra = row_tile(P, p, 0, tok1), rb = row_tile(P, p, 1, tok1);
+    const int n = max(ra.n, rb.n);
+    const int32_t* table = P.block_table + (int64_t)p.seq * P.table_stride;
+    auto load_q = [&](const RowTile& rt) {
+      if (!sy.wait_warp(&sh->q_empty[qb], q_par)) return false;
+      if (lane == 0) {
+        uint64_t* bar = kTurn ? &sh->q_land[qb] : &sh->q_full[qb];
+        mbar_arrive_expect_tx(bar, q_bytes);
+#pragma unroll
+        for (int h = 0; h < kH; ++h)
+          tma_4d(smem_u32(sh->q[qb]) + h * kTileM * 128, &M.q, h * 64, 0, p.head,
+                 p.q_tok + rt.tok0, bar);
+      }
+      __syncwarp();
+      if (++qb == kQBufs) qb = 0, q_par ^= 1u;
+      return true;
+    };
+    if (ra.n > 0) ok = load_q(ra);
+    for (int j = 0; j < n && ok; ++j) {
+      const int key0 = (p.t0 + j) * kTileK;
+      const int b0 = p.lo > key0 ? (p.lo - key0) / r : 0;
+      const int b1 = min(boxes, (p.hi - key0 + r - 1) / r);
+      // page of this lane's group of keys, and its scales
+      const int key = key0 + lane * kGroup, box_of = lane * kGroup / r;
+      const bool has = lane < kGroups && box_of >= b0 && box_of < b1;
+      int id = 0;
+      if (has) {
+        id = __ldg(table + (key >> P.page_log2));
+        if (id < 0 || id >= P.num_pages) {
+          atomicOr(P.status, kAttnBadPage);
+          id = (int)P.num_pages;  // outside the tensor: reads zeros
+        }
+      }
+      float ks = 1.f, vs = 1.f;
+      if (has && id < P.num_pages) {
+        const int block = (key & (page - 1)) >> P.block_log2;
+        ks = __ldg(P.k_scale + id * P.ks_st[0] + block * P.ks_st[1] + p.head * P.ks_st[2]);
+        vs = __ldg(P.v_scale + id * P.vs_st[0] + block * P.vs_st[1] + p.head * P.vs_st[2]);
+      }
+      const int box_id = __shfl_sync(0xffffffffu, id, (lane * r / kGroup) & (kGroups - 1));
+      const bool mine = lane >= b0 && lane < b1;
+      for (int v = 0; v < 2 && ok; ++v) {
+        ok = sy.wait_warp(&sh->empty[stage], parity);
+        if (!ok) break;
+        uint64_t* bar = &sh->land[stage];
+        used |= 1u << stage;
+        land_next ^= 1u << stage;
+        if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(b1 - b0) * (uint32_t)r * 128u);
+        __syncwarp();
+        if (mine)
+          tma_5d(smem_u32(sh->ring[stage]) + raw_at(Smem::kTileBytes) + lane * r * 128, v ? &M.v : &M.k, 0,
+                 (key0 + lane * r) & (page - 1), p.head, box_id, 0, bar);
+        if (++stage == kStages) stage = 0, parity ^= 1u;
+        if (v == 0) {
+          const BlockScale b = block_scale(ks, vs);
+          float low = has ? b.v_log2 : INFINITY;
+#pragma unroll
+          for (int o = 1; o < kGroups; o <<= 1) low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+          if (lane < kGroups) sh->scale[sc][lane] = make_float4(b.k, b.v_log2, b.v_inv, low);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh->scale_full[sc]);
+          if (++sc == kScaleRing) sc = 0;
+          if (j == 0 && rb.n > 0) ok = load_q(rb);
+        }
+      }
+    }
+    if (!ok) break;
+    int next = 0;
+    if (lane == 0) next = atomicAdd(plan.head + kPlanNext, 1);
+    next = __shfl_sync(0xffffffffu, next, 0);
+    if (next < n_pieces)
+      p = load_piece(plan.pieces + next);
+    else
+      p.seq = -1;
+  }
+  // Stay until the last copies have landed, as above.
+  for (int i = 0; i < kStages; ++i) {
+    if (!(used >> i & 1u)) continue;
+    for (uint32_t k = 0; k < kSpinLimit; ++k)
+      if (mbar_try_wait(&sh->land[i], (land_next >> i & 1u) ^ 1u)) break;
+  }
+  for (int i = 0; i < kQBufs; ++i)
+    for (uint32_t k = 0; k < kSpinLimit; ++k)
+      if (mbar_try_wait(kTurn ? &sh->q_land[i] : &sh->q_full[i], i < qb ? q_par ^ 1u : q_par)) break;
+}
+
+// 16 codes as f16 numbers.
+__device__ __forceinline__ void codes16(const uint4& x, uint32_t (&f)[8]) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = e4m3x2_to_f16x2((uint16_t)(w[i] & 0xffffu));
+    f[2 * i + 1] = e4m3x2_to_f16x2((uint16_t)(w[i] >> 16));
+  }
+}
+
+// Two warps (part 0 and 1, half of the rows each) turn what lands into f16 operands, in place. A row's
+// bytes become (DP = 128) a row of the first 64 elements in the lower half of the stage and one of the
+// others where the bytes were, so no row waits for another. V rows that no token sees become zeros.
+// Queries in bf16 become f16 too, a row that f16 would not hold times a power of two. Shared memory
+// moves 48 KB per tile for this, beside the 128 KB that its MMAs read.
+template <typename T, int DP>
+__device__ void chunk_turn(const AttnParams& P, int tok1, int part, ChunkSmem<DP, true>* sh) {
+  using Smem = ChunkSmem<DP, true>;
+  constexpr int kStages = Smem::kStages, kH = DP / 64;
+  const int lane = threadIdx.x & 31;
+  const ChunkSync<DP, true> sy{sh, P.status};
+  int stage = 0, qb = 0;
+  uint32_t land_par = 0, q_par = 0;  // (land_par: a bit per stage)
+  auto turn_q = [&] {
+    if constexpr (!std::is_same<T, __half>::value) {
+      if (!sy.wait_warp(&sh->q_land[qb], q_par)) return false;
+      uint8_t* q = sh->q[qb];
+      const int c = lane & 7;
+#pragma unroll 1
+      for (int i = 0; i < kTileM / 2 / 4; ++i) {  // 8 lanes a row
+        const int row = part * (kTileM / 2) + i * 4 + (lane >> 3);
+        uint4 x[kH];
+        uint32_t top = 0;  // largest |x|: bf16 bits in the upper half
+#pragma unroll
+        for (int h = 0; h < kH; ++h) {
+          x[h] = *reinterpret_cast<const uint4*>(q + h * kTileM * 128 + row * 128 + c * 16);
+          const uint32_t w[4] = {x[h].x, x[h].y, x[h].z, x[h].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) top = max(top, max(w[k] << 16 & 0x7fff0000u, w[k] & 0x7fff0000u));
+        }
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const int ex = (int)(top >> 23) - 127;
+        const int e = top && ex < 128 && (ex < -4 || ex > 14) ? (ex > 14 ? ex - 14 : max(ex, -126)) : 0;
+        const float by = __uint_as_float((uint32_t)(127 - e) << 23);
+        if (c == 0) sh->q_log2[qb][row] = (int8_t)e;
+#pragma unroll
+        for (int h = 0; h < kH; ++h) {
+          uint32_t w[4] = {x[h].x, x[h].y, x[h].z, x[h].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 f = unpack2<T>(w[k]);
+            w[k] = pack2<__half>(f.x * by, f.y * by);
+          }
+          *reinterpret_cast<uint4*>(q + h * kTileM * 128 + row * 128 + c * 16) =
+              make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->q_full[qb]);
+      if (++qb == kQBufs) qb = 0, q_par ^= 1u;
+    }
+    return true;
+  };
+  constexpr int kLanes = DP / 16;          // lanes of a row, 16 bytes each
+  constexpr int kRows = 32 / kLanes;       // rows of an access of the warp
+  constexpr int kAtOnce = 4;               // accesses in flight
+  const int c = lane % kLanes;
+  // (DP = 64: rows 4 apart side by side, whose chunks lie in other banks)
+  const int r_in = DP == 64 ? (lane / kLanes >> 1) + 4 * (lane / kLanes & 1) : lane / kLanes;
+  PieceReader<DP, true> pieces;
+  for (Piece p; pieces.next(sy, p);) {
+    const RowTile ra = row_tile(P, p, 0, tok1), rb = row_tile(P, p, 1, tok1);
+    const int n = max(ra.n, rb.n);
+    if (ra.n > 0 && !turn_q()) return;
+    for (int j = 0; j < 2 * n; ++j) {
+      const int key0 = (p.t0 + (j >> 1)) * kTileK;
+      if (!sy.wait_warp(&sh->land[stage], (land_par >> stage) & 1u)) return;
+      land_par ^= 1u << stage;
+      uint8_t* tile = sh->ring[stage];
+      const bool cut = (j & 1) && (key0 < p.lo || key0 + kTileK > p.hi);
+#pragma unroll 1
+      for (int i = 0; i < kTileK / 2 / kRows; i += kAtOnce) {
+        uint4 x[kAtOnce];
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+          const int row = part * (kTileK / 2) + (i + u) * kRows + r_in;
+          x[u] = *reinterpret_cast<const uint4*>(tile + raw_at(Smem::kTileBytes) + row * 128 + ((c ^ (row & 7)) << 4));
+        }
+        __syncwarp();  // a row's bytes have been read before they are written over
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+          const int row = part * (kTileK / 2) + (i + u) * kRows + r_in;
+          uint32_t f[8];
+          codes16(x[u], f);
+          if (cut && (key0 + row < p.lo || key0 + row >= p.hi)) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) f[k] = 0u;
+          }
+          // elements 16 c ..: two 16-byte chunks of half h; the halves' lanes store theirs in opposite
+          // orders, so that the eight of a row meet eight different chunks
+          const int h = c >> 2, o = 2 * (c & 3);
+          uint8_t* to = tile + h * kTileK * 128 + row * 128;
+          const uint4 first = make_uint4(f[0], f[1], f[2], f[3]), second = make_uint4(f[4], f[5], f[6], f[7]);
+          *reinterpret_cast<uint4*>(to + (((h ? o + 1 : o) ^ (row & 7)) << 4)) = h ? second : first;
+          *reinterpret_cast<uint4*>(to + (((h ? o : o + 1) ^ (row & 7)) << 4)) = h ? first : second;
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->full[stage]);
+      if (++stage == kStages) stage = 0;
+      if (j == 0 && rb.n > 0 && !turn_q()) return;
+    }
+  }
+}
+
+// T: the operands' type.
+template <typename T, int DP, bool C8>
+__device__ void chunk_mma(const AttnParams& P, int tok1, ChunkSmem<DP, C8>* sh) {
+  constexpr int kStages = ChunkSmem<DP, C8>::kStages;
+  constexpr int kTileBytes = ChunkSmem<DP, C8>::kTileBytes;
+  const ChunkSync<DP, C8> sy{sh, P.status};
   const uint32_t tb = sh->tmem;
   const uint32_t qd = desc_low(smem_u32(sh->q[0]), 16);
   const uint32_t kd = desc_low(smem_u32(sh->ring[0]), 16);
@@ -769,7 +1019,7 @@ __device__ void chunk_mma(const AttnParams& P, int tok1, ChunkSmem<DP>* sh) {
     pend[x] = false;
   };
 
-  PieceReader<DP> pieces;
+  PieceReader<DP, C8> pieces;
   for (Piece p; ok && pieces.next(sy, p);) {
     const int nx[2] = {row_tile(P, p, 0, tok1).n, row_tile(P, p, 1, tok1).n};
     const int n = max(nx[0], nx[1]);
@@ -824,9 +1074,11 @@ __device__ __forceinline__ void st_sector(void* p, const uint32_t (&w)[8]) {
                : "memory");
 }
 
-template <typename T, int DP>
-__device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP>* sh) {
-  const ChunkSync<DP> sy{sh, P.status};
+template <typename T, int DP, bool C8>
+__device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP, C8>* sh) {
+  using TP = typename std::conditional<C8, __half, T>::type;  // P's type
+  constexpr bool kTurn = C8 && !std::is_same<T, __half>::value;
+  const ChunkSync<DP, C8> sy{sh, P.status};
   const int row = threadIdx.x & 127, lane = threadIdx.x & 31;
   const uint32_t lanes = (uint32_t)(row & ~31) << 16;
   const uint32_t ts = sh->tmem + kTmemS + x * 128 + lanes, to = sh->tmem + kTmemO + x * 128 + lanes;
@@ -836,18 +1088,31 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
   const bool flip = P.scale_log2 < 0.f;
   const float sc = fmaxf(fabsf(P.scale_log2), 1e-30f);
   int q_next = 0;
+  uint32_t q_wrap = 0;  // C8: parity of the next Q buffer's phase
+  uint32_t tile_at = 0;  // C8: key tiles of the pieces before
   uint32_t s_par = 0, o_par = 0;
   constexpr int kSlot = 2 * kTileM * (DP + 2);
-  PieceReader<DP> pieces;
+  PieceReader<DP, C8> pieces;
   for (Piece p; pieces.next(sy, p);) {
     const RowTile rt = row_tile(P, p, x, tok1);
     // Q buffers are taken in order: A's, B's, the next item's A's, ...
     const int n_other = row_tile(P, p, x ^ 1, tok1).n;
     int q_mine = q_next;
-    if (rt.n > 0 && x == 1 && n_other > 0) q_mine = q_mine + 1 == kQBufs ? 0 : q_mine + 1;
+    uint32_t q_par = q_wrap;
+    if (rt.n > 0 && x == 1 && n_other > 0) q_mine = q_mine + 1 == kQBufs ? (q_par ^= 1u, 0) : q_mine + 1;
     q_next += (rt.n > 0) + (n_other > 0);
-    if (q_next >= kQBufs) q_next -= kQBufs;
+    if (q_next >= kQBufs) q_next -= kQBufs, q_wrap ^= 1u;
+    const uint32_t tile0 = tile_at;
+    if constexpr (C8) tile_at += max(rt.n, n_other);
     if (rt.toks == 0) continue;
+    // C8: scores are those of the codes, times this and the scale of the keys
+    float sc_row = sc;
+    if constexpr (kTurn) {
+      if (rt.n > 0) {
+        if (!sy.wait_warp(&sh->q_full[q_mine], q_par)) return;
+        sc_row *= __uint_as_float((uint32_t)(127 + sh->q_log2[q_mine][row]) << 23);
+      }
+    }
     const bool live = tok < rt.toks;
     // keys this row sees: [kmin, kmax); the tile's rows all see [tile_min, tile_max)
     const int pos0 = p.pos + rt.tok0;
@@ -860,6 +1125,12 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
       if (!sy.wait_warp(&sh->s_full[x], s_par)) return;
       s_par ^= 1u;
       tc_after();
+      const float4* scales = nullptr;
+      if constexpr (C8) {
+        const uint32_t at = tile0 + j;
+        if (!sy.wait_warp(&sh->scale_full[at % kScaleRing], at / kScaleRing & 1u)) return;
+        scales = sh->scale[at % kScaleRing];
+      }
       float s[kTileK];
       const int key0 = (p.t0 + j) * kTileK;
       const bool masked = key0 < all_min || key0 + kTileK > all_max;
@@ -894,14 +1165,16 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
       // A row is off where a score exceeds the reference by more than 2^kLazy, or all fall short of
       // it by more than 2^kShort with nothing summed yet (`high` in powers of two above it).
       auto is_off = [&](float high) {
-        return high > kLazy || (l == 0.f && high < -kShort<T> && high != -INFINITY);
+        return high > kLazy || (l == 0.f && high < -kShort<TP> && high != -INFINITY);
       };
       // Makes this tile's maximum the reference of the rows that are off, and moves what was summed
-      // with the old one.
+      // with the old one. (C8: the first pass has found which rows are off; theirs are exponents by
+      // then, base-2 logarithms like the reference.)
+      bool off_row = false;
       auto move = [&] {
-        const float mx = highest();
-        const bool off = is_off((mx - ref) * sc);
-        const float f = off && l > 0.f ? ex2((ref - mx) * sc) : 1.f;  // (nothing summed: O is 0)
+        const float mx = highest(), by = C8 ? 1.f : sc;
+        const bool off = C8 ? off_row : is_off((mx - ref) * by);
+        const float f = off && l > 0.f ? ex2((ref - mx) * by) : 1.f;  // (nothing summed: O is 0)
         if (off) ref = mx;
         l *= f;
         if (j == 0) return;
@@ -920,7 +1193,8 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
       // rarely news after the first tile. So it is taken beside the exponentials with the
       // reference so far, and looked at before any of P is announced; where a row of the warp is
       // off, the tile is begun again.
-      if (j == 0) ref = 0.f;
+      // (C8: at the lowest scale of V among the tile's keys, a term of their exponents)
+      if (j == 0) ref = C8 ? scales[0].w : 0.f;
       bool moved = false;
       // The instructions of other pairs are laid between the two exponentials of a pair, which keep
       // the special-function unit busy for 16 cycles: the products of pairs to come (all of them,
@@ -929,24 +1203,57 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
       // unit waits. P goes out in two halves: the MMAs of the first run beside the exponentials of
       // the second.
       constexpr int kPairs = kTileK / 2, kAhead = 4;
+      // C8: a factor of scores is not 0, so that a masked -inf stays -inf
+      constexpr float kLeast = 1e-35f;
       uint64_t l0, l1;
       for (;;) {
         load();
+        if (C8 && moved) {
+          // Exponents first, each rounded by itself: the largest is then no higher than the reference
+          // that it gives, however large it is. (Rows that are not off stay as in the first pass:
+          // no row's result goes by the others of its warp.)
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) {
+            const float4 u = scales[i / (kGroup / 2)];
+            const float a = off_row ? fmaxf(u.x * sc_row, kLeast) : 1.f, b = off_row ? u.y : 0.f;
+            unpair(fma2v(pair(s[2 * i], s[2 * i + 1]), pair(a, a), pair(b, b)), s[2 * i], s[2 * i + 1]);
+          }
+        }
         if (moved) move();
         const float off = -ref * sc;
-        const uint64_t sc2 = pair(sc, sc), off2 = pair(off, off);
+        uint64_t sc2 = pair(sc, sc), off2 = pair(off, off), inv2 = 0;
+        float4 ahead;  // C8: scales of the next group of keys
+        if constexpr (C8) ahead = scales[0];
         uint32_t pk[kPairs / 2];
         float m0 = -INFINITY, m1 = -INFINITY;
         l0 = l1 = 0;
+        constexpr int kGroupPairs = kGroup / 2;
         auto scaled = [&](int i, float& m) {
+          if constexpr (C8) {
+            if (i % kGroupPairs == 0) {
+              const float a = off_row ? 1.f : fmaxf(ahead.x * sc_row, kLeast);
+              const float b = off_row ? -ref : ahead.y - ref;
+              sc2 = pair(a, a), off2 = pair(b, b);
+            } else if (i % kGroupPairs == 1 && i + kGroupPairs < kPairs) {
+              ahead = scales[i / kGroupPairs + 1];
+            }
+          }
           unpair(fma2v(pair(s[2 * i], s[2 * i + 1]), sc2, off2), s[2 * i], s[2 * i + 1]);
           // (two pairs behind: a warp issues in order, and would wait for the product)
           if (i >= 2) m = max3v(m, s[2 * i - 4], s[2 * i - 3]);
         };
         auto done = [&](int d) {
-          pk[d % (kPairs / 2)] = pack2v<T>(s[2 * d], s[2 * d + 1]);
+          pk[d % (kPairs / 2)] = pack2v<TP>(s[2 * d], s[2 * d + 1]);
           uint64_t& sum = d & 1 ? l1 : l0;
-          sum = add2v(sum, pair(s[2 * d], s[2 * d + 1]));
+          if constexpr (C8) {
+            if (d % kGroupPairs == 0) {
+              const float inv = scales[d / kGroupPairs].z;
+              inv2 = pair(inv, inv);
+            }
+            sum = fma2v(pair(s[2 * d], s[2 * d + 1]), inv2, sum);
+          } else {
+            sum = add2v(sum, pair(s[2 * d], s[2 * d + 1]));
+          }
         };
         auto announce = [&](int half) {
           tm_st16(ts + half * 32, pk);
@@ -971,6 +1278,7 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
           if (i >= kAhead) done(i - kAhead);
         }
         if (!moved && __any_sync(0xffffffffu, is_off(fmaxf(m0, m1)))) {
+          if constexpr (C8) off_row = is_off(fmaxf(m0, m1));
           moved = true;
           continue;
         }
@@ -989,6 +1297,7 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
       l += la + lb;
     }
     // output of the row tile
+    const float ref_log2 = C8 ? ref : ref * sc;
     if (rt.n > 0) {
       if (!sy.wait_warp(&sh->o_full[x], o_par)) return;
       o_par ^= 1u;
@@ -999,7 +1308,7 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
       if (live) {
         // (a row that summed nothing here has no reference: the one it started from, 0, may lie so
         // far above those of the other parts that the join would weigh them as nothing)
-        part[kTileM * DP + row] = l == 0.f ? -INFINITY : ref * sc;
+        part[kTileM * DP + row] = l == 0.f ? -INFINITY : ref_log2;
         part[kTileM * DP + kTileM + row] = l;
       }
 #pragma unroll 1
@@ -1053,7 +1362,7 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
       }
       if (live && P.lse)
         P.lse[(int64_t)(p.q_tok + rt.tok0 + tok) * P.Hq + p.head * P.G + g] =
-            l == 0.f ? -INFINITY : (ref * sc + log2f(l)) * 0.69314718055994531f;
+            l == 0.f ? -INFINITY : (ref_log2 + log2f(l)) * 0.69314718055994531f;
     }
     if (rt.n > 0) {  // the Q buffer goes back to the copies
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -1064,23 +1373,25 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
   }
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool C8>
 __global__ void __launch_bounds__(kThreadsC, 1)
     k_attn_chunk(const __grid_constant__ AttnMaps M, const __grid_constant__ AttnParams P,
                  const __grid_constant__ Plan plan, int tok1) {
   extern __shared__ uint8_t smem_raw[];
-  ChunkSmem<DP>* sh = reinterpret_cast<ChunkSmem<DP>*>(
+  ChunkSmem<DP, C8>* sh = reinterpret_cast<ChunkSmem<DP, C8>*>(
       smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023));
   const int warp = threadIdx.x >> 5;
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
-    for (int i = 0; i < ChunkSmem<DP>::kStages; ++i) {
-      mbar_init(&sh->full[i], 1);
+    constexpr bool kTurn = C8 && !std::is_same<T, __half>::value;
+    for (int i = 0; i < ChunkSmem<DP, C8>::kStages; ++i) {
+      mbar_init(&sh->full[i], C8 ? 2 : 1);  // (two warps turn a tile)
       mbar_init(&sh->empty[i], 1);
       mbar_init(&sh->land[i], 1);
     }
     for (int i = 0; i < kQBufs; ++i) {
-      mbar_init(&sh->q_full[i], 1);
+      mbar_init(&sh->q_full[i], kTurn ? 2 : 1);
+      if (kTurn) mbar_init(&sh->q_land[i], 1);
       mbar_init(&sh->q_empty[i], 4);  // the tile's softmax warps
     }
     for (int x = 0; x < 2; ++x) {
@@ -1091,8 +1402,9 @@ __global__ void __launch_bounds__(kThreadsC, 1)
     }
     for (int i = 0; i < kPieceRing; ++i) {
       mbar_init(&sh->piece_full[i], 1);
-      mbar_init(&sh->piece_empty[i], kPieceReaders);
+      mbar_init(&sh->piece_empty[i], kPieceReaders + C8);
     }
+    for (int i = 0; C8 && i < kScaleRing; ++i) mbar_init(&sh->scale_full[i], 1);
     mbar_init(&sh->drain, 1);
     sh->abort = 0;
     fence_mbar_init();
@@ -1112,15 +1424,22 @@ __global__ void __launch_bounds__(kThreadsC, 1)
   pdl_wait();
   if (warp < kWarpMma) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-    chunk_softmax<T, DP>(P, tok1, warp >> 2, sh);
+    chunk_softmax<T, DP, C8>(P, tok1, warp >> 2, sh);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
-    if (warp == kWarpMma)
-      chunk_mma<T, DP>(P, tok1, sh);
-    else if (warp == kWarpLoad)
-      chunk_load<DP>(P, M, plan, tok1, sh);
-    else if (warp == kWarpFix)
-      chunk_fix<DP>(P, tok1, sh);
+    if (warp == kWarpMma) {
+      chunk_mma<typename std::conditional<C8, __half, T>::type, DP, C8>(P, tok1, sh);
+    } else if constexpr (C8) {
+      if (warp == kWarpLoad)
+        chunk_load8<T, DP>(P, M, plan, tok1, sh);
+      else
+        chunk_turn<T, DP>(P, tok1, warp - kWarpFix, sh);
+    } else {
+      if (warp == kWarpLoad)
+        chunk_load<DP>(P, M, plan, tok1, sh);
+      else if (warp == kWarpFix)
+        chunk_fix<DP>(P, tok1, sh);
+    }
   }
   tc_before();
   __syncthreads();
@@ -1211,20 +1530,20 @@ int64_t chunk_groups(int64_t total_q, int batch, int G) {
   return total_q / (2 * (kTileM / G)) + batch;
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool C8>
 int run_chunk(const AttnMaps& M, const AttnParams& P, const Plan& plan, int tok1, int64_t groups,
               cudaStream_t stream) {
-  constexpr size_t smem = sizeof(ChunkSmem<DP>) + 1024;
+  constexpr size_t smem = sizeof(ChunkSmem<DP, C8>) + 1024;
   static_assert(smem <= 227 * 1024, "shared memory");
   // the warpgroups' shares must add up to what a block is launched with
   static const bool fits = [] {
     cudaFuncAttributes at;
-    return cudaFuncGetAttributes(&at, k_attn_chunk<T, DP>) == cudaSuccess &&
+    return cudaFuncGetAttributes(&at, k_attn_chunk<T, DP, C8>) == cudaSuccess &&
            at.numRegs >= kRegsLaunch;
   }();
   if (!fits) return FTB_ERR_NOT_BUILT;
   static std::atomic<uint64_t> done{0}, plan_done{0};
-  cudaError_t err = allow_smem(k_attn_chunk<T, DP>, smem, done);
+  cudaError_t err = allow_smem(k_attn_chunk<T, DP, C8>, smem, done);
   if (err == cudaSuccess) err = allow_smem(k_attn_plan, kPlanSmem, plan_done);
   if (err != cudaSuccess) return cuda_status(err);
   const int sms = sm_count();
@@ -1234,11 +1553,21 @@ int run_chunk(const AttnMaps& M, const AttnParams& P, const Plan& plan, int tok1
   err = launch_pdl(k_attn_plan, dim3(1), dim3(kPlanThreads), plan_smem, stream, P, plan, 2 * tok1,
                    sms);
   if (err != cudaSuccess) return cuda_status(err);
-  err = launch_pdl(k_attn_chunk<T, DP>, dim3((unsigned)sms), dim3(kThreadsC), smem, stream, M, P,
+  err = launch_pdl(k_attn_chunk<T, DP, C8>, dim3((unsigned)sms), dim3(kThreadsC), smem, stream, M, P,
                    plan, tok1);
   if (err != cudaSuccess) return cuda_status(err);
   return cuda_status(launch_pdl(k_attn_join<T, DP>, dim3((unsigned)sms * 8), dim3(256), 0, stream,
                                 P, plan, tok1));
+}
+
+template <bool C8>
+int pick_chunk(const ftb_attn_args& a, const AttnMaps& M, const AttnParams& P, const Plan& plan,
+               int tok1, int64_t groups, cudaStream_t stream) {
+  if (a.type == FTB_TYPE_BF16)
+    return a.D <= 64 ? run_chunk<__nv_bfloat16, 64, C8>(M, P, plan, tok1, groups, stream)
+                     : run_chunk<__nv_bfloat16, 128, C8>(M, P, plan, tok1, groups, stream);
+  return a.D <= 64 ? run_chunk<__half, 64, C8>(M, P, plan, tok1, groups, stream)
+                   : run_chunk<__half, 128, C8>(M, P, plan, tok1, groups, stream);
 }
 
 }  // namespace
@@ -1256,25 +1585,24 @@ bool attn_chunk_fits(const ftb_attn_args& a) {
          chunk_groups(a.total_q, a.batch, a.Hq / a.Hkv) * a.Hkv <= 0x3fffffff;
 }
 
-int launch_attn_chunk(const ftb_attn_args& a, AttnParams P, cudaStream_t stream) {
+int launch_attn_chunk(const ftb_attn_args& a, AttnParams P, bool fp8, cudaStream_t stream) {
   if (!attn_chunk_fits(a)) return FTB_ERR_SHAPE;
   const int tok1 = kTileM / P.G;
   const int64_t groups = chunk_groups(a.total_q, a.batch, P.G);
   AttnMaps M;
   const uint32_t r = a.page < kTileK ? a.page : kTileK;
-  int st = attn_cache_map(&M.k, a.k_cache, a, a.k_strides, r, 1);
-  if (!st) st = attn_cache_map(&M.v, a.v_cache, a, a.v_strides, r, 1);
+  int st = fp8 ? attn_cache_map8(&M.k, a.k_cache, a, a.k_strides, r)
+               : attn_cache_map(&M.k, a.k_cache, a, a.k_strides, r, 1);
+  if (!st)
+    st = fp8 ? attn_cache_map8(&M.v, a.v_cache, a, a.v_strides, r)
+             : attn_cache_map(&M.v, a.v_cache, a, a.v_strides, r, 1);
   if (!st) st = attn_q_map(&M.q, a, (uint32_t)P.G, (uint32_t)tok1);
   if (st) return st;
   size_t bytes;
   const Plan plan = carve_plan(reinterpret_cast<char*>(P.partial), groups, a.Hkv, &bytes);
   P.partial = reinterpret_cast<float*>(reinterpret_cast<char*>(P.partial) + bytes);
-  const int dp = a.D <= 64 ? 64 : 128;
-  if (a.type == FTB_TYPE_BF16)
-    return dp == 64 ? run_chunk<__nv_bfloat16, 64>(M, P, plan, tok1, groups, stream)
-                    : run_chunk<__nv_bfloat16, 128>(M, P, plan, tok1, groups, stream);
-  return dp == 64 ? run_chunk<__half, 64>(M, P, plan, tok1, groups, stream)
-                  : run_chunk<__half, 128>(M, P, plan, tok1, groups, stream);
+  return fp8 ? pick_chunk<true>(a, M, P, plan, tok1, groups, stream)
+             : pick_chunk<false>(a, M, P, plan, tok1, groups, stream);
 }
 
 }  // namespace ftb
