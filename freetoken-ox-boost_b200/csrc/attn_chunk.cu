@@ -48,13 +48,24 @@ namespace {
 
 constexpr int kTileK = 128;   // keys per tile
 constexpr int kTileM = 128;   // rows per tile
-constexpr int kThreadsC = 384;
 constexpr int kWarpMma = 8, kWarpLoad = 9, kWarpFix = 10;
-// registers: softmax 2 x 128 threads x 216 + 128 x 72 = 64512 = 384 x 168 at launch
-constexpr int kRegsLaunch = 168, kRegsSoftmax = 216, kRegsOther = 72;
-static_assert(2 * 128 * kRegsSoftmax + 128 * kRegsOther <= kThreadsC * kRegsLaunch, "registers");
+constexpr int kTurners = 4, kWarpTurnQ = kWarpFix + kTurners;  // C8: 10-13 turn keys, 14 and 15 queries
+// registers: softmax 2 x 128 threads x 216 + 128 x 72 = 64512 = 384 x 168 at launch; for a cache of bytes
+// (C8), whose tiles four more warps turn, 2 x 128 x 200 + 256 x 56 = 65536 = 512 x 128
+template <bool C8>
+struct ChunkShape {
+  static constexpr int kThreads = C8 ? 512 : 384;
+  static constexpr int kRegsLaunch = C8 ? 128 : 168, kRegsSoftmax = C8 ? 200 : 216,
+                       kRegsOther = C8 ? 56 : 72;
+  static_assert(2 * 128 * kRegsSoftmax + (kThreads - 256) * kRegsOther <= kThreads * kRegsLaunch,
+                "registers");
+};
 constexpr int kTmemS = 0, kTmemO = 256;  // + 128 for tile B
 constexpr float kLazy = 8.f;             // log2 of what a score may exceed the reference by
+// The same for a cache of bytes, whose P is always f16: as far as f16 goes. The scales' logarithms are
+// terms of the exponents and widen their range, and a row that moves costs its warp a second pass (with 8
+// in place of 14, 4093 tokens at 32771 keys whose scales differ by 4 took 4.1 ms).
+constexpr float kLazyBytes = 14.f;
 // log2 of what a row's maximum may fall short of it. f16 has no exponents to spare: 2^8 above the
 // maximum, weights of 2^-17 of the largest would be rounded away, and many of those can hold much
 // of the sum.
@@ -497,7 +508,7 @@ __device__ __forceinline__ float max3v(float a, float b, float c) {
 
 // ---- the kernel --------------------------------------------------------------------------------
 
-constexpr int kPieceRing = 4, kPieceReaders = 8 + 2;  // softmax warps, MMA, fixer (C8: two)
+constexpr int kPieceRing = 4, kPieceReaders = 8 + 2;  // softmax warps, MMA, fixer
 // Three Q buffers for the two tiles: the next item's A comes in while this one is still in use.
 constexpr int kQBufs = 3;
 constexpr int chunk_stages(int DP) { return DP == 128 ? 4 : 8; }
@@ -866,25 +877,81 @@ __device__ __forceinline__ void codes16(const uint4& x, uint32_t (&f)[8]) {
   }
 }
 
-// Two warps (part 0 and 1, half of the rows each) turn what lands into f16 operands, in place. A row's
-// bytes become (DP = 128) a row of the first 64 elements in the lower half of the stage and one of the
-// others where the bytes were, so no row waits for another. V rows that no token sees become zeros.
-// Queries in bf16 become f16 too, a row that f16 would not hold times a power of two. Shared memory
-// moves 48 KB per tile for this, beside the 128 KB that its MMAs read.
-template <typename T, int DP>
+// kTurners warps (`part` of the rows each) turn what lands into f16 operands, in place. A row's bytes
+// become (DP = 128) a row of the first 64 elements in the lower half of the stage and one of the others
+// where the bytes were, so no row waits for another. V rows that no token sees become zeros. A warp has
+// all of its part in flight at once: the MMAs keep shared memory busy, and its loads wait long (two
+// warps, 4 or 8 loads at once: 2.68 and 2.45 ms for the chunk at 32771 keys).
+template <int DP>
 __device__ void chunk_turn(const AttnParams& P, int tok1, int part, ChunkSmem<DP, true>* sh) {
   using Smem = ChunkSmem<DP, true>;
-  constexpr int kStages = Smem::kStages, kH = DP / 64;
+  constexpr int kStages = Smem::kStages;
   const int lane = threadIdx.x & 31;
   const ChunkSync<DP, true> sy{sh, P.status};
-  int stage = 0, qb = 0;
-  uint32_t land_par = 0, q_par = 0;  // (land_par: a bit per stage)
-  auto turn_q = [&] {
-    if constexpr (!std::is_same<T, __half>::value) {
-      if (!sy.wait_warp(&sh->q_land[qb], q_par)) return false;
+  constexpr int kLanes = DP / 16;        // lanes of a row, 16 bytes each
+  constexpr int kRows = 32 / kLanes;     // rows of an access of the warp
+  constexpr int kAccesses = kTileK / kTurners / kRows;
+  const int c = lane % kLanes;
+  // (DP = 64: rows 4 apart side by side, whose chunks lie in other banks)
+  const int row0 = part * (kTileK / kTurners) +
+                   (DP == 64 ? (lane / kLanes >> 1) + 4 * (lane / kLanes & 1) : lane / kLanes);
+  // elements 16 c ..: two 16-byte chunks of half h; the halves' lanes store theirs in opposite orders, so
+  // that the eight of a row meet eight different chunks
+  const int h = c >> 2, o0 = 2 * (c & 3) + h, o1 = o0 ^ 1;
+  int stage = 0;
+  uint32_t land_par = 0;  // a bit per stage
+  PieceReader<DP, true> pieces;
+  for (Piece p; pieces.next(sy, p);) {
+    const int n = max(row_tile(P, p, 0, tok1).n, row_tile(P, p, 1, tok1).n);
+    for (int j = 0; j < 2 * n; ++j) {
+      const int key0 = (p.t0 + (j >> 1)) * kTileK;
+      if (!sy.wait_warp(&sh->land[stage], (land_par >> stage) & 1u)) return;
+      land_par ^= 1u << stage;
+      uint8_t* tile = sh->ring[stage];
+      const bool cut = (j & 1) && (key0 < p.lo || key0 + kTileK > p.hi);
+      uint4 x[kAccesses];
+#pragma unroll
+      for (int u = 0; u < kAccesses; ++u) {
+        const int row = row0 + u * kRows;
+        x[u] = *reinterpret_cast<const uint4*>(tile + raw_at(Smem::kTileBytes) + row * 128 +
+                                               ((c ^ (row & 7)) << 4));
+        if (cut && (key0 + row < p.lo || key0 + row >= p.hi)) x[u] = make_uint4(0, 0, 0, 0);
+      }
+      __syncwarp();  // a row's bytes have been read before they are written over
+#pragma unroll
+      for (int u = 0; u < kAccesses; ++u) {
+        const int row = row0 + u * kRows;
+        uint32_t f[8];
+        codes16(x[u], f);
+        const uint4 first = make_uint4(f[0], f[1], f[2], f[3]), second = make_uint4(f[4], f[5], f[6], f[7]);
+        uint8_t* to = tile + h * kTileK * 128 + row * 128;
+        *reinterpret_cast<uint4*>(to + ((o0 ^ (row & 7)) << 4)) = h ? second : first;
+        *reinterpret_cast<uint4*>(to + ((o1 ^ (row & 7)) << 4)) = h ? first : second;
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->full[stage]);
+      if (++stage == kStages) stage = 0;
+    }
+  }
+}
+
+// Two warps turn bf16 queries into f16, in place, a row that f16 would not hold with all its bits times a
+// power of two.
+template <int DP>
+__device__ void chunk_turn_q(const AttnParams& P, int tok1, int part, ChunkSmem<DP, true>* sh) {
+  constexpr int kH = DP / 64;
+  const int lane = threadIdx.x & 31, c = lane & 7;
+  const ChunkSync<DP, true> sy{sh, P.status};
+  int qb = 0;
+  uint32_t q_par = 0;
+  PieceReader<DP, true> pieces;
+  for (Piece p; pieces.next(sy, p);) {
+    for (int t = 0; t < 2; ++t) {
+      if (row_tile(P, p, t, tok1).n == 0) continue;
+      if (!sy.wait_warp(&sh->q_land[qb], q_par)) return;
       uint8_t* q = sh->q[qb];
-      const int c = lane & 7;
-#pragma unroll 1
+#pragma unroll 2
       for (int i = 0; i < kTileM / 2 / 4; ++i) {  // 8 lanes a row
         const int row = part * (kTileM / 2) + i * 4 + (lane >> 3);
         uint4 x[kH];
@@ -907,7 +974,7 @@ __device__ void chunk_turn(const AttnParams& P, int tok1, int part, ChunkSmem<DP
           uint32_t w[4] = {x[h].x, x[h].y, x[h].z, x[h].w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const float2 f = unpack2<T>(w[k]);
+            const float2 f = unpack2<__nv_bfloat16>(w[k]);
             w[k] = pack2<__half>(f.x * by, f.y * by);
           }
           *reinterpret_cast<uint4*>(q + h * kTileM * 128 + row * 128 + c * 16) =
@@ -918,58 +985,6 @@ __device__ void chunk_turn(const AttnParams& P, int tok1, int part, ChunkSmem<DP
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->q_full[qb]);
       if (++qb == kQBufs) qb = 0, q_par ^= 1u;
-    }
-    return true;
-  };
-  constexpr int kLanes = DP / 16;          // lanes of a row, 16 bytes each
-  constexpr int kRows = 32 / kLanes;       // rows of an access of the warp
-  constexpr int kAtOnce = 4;               // accesses in flight
-  const int c = lane % kLanes;
-  // (DP = 64: rows 4 apart side by side, whose chunks lie in other banks)
-  const int r_in = DP == 64 ? (lane / kLanes >> 1) + 4 * (lane / kLanes & 1) : lane / kLanes;
-  PieceReader<DP, true> pieces;
-  for (Piece p; pieces.next(sy, p);) {
-    const RowTile ra = row_tile(P, p, 0, tok1), rb = row_tile(P, p, 1, tok1);
-    const int n = max(ra.n, rb.n);
-    if (ra.n > 0 && !turn_q()) return;
-    for (int j = 0; j < 2 * n; ++j) {
-      const int key0 = (p.t0 + (j >> 1)) * kTileK;
-      if (!sy.wait_warp(&sh->land[stage], (land_par >> stage) & 1u)) return;
-      land_par ^= 1u << stage;
-      uint8_t* tile = sh->ring[stage];
-      const bool cut = (j & 1) && (key0 < p.lo || key0 + kTileK > p.hi);
-#pragma unroll 1
-      for (int i = 0; i < kTileK / 2 / kRows; i += kAtOnce) {
-        uint4 x[kAtOnce];
-#pragma unroll
-        for (int u = 0; u < kAtOnce; ++u) {
-          const int row = part * (kTileK / 2) + (i + u) * kRows + r_in;
-          x[u] = *reinterpret_cast<const uint4*>(tile + raw_at(Smem::kTileBytes) + row * 128 + ((c ^ (row & 7)) << 4));
-        }
-        __syncwarp();  // a row's bytes have been read before they are written over
-#pragma unroll
-        for (int u = 0; u < kAtOnce; ++u) {
-          const int row = part * (kTileK / 2) + (i + u) * kRows + r_in;
-          uint32_t f[8];
-          codes16(x[u], f);
-          if (cut && (key0 + row < p.lo || key0 + row >= p.hi)) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) f[k] = 0u;
-          }
-          // elements 16 c ..: two 16-byte chunks of half h; the halves' lanes store theirs in opposite
-          // orders, so that the eight of a row meet eight different chunks
-          const int h = c >> 2, o = 2 * (c & 3);
-          uint8_t* to = tile + h * kTileK * 128 + row * 128;
-          const uint4 first = make_uint4(f[0], f[1], f[2], f[3]), second = make_uint4(f[4], f[5], f[6], f[7]);
-          *reinterpret_cast<uint4*>(to + (((h ? o + 1 : o) ^ (row & 7)) << 4)) = h ? second : first;
-          *reinterpret_cast<uint4*>(to + (((h ? o : o + 1) ^ (row & 7)) << 4)) = h ? first : second;
-        }
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh->full[stage]);
-      if (++stage == kStages) stage = 0;
-      if (j == 0 && rb.n > 0 && !turn_q()) return;
     }
   }
 }
@@ -1165,7 +1180,7 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
       // A row is off where a score exceeds the reference by more than 2^kLazy, or all fall short of
       // it by more than 2^kShort with nothing summed yet (`high` in powers of two above it).
       auto is_off = [&](float high) {
-        return high > kLazy || (l == 0.f && high < -kShort<TP> && high != -INFINITY);
+        return high > (C8 ? kLazyBytes : kLazy) || (l == 0.f && high < -kShort<TP> && high != -INFINITY);
       };
       // Makes this tile's maximum the reference of the rows that are off, and moves what was summed
       // with the old one. (C8: the first pass has found which rows are off; theirs are exponents by
@@ -1374,7 +1389,7 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
 }
 
 template <typename T, int DP, bool C8>
-__global__ void __launch_bounds__(kThreadsC, 1)
+__global__ void __launch_bounds__(ChunkShape<C8>::kThreads, 1)
     k_attn_chunk(const __grid_constant__ AttnMaps M, const __grid_constant__ AttnParams P,
                  const __grid_constant__ Plan plan, int tok1) {
   extern __shared__ uint8_t smem_raw[];
@@ -1385,7 +1400,7 @@ __global__ void __launch_bounds__(kThreadsC, 1)
   if (threadIdx.x == 0) {
     constexpr bool kTurn = C8 && !std::is_same<T, __half>::value;
     for (int i = 0; i < ChunkSmem<DP, C8>::kStages; ++i) {
-      mbar_init(&sh->full[i], C8 ? 2 : 1);  // (two warps turn a tile)
+      mbar_init(&sh->full[i], C8 ? kTurners : 1);
       mbar_init(&sh->empty[i], 1);
       mbar_init(&sh->land[i], 1);
     }
@@ -1402,7 +1417,7 @@ __global__ void __launch_bounds__(kThreadsC, 1)
     }
     for (int i = 0; i < kPieceRing; ++i) {
       mbar_init(&sh->piece_full[i], 1);
-      mbar_init(&sh->piece_empty[i], kPieceReaders + C8);
+      mbar_init(&sh->piece_empty[i], C8 ? 8 + 1 + kTurners + 2 * kTurn : kPieceReaders);
     }
     for (int i = 0; C8 && i < kScaleRing; ++i) mbar_init(&sh->scale_full[i], 1);
     mbar_init(&sh->drain, 1);
@@ -1423,17 +1438,19 @@ __global__ void __launch_bounds__(kThreadsC, 1)
   tc_after();
   pdl_wait();
   if (warp < kWarpMma) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(ChunkShape<C8>::kRegsSoftmax));
     chunk_softmax<T, DP, C8>(P, tok1, warp >> 2, sh);
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(ChunkShape<C8>::kRegsOther));
     if (warp == kWarpMma) {
       chunk_mma<typename std::conditional<C8, __half, T>::type, DP, C8>(P, tok1, sh);
     } else if constexpr (C8) {
       if (warp == kWarpLoad)
         chunk_load8<T, DP>(P, M, plan, tok1, sh);
-      else
-        chunk_turn<T, DP>(P, tok1, warp - kWarpFix, sh);
+      else if (warp < kWarpTurnQ)
+        chunk_turn<DP>(P, tok1, warp - kWarpFix, sh);
+      else if (!std::is_same<T, __half>::value)
+        chunk_turn_q<DP>(P, tok1, warp - kWarpTurnQ, sh);
     } else {
       if (warp == kWarpLoad)
         chunk_load<DP>(P, M, plan, tok1, sh);
@@ -1539,7 +1556,7 @@ int run_chunk(const AttnMaps& M, const AttnParams& P, const Plan& plan, int tok1
   static const bool fits = [] {
     cudaFuncAttributes at;
     return cudaFuncGetAttributes(&at, k_attn_chunk<T, DP, C8>) == cudaSuccess &&
-           at.numRegs >= kRegsLaunch;
+           at.numRegs >= ChunkShape<C8>::kRegsLaunch;
   }();
   if (!fits) return FTB_ERR_NOT_BUILT;
   static std::atomic<uint64_t> done{0}, plan_done{0};
@@ -1553,7 +1570,7 @@ int run_chunk(const AttnMaps& M, const AttnParams& P, const Plan& plan, int tok1
   err = launch_pdl(k_attn_plan, dim3(1), dim3(kPlanThreads), plan_smem, stream, P, plan, 2 * tok1,
                    sms);
   if (err != cudaSuccess) return cuda_status(err);
-  err = launch_pdl(k_attn_chunk<T, DP, C8>, dim3((unsigned)sms), dim3(kThreadsC), smem, stream, M, P,
+  err = launch_pdl(k_attn_chunk<T, DP, C8>, dim3((unsigned)sms), dim3(ChunkShape<C8>::kThreads), smem, stream, M, P,
                    plan, tok1);
   if (err != cudaSuccess) return cuda_status(err);
   return cuda_status(launch_pdl(k_attn_join<T, DP>, dim3((unsigned)sms * 8), dim3(256), 0, stream,
