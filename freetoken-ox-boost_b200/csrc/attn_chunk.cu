@@ -1038,6 +1038,13 @@ __device__ void chunk_mma(const AttnParams& P, int tok1, ChunkSmem<DP, C8>* sh) 
   for (Piece p; ok && pieces.next(sy, p);) {
     const int nx[2] = {row_tile(P, p, 0, tok1).n, row_tile(P, p, 1, tok1).n};
     const int n = max(nx[0], nx[1]);
+    // An item without keys brings no step to issue the last P V of the one before in. The softmax warps
+    // wait for that before they take another item, so a ring full of such items would never move on.
+    if (n == 0) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        if (ok && pend[x]) pv(x);
+    }
     for (int j = 0; j < n && ok; ++j) {
       ok = sy.wait_warp(&sh->full[stage], parity);
       if (!ok) break;
