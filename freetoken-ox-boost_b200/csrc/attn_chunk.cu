@@ -514,12 +514,17 @@ constexpr int kQBufs = 3;
 constexpr int chunk_stages(int DP) { return DP == 128 ? 4 : 8; }
 // C8: the cache is one of bytes. A tile's rows of 128 bytes land in the last 16 KB of its stage and are
 // turned into f16 in place.
-constexpr int kScaleRing = 4;   // key tiles whose scales are kept
+// Key tiles whose scales are kept. A tile's scales come when its K stage is free, that is after S of the
+// tile kStages / 2 before it, which followed P of the one before that: so many tiles and one more may
+// still be read, and a tile further back is not.
+constexpr int scale_ring(int DP) { return DP == 128 ? 4 : 8; }
 constexpr int kGroup = 16;      // keys that share their scales for certain
 template <int DP, bool C8>
 struct ChunkSmem {
   static constexpr int kStages = chunk_stages(DP);
   static constexpr int kTileBytes = kTileK * DP * 2;
+  static constexpr int kScaleRing = scale_ring(DP);
+  static_assert(kScaleRing > kStages / 2, "no scales are written over that are still read");
   alignas(1024) uint8_t q[kQBufs][kTileBytes];      // [half][row][64]
   alignas(1024) uint8_t ring[kStages][kTileBytes];  // [half][key][64]
   // of each kGroup keys: the scale of K, log2 and reciprocal of V's, and (in the first) the lowest log2
@@ -748,8 +753,7 @@ __device__ void chunk_fix(const AttnParams& P, int tok1, ChunkSmem<DP, false>* s
 constexpr int raw_at(int tile_bytes) { return tile_bytes - kTileK * 128; }
 
 // chunk_load for a cache of bytes. All tiles signal land[]; lanes 0..7 bring the scales of the tile's
-// groups of keys. A tile's scales take the place of those of four tiles before, which nobody reads any
-// more: its K stage came free after S of the tile two before, which came after P of the one before that.
+// groups of keys.
 template <typename T, int DP>
 __device__ void chunk_load8(const AttnParams& P, const AttnMaps& M, const Plan& plan, int tok1,
                             ChunkSmem<DP, true>* sh) {
@@ -842,7 +846,7 @@ __device__ void chunk_load8(const AttnParams& P, const AttnMaps& M, const Plan& 
           if (lane < kGroups) sh->scale[sc][lane] = make_float4(b.k, b.v_log2, b.v_inv, low);
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh->scale_full[sc]);
-          if (++sc == kScaleRing) sc = 0;
+          if (++sc == Smem::kScaleRing) sc = 0;
           if (j == 0 && rb.n > 0) ok = load_q(rb);
         }
       }
@@ -1127,14 +1131,7 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
     const uint32_t tile0 = tile_at;
     if constexpr (C8) tile_at += max(rt.n, n_other);
     if (rt.toks == 0) continue;
-    // C8: scores are those of the codes, times this and the scale of the keys
-    float sc_row = sc;
-    if constexpr (kTurn) {
-      if (rt.n > 0) {
-        if (!sy.wait_warp(&sh->q_full[q_mine], q_par)) return;
-        sc_row *= __uint_as_float((uint32_t)(127 + sh->q_log2[q_mine][row]) << 23);
-      }
-    }
+    float sc_row = sc;  // C8: scores are those of the codes, times this and the scale of the keys
     const bool live = tok < rt.toks;
     // keys this row sees: [kmin, kmax); the tile's rows all see [tile_min, tile_max)
     const int pos0 = p.pos + rt.tok0;
@@ -1148,7 +1145,16 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
       s_par ^= 1u;
       tc_after();
       const float4* scales = nullptr;
+      if constexpr (kTurn) {
+        // (S is there, so this phase has passed, and no later one: this warp still holds the buffer.
+        // Waited for before S, a warp that had no keys in the items before could be a phase too early.)
+        if (j == 0) {
+          if (!sy.wait_warp(&sh->q_full[q_mine], q_par)) return;
+          sc_row *= __uint_as_float((uint32_t)(127 + sh->q_log2[q_mine][row]) << 23);
+        }
+      }
       if constexpr (C8) {
+        constexpr uint32_t kScaleRing = ChunkSmem<DP, C8>::kScaleRing;
         const uint32_t at = tile0 + j;
         if (!sy.wait_warp(&sh->scale_full[at % kScaleRing], at / kScaleRing & 1u)) return;
         scales = sh->scale[at % kScaleRing];
@@ -1426,7 +1432,7 @@ __global__ void __launch_bounds__(ChunkShape<C8>::kThreads, 1)
       mbar_init(&sh->piece_full[i], 1);
       mbar_init(&sh->piece_empty[i], C8 ? 8 + 1 + kTurners + 2 * kTurn : kPieceReaders);
     }
-    for (int i = 0; C8 && i < kScaleRing; ++i) mbar_init(&sh->scale_full[i], 1);
+    for (int i = 0; C8 && i < ChunkSmem<DP, C8>::kScaleRing; ++i) mbar_init(&sh->scale_full[i], 1);
     mbar_init(&sh->drain, 1);
     sh->abort = 0;
     fence_mbar_init();

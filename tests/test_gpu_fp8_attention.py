@@ -92,6 +92,25 @@ def test_chunk_head_groups(heads):
     check(Fp8Case([(400, 2300)], q_heads=heads[0], kv_heads=heads[1]))
 
 
+@pytest.mark.parametrize("head", [64, 128])
+@pytest.mark.parametrize("dtype", [BF, F16])
+def test_more_items_than_multiprocessors(dtype, head):
+    """A block takes several items one after another: with keys for both row tiles, for one of them
+    (windows, ends of sequences) and for none, of one key tile and of many; rows of q that f16 holds and
+    rows that are scaled."""
+    pairs = [(300, 2900), (58, 1860), (3, 1200), (260, 1500), (1, 0), (280, 280), (19, 2100), (400, 300)]
+    c = Fp8Case(pairs * 3, q_heads=24, kv_heads=8, head=head, page=32, block=32, dtype=dtype, window=900)
+    q, keys = build(c)
+    if dtype == BF:
+        lift = torch.ones(q.shape[:2] + (1,))
+        lift[::3, ::2] = 2.0 ** -12
+        q = (q.float() * lift).to(BF)
+        c.t["q"] = q.cuda()
+    for _ in range(20):
+        out, lse = ftb.paged_attention(**c.t, window=c.window, return_lse=True, check_status=True)
+    compare(c, out, lse, *reference(c, q, keys))
+
+
 @pytest.mark.parametrize("window", [1, 16, 100, 128, 129, 1000])
 def test_chunk_window(window):
     check(Fp8Case([(200, 600), (40, 40), (1, 333)], window=window))
