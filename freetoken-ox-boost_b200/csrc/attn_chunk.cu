@@ -48,18 +48,15 @@ namespace {
 
 constexpr int kTileK = 128;   // keys per tile
 constexpr int kTileM = 128;   // rows per tile
+constexpr int kThreadsC = 384;
 constexpr int kWarpMma = 8, kWarpLoad = 9, kWarpFix = 10;
-constexpr int kTurners = 4, kWarpTurnQ = kWarpFix + kTurners;  // C8: 10-13 turn keys, 14 and 15 queries
-// registers: softmax 2 x 128 threads x 216 + 128 x 72 = 64512 = 384 x 168 at launch; for a cache of bytes
-// (C8), whose tiles four more warps turn, 2 x 128 x 200 + 256 x 56 = 65536 = 512 x 128
-template <bool C8>
-struct ChunkShape {
-  static constexpr int kThreads = C8 ? 512 : 384;
-  static constexpr int kRegsLaunch = C8 ? 128 : 168, kRegsSoftmax = C8 ? 200 : 216,
-                       kRegsOther = C8 ? 56 : 72;
-  static_assert(2 * 128 * kRegsSoftmax + (kThreads - 256) * kRegsOther <= kThreads * kRegsLaunch,
-                "registers");
-};
+// C8 (a cache of bytes): warps 10 and 11 turn the tiles, each with so many 16-byte loads at once. More
+// disturb the MMAs' reads of shared memory (1, 2, 4, 8: 2.50, 2.24, 2.55, 2.72 ms for 4093 tokens at 32771
+// keys), and four such warps, which leave the softmax 200 registers, are no faster (2.36 ms).
+constexpr int kTurners = 2, kInFlight = 2;
+// registers: softmax 2 x 128 threads x 216 + 128 x 72 = 64512 = 384 x 168 at launch
+constexpr int kRegsLaunch = 168, kRegsSoftmax = 216, kRegsOther = 72;
+static_assert(2 * 128 * kRegsSoftmax + 128 * kRegsOther <= kThreadsC * kRegsLaunch, "registers");
 constexpr int kTmemS = 0, kTmemO = 256;  // + 128 for tile B
 constexpr float kLazy = 8.f;             // log2 of what a score may exceed the reference by
 // The same for a cache of bytes, whose P is always f16: as far as f16 goes. The scales' logarithms are
@@ -508,7 +505,7 @@ __device__ __forceinline__ float max3v(float a, float b, float c) {
 
 // ---- the kernel --------------------------------------------------------------------------------
 
-constexpr int kPieceRing = 4, kPieceReaders = 8 + 2;  // softmax warps, MMA, fixer
+constexpr int kPieceRing = 4, kPieceReaders = 8 + 2;  // softmax warps, MMA, fixer (C8: kTurners)
 // Three Q buffers for the two tiles: the next item's A comes in while this one is still in use.
 constexpr int kQBufs = 3;
 constexpr int chunk_stages(int DP) { return DP == 128 ? 4 : 8; }
@@ -529,10 +526,9 @@ struct ChunkSmem {
   alignas(1024) uint8_t ring[kStages][kTileBytes];  // [half][key][64]
   // of each kGroup keys: the scale of K, log2 and reciprocal of V's, and (in the first) the lowest log2
   float4 scale[C8 ? kScaleRing : 1][kTileK / kGroup];
-  int8_t q_log2[C8 ? kQBufs : 1][kTileM];  // what a row of q was divided by
   uint64_t full[kStages], empty[kStages];
   uint64_t land[kStages];  // a V tile that the fixer completes has landed (C8: any tile)
-  uint64_t q_full[kQBufs], q_empty[kQBufs], q_land[C8 ? kQBufs : 1];
+  uint64_t q_full[kQBufs], q_empty[kQBufs];
   uint64_t scale_full[C8 ? kScaleRing : 1];
   uint64_t s_full[2], p_ready[2][2], o_full[2];  // p_ready: by halves of the keys
   Piece piece[kPieceRing];
@@ -754,12 +750,11 @@ constexpr int raw_at(int tile_bytes) { return tile_bytes - kTileK * 128; }
 
 // chunk_load for a cache of bytes. All tiles signal land[]; lanes 0..7 bring the scales of the tile's
 // groups of keys.
-template <typename T, int DP>
+template <int DP>
 __device__ void chunk_load8(const AttnParams& P, const AttnMaps& M, const Plan& plan, int tok1,
                             ChunkSmem<DP, true>* sh) {
   using Smem = ChunkSmem<DP, true>;
   constexpr int kStages = Smem::kStages, kH = DP / 64, kGroups = kTileK / kGroup;
-  constexpr bool kTurn = !std::is_same<T, __half>::value;  // q is turned into f16 too
   const int lane = threadIdx.x & 31;
   const ChunkSync<DP, true> sy{sh, P.status};
   const int page = 1 << P.page_log2;
@@ -791,12 +786,11 @@ __device__ void chunk_load8(const AttnParams& P, const AttnMaps& M, const Plan& 
     auto load_q = [&](const RowTile& rt) {
       if (!sy.wait_warp(&sh->q_empty[qb], q_par)) return false;
       if (lane == 0) {
-        uint64_t* bar = kTurn ? &sh->q_land[qb] : &sh->q_full[qb];
-        mbar_arrive_expect_tx(bar, q_bytes);
+        mbar_arrive_expect_tx(&sh->q_full[qb], q_bytes);
 #pragma unroll
         for (int h = 0; h < kH; ++h)
           tma_4d(smem_u32(sh->q[qb]) + h * kTileM * 128, &M.q, h * 64, 0, p.head,
-                 p.q_tok + rt.tok0, bar);
+                 p.q_tok + rt.tok0, &sh->q_full[qb]);
       }
       __syncwarp();
       if (++qb == kQBufs) qb = 0, q_par ^= 1u;
@@ -868,10 +862,11 @@ __device__ void chunk_load8(const AttnParams& P, const AttnMaps& M, const Plan& 
   }
   for (int i = 0; i < kQBufs; ++i)
     for (uint32_t k = 0; k < kSpinLimit; ++k)
-      if (mbar_try_wait(kTurn ? &sh->q_land[i] : &sh->q_full[i], i < qb ? q_par ^ 1u : q_par)) break;
+      if (mbar_try_wait(&sh->q_full[i], i < qb ? q_par ^ 1u : q_par)) break;
 }
 
-// 16 codes as f16 numbers.
+// 16 codes as numbers of T (exact, NaN among them).
+template <typename T>
 __device__ __forceinline__ void codes16(const uint4& x, uint32_t (&f)[8]) {
   const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
@@ -879,14 +874,21 @@ __device__ __forceinline__ void codes16(const uint4& x, uint32_t (&f)[8]) {
     f[2 * i] = e4m3x2_to_f16x2((uint16_t)(w[i] & 0xffffu));
     f[2 * i + 1] = e4m3x2_to_f16x2((uint16_t)(w[i] >> 16));
   }
+  if constexpr (!std::is_same<T, __half>::value) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 v = unpack2<__half>(f[i]);
+      f[i] = pack2<T>(v.x, v.y);
+    }
+  }
 }
 
-// kTurners warps (`part` of the rows each) turn what lands into f16 operands, in place. A row's bytes
+// kTurners warps (`part` of the rows each) turn what lands into 16-bit operands, in place: K into q's type
+// T, since both operands of a product have one, V into f16, like P. (Turning bf16 queries into f16
+// instead kept the start of an item waiting: 8 prompts 144 us against 129.) A row's bytes
 // become (DP = 128) a row of the first 64 elements in the lower half of the stage and one of the others
-// where the bytes were, so no row waits for another. V rows that no token sees become zeros. A warp has
-// all of its part in flight at once: the MMAs keep shared memory busy, and its loads wait long (two
-// warps, 4 or 8 loads at once: 2.68 and 2.45 ms for the chunk at 32771 keys).
-template <int DP>
+// where the bytes were, so no row waits for another. V rows that no token sees become zeros.
+template <typename T, int DP>
 __device__ void chunk_turn(const AttnParams& P, int tok1, int part, ChunkSmem<DP, true>* sh) {
   using Smem = ChunkSmem<DP, true>;
   constexpr int kStages = Smem::kStages;
@@ -895,13 +897,13 @@ __device__ void chunk_turn(const AttnParams& P, int tok1, int part, ChunkSmem<DP
   constexpr int kLanes = DP / 16;        // lanes of a row, 16 bytes each
   constexpr int kRows = 32 / kLanes;     // rows of an access of the warp
   constexpr int kAccesses = kTileK / kTurners / kRows;
-  const int c = lane % kLanes;
-  // (DP = 64: rows 4 apart side by side, whose chunks lie in other banks)
+  const int c = lane % kLanes;           // elements 16 c ..: two 16-byte chunks of half h
+  const int h = c >> 2, o = 2 * (c & 3);
+  // The rows that eight lanes meet together. DP = 128: the second half of the row beside the one whose
+  // first half the others turn, which the swizzle puts into the other eight chunks' banks. DP = 64: rows
+  // 4 apart, for the same reason.
   const int row0 = part * (kTileK / kTurners) +
-                   (DP == 64 ? (lane / kLanes >> 1) + 4 * (lane / kLanes & 1) : lane / kLanes);
-  // elements 16 c ..: two 16-byte chunks of half h; the halves' lanes store theirs in opposite orders, so
-  // that the eight of a row meet eight different chunks
-  const int h = c >> 2, o0 = 2 * (c & 3) + h, o1 = o0 ^ 1;
+                   (DP == 64 ? (lane / kLanes >> 1) + 4 * (lane / kLanes & 1) : lane / kLanes ^ h);
   int stage = 0;
   uint32_t land_par = 0;  // a bit per stage
   PieceReader<DP, true> pieces;
@@ -912,26 +914,34 @@ __device__ void chunk_turn(const AttnParams& P, int tok1, int part, ChunkSmem<DP
       if (!sy.wait_warp(&sh->land[stage], (land_par >> stage) & 1u)) return;
       land_par ^= 1u << stage;
       uint8_t* tile = sh->ring[stage];
-      const bool cut = (j & 1) && (key0 < p.lo || key0 + kTileK > p.hi);
-      uint4 x[kAccesses];
+      constexpr int kAtOnce = kAccesses < kInFlight ? kAccesses : kInFlight;
+      auto turn = [&](auto type, bool cut) {
+#pragma unroll 1
+        for (int u0 = 0; u0 < kAccesses; u0 += kAtOnce) {
+          uint4 x[kAtOnce];
 #pragma unroll
-      for (int u = 0; u < kAccesses; ++u) {
-        const int row = row0 + u * kRows;
-        x[u] = *reinterpret_cast<const uint4*>(tile + raw_at(Smem::kTileBytes) + row * 128 +
-                                               ((c ^ (row & 7)) << 4));
-        if (cut && (key0 + row < p.lo || key0 + row >= p.hi)) x[u] = make_uint4(0, 0, 0, 0);
-      }
-      __syncwarp();  // a row's bytes have been read before they are written over
+          for (int u = 0; u < kAtOnce; ++u) {
+            const int row = row0 + (u0 + u) * kRows;
+            x[u] = *reinterpret_cast<const uint4*>(tile + raw_at(Smem::kTileBytes) + row * 128 +
+                                                   ((c ^ (row & 7)) << 4));
+            if (cut && (key0 + row < p.lo || key0 + row >= p.hi)) x[u] = make_uint4(0, 0, 0, 0);
+          }
+          __syncwarp();  // a row's bytes have been read before they are written over
 #pragma unroll
-      for (int u = 0; u < kAccesses; ++u) {
-        const int row = row0 + u * kRows;
-        uint32_t f[8];
-        codes16(x[u], f);
-        const uint4 first = make_uint4(f[0], f[1], f[2], f[3]), second = make_uint4(f[4], f[5], f[6], f[7]);
-        uint8_t* to = tile + h * kTileK * 128 + row * 128;
-        *reinterpret_cast<uint4*>(to + ((o0 ^ (row & 7)) << 4)) = h ? second : first;
-        *reinterpret_cast<uint4*>(to + ((o1 ^ (row & 7)) << 4)) = h ? first : second;
-      }
+          for (int u = 0; u < kAtOnce; ++u) {
+            const int row = row0 + (u0 + u) * kRows;
+            uint32_t f[8];
+            codes16<decltype(type)>(x[u], f);
+            uint8_t* to = tile + h * kTileK * 128 + row * 128;
+            *reinterpret_cast<uint4*>(to + ((o ^ (row & 7)) << 4)) = make_uint4(f[0], f[1], f[2], f[3]);
+            *reinterpret_cast<uint4*>(to + ((o + 1 ^ (row & 7)) << 4)) = make_uint4(f[4], f[5], f[6], f[7]);
+          }
+        }
+      };
+      if (j & 1)
+        turn(__half(), key0 < p.lo || key0 + kTileK > p.hi);
+      else
+        turn(T(), false);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->full[stage]);
@@ -940,60 +950,7 @@ __device__ void chunk_turn(const AttnParams& P, int tok1, int part, ChunkSmem<DP
   }
 }
 
-// Two warps turn bf16 queries into f16, in place, a row that f16 would not hold with all its bits times a
-// power of two.
-template <int DP>
-__device__ void chunk_turn_q(const AttnParams& P, int tok1, int part, ChunkSmem<DP, true>* sh) {
-  constexpr int kH = DP / 64;
-  const int lane = threadIdx.x & 31, c = lane & 7;
-  const ChunkSync<DP, true> sy{sh, P.status};
-  int qb = 0;
-  uint32_t q_par = 0;
-  PieceReader<DP, true> pieces;
-  for (Piece p; pieces.next(sy, p);) {
-    for (int t = 0; t < 2; ++t) {
-      if (row_tile(P, p, t, tok1).n == 0) continue;
-      if (!sy.wait_warp(&sh->q_land[qb], q_par)) return;
-      uint8_t* q = sh->q[qb];
-#pragma unroll 2
-      for (int i = 0; i < kTileM / 2 / 4; ++i) {  // 8 lanes a row
-        const int row = part * (kTileM / 2) + i * 4 + (lane >> 3);
-        uint4 x[kH];
-        uint32_t top = 0;  // largest |x|: bf16 bits in the upper half
-#pragma unroll
-        for (int h = 0; h < kH; ++h) {
-          x[h] = *reinterpret_cast<const uint4*>(q + h * kTileM * 128 + row * 128 + c * 16);
-          const uint32_t w[4] = {x[h].x, x[h].y, x[h].z, x[h].w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) top = max(top, max(w[k] << 16 & 0x7fff0000u, w[k] & 0x7fff0000u));
-        }
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const int ex = (int)(top >> 23) - 127;
-        const int e = top && ex < 128 && (ex < -4 || ex > 14) ? (ex > 14 ? ex - 14 : max(ex, -126)) : 0;
-        const float by = __uint_as_float((uint32_t)(127 - e) << 23);
-        if (c == 0) sh->q_log2[qb][row] = (int8_t)e;
-#pragma unroll
-        for (int h = 0; h < kH; ++h) {
-          uint32_t w[4] = {x[h].x, x[h].y, x[h].z, x[h].w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float2 f = unpack2<__nv_bfloat16>(w[k]);
-            w[k] = pack2<__half>(f.x * by, f.y * by);
-          }
-          *reinterpret_cast<uint4*>(q + h * kTileM * 128 + row * 128 + c * 16) =
-              make_uint4(w[0], w[1], w[2], w[3]);
-        }
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh->q_full[qb]);
-      if (++qb == kQBufs) qb = 0, q_par ^= 1u;
-    }
-  }
-}
-
-// T: the operands' type.
+// T: q's type.
 template <typename T, int DP, bool C8>
 __device__ void chunk_mma(const AttnParams& P, int tok1, ChunkSmem<DP, C8>* sh) {
   constexpr int kStages = ChunkSmem<DP, C8>::kStages;
@@ -1003,7 +960,8 @@ __device__ void chunk_mma(const AttnParams& P, int tok1, ChunkSmem<DP, C8>* sh) 
   const uint32_t qd = desc_low(smem_u32(sh->q[0]), 16);
   const uint32_t kd = desc_low(smem_u32(sh->ring[0]), 16);
   const uint32_t vd = desc_low(smem_u32(sh->ring[0]), kTileK * 128);
-  constexpr uint32_t kIdS = idesc<T>(kTileK, false), kIdO = idesc<T>(DP, true);
+  using TP = typename std::conditional<C8, __half, T>::type;  // P's and V's type
+  constexpr uint32_t kIdS = idesc<T>(kTileK, false), kIdO = idesc<TP>(DP, true);
   int stage = 0;
   int qb = 0, q_of[2] = {0, 0};  // next Q buffer; the tiles' buffers
   uint32_t parity = 0, q_par = 0, p_par[2] = {0, 0};
@@ -1103,7 +1061,6 @@ __device__ __forceinline__ void st_sector(void* p, const uint32_t (&w)[8]) {
 template <typename T, int DP, bool C8>
 __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP, C8>* sh) {
   using TP = typename std::conditional<C8, __half, T>::type;  // P's type
-  constexpr bool kTurn = C8 && !std::is_same<T, __half>::value;
   const ChunkSync<DP, C8> sy{sh, P.status};
   const int row = threadIdx.x & 127, lane = threadIdx.x & 31;
   const uint32_t lanes = (uint32_t)(row & ~31) << 16;
@@ -1114,7 +1071,6 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
   const bool flip = P.scale_log2 < 0.f;
   const float sc = fmaxf(fabsf(P.scale_log2), 1e-30f);
   int q_next = 0;
-  uint32_t q_wrap = 0;  // C8: parity of the next Q buffer's phase
   uint32_t tile_at = 0;  // C8: key tiles of the pieces before
   uint32_t s_par = 0, o_par = 0;
   constexpr int kSlot = 2 * kTileM * (DP + 2);
@@ -1124,14 +1080,12 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
     // Q buffers are taken in order: A's, B's, the next item's A's, ...
     const int n_other = row_tile(P, p, x ^ 1, tok1).n;
     int q_mine = q_next;
-    uint32_t q_par = q_wrap;
-    if (rt.n > 0 && x == 1 && n_other > 0) q_mine = q_mine + 1 == kQBufs ? (q_par ^= 1u, 0) : q_mine + 1;
+    if (rt.n > 0 && x == 1 && n_other > 0) q_mine = q_mine + 1 == kQBufs ? 0 : q_mine + 1;
     q_next += (rt.n > 0) + (n_other > 0);
-    if (q_next >= kQBufs) q_next -= kQBufs, q_wrap ^= 1u;
+    if (q_next >= kQBufs) q_next -= kQBufs;
     const uint32_t tile0 = tile_at;
     if constexpr (C8) tile_at += max(rt.n, n_other);
     if (rt.toks == 0) continue;
-    float sc_row = sc;  // C8: scores are those of the codes, times this and the scale of the keys
     const bool live = tok < rt.toks;
     // keys this row sees: [kmin, kmax); the tile's rows all see [tile_min, tile_max)
     const int pos0 = p.pos + rt.tok0;
@@ -1145,14 +1099,6 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
       s_par ^= 1u;
       tc_after();
       const float4* scales = nullptr;
-      if constexpr (kTurn) {
-        // (S is there, so this phase has passed, and no later one: this warp still holds the buffer.
-        // Waited for before S, a warp that had no keys in the items before could be a phase too early.)
-        if (j == 0) {
-          if (!sy.wait_warp(&sh->q_full[q_mine], q_par)) return;
-          sc_row *= __uint_as_float((uint32_t)(127 + sh->q_log2[q_mine][row]) << 23);
-        }
-      }
       if constexpr (C8) {
         constexpr uint32_t kScaleRing = ChunkSmem<DP, C8>::kScaleRing;
         const uint32_t at = tile0 + j;
@@ -1243,7 +1189,7 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
 #pragma unroll
           for (int i = 0; i < kPairs; ++i) {
             const float4 u = scales[i / (kGroup / 2)];
-            const float a = off_row ? fmaxf(u.x * sc_row, kLeast) : 1.f, b = off_row ? u.y : 0.f;
+            const float a = off_row ? fmaxf(u.x * sc, kLeast) : 1.f, b = off_row ? u.y : 0.f;
             unpair(fma2v(pair(s[2 * i], s[2 * i + 1]), pair(a, a), pair(b, b)), s[2 * i], s[2 * i + 1]);
           }
         }
@@ -1259,7 +1205,7 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
         auto scaled = [&](int i, float& m) {
           if constexpr (C8) {
             if (i % kGroupPairs == 0) {
-              const float a = off_row ? 1.f : fmaxf(ahead.x * sc_row, kLeast);
+              const float a = off_row ? 1.f : fmaxf(ahead.x * sc, kLeast);
               const float b = off_row ? -ref : ahead.y - ref;
               sc2 = pair(a, a), off2 = pair(b, b);
             } else if (i % kGroupPairs == 1 && i + kGroupPairs < kPairs) {
@@ -1402,7 +1348,7 @@ __device__ void chunk_softmax(const AttnParams& P, int tok1, int x, ChunkSmem<DP
 }
 
 template <typename T, int DP, bool C8>
-__global__ void __launch_bounds__(ChunkShape<C8>::kThreads, 1)
+__global__ void __launch_bounds__(kThreadsC, 1)
     k_attn_chunk(const __grid_constant__ AttnMaps M, const __grid_constant__ AttnParams P,
                  const __grid_constant__ Plan plan, int tok1) {
   extern __shared__ uint8_t smem_raw[];
@@ -1411,15 +1357,13 @@ __global__ void __launch_bounds__(ChunkShape<C8>::kThreads, 1)
   const int warp = threadIdx.x >> 5;
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
-    constexpr bool kTurn = C8 && !std::is_same<T, __half>::value;
     for (int i = 0; i < ChunkSmem<DP, C8>::kStages; ++i) {
       mbar_init(&sh->full[i], C8 ? kTurners : 1);
       mbar_init(&sh->empty[i], 1);
       mbar_init(&sh->land[i], 1);
     }
     for (int i = 0; i < kQBufs; ++i) {
-      mbar_init(&sh->q_full[i], kTurn ? 2 : 1);
-      if (kTurn) mbar_init(&sh->q_land[i], 1);
+      mbar_init(&sh->q_full[i], 1);
       mbar_init(&sh->q_empty[i], 4);  // the tile's softmax warps
     }
     for (int x = 0; x < 2; ++x) {
@@ -1430,7 +1374,7 @@ __global__ void __launch_bounds__(ChunkShape<C8>::kThreads, 1)
     }
     for (int i = 0; i < kPieceRing; ++i) {
       mbar_init(&sh->piece_full[i], 1);
-      mbar_init(&sh->piece_empty[i], C8 ? 8 + 1 + kTurners + 2 * kTurn : kPieceReaders);
+      mbar_init(&sh->piece_empty[i], kPieceReaders + (C8 ? kTurners - 1 : 0));
     }
     for (int i = 0; C8 && i < ChunkSmem<DP, C8>::kScaleRing; ++i) mbar_init(&sh->scale_full[i], 1);
     mbar_init(&sh->drain, 1);
@@ -1451,19 +1395,17 @@ __global__ void __launch_bounds__(ChunkShape<C8>::kThreads, 1)
   tc_after();
   pdl_wait();
   if (warp < kWarpMma) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(ChunkShape<C8>::kRegsSoftmax));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
     chunk_softmax<T, DP, C8>(P, tok1, warp >> 2, sh);
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(ChunkShape<C8>::kRegsOther));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
     if (warp == kWarpMma) {
-      chunk_mma<typename std::conditional<C8, __half, T>::type, DP, C8>(P, tok1, sh);
+      chunk_mma<T, DP, C8>(P, tok1, sh);
     } else if constexpr (C8) {
       if (warp == kWarpLoad)
-        chunk_load8<T, DP>(P, M, plan, tok1, sh);
-      else if (warp < kWarpTurnQ)
-        chunk_turn<DP>(P, tok1, warp - kWarpFix, sh);
-      else if (!std::is_same<T, __half>::value)
-        chunk_turn_q<DP>(P, tok1, warp - kWarpTurnQ, sh);
+        chunk_load8<DP>(P, M, plan, tok1, sh);
+      else
+        chunk_turn<T, DP>(P, tok1, warp - kWarpFix, sh);
     } else {
       if (warp == kWarpLoad)
         chunk_load<DP>(P, M, plan, tok1, sh);
@@ -1569,7 +1511,7 @@ int run_chunk(const AttnMaps& M, const AttnParams& P, const Plan& plan, int tok1
   static const bool fits = [] {
     cudaFuncAttributes at;
     return cudaFuncGetAttributes(&at, k_attn_chunk<T, DP, C8>) == cudaSuccess &&
-           at.numRegs >= ChunkShape<C8>::kRegsLaunch;
+           at.numRegs >= kRegsLaunch;
   }();
   if (!fits) return FTB_ERR_NOT_BUILT;
   static std::atomic<uint64_t> done{0}, plan_done{0};
@@ -1583,7 +1525,7 @@ int run_chunk(const AttnMaps& M, const AttnParams& P, const Plan& plan, int tok1
   err = launch_pdl(k_attn_plan, dim3(1), dim3(kPlanThreads), plan_smem, stream, P, plan, 2 * tok1,
                    sms);
   if (err != cudaSuccess) return cuda_status(err);
-  err = launch_pdl(k_attn_chunk<T, DP, C8>, dim3((unsigned)sms), dim3(ChunkShape<C8>::kThreads), smem, stream, M, P,
+  err = launch_pdl(k_attn_chunk<T, DP, C8>, dim3((unsigned)sms), dim3(kThreadsC), smem, stream, M, P,
                    plan, tok1);
   if (err != cudaSuccess) return cuda_status(err);
   return cuda_status(launch_pdl(k_attn_join<T, DP>, dim3((unsigned)sms * 8), dim3(256), 0, stream,
