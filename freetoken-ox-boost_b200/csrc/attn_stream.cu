@@ -61,6 +61,26 @@ struct StreamSmem {
   int abort;
 };
 
+// The form for up to 8 rows over a cache of bytes.
+constexpr int kRows8 = 8, kCtasPerSm8 = 3;
+template <int DP>
+struct StreamSmem8 {
+  static constexpr int kStages = 4;
+  alignas(1024) uint8_t ring[kStages][2][kTile * 128];
+  alignas(16) float merge[kConsumers][kRows8][DP / 2 + 4];  // half of the columns
+  BlockScale scale[kStages][kConsumers];
+  float ml[kConsumers][kRows8][2];
+  float fac[kConsumers][kRows8];
+  float row_m[kRows8], row_l[kRows8];
+  uint64_t full[kStages], empty[kStages];
+  int64_t scan[kThreads / kWarp];
+  int64_t start_item;
+  int64_t total;
+  int start_seq;
+  int flag;
+  int abort;
+};
+
 __device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -91,11 +111,12 @@ struct PairTiles {
   int lo, hi;  // keys
   int t0, t1;  // tiles
 };
+template <int R>  // rows of a row tile
 __device__ __forceinline__ PairTiles pair_tiles(const AttnParams& P, const AttnSeq& s, int row0) {
   PairTiles t{0, 0, 0, 0};
   const int64_t rows = (int64_t)s.n * P.G;
   if (row0 >= rows) return t;
-  const int last = (int)(rows < row0 + kRows ? rows : row0 + kRows) - 1;
+  const int last = (int)(rows < row0 + R ? rows : row0 + R) - 1;
   const KeyRange k = attn_range(P, s, row0 / P.G, last / P.G);
   if (k.lo >= k.hi) return t;
   t.lo = k.lo, t.hi = k.hi, t.t0 = k.lo / kTile, t.t1 = (k.hi + kTile - 1) / kTile;
@@ -103,6 +124,7 @@ __device__ __forceinline__ PairTiles pair_tiles(const AttnParams& P, const AttnS
 }
 
 // The walk over a block's share of the line; producer and consumers take the same steps.
+template <int R>
 struct Walk {
   int seq, head, tile;  // next tile of pair (seq, head)
   int64_t item;         // line position of the pair's first tile
@@ -113,7 +135,7 @@ struct Walk {
                         int64_t count) {
     seq = seq0;
     s = attn_seq(P, seq);
-    t = pair_tiles(P, s, row0);
+    t = pair_tiles<R>(P, s, row0);
     const int64_t off = at - seq_at;  // into the sequence's Hkv pairs
     const int n = t.t1 - t.t0;
     head = (int)(off / n);
@@ -136,16 +158,16 @@ struct Walk {
       do {
         ++seq;  // left > 0: a later sequence has tiles
         s = attn_seq(P, seq);
-        t = pair_tiles(P, s, row0);
+        t = pair_tiles<R>(P, s, row0);
       } while (t.t1 == t.t0);
     }
     tile = t.t0;
   }
 };
 
-template <int DP, bool C8>
+template <class Smem>
 struct StreamSync {
-  StreamSmem<DP, C8>* sh;
+  Smem* sh;
   uint32_t* status;
   __device__ bool wait(uint64_t* bar, uint32_t parity) const {
     if (mbar_try_wait(bar, parity)) return true;
@@ -164,10 +186,10 @@ struct StreamSync {
 // One warp. Copies the tiles of the share into the ring.
 template <int DP>
 __device__ void stream_producer(const AttnParams& P, const AttnMaps& M, StreamSmem<DP, false>* sh,
-                                Walk w, int row0) {
+                                Walk<kRows> w, int row0) {
   constexpr int kStages = StreamSmem<DP, false>::kStages;
   const int lane = threadIdx.x & 31;
-  const StreamSync<DP, false> sy{sh, P.status};
+  const StreamSync<StreamSmem<DP, false>> sy{sh, P.status};
   const int page = 1 << P.page_log2;
   const int r = page < kTile ? page : kTile;  // keys per box
   const int boxes = kTile / r;                // <= 8
@@ -226,63 +248,96 @@ __device__ void stream_producer(const AttnParams& P, const AttnMaps& M, StreamSm
       if (mbar_try_wait(&sh->full[u % kStages], (u / kStages) & 1u)) break;
 }
 
-// The same for a cache of bytes. Lanes 0..3 also bring the scales of the tile's 4 x 16 keys (a block of
-// tokens is 16 keys or more), while the tile's copies are on their way.
-template <int DP>
-__device__ void stream_producer8(const AttnParams& P, const AttnMaps& M, StreamSmem<DP, true>* sh,
-                                 Walk w, int row0) {
-  constexpr int kStages = StreamSmem<DP, true>::kStages;
+// A load that keeps its place among volatile statements: asked for before the waits that hide it.
+__device__ __forceinline__ int ldg_now(const int32_t* p) {
+  int r;
+  asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(r) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ float ldg_now(const float* p) {
+  float r;
+  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(r) : "l"(p));
+  return r;
+}
+
+// The same for a cache of bytes, whose scales come by plain loads: four groups of 16 keys per tile (a
+// block of tokens is 16 keys or more). A tile takes half as long as one of 16 bits, about as long as a
+// page id and the scales behind it take to come, so the lanes look after eight tiles at once, lane l after
+// group l % 4 of tile l / 4, and ask for the scales of the next eight and the ids of those after them
+// before they turn to these (one tile at a time: 123 us for 61 tokens at up to 8192 keys).
+template <class Smem, int R>
+__device__ void stream_producer8(const AttnParams& P, const AttnMaps& M, Smem* sh, Walk<R> w, int row0) {
+  constexpr int kStages = Smem::kStages;
+  constexpr int kGroups = kTile / 16, kAhead = kWarp / kGroups;
   const int lane = threadIdx.x & 31;
-  const StreamSync<DP, true> sy{sh, P.status};
+  const StreamSync<Smem> sy{sh, P.status};
   const int page = 1 << P.page_log2;
   const int r = page < kTile ? page : kTile;  // keys per box, >= 16
-  const int boxes = kTile / r;                // <= 4
+  const int boxes = kTile / r;                // <= kGroups
+  const int my_box = (lane & (kGroups - 1)) * 16 / r;
   int stage = 0;
   uint32_t parity = 1, issued = 0;
   bool ok = true;
   while (w.left > 0 && ok) {
     const int n = w.take();
-    for (int j = 0; j < n && ok; ++j) {
-      const int key0 = (w.tile + j) * kTile;
-      // boxes with a key in [lo, hi)
-      const int b0 = w.t.lo > key0 ? (w.t.lo - key0) / r : 0;
-      int b1 = (w.t.hi - key0 + r - 1) / r;
-      if (b1 > boxes) b1 = boxes;
-      int id = 0;  // page of keys 16 lane ..
-      const int key = key0 + lane * 16, box_of = lane * 16 / r;
-      const bool has = lane < kTile / 16 && box_of >= b0 && box_of < b1;
-      if (has) {
-        id = P.block_table[(int64_t)w.seq * P.table_stride + (key >> P.page_log2)];
-        if (id < 0 || id >= P.num_pages) {
-          atomicOr(P.status, kAttnBadPage);
-          id = (int)P.num_pages;  // outside the tensor: reads zeros
+    const int32_t* table = P.block_table + (int64_t)w.seq * P.table_stride;
+    const float* ks_of = P.k_scale + w.head * P.ks_st[2];
+    const float* vs_of = P.v_scale + w.head * P.vs_st[2];
+    // boxes [b0, b1) of a tile have a key in [lo, hi)
+    auto box0 = [&](int key0) { return w.t.lo > key0 ? (w.t.lo - key0) / r : 0; };
+    auto box1 = [&](int key0) { return min(boxes, (w.t.hi - key0 + r - 1) / r); };
+    // the first key of this lane's group of the tiles from j0 on; whether anybody reads it
+    auto key_at = [&](int j0) { return (w.tile + j0) * kTile + lane * 16; };
+    auto wanted = [&](int j0) {
+      const int key0 = (w.tile + j0 + lane / kGroups) * kTile;
+      return j0 + lane / kGroups < n && my_box >= box0(key0) && my_box < box1(key0);
+    };
+    auto load_id = [&](int j0) {  // -1: not wanted
+      return wanted(j0) ? ldg_now(table + (key_at(j0) >> P.page_log2)) : -1;
+    };
+    auto load_scales = [&](int j0, int id, float& ks, float& vs) {
+      ks = vs = 1.f;
+      if (id >= 0 && id < P.num_pages) {
+        const int block = (key_at(j0) & (page - 1)) >> P.block_log2;
+        ks = ldg_now(ks_of + id * P.ks_st[0] + block * P.ks_st[1]);
+        vs = ldg_now(vs_of + id * P.vs_st[0] + block * P.vs_st[1]);
+      }
+    };
+    int id = load_id(0), id_next = load_id(kAhead);
+    float ks, vs;
+    load_scales(0, id, ks, vs);
+    for (int j0 = 0; j0 < n && ok; j0 += kAhead) {
+      float ks_next, vs_next;
+      load_scales(j0 + kAhead, id_next, ks_next, vs_next);
+      const int id_after = load_id(j0 + 2 * kAhead);
+      if (wanted(j0) && (id < 0 || id >= P.num_pages)) {
+        atomicOr(P.status, kAttnBadPage);
+        id = (int)P.num_pages;  // outside the tensor: reads zeros
+      }
+      const int count = min(kAhead, n - j0);
+      for (int j = 0; j < count; ++j) {
+        const int key0 = (w.tile + j0 + j) * kTile;
+        const int b0 = box0(key0), b1 = box1(key0);
+        // (a box's groups are of one page)
+        const int box_id = __shfl_sync(0xffffffffu, id, j * kGroups + ((lane * r >> 4) & (kGroups - 1)));
+        ok = __all_sync(0xffffffffu, sy.wait(&sh->empty[stage], parity));
+        if (!ok) break;
+        ++issued;
+        if (lane >= b0 && lane < b1) {
+          const uint32_t at = lane * r * 128;
+          const int row = (key0 + lane * r) & (page - 1);
+          tma_5d(smem_u32(sh->ring[stage][0]) + at, &M.k, 0, row, w.head, box_id, 0, &sh->full[stage]);
+          tma_5d(smem_u32(sh->ring[stage][1]) + at, &M.v, 0, row, w.head, box_id, 0, &sh->full[stage]);
         }
+        if (lane / kGroups == j) sh->scale[stage][lane & (kGroups - 1)] = block_scale(ks, vs);
+        __syncwarp();
+        // (the phase stays open for this arrival, whatever has landed by now)
+        if (lane == 0)
+          mbar_arrive_expect_tx(&sh->full[stage], 2u * (uint32_t)(b1 - b0) * (uint32_t)r * 128u);
+        __syncwarp();
+        if (++stage == kStages) stage = 0, parity ^= 1u;
       }
-      const int box_id = __shfl_sync(0xffffffffu, id, (lane * r >> 4) & 3);
-      ok = __all_sync(0xffffffffu, sy.wait(&sh->empty[stage], parity));
-      if (!ok) break;
-      ++issued;
-      if (lane >= b0 && lane < b1) {
-        const uint32_t at = lane * r * 128;
-        const int row = (key0 + lane * r) & (page - 1);
-        tma_5d(smem_u32(sh->ring[stage][0]) + at, &M.k, 0, row, w.head, box_id, 0, &sh->full[stage]);
-        tma_5d(smem_u32(sh->ring[stage][1]) + at, &M.v, 0, row, w.head, box_id, 0, &sh->full[stage]);
-      }
-      if (lane < kTile / 16) {
-        float ks = 1.f, vs = 1.f;
-        if (has && id < P.num_pages) {
-          const int block = (key & (page - 1)) >> P.block_log2;
-          ks = __ldg(P.k_scale + id * P.ks_st[0] + block * P.ks_st[1] + w.head * P.ks_st[2]);
-          vs = __ldg(P.v_scale + id * P.vs_st[0] + block * P.vs_st[1] + w.head * P.vs_st[2]);
-        }
-        sh->scale[stage][lane] = block_scale(ks, vs);
-      }
-      __syncwarp();
-      // (the phase stays open for this arrival, whatever has landed by now)
-      if (lane == 0)
-        mbar_arrive_expect_tx(&sh->full[stage], 2u * (uint32_t)(b1 - b0) * (uint32_t)r * 128u);
-      __syncwarp();
-      if (++stage == kStages) stage = 0, parity ^= 1u;
+      id = id_next, id_next = id_after, ks = ks_next, vs = vs_next;
     }
     w.next(P, row0, n);
   }
@@ -300,8 +355,8 @@ __device__ __forceinline__ int key_of(int n) { return n & 1 ? (n - 1) ^ 5 : n; }
 // of each 64, as K's bytes lie in a lane. bf16 rows whose largest element f16 would not hold with all
 // its bits are taken times a power of two (returned: its inverse).
 template <typename T, int DP>
-__device__ __forceinline__ float load_q8(const uint16_t* qp, bool in, int D, int e,
-                                         uint32_t (&qa)[DP / 16][4]) {
+__device__ __forceinline__ float load_q8(const uint16_t* qp, bool in, int D,
+                                         uint32_t (&lo)[DP / 16], uint32_t (&hi)[DP / 16]) {
   const int tig = threadIdx.x & 3;
   uint4 w[DP / 64][2];
 #pragma unroll
@@ -347,19 +402,362 @@ __device__ __forceinline__ float load_q8(const uint16_t* qp, bool in, int D, int
 #pragma unroll
       for (int k = 0; k < 4; k += 2) {
         const int c = h * 4 + i * 2 + (k >> 1);
-        qa[c][e] = v[k], qa[c][2 + e] = v[k + 1];
+        lo[c] = v[k], hi[c] = v[k + 1];
       }
     }
   return back;
 }
 
+// An 8 x 8 matrix of 16-bit elements, a row's pair per lane, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+// Up to 8 rows over a cache of bytes. The rows are the N of the products, so that none of their 16 M is
+// wasted on rows that are not there:
+//   S^T = K Q^T    M = 16 keys of the warp, K = 16 elements
+//   O^T = V^T P^T  M = 16 columns of V, K = 16 keys; P goes from the accumulators of S^T to the operand by
+//                  a transposition of 8 x 8 (movmatrix)
+// Half the products, exponentials and registers of the form above, and three blocks per SM: the work is
+// bound by latencies (61 tokens at up to 8192 keys 130 us with it).
+// A row's reference moves to a tile's maximum where that exceeds it by more than 2^kLazy (P reaches
+// 2^kLazy, f16 holds it), so the warp's maxima are rarely brought together: one vote per tile.
+template <typename T, int DP>
+__device__ void stream_consumer8(const AttnParams& P, StreamSmem8<DP>* sh, Walk<kRows8> w, int row0,
+                                 int64_t share) {
+  using Smem = StreamSmem8<DP>;
+  constexpr int kStages = Smem::kStages, VB = DP / 8;
+  constexpr float kLazy = 10.f;
+  constexpr bool kRest = std::is_same<T, __half>::value;  // (as above)
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t2 = (lane & 3) * 2;  // key (or columns) of the lane; its rows t2, t2 + 1
+  const StreamSync<Smem> sy{sh, P.status};
+  // K: keys kr, kr + 8 of the tile, chunk lane % 4 of each 64 elements; V: keys kv[e], kv[e] + 8, VB bytes
+  const int kr = warp * 16 + key_of(g), kv0 = warp * 16 + key_of(t2), kv1 = warp * 16 + key_of(t2 + 1);
+  auto v_at = [&](int key) {
+    const int byte = g * VB;
+    return key * 128 + (((byte >> 4) ^ (key & 7)) << 4) + (byte & 15);
+  };
+  int stage = 0;
+  uint32_t parity = 0;  // + kGaveUp once a wait did
+  constexpr uint32_t kGaveUp = 2;
+  while (w.left > 0) {
+    const int n = w.take();
+    const AttnSeq s = w.s;
+    const int rows_all = s.n * P.G - row0;
+    const int rows = rows_all < kRows8 ? rows_all : kRows8;
+    int kmin[2], kmax[2];  // keys of rows t2, t2 + 1
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      kmin[e] = kmax[e] = 0;
+      if (t2 + e < rows) {
+        const int i = (row0 + t2 + e) / P.G;
+        const KeyRange k = attn_range(P, s, i, i);
+        kmin[e] = k.lo, kmax[e] = k.hi;
+      }
+    }
+    uint32_t q_lo[DP / 16], q_hi[DP / 16];  // row g
+    float factor[2];                        // of the codes' scores, rows t2, t2 + 1
+    {
+      const int row = row0 + g;
+      const uint16_t* qp =
+          P.q + (int64_t)(s.q0 + row / P.G) * P.q_st + (int64_t)(w.head * P.G + row % P.G) * P.q_sh;
+      const float back = load_q8<T, DP>(qp, g < rows, P.D, q_lo, q_hi) * P.scale_log2;
+      factor[0] = __shfl_sync(0xffffffffu, back, t2 * 4);
+      factor[1] = __shfl_sync(0xffffffffu, back, t2 * 4 + 4);
+    }
+    float ref[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    float o[VB / 2][4];  // columns VB g + 2 j, + 1 of rows t2, t2 + 1
+#pragma unroll
+    for (int j = 0; j < VB / 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[j][i] = 0.f;
+    for (int j = 0; j < n && parity < kGaveUp; ++j) {
+      const int key0 = (w.tile + j) * kTile + warp * 16;
+      if (!__all_sync(0xffffffffu, sy.wait(&sh->full[stage], parity))) {
+        parity = kGaveUp;
+        break;
+      }
+      const uint8_t *kb = sh->ring[stage][0], *vb = sh->ring[stage][1];
+      const BlockScale bs = sh->scale[stage][warp];
+      float sc[4] = {}, sd[4] = {};
+#pragma unroll
+      for (int c = 0; c < DP / 64; ++c) {
+        uint4 b[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          b[h] = *reinterpret_cast<const uint4*>(kb + (kr + 8 * h) * 128 +
+                                                 (((4 * c + (lane & 3)) ^ (kr & 7)) << 4));
+        const uint32_t v[2][4] = {{b[0].x, b[0].y, b[0].z, b[0].w}, {b[1].x, b[1].y, b[1].z, b[1].w}};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t a[4] = {e4m3x2_to_f16x2((uint16_t)(v[0][k] & 0xffffu)),
+                                 e4m3x2_to_f16x2((uint16_t)(v[1][k] & 0xffffu)),
+                                 e4m3x2_to_f16x2((uint16_t)(v[0][k] >> 16)),
+                                 e4m3x2_to_f16x2((uint16_t)(v[1][k] >> 16))};
+          mma16816<__half>(k & 1 ? sd : sc, a, q_lo[4 * c + k], q_hi[4 * c + k]);
+        }
+      }
+      // V's bytes, asked for before the exponentials; rows outside [lo, hi) may hold NaN: made zero
+      const bool inside = key0 >= w.t.lo && key0 + 16 <= w.t.hi;
+      uint32_t v[2][2][VB / 4];  // [key group][key's parity][bytes]
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int row = (e ? kv1 : kv0) + 8 * h;
+          if constexpr (VB == 16) {
+            const uint4 b = *reinterpret_cast<const uint4*>(vb + v_at(row));
+            v[h][e][0] = b.x, v[h][e][1] = b.y, v[h][e][2] = b.z, v[h][e][3] = b.w;
+          } else {
+            const uint2 b = *reinterpret_cast<const uint2*>(vb + v_at(row));
+            v[h][e][0] = b.x, v[h][e][1] = b.y;
+          }
+          const int key = key0 - warp * 16 + row;
+          if (!inside && (key < w.t.lo || key >= w.t.hi)) {
+#pragma unroll
+            for (int k = 0; k < VB / 4; ++k) v[h][e][k] = 0u;
+          }
+        }
+      const bool clean = inside && (!P.causal || s.n == 1) && (P.window <= 0 || s.n == 1);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = key0 + (i >> 1) * 8 + kr - warp * 16;
+        const bool seen = clean || (key >= kmin[i & 1] && key < kmax[i & 1]);
+        sc[i] = seen ? fmaf(sc[i] + sd[i], bs.k * factor[i & 1], bs.v_log2) : -INFINITY;
+      }
+      if (__any_sync(0xffffffffu, fmaxf(sc[0], sc[2]) > ref[0] + kLazy || fmaxf(sc[1], sc[3]) > ref[1] + kLazy)) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float mx = fmaxf(sc[e], sc[2 + e]);
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+          if (mx > ref[e] + kLazy) {  // (the same for all lanes of the row)
+            const float f = ex2(ref[e] - mx);
+            ref[e] = mx;
+            l[e] *= f;
+#pragma unroll
+            for (int jj = 0; jj < VB / 2; ++jj) o[jj][e] *= f, o[jj][2 + e] *= f;
+          }
+        }
+      }
+      float p[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] = ex2(sc[i] - (ref[i & 1] == -INFINITY ? 0.f : ref[i & 1]));
+#pragma unroll
+      for (int e = 0; e < 2; ++e) l[e] = fmaf(p[e] + p[2 + e], bs.v_inv, l[e]);
+      uint32_t pb[2], rb[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        pb[h] = pack2<__half>(p[2 * h], p[2 * h + 1]);
+        if constexpr (kRest) {
+          const float2 a = unpack2<__half>(pb[h]);
+          rb[h] = transpose8(pack2<__half>(p[2 * h] - a.x, p[2 * h + 1] - a.y));
+        }
+        pb[h] = transpose8(pb[h]);
+      }
+#pragma unroll
+      for (int k = 0; k < VB / 4; ++k) {
+        // bytes of two keys side by side, two columns to a word
+        uint32_t x[2][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          x[h][0] = __byte_perm(v[h][0][k], v[h][1][k], 0x5140);
+          x[h][1] = __byte_perm(v[h][0][k], v[h][1][k], 0x7362);
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const uint32_t a[4] = {e4m3x2_to_f16x2((uint16_t)(x[0][c] & 0xffffu)),
+                                 e4m3x2_to_f16x2((uint16_t)(x[0][c] >> 16)),
+                                 e4m3x2_to_f16x2((uint16_t)(x[1][c] & 0xffffu)),
+                                 e4m3x2_to_f16x2((uint16_t)(x[1][c] >> 16))};
+          mma16816<__half>(o[2 * k + c], a, pb[0], pb[1]);
+          if constexpr (kRest) mma16816<__half>(o[2 * k + c], a, rb[0], rb[1]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->empty[stage]);
+      if (++stage == kStages) stage = 0, parity ^= 1u;
+    }
+    if (parity >= kGaveUp) l[0] = l[1] = NAN;
+    // join the four warps' parts of the rows
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], x);
+      if (g == 0) {
+        sh->ml[warp][t2 + e][0] = ref[e];
+        sh->ml[warp][t2 + e][1] = l[e];
+      }
+    }
+    named_bar(1, kConsumers * kWarp);
+    if (threadIdx.x < kRows8) {
+      const int row = threadIdx.x;
+      float mm = sh->ml[0][row][0];
+      for (int i = 1; i < kConsumers; ++i) mm = fmaxf(mm, sh->ml[i][row][0]);
+      const float top = mm == -INFINITY ? 0.f : mm;
+      float ll = 0.f;
+      for (int i = 0; i < kConsumers; ++i) {
+        const float f = ex2(sh->ml[i][row][0] - top);
+        sh->fac[i][row] = f;
+        ll += f * sh->ml[i][row][1];
+      }
+      sh->row_m[row] = mm;
+      sh->row_l[row] = ll;
+    }
+    named_bar(1, kConsumers * kWarp);
+    const bool begins = w.tile == w.t.t0, ends = w.tile + n == w.t.t1;
+    const bool whole = begins && ends;
+    const int64_t blk = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+    constexpr int kSlot = kRows8 * DP + 2 * kRows8;
+    float* slot = P.partial + (2 * blk + (begins ? 1 : 0)) * kSlot;  // (as above)
+    const float f0 = sh->fac[warp][t2], f1 = sh->fac[warp][t2 + 1];
+    constexpr int kHalf = DP / 2, kPer = kHalf / 4;  // columns of a pass, threads of a row
+    const int orow = threadIdx.x / kPer, oc = threadIdx.x % kPer * 4;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      if (g >> 2 == c) {
+#pragma unroll
+        for (int i = 0; i < VB / 4; ++i) {
+          const float(&a)[4] = o[2 * i], (&b)[4] = o[2 * i + 1];
+          const int at = (g & 3) * VB + 4 * i;
+          *reinterpret_cast<float4*>(&sh->merge[warp][t2][at]) =
+              make_float4(a[0] * f0, a[2] * f0, b[0] * f0, b[2] * f0);
+          *reinterpret_cast<float4*>(&sh->merge[warp][t2 + 1][at]) =
+              make_float4(a[1] * f1, a[3] * f1, b[1] * f1, b[3] * f1);
+        }
+      }
+      named_bar(1, kConsumers * kWarp);
+      const int d = c * kHalf + oc;
+      if (orow < rows) {
+        float4 a = *reinterpret_cast<float4*>(&sh->merge[0][orow][oc]);
+#pragma unroll
+        for (int i = 1; i < kConsumers; ++i) {
+          const float4 b = *reinterpret_cast<float4*>(&sh->merge[i][orow][oc]);
+          a.x += b.x, a.y += b.y, a.z += b.z, a.w += b.w;
+        }
+        if (!whole) {
+          *reinterpret_cast<float4*>(slot + orow * DP + d) = a;
+        } else if (d < P.D) {
+          const float ll = sh->row_l[orow], inv = ll > 0.f || ll != ll ? 1.f / ll : 0.f;
+          const int row = row0 + orow;
+          uint16_t* op = P.out + ((int64_t)(s.q0 + row / P.G) * P.Hq + w.head * P.G + row % P.G) * P.D + d;
+          *reinterpret_cast<uint2*>(op) =
+              make_uint2(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv));
+        }
+      }
+      named_bar(1, kConsumers * kWarp);
+    }
+    if (whole) {
+      if (P.lse && threadIdx.x < rows) {
+        const int row = row0 + threadIdx.x;
+        P.lse[(int64_t)(s.q0 + row / P.G) * P.Hq + w.head * P.G + row % P.G] =
+            sh->row_l[threadIdx.x] == 0.f
+                ? -INFINITY
+                : (sh->row_m[threadIdx.x] + log2f(sh->row_l[threadIdx.x])) * 0.69314718055994531f;
+      }
+    } else {
+      if (threadIdx.x < rows) {
+        slot[kRows8 * DP + threadIdx.x] = sh->row_m[threadIdx.x];
+        slot[kRows8 * DP + kRows8 + threadIdx.x] = sh->row_l[threadIdx.x];
+      }
+      // blocks c0..c1 hold the pair's parts: the last one to get here joins them
+      const int64_t c0 = w.item / share, c1 = (w.item + (w.t.t1 - w.t.t0) - 1) / share;
+      const int64_t blk0 = (int64_t)blockIdx.y * gridDim.x + c0;
+      const int parts = (int)(c1 - c0) + 1;
+      __threadfence();
+      named_bar(1, kConsumers * kWarp);
+      if (threadIdx.x == 0) {
+        const bool last = atomicAdd(&P.counters[blk0], 1) == parts - 1;
+        if (last) P.counters[blk0] = 0;
+        sh->flag = last;
+        __threadfence();
+      }
+      named_bar(1, kConsumers * kWarp);
+      if (sh->flag) {
+        const float* p0 = P.partial + (2 * blk0 + 1) * kSlot;
+        const float* p1 = P.partial + 2 * (blk0 + 1) * kSlot;
+        // 16 threads a row, DP / 64 x 4 columns each; the threads of rows that are not there take their
+        // share of the parts: part i goes to way i % ways of its row
+        constexpr int kCols = DP / 64;
+        const int jc = (threadIdx.x & 15) * 4, trow = threadIdx.x >> 4;
+        const int lg = rows > 1 ? 32 - __clz(rows - 1) : 0, ways = kRows8 >> lg;
+        const int jrow = trow & ((1 << lg) - 1), way = trow >> lg;
+        const bool mine = jrow < rows;
+        float mm = -INFINITY, ll = 0.f;
+        float4 acc[kCols];
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+        auto add = [&](float f, const float4& b, int c) {
+          acc[c].x += f * b.x, acc[c].y += f * b.y, acc[c].z += f * b.z, acc[c].w += f * b.w;
+        };
+        if (mine) {
+          for (int i = way; i < parts; i += ways) {
+            const float* q = i == 0 ? p0 : p1 + (int64_t)(i - 1) * 2 * kSlot;
+            mm = fmaxf(mm, __ldcg(q + kRows8 * DP + jrow));
+          }
+          const float top = mm == -INFINITY ? 0.f : mm;
+          for (int i = way; i < parts; i += ways) {
+            const float* q = i == 0 ? p0 : p1 + (int64_t)(i - 1) * 2 * kSlot;
+            const float f = ex2(__ldcg(q + kRows8 * DP + jrow) - top);
+            ll += f * __ldcg(q + kRows8 * DP + kRows8 + jrow);
+#pragma unroll
+            for (int c = 0; c < kCols; ++c)
+              add(f, __ldcg(reinterpret_cast<const float4*>(q + jrow * DP + c * 64 + jc)), c);
+          }
+        }
+        if (ways > 1) {
+          static_assert(sizeof(sh->merge) >= kRows8 * DP * sizeof(float), "the ways' sums fit");
+          float* all = &sh->merge[0][0][0];
+#pragma unroll
+          for (int c = 0; c < kCols; ++c)
+            *reinterpret_cast<float4*>(all + trow * DP + c * 64 + jc) = acc[c];
+          if (jc == 0) sh->ml[0][trow][0] = mm, sh->ml[0][trow][1] = ll;
+          named_bar(1, kConsumers * kWarp);
+          if (mine && way == 0) {
+            for (int i = 1; i < ways; ++i) mm = fmaxf(mm, sh->ml[0][jrow + (i << lg)][0]);
+            const float top = mm == -INFINITY ? 0.f : mm;
+            ll = 0.f;
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int i = 0; i < ways; ++i) {
+              const int at = jrow + (i << lg);
+              const float f = ex2(sh->ml[0][at][0] - top);
+              ll += f * sh->ml[0][at][1];
+#pragma unroll
+              for (int c = 0; c < kCols; ++c)
+                add(f, *reinterpret_cast<const float4*>(all + at * DP + c * 64 + jc), c);
+            }
+          }
+          named_bar(1, kConsumers * kWarp);  // (the next pair writes the merge buffer)
+        }
+        if (mine && way == 0) {
+          const float inv = ll > 0.f || ll != ll ? 1.f / ll : 0.f;
+          const int row = row0 + jrow;
+          const int64_t at = (int64_t)(s.q0 + row / P.G) * P.Hq + w.head * P.G + row % P.G;
+#pragma unroll
+          for (int c = 0; c < kCols; ++c)
+            if (c * 64 + jc < P.D)
+              *reinterpret_cast<uint2*>(P.out + at * P.D + c * 64 + jc) = make_uint2(
+                  pack2<T>(acc[c].x * inv, acc[c].y * inv), pack2<T>(acc[c].z * inv, acc[c].w * inv));
+          if (P.lse && jc == 0)
+            P.lse[at] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) * 0.69314718055994531f;
+        }
+      }
+    }
+    w.next(P, row0, n);
+  }
+}
+
 template <typename T, int DP, bool C8>
-__device__ void stream_consumer(const AttnParams& P, StreamSmem<DP, C8>* sh, Walk w, int row0,
+__device__ void stream_consumer(const AttnParams& P, StreamSmem<DP, C8>* sh, Walk<kRows> w, int row0,
                                 int64_t share) {
   constexpr int kStages = StreamSmem<DP, C8>::kStages;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t2 = (lane & 3) * 2;
-  const StreamSync<DP, C8> sy{sh, P.status};
+  const StreamSync<StreamSmem<DP, C8>> sy{sh, P.status};
   // P's type: the tensors', or f16 beside V's codes, which are f16 numbers. The rounding's rest goes
   // along where the output is as fine as P.
   using TP = typename std::conditional<C8, __half, T>::type;
@@ -398,7 +796,10 @@ __device__ void stream_consumer(const AttnParams& P, StreamSmem<DP, C8>* sh, Wal
       }
       const uint16_t* qp = P.q + (int64_t)(s.q0 + i) * P.q_st + (int64_t)hq * P.q_sh;
       if constexpr (C8) {
-        q_back[e] = load_q8<T, DP>(qp, in, P.D, e, qa);
+        uint32_t lo[DP / 16], hi[DP / 16];
+        q_back[e] = load_q8<T, DP>(qp, in, P.D, lo, hi);
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) qa[c][e] = lo[c], qa[c][2 + e] = hi[c];
       } else {
 #pragma unroll
         for (int c = 0; c < DP / 16; ++c) {
@@ -740,17 +1141,19 @@ __device__ void stream_consumer(const AttnParams& P, StreamSmem<DP, C8>* sh, Wal
   }
 }
 
-template <typename T, int DP, bool C8>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm)
+// R: rows of a row tile. 8 is the form for few rows over a cache of bytes.
+template <typename T, int DP, bool C8, int R>
+__global__ void __launch_bounds__(kThreads, R == kRows8 ? kCtasPerSm8 : kCtasPerSm)
     k_attn_stream(const __grid_constant__ AttnMaps M, const __grid_constant__ AttnParams P) {
   extern __shared__ uint8_t smem_raw[];
-  StreamSmem<DP, C8>* sh = reinterpret_cast<StreamSmem<DP, C8>*>(
+  using Smem = typename std::conditional<R == kRows8, StreamSmem8<DP>, StreamSmem<DP, C8>>::type;
+  Smem* sh = reinterpret_cast<Smem*>(
       smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int row0 = blockIdx.y * kRows;
+  const int row0 = blockIdx.y * R;
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
-    for (int i = 0; i < StreamSmem<DP, C8>::kStages; ++i) {
+    for (int i = 0; i < Smem::kStages; ++i) {
       mbar_init(&sh->full[i], 1);
       mbar_init(&sh->empty[i], kConsumers);
     }
@@ -767,7 +1170,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   bool empty = false;
   for (int b = b0; b < b1; ++b) {
     const AttnSeq s = attn_seq(P, b);
-    const PairTiles t = pair_tiles(P, s, row0);
+    const PairTiles t = pair_tiles<R>(P, s, row0);
     mine += (int64_t)(t.t1 - t.t0) * P.Hkv;
     if (blockIdx.x == 0 && blockIdx.y == 0 && (s.bad_len || s.bad_rows))
       atomicOr(P.status, (s.bad_len ? kAttnBadPage : 0u) | (s.bad_rows ? kAttnBadRows : 0u));
@@ -792,7 +1195,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   if (at >= excl && at < excl + mine) {
     int64_t pos = excl;
     for (int b = b0; b < b1; ++b) {
-      const PairTiles t = pair_tiles(P, attn_seq(P, b), row0);
+      const PairTiles t = pair_tiles<R>(P, attn_seq(P, b), row0);
       const int64_t n = (int64_t)(t.t1 - t.t0) * P.Hkv;
       if (at < pos + n) {
         sh->start_seq = b;
@@ -807,10 +1210,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   if (any_empty) {
     for (int b = blockIdx.x; b < P.batch; b += gridDim.x) {
       const AttnSeq s = attn_seq(P, b);
-      const PairTiles t = pair_tiles(P, s, row0);
+      const PairTiles t = pair_tiles<R>(P, s, row0);
       const int64_t all = (int64_t)s.n * P.G - row0;
       if (t.t1 != t.t0 || all <= 0) continue;
-      const int rows = all < kRows ? (int)all : kRows;
+      const int rows = all < R ? (int)all : R;
       for (int i = threadIdx.x; i < rows * P.Hkv; i += kThreads) {
         const int row = row0 + i % rows, head = i / rows;
         const int64_t to = (int64_t)(s.q0 + row / P.G) * P.Hq + head * P.G + row % P.G;
@@ -822,31 +1225,33 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   }
   if (at >= total) return;
   const int64_t count = total - at < share ? total - at : share;
-  Walk w;
+  Walk<R> w;
   w.start(P, row0, sh->start_seq, sh->start_item, at, count);
   if (warp == kConsumers) {
     if constexpr (C8)
-      stream_producer8<DP>(P, M, sh, w, row0);
+      stream_producer8(P, M, sh, w, row0);
     else
       stream_producer<DP>(P, M, sh, w, row0);
+  } else if constexpr (R == kRows8) {
+    stream_consumer8<T, DP>(P, sh, w, row0, share);
   } else {
     stream_consumer<T, DP, C8>(P, sh, w, row0, share);
   }
 }
 
-template <typename T, int DP, bool C8>
+template <typename T, int DP, bool C8, int R>
 int run_stream(const AttnMaps& M, const AttnParams& P, dim3 grid, cudaStream_t stream) {
-  constexpr size_t smem = sizeof(StreamSmem<DP, C8>) + 1024;
-  static_assert(smem <= 113 * 1024, "two blocks per SM");
+  constexpr size_t smem = (R == kRows8 ? sizeof(StreamSmem8<DP>) : sizeof(StreamSmem<DP, C8>)) + 1024;
+  static_assert((smem + 1024) * (R == kRows8 ? kCtasPerSm8 : kCtasPerSm) <= 228 * 1024, "blocks per SM");
   static std::atomic<uint64_t> done{0};
-  cudaError_t err = allow_smem(k_attn_stream<T, DP, C8>, smem, done);
+  cudaError_t err = allow_smem(k_attn_stream<T, DP, C8, R>, smem, done);
   if (err != cudaSuccess) return cuda_status(err);
-  return cuda_status(launch_pdl(k_attn_stream<T, DP, C8>, grid, dim3(kThreads), smem, stream, M, P));
+  return cuda_status(launch_pdl(k_attn_stream<T, DP, C8, R>, grid, dim3(kThreads), smem, stream, M, P));
 }
 
-// Blocks per row tile: two per SM over all row tiles, at least one.
-int stream_blocks(int64_t row_tiles) {
-  int64_t w = (int64_t)kCtasPerSm * sm_count() / row_tiles;
+// Blocks per row tile: so many per SM over all row tiles, at least one.
+int stream_blocks(int64_t row_tiles, int per_sm = kCtasPerSm) {
+  int64_t w = (int64_t)per_sm * sm_count() / row_tiles;
   if (w < 1) w = 1;
   return (int)w;
 }
@@ -861,14 +1266,14 @@ size_t attn_stream_partial_bytes(int64_t rows_max, int D) {
   return (size_t)(tiles * w) * 2 * (kRows * dp + 2 * kRows) * sizeof(float);
 }
 
-template <bool C8>
+template <bool C8, int R>
 int pick_stream(const ftb_attn_args& a, const AttnMaps& M, const AttnParams& P, int dp, dim3 grid,
                 cudaStream_t stream) {
   if (a.type == FTB_TYPE_BF16)
-    return dp == 64 ? run_stream<__nv_bfloat16, 64, C8>(M, P, grid, stream)
-                    : run_stream<__nv_bfloat16, 128, C8>(M, P, grid, stream);
-  return dp == 64 ? run_stream<__half, 64, C8>(M, P, grid, stream)
-                  : run_stream<__half, 128, C8>(M, P, grid, stream);
+    return dp == 64 ? run_stream<__nv_bfloat16, 64, C8, R>(M, P, grid, stream)
+                    : run_stream<__nv_bfloat16, 128, C8, R>(M, P, grid, stream);
+  return dp == 64 ? run_stream<__half, 64, C8, R>(M, P, grid, stream)
+                  : run_stream<__half, 128, C8, R>(M, P, grid, stream);
 }
 
 int launch_attn_stream(const ftb_attn_args& a, AttnParams P, bool fp8, cudaStream_t stream) {
@@ -883,12 +1288,19 @@ int launch_attn_stream(const ftb_attn_args& a, AttnParams P, bool fp8, cudaStrea
              : attn_cache_map(&M.v, a.v_cache, a, a.v_strides, r, halves);
   if (st) return st;
   M.q = M.k;  // unused
+  if (fp8 && (int64_t)a.max_q * P.G <= kRows8) {
+    // (its parts are fewer and smaller than the workspace allows: 3 blocks' of 8 rows against 2 of 16)
+    static_assert(kCtasPerSm8 * kRows8 <= kCtasPerSm * kRows, "parts fit the workspace");
+    const int64_t w = stream_blocks(1, kCtasPerSm8);
+    if (w > kAttnCounters) return FTB_ERR_SHAPE;
+    return pick_stream<true, kRows8>(a, M, P, dp, dim3((unsigned)w), stream);
+  }
   const int64_t tiles = ceil_div((int64_t)a.max_q * P.G, kRows);
   const int64_t w = stream_blocks(tiles);
   if (tiles > 65535 || (w > 1 && tiles * w > kAttnCounters)) return FTB_ERR_SHAPE;
   const dim3 grid((unsigned)w, (unsigned)tiles);
-  return fp8 ? pick_stream<true>(a, M, P, dp, grid, stream)
-             : pick_stream<false>(a, M, P, dp, grid, stream);
+  return fp8 ? pick_stream<true, kRows>(a, M, P, dp, grid, stream)
+             : pick_stream<false, kRows>(a, M, P, dp, grid, stream);
 }
 
 }  // namespace ftb
