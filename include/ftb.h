@@ -541,7 +541,7 @@ FTB_API int ftb_attention(const ftb_attn_args* args, ftb_stream_t stream);
  * are. Tokens may come in any order; of two tokens with the same slot one is kept, whole.
  * workspace: ftb_rope_fp8_workspace_bytes() bytes, 4-byte aligned, for calls of one stream order. It
  * may be the one of ftb_attention(): its first FTB_ATTN_ZERO_BYTES bytes are not touched, and the rest
- * may hold anything. Calls of up to 512 tokens take none (it may be NULL).
+ * may hold anything. Calls of up to 2048 tokens take none (it may be NULL).
  */
 typedef struct ftb_rope_fp8_args {
   ftb_rope_args rope;

@@ -31,8 +31,8 @@ def rope(**kw):
     (dict(type=2), ARG), (dict(tokens=4, slots=0), ARG), (dict(tokens=4, slots=0, v_dst=0), ARG),
     (dict(tokens=4, k_scale=0), ARG), (dict(tokens=4, v_scale=0), ARG), (dict(tokens=4, q=0), ARG),
     (dict(tokens=4, n_slots=63), SHAPE), (dict(tokens=4, n_slots=-16), SHAPE),
-    (dict(tokens=513), WORKSPACE), (dict(tokens=513, workspace=16, workspace_bytes=65536), WORKSPACE),
-    (dict(tokens=513, workspace=18, workspace_bytes=1 << 20), ALIGN),
+    (dict(tokens=2049), WORKSPACE), (dict(tokens=2049, workspace=16, workspace_bytes=65536), WORKSPACE),
+    (dict(tokens=2049, workspace=18, workspace_bytes=1 << 20), ALIGN),
     (dict(tokens=4, Hkv=1025), SHAPE)])
 def test_rope(kw, status):
     assert rope(**kw) == status
@@ -44,8 +44,8 @@ def test_rope_null():
 
 def test_rope_workspace_bytes():
     size = _lib.load().ftb_rope_fp8_workspace_bytes
-    assert size(512, 1 << 20) == _lib.FTB_ATTN_ZERO_BYTES
-    assert size(513, 1 << 20) == _lib.FTB_ATTN_ZERO_BYTES + (4 << 20)
+    assert size(2048, 1 << 20) == _lib.FTB_ATTN_ZERO_BYTES
+    assert size(2049, 1 << 20) == _lib.FTB_ATTN_ZERO_BYTES + (4 << 20)
     assert size(-1, 5) == 0
 
 

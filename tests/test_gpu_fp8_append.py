@@ -82,9 +82,9 @@ def test_joins_a_block(first, tokens):
 
 @pytest.mark.parametrize("page,block", [(16, 16), (32, 32), (64, 64), (128, 128), (128, 32), (48, 16),
                                         (256, 128)])
-@pytest.mark.parametrize("tokens", [1, 60, 300, 700])
+@pytest.mark.parametrize("tokens", [1, 60, 300, 2300])
 def test_pages_and_blocks(page, block, tokens):
-    """(700 tokens go through the table of slots, the others through a scan)"""
+    """(2300 tokens go through the table of slots, the others through a scan)"""
     pages = -(-(tokens + page) // page) + 1
     check(make(tokens, range(page - 5, page - 5 + tokens), page=page, block=block, pages=pages))
 
@@ -93,18 +93,18 @@ def test_pages_and_blocks(page, block, tokens):
                                          (112, 112, "half"), (64, 24, "half"), (72, 20, "half"),
                                          (66, 6, "adjacent"), (16, 16, "half"), (256, 128, "half"),
                                          (512, 256, "half")])
-@pytest.mark.parametrize("tokens", [1, 40, 600])
+@pytest.mark.parametrize("tokens", [1, 40, 600, 2100])
 def test_heads_and_rotations(D, rot, pairs, tokens):
-    check(make(tokens, range(7, 7 + tokens), D=D, rot=rot, pairs=pairs, pages=20, dtype=F16))
+    check(make(tokens, range(7, 7 + tokens), D=D, rot=rot, pairs=pairs, pages=70, dtype=F16))
 
 
 @pytest.mark.parametrize("heads", [(1, 1), (3, 1), (8, 8), (40, 5), (32, 33), (2, 130)])
-@pytest.mark.parametrize("tokens", [1, 50, 520])
+@pytest.mark.parametrize("tokens", [1, 50, 520, 2050])
 def test_head_counts(heads, tokens):
-    check(make(tokens, range(3, 3 + tokens), heads=heads, pages=20, D=32, rot=32))
+    check(make(tokens, range(3, 3 + tokens), heads=heads, pages=70, D=32, rot=32))
 
 
-@pytest.mark.parametrize("tokens", [12, 200, 513, 2000])
+@pytest.mark.parametrize("tokens", [12, 200, 513, 2000, 2049, 5000])
 @pytest.mark.parametrize("slot_type", [torch.int32, torch.int64])
 def test_any_order_of_slots(tokens, slot_type):
     """A decode batch, and tokens whose blocks are met in any order, some of them stored nowhere."""
@@ -118,7 +118,7 @@ def test_any_order_of_slots(tokens, slot_type):
 
 
 def test_every_slot_nowhere():
-    for tokens in (5, 600):
+    for tokens in (5, 600, 2500):
         check(make(tokens, [-1] * tokens))
 
 
@@ -126,8 +126,8 @@ def test_every_slot_nowhere():
 @pytest.mark.parametrize("axes,sections,order", [(3, (12, 10, 10), "cyclic"), (2, (32, 0), "blocks"),
                                                  (4, (8, 8, 8, 8), "blocks")])
 def test_axes_and_layouts(layout, axes, sections, order):
-    for tokens in (9, 530):
-        check(make(tokens, range(20, 20 + tokens), axes=axes, sections=sections, order=order, pages=20,
+    for tokens in (9, 530, 2100):
+        check(make(tokens, range(20, 20 + tokens), axes=axes, sections=sections, order=order, pages=70,
                    layout=layout))
 
 
@@ -161,10 +161,10 @@ def test_numbers_at_the_limits():
 
 
 @pytest.mark.parametrize("old", [0.0, -1.0, math.nan, math.inf, 0.3, 1e-30, 1e30, 5.0])
-@pytest.mark.parametrize("tokens", [2, 600])
+@pytest.mark.parametrize("tokens", [2, 600, 2100])
 def test_scales_so_far(old, tokens):
     """Scales that are none start anew, others go up to a power of two within the limits."""
-    c = make(tokens, range(5, 5 + tokens), pages=20)
+    c = make(tokens, range(5, 5 + tokens), pages=70)
     c["k_scale"][:], c["v_scale"][:] = old, old
     check(c)
 
@@ -177,10 +177,10 @@ def test_nan_codes_stay():
 
 
 def test_one_of_two_tokens_with_a_slot_is_kept_whole():
-    for tokens in (10, 600):
+    for tokens in (10, 600, 2100):
         slots = torch.arange(tokens)
         slots[tokens // 2:] = slots[:tokens - tokens // 2].clone()
-        c = make(tokens, slots, pages=20)
+        c = make(tokens, slots, pages=70)
         got = call(c)
         _, k, v = c["qkv"].split([4, 2, 2], 1)
         k = turned(k, c["positions"], c["table"], "half")
@@ -213,8 +213,8 @@ def test_step_by_step_and_at_once():
 
 
 def test_captured_and_replayed():
-    for tokens in (6, 700):
-        c = make(tokens, range(3, 3 + tokens), pages=30)
+    for tokens in (6, 700, 2100):
+        c = make(tokens, range(3, 3 + tokens), pages=70)
         dev = {n: c[n].cuda() for n in ("qkv", "positions", "table", "slots", "k_scale", "v_scale")}
         caches = [c[n].cuda() for n in ("k_cache", "v_cache")]
         q, k, v = dev["qkv"].split([4, 2, 2], 1)
@@ -228,7 +228,7 @@ def test_captured_and_replayed():
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             out = run()
-        other = make(tokens, range(40, 40 + tokens), pages=30, seed=4)
+        other = make(tokens, range(40, 40 + tokens), pages=70, seed=4)
         for n in dev:
             dev[n].copy_(other[n])
         for a, n in zip(caches, ("k_cache", "v_cache")):
@@ -249,7 +249,7 @@ def test_after_an_attention_on_the_same_stream():
     ref = reference(a, *build(a))
     for i in range(3):
         compare(a, *ftb.paged_attention(**a.t, return_lse=True, check_status=True), *ref)
-        check(make(700, range(700), pages=30, seed=i))
+        check(make(2100, range(2100), pages=70, seed=i))
 
 
 def test_q_in_place():
