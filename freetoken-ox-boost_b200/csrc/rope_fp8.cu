@@ -33,6 +33,7 @@ constexpr int kPerSm = 4;        // thread blocks per SM
 constexpr int kKept = 1;         // items of a thread that stay in registers
 constexpr int kItems = 8;        // items of a thread that a thread block is made for
 constexpr int kMaxBlock = 128;   // tokens per scale
+constexpr int kMaxHeads = 256;   // of a thread block
 constexpr int kScan = 2048;      // tokens up to which an owner scans all slots
 constexpr int kMaxRange = 64;    // tokens per thread block beyond that, at most
 constexpr int kManyTokens = 4096;  // from here on a thread block turns q of eight tokens
@@ -233,9 +234,9 @@ struct AppendShared {
   int row[kMaxBlock], tok[kMaxBlock];  // the written rows, ascending
   int n, last;
   uint32_t candidates[kMaxRange / 32];
-  uint32_t top[kThreads * kItems];  // by head: largest |x|, as bits
-  float by[kThreads * kItems];      // 1 / scale
-  float again[kThreads * kItems];   // old scale / scale where they differ, else 0
+  uint32_t top[kMaxHeads];  // by head: largest |x|, as bits
+  float by[kMaxHeads];      // 1 / scale
+  float again[kMaxHeads];   // old scale / scale where they differ, else 0
 };
 
 // The block with token t's slot, if t is its owner: heads [h0, h0 + nh) of K (kind 0) or V.
@@ -471,6 +472,7 @@ int run_append(AppendParams A, cudaStream_t stream) {
   // heads per thread block: as many as its registers hold of a full block of tokens
   const int rows = (int)(T0 < (1 << A.block_log2) ? T0 : (1 << A.block_log2));
   int per = step * kItems / rows;
+  per = per > kMaxHeads ? kMaxHeads : per;
   per = per < 1 ? 1 : per > P.Hkv ? P.Hkv : per;
   A.per_split = per;
   A.splits = 2 * (int)ceil_div(P.Hkv, per);
@@ -525,7 +527,7 @@ int ftb_rope_fp8(const ftb_rope_fp8_args* args, ftb_stream_t stream) {
   if (a->tokens == 0) return FTB_OK;
   if (!a->slots || !args->k_scale || !args->v_scale) return FTB_ERR_ARG;
   if (a->n_slots < 0 || a->n_slots % a->page) return FTB_ERR_SHAPE;
-  if (a->Hkv > kThreads * kItems) return FTB_ERR_SHAPE;
+  if (a->Hkv > 1024) return FTB_ERR_SHAPE;
   while ((1 << A.block_log2) < size) ++A.block_log2;
   A.dst[0] = reinterpret_cast<uint8_t*>(a->k_dst), A.dst[1] = reinterpret_cast<uint8_t*>(a->v_dst);
   A.scale[0] = args->k_scale, A.scale[1] = args->v_scale;
