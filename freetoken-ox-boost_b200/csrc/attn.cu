@@ -58,14 +58,14 @@ int attn_cache_map(CUtensorMap* m, const void* base, const ftb_attn_args& a,
 }
 
 int attn_cache_map8(CUtensorMap* m, const void* base, const ftb_attn_args& a,
-                    const int64_t (&strides)[3], uint32_t box_rows) {
+                    const int64_t (&strides)[3], uint32_t box_rows, uint32_t box_heads) {
   PFN_cuTensorMapEncodeTiled fn = encode_fn();
   if (!fn) return FTB_ERR_CUDA;
   const cuuint64_t dims[5] = {(cuuint64_t)a.D, (cuuint64_t)a.page, (cuuint64_t)a.Hkv,
                               (cuuint64_t)a.num_pages, 1};
   const cuuint64_t st[4] = {(cuuint64_t)strides[1], (cuuint64_t)strides[2], (cuuint64_t)strides[0],
                             128};
-  const cuuint32_t box[5] = {128, box_rows, 1, 1, 1};
+  const cuuint32_t box[5] = {128, box_rows, box_heads, 1, 1};
   const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   // A head's row, no more: with 256 bytes the next head's, which is read at another time, came along (3
   // tokens at up to 131072 keys moved 969 MB instead of 719).

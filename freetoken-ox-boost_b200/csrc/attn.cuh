@@ -45,9 +45,10 @@ struct AttnMaps {
 
 int attn_cache_map(CUtensorMap* m, const void* base, const ftb_attn_args& a,
                    const int64_t (&strides)[3], uint32_t box_rows, uint32_t halves);
-// The same for a cache of bytes: boxes of `box_rows` key rows by 128 bytes (D and zeros behind it).
+// The same for a cache of bytes: boxes of `box_rows` key rows of
+// `box_heads` kv heads by 128 bytes (D and zeros behind it).
 int attn_cache_map8(CUtensorMap* m, const void* base, const ftb_attn_args& a,
-                    const int64_t (&strides)[3], uint32_t box_rows);
+                    const int64_t (&strides)[3], uint32_t box_rows, uint32_t box_heads = 1);
 // Query rows of one kv head: boxes of `tokens` tokens x `group` heads x 64 elements.
 int attn_q_map(CUtensorMap* m, const ftb_attn_args& a, uint32_t group, uint32_t tokens);
 

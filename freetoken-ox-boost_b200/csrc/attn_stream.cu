@@ -61,17 +61,20 @@ struct StreamSmem {
   int abort;
 };
 
-// The form for up to 8 rows over a cache of bytes.
-constexpr int kRows8 = 8, kCtasPerSm8 = 3;
-template <int DP>
+// The form for up to 8 rows over a cache of bytes. A stage is 64 rows of 128 bytes of K and of V: 64
+// keys of a head, or (HP = 2, an even number of kv heads) 32 keys of two heads that lie side by side. Pairs
+// because memory is read faster in 256 bytes than in 128: copies alone, without any products, took 83 us
+// for 61 tokens at up to 8192 keys one head at a time and 74 us by pairs.
+constexpr int kRows8 = 8;
+template <int DP, int HP>
 struct StreamSmem8 {
-  static constexpr int kStages = 4;
-  alignas(1024) uint8_t ring[kStages][2][kTile * 128];
+  static constexpr int kStages = 6;
+  alignas(1024) uint8_t ring[kStages][2][64 * 128];  // [box][head][row][128]
   alignas(16) float merge[kConsumers][kRows8][DP / 2 + 4];  // half of the columns
-  BlockScale scale[kStages][kConsumers];
+  BlockScale scale[kStages][kConsumers];  // of each warp's keys
   float ml[kConsumers][kRows8][2];
   float fac[kConsumers][kRows8];
-  float row_m[kRows8], row_l[kRows8];
+  float row_m[HP][kRows8], row_l[HP][kRows8];
   uint64_t full[kStages], empty[kStages];
   int64_t scan[kThreads / kWarp];
   int64_t start_item;
@@ -111,7 +114,7 @@ struct PairTiles {
   int lo, hi;  // keys
   int t0, t1;  // tiles
 };
-template <int R>  // rows of a row tile
+template <int R, int KT>  // rows of a row tile, keys of a stage
 __device__ __forceinline__ PairTiles pair_tiles(const AttnParams& P, const AttnSeq& s, int row0) {
   PairTiles t{0, 0, 0, 0};
   const int64_t rows = (int64_t)s.n * P.G;
@@ -119,23 +122,26 @@ __device__ __forceinline__ PairTiles pair_tiles(const AttnParams& P, const AttnS
   const int last = (int)(rows < row0 + R ? rows : row0 + R) - 1;
   const KeyRange k = attn_range(P, s, row0 / P.G, last / P.G);
   if (k.lo >= k.hi) return t;
-  t.lo = k.lo, t.hi = k.hi, t.t0 = k.lo / kTile, t.t1 = (k.hi + kTile - 1) / kTile;
+  t.lo = k.lo, t.hi = k.hi, t.t0 = k.lo / KT, t.t1 = (k.hi + KT - 1) / KT;
   return t;
 }
 
 // The walk over a block's share of the line; producer and consumers take the same steps.
-template <int R>
+// (heads: the kv heads, or pairs of them, that the line has one after another)
+template <int R, int KT>
 struct Walk {
   int seq, head, tile;  // next tile of pair (seq, head)
+  int heads;
   int64_t item;         // line position of the pair's first tile
   int64_t left;         // tiles of the share still to do
   AttnSeq s;
   PairTiles t;
   __device__ void start(const AttnParams& P, int row0, int seq0, int64_t seq_at, int64_t at,
-                        int64_t count) {
+                        int64_t count, int n_heads) {
     seq = seq0;
+    heads = n_heads;
     s = attn_seq(P, seq);
-    t = pair_tiles<R>(P, s, row0);
+    t = pair_tiles<R, KT>(P, s, row0);
     const int64_t off = at - seq_at;  // into the sequence's Hkv pairs
     const int n = t.t1 - t.t0;
     head = (int)(off / n);
@@ -153,12 +159,12 @@ struct Walk {
     tile += done;
     if (left <= 0) return;
     item += t.t1 - t.t0;  // left > 0: the pair is done
-    if (++head == P.Hkv) {
+    if (++head == heads) {
       head = 0;
       do {
         ++seq;  // left > 0: a later sequence has tiles
         s = attn_seq(P, seq);
-        t = pair_tiles<R>(P, s, row0);
+        t = pair_tiles<R, KT>(P, s, row0);
       } while (t.t1 == t.t0);
     }
     tile = t.t0;
@@ -186,7 +192,7 @@ struct StreamSync {
 // One warp. Copies the tiles of the share into the ring.
 template <int DP>
 __device__ void stream_producer(const AttnParams& P, const AttnMaps& M, StreamSmem<DP, false>* sh,
-                                Walk<kRows> w, int row0) {
+                                Walk<kRows, kTile> w, int row0) {
   constexpr int kStages = StreamSmem<DP, false>::kStages;
   const int lane = threadIdx.x & 31;
   const StreamSync<StreamSmem<DP, false>> sy{sh, P.status};
@@ -263,34 +269,37 @@ __device__ __forceinline__ float ldg_now(const float* p) {
 // The same for a cache of bytes, whose scales come by plain loads: four groups of 16 keys per tile (a
 // block of tokens is 16 keys or more). A tile takes half as long as one of 16 bits, about as long as a
 // page id and the scales behind it take to come, so the lanes look after eight tiles at once, lane l after
-// group l % 4 of tile l / 4, and ask for the scales of the next eight and the ids of those after them
+// 16 keys of one head of tile l / 4, and ask for the scales of the next eight and the ids of those after them
 // before they turn to these (one tile at a time: 123 us for 61 tokens at up to 8192 keys).
-template <class Smem, int R>
-__device__ void stream_producer8(const AttnParams& P, const AttnMaps& M, Smem* sh, Walk<R> w, int row0) {
+template <int HP, class Smem, int R, int KT>
+__device__ void stream_producer8(const AttnParams& P, const AttnMaps& M, Smem* sh, Walk<R, KT> w,
+                                 int row0) {
   constexpr int kStages = Smem::kStages;
-  constexpr int kGroups = kTile / 16, kAhead = kWarp / kGroups;
+  // a lane's group of keys, of kGroups per tile, and its head: four lanes per tile
+  constexpr int kGroups = KT / 16, kLanes = kGroups * HP, kAhead = kWarp / kLanes;
   const int lane = threadIdx.x & 31;
   const StreamSync<Smem> sy{sh, P.status};
   const int page = 1 << P.page_log2;
-  const int r = page < kTile ? page : kTile;  // keys per box, >= 16
-  const int boxes = kTile / r;                // <= kGroups
-  const int my_box = (lane & (kGroups - 1)) * 16 / r;
+  const int r = page < KT ? page : KT;  // keys per box, >= 16
+  const int boxes = KT / r;             // <= kGroups
+  const int my_key = (lane & (kGroups - 1)) * 16, my_box = my_key / r;
+  const int my_head = (lane & (kLanes - 1)) / kGroups;
   int stage = 0;
   uint32_t parity = 1, issued = 0;
   bool ok = true;
   while (w.left > 0 && ok) {
     const int n = w.take();
     const int32_t* table = P.block_table + (int64_t)w.seq * P.table_stride;
-    const float* ks_of = P.k_scale + w.head * P.ks_st[2];
-    const float* vs_of = P.v_scale + w.head * P.vs_st[2];
+    const float* ks_of = P.k_scale + (w.head * HP + my_head) * P.ks_st[2];
+    const float* vs_of = P.v_scale + (w.head * HP + my_head) * P.vs_st[2];
     // boxes [b0, b1) of a tile have a key in [lo, hi)
     auto box0 = [&](int key0) { return w.t.lo > key0 ? (w.t.lo - key0) / r : 0; };
     auto box1 = [&](int key0) { return min(boxes, (w.t.hi - key0 + r - 1) / r); };
     // the first key of this lane's group of the tiles from j0 on; whether anybody reads it
-    auto key_at = [&](int j0) { return (w.tile + j0) * kTile + lane * 16; };
+    auto key_at = [&](int j0) { return (w.tile + j0 + lane / kLanes) * KT + my_key; };
     auto wanted = [&](int j0) {
-      const int key0 = (w.tile + j0 + lane / kGroups) * kTile;
-      return j0 + lane / kGroups < n && my_box >= box0(key0) && my_box < box1(key0);
+      const int key0 = (w.tile + j0 + lane / kLanes) * KT;
+      return j0 + lane / kLanes < n && my_box >= box0(key0) && my_box < box1(key0);
     };
     auto load_id = [&](int j0) {  // -1: not wanted
       return wanted(j0) ? ldg_now(table + (key_at(j0) >> P.page_log2)) : -1;
@@ -316,24 +325,24 @@ __device__ void stream_producer8(const AttnParams& P, const AttnMaps& M, Smem* s
       }
       const int count = min(kAhead, n - j0);
       for (int j = 0; j < count; ++j) {
-        const int key0 = (w.tile + j0 + j) * kTile;
+        const int key0 = (w.tile + j0 + j) * KT;
         const int b0 = box0(key0), b1 = box1(key0);
         // (a box's groups are of one page)
-        const int box_id = __shfl_sync(0xffffffffu, id, j * kGroups + ((lane * r >> 4) & (kGroups - 1)));
+        const int box_id = __shfl_sync(0xffffffffu, id, j * kLanes + ((lane * r >> 4) & (kGroups - 1)));
         ok = __all_sync(0xffffffffu, sy.wait(&sh->empty[stage], parity));
         if (!ok) break;
         ++issued;
         if (lane >= b0 && lane < b1) {
-          const uint32_t at = lane * r * 128;
+          const uint32_t at = lane * r * 128 * HP;
           const int row = (key0 + lane * r) & (page - 1);
-          tma_5d(smem_u32(sh->ring[stage][0]) + at, &M.k, 0, row, w.head, box_id, 0, &sh->full[stage]);
-          tma_5d(smem_u32(sh->ring[stage][1]) + at, &M.v, 0, row, w.head, box_id, 0, &sh->full[stage]);
+          tma_5d(smem_u32(sh->ring[stage][0]) + at, &M.k, 0, row, w.head * HP, box_id, 0, &sh->full[stage]);
+          tma_5d(smem_u32(sh->ring[stage][1]) + at, &M.v, 0, row, w.head * HP, box_id, 0, &sh->full[stage]);
         }
-        if (lane / kGroups == j) sh->scale[stage][lane & (kGroups - 1)] = block_scale(ks, vs);
+        if (lane / kLanes == j) sh->scale[stage][lane & (kLanes - 1)] = block_scale(ks, vs);
         __syncwarp();
         // (the phase stays open for this arrival, whatever has landed by now)
         if (lane == 0)
-          mbar_arrive_expect_tx(&sh->full[stage], 2u * (uint32_t)(b1 - b0) * (uint32_t)r * 128u);
+          mbar_arrive_expect_tx(&sh->full[stage], 2u * HP * (uint32_t)(b1 - b0) * (uint32_t)r * 128u);
         __syncwarp();
         if (++stage == kStages) stage = 0, parity ^= 1u;
       }
@@ -420,22 +429,26 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
 //   S^T = K Q^T    M = 16 keys of the warp, K = 16 elements
 //   O^T = V^T P^T  M = 16 columns of V, K = 16 keys; P goes from the accumulators of S^T to the operand by
 //                  a transposition of 8 x 8 (movmatrix)
-// Half the products, exponentials and registers of the form above, and three blocks per SM: the work is
-// bound by latencies (61 tokens at up to 8192 keys 130 us with it).
+// Half the products, exponentials and registers of the form above, whose chain of instructions bound it (61
+// tokens at up to 8192 keys 130 us). Each warp has 16 keys of one head of a stage.
 // A row's reference moves to a tile's maximum where that exceeds it by more than 2^kLazy (P reaches
 // 2^kLazy, f16 holds it), so the warp's maxima are rarely brought together: one vote per tile.
-template <typename T, int DP>
-__device__ void stream_consumer8(const AttnParams& P, StreamSmem8<DP>* sh, Walk<kRows8> w, int row0,
-                                 int64_t share) {
-  using Smem = StreamSmem8<DP>;
+template <typename T, int DP, int HP>
+__device__ void stream_consumer8(const AttnParams& P, StreamSmem8<DP, HP>* sh, Walk<kRows8, 64 / HP> w,
+                                 int row0, int64_t share) {
+  using Smem = StreamSmem8<DP, HP>;
+  constexpr int kWarps = kConsumers / HP, KT = 64 / HP;  // warps of a head, keys of a stage
   constexpr int kStages = Smem::kStages, VB = DP / 8;
   constexpr float kLazy = 10.f;
   constexpr bool kRest = std::is_same<T, __half>::value;  // (as above)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t2 = (lane & 3) * 2;  // key (or columns) of the lane; its rows t2, t2 + 1
   const StreamSync<Smem> sy{sh, P.status};
-  // K: keys kr, kr + 8 of the tile, chunk lane % 4 of each 64 elements; V: keys kv[e], kv[e] + 8, VB bytes
-  const int kr = warp * 16 + key_of(g), kv0 = warp * 16 + key_of(t2), kv1 = warp * 16 + key_of(t2 + 1);
+  const int wh = warp / kWarps, wk = warp % kWarps * 16;  // the warp's head and first key of a stage
+  const int page = 1 << P.page_log2, r = page < KT ? page : KT;  // keys per box
+  const int base = (wk / r * HP + wh) * r * 128 + wk % r * 128;  // its rows
+  // K: keys kr, kr + 8 of the warp's, chunk lane % 4 of each 64 elements; V: keys kv0, kv1, + 8, VB bytes
+  const int kr = key_of(g), kv0 = key_of(t2), kv1 = key_of(t2 + 1);
   auto v_at = [&](int key) {
     const int byte = g * VB;
     return key * 128 + (((byte >> 4) ^ (key & 7)) << 4) + (byte & 15);
@@ -463,7 +476,7 @@ __device__ void stream_consumer8(const AttnParams& P, StreamSmem8<DP>* sh, Walk<
     {
       const int row = row0 + g;
       const uint16_t* qp =
-          P.q + (int64_t)(s.q0 + row / P.G) * P.q_st + (int64_t)(w.head * P.G + row % P.G) * P.q_sh;
+          P.q + (int64_t)(s.q0 + row / P.G) * P.q_st + (int64_t)((w.head * HP + wh) * P.G + row % P.G) * P.q_sh;
       const float back = load_q8<T, DP>(qp, g < rows, P.D, q_lo, q_hi) * P.scale_log2;
       factor[0] = __shfl_sync(0xffffffffu, back, t2 * 4);
       factor[1] = __shfl_sync(0xffffffffu, back, t2 * 4 + 4);
@@ -475,12 +488,12 @@ __device__ void stream_consumer8(const AttnParams& P, StreamSmem8<DP>* sh, Walk<
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[j][i] = 0.f;
     for (int j = 0; j < n && parity < kGaveUp; ++j) {
-      const int key0 = (w.tile + j) * kTile + warp * 16;
+      const int key0 = (w.tile + j) * KT + wk;
       if (!__all_sync(0xffffffffu, sy.wait(&sh->full[stage], parity))) {
         parity = kGaveUp;
         break;
       }
-      const uint8_t *kb = sh->ring[stage][0], *vb = sh->ring[stage][1];
+      const uint8_t *kb = sh->ring[stage][0] + base, *vb = sh->ring[stage][1] + base;
       const BlockScale bs = sh->scale[stage][warp];
       float sc[4] = {}, sd[4] = {};
 #pragma unroll
@@ -515,7 +528,7 @@ __device__ void stream_consumer8(const AttnParams& P, StreamSmem8<DP>* sh, Walk<
             const uint2 b = *reinterpret_cast<const uint2*>(vb + v_at(row));
             v[h][e][0] = b.x, v[h][e][1] = b.y;
           }
-          const int key = key0 - warp * 16 + row;
+          const int key = key0 + row;
           if (!inside && (key < w.t.lo || key >= w.t.hi)) {
 #pragma unroll
             for (int k = 0; k < VB / 4; ++k) v[h][e][k] = 0u;
@@ -524,7 +537,7 @@ __device__ void stream_consumer8(const AttnParams& P, StreamSmem8<DP>* sh, Walk<
       const bool clean = inside && (!P.causal || s.n == 1) && (P.window <= 0 || s.n == 1);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int key = key0 + (i >> 1) * 8 + kr - warp * 16;
+        const int key = key0 + (i >> 1) * 8 + kr;
         const bool seen = clean || (key >= kmin[i & 1] && key < kmax[i & 1]);
         sc[i] = seen ? fmaf(sc[i] + sd[i], bs.k * factor[i & 1], bs.v_log2) : -INFINITY;
       }
@@ -593,25 +606,28 @@ __device__ void stream_consumer8(const AttnParams& P, StreamSmem8<DP>* sh, Walk<
       }
     }
     named_bar(1, kConsumers * kWarp);
-    if (threadIdx.x < kRows8) {
-      const int row = threadIdx.x;
-      float mm = sh->ml[0][row][0];
-      for (int i = 1; i < kConsumers; ++i) mm = fmaxf(mm, sh->ml[i][row][0]);
+    if (threadIdx.x < HP * kRows8) {
+      const int row = threadIdx.x % kRows8, hh = threadIdx.x / kRows8, w0 = hh * kWarps;
+      float mm = sh->ml[w0][row][0];
+      for (int i = 1; i < kWarps; ++i) mm = fmaxf(mm, sh->ml[w0 + i][row][0]);
       const float top = mm == -INFINITY ? 0.f : mm;
       float ll = 0.f;
-      for (int i = 0; i < kConsumers; ++i) {
-        const float f = ex2(sh->ml[i][row][0] - top);
-        sh->fac[i][row] = f;
-        ll += f * sh->ml[i][row][1];
+      for (int i = 0; i < kWarps; ++i) {
+        const float f = ex2(sh->ml[w0 + i][row][0] - top);
+        sh->fac[w0 + i][row] = f;
+        ll += f * sh->ml[w0 + i][row][1];
       }
-      sh->row_m[row] = mm;
-      sh->row_l[row] = ll;
+      sh->row_m[hh][row] = mm;
+      sh->row_l[hh][row] = ll;
     }
     named_bar(1, kConsumers * kWarp);
     const bool begins = w.tile == w.t.t0, ends = w.tile + n == w.t.t1;
     const bool whole = begins && ends;
     const int64_t blk = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
-    constexpr int kSlot = kRows8 * DP + 2 * kRows8;
+    constexpr int kPart = kRows8 * DP + 2 * kRows8, kSlot = HP * kPart;  // of a head; of all
+    auto out_row = [&](int row, int hh) {  // of the outputs
+      return (int64_t)(s.q0 + row / P.G) * P.Hq + (w.head * HP + hh) * P.G + row % P.G;
+    };
     float* slot = P.partial + (2 * blk + (begins ? 1 : 0)) * kSlot;  // (as above)
     const float f0 = sh->fac[warp][t2], f1 = sh->fac[warp][t2 + 1];
     constexpr int kHalf = DP / 2, kPer = kHalf / 4;  // columns of a pass, threads of a row
@@ -631,37 +647,37 @@ __device__ void stream_consumer8(const AttnParams& P, StreamSmem8<DP>* sh, Walk<
       }
       named_bar(1, kConsumers * kWarp);
       const int d = c * kHalf + oc;
-      if (orow < rows) {
-        float4 a = *reinterpret_cast<float4*>(&sh->merge[0][orow][oc]);
 #pragma unroll
-        for (int i = 1; i < kConsumers; ++i) {
-          const float4 b = *reinterpret_cast<float4*>(&sh->merge[i][orow][oc]);
+      for (int hh = 0; hh < HP; ++hh) {
+        if (orow >= rows) continue;
+        float4 a = *reinterpret_cast<float4*>(&sh->merge[hh * kWarps][orow][oc]);
+#pragma unroll
+        for (int i = 1; i < kWarps; ++i) {
+          const float4 b = *reinterpret_cast<float4*>(&sh->merge[hh * kWarps + i][orow][oc]);
           a.x += b.x, a.y += b.y, a.z += b.z, a.w += b.w;
         }
         if (!whole) {
-          *reinterpret_cast<float4*>(slot + orow * DP + d) = a;
+          *reinterpret_cast<float4*>(slot + hh * kPart + orow * DP + d) = a;
         } else if (d < P.D) {
-          const float ll = sh->row_l[orow], inv = ll > 0.f || ll != ll ? 1.f / ll : 0.f;
-          const int row = row0 + orow;
-          uint16_t* op = P.out + ((int64_t)(s.q0 + row / P.G) * P.Hq + w.head * P.G + row % P.G) * P.D + d;
-          *reinterpret_cast<uint2*>(op) =
+          const float ll = sh->row_l[hh][orow], inv = ll > 0.f || ll != ll ? 1.f / ll : 0.f;
+          *reinterpret_cast<uint2*>(P.out + out_row(row0 + orow, hh) * P.D + d) =
               make_uint2(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv));
         }
       }
       named_bar(1, kConsumers * kWarp);
     }
     if (whole) {
-      if (P.lse && threadIdx.x < rows) {
-        const int row = row0 + threadIdx.x;
-        P.lse[(int64_t)(s.q0 + row / P.G) * P.Hq + w.head * P.G + row % P.G] =
-            sh->row_l[threadIdx.x] == 0.f
-                ? -INFINITY
-                : (sh->row_m[threadIdx.x] + log2f(sh->row_l[threadIdx.x])) * 0.69314718055994531f;
+      const int row = threadIdx.x % kRows8, hh = threadIdx.x / kRows8;
+      if (P.lse && hh < HP && row < rows) {
+        const float ll = sh->row_l[hh][row];
+        P.lse[out_row(row0 + row, hh)] =
+            ll == 0.f ? -INFINITY : (sh->row_m[hh][row] + log2f(ll)) * 0.69314718055994531f;
       }
     } else {
-      if (threadIdx.x < rows) {
-        slot[kRows8 * DP + threadIdx.x] = sh->row_m[threadIdx.x];
-        slot[kRows8 * DP + kRows8 + threadIdx.x] = sh->row_l[threadIdx.x];
+      const int row = threadIdx.x % kRows8, hh = threadIdx.x / kRows8;
+      if (hh < HP && row < rows) {
+        slot[hh * kPart + kRows8 * DP + row] = sh->row_m[hh][row];
+        slot[hh * kPart + kRows8 * DP + kRows8 + row] = sh->row_l[hh][row];
       }
       // blocks c0..c1 hold the pair's parts: the last one to get here joins them
       const int64_t c0 = w.item / share, c1 = (w.item + (w.t.t1 - w.t.t0) - 1) / share;
@@ -679,10 +695,11 @@ __device__ void stream_consumer8(const AttnParams& P, StreamSmem8<DP>* sh, Walk<
       if (sh->flag) {
         const float* p0 = P.partial + (2 * blk0 + 1) * kSlot;
         const float* p1 = P.partial + 2 * (blk0 + 1) * kSlot;
-        // 16 threads a row, DP / 64 x 4 columns each; the threads of rows that are not there take their
-        // share of the parts: part i goes to way i % ways of its row
-        constexpr int kCols = DP / 64;
-        const int jc = (threadIdx.x & 15) * 4, trow = threadIdx.x >> 4;
+        // All heads' rows at once, 16 / HP threads a row, kCols x 4 columns each; the threads of rows that
+        // are not there take their share of the parts: part i goes to way i % ways of its row.
+        constexpr int kRowThreads = 16 / HP, kStep = kRowThreads * 4, kCols = DP / kStep;
+        const int jc = threadIdx.x % kRowThreads * 4, any = threadIdx.x / kRowThreads;
+        const int hh = any / kRows8, trow = any % kRows8;
         const int lg = rows > 1 ? 32 - __clz(rows - 1) : 0, ways = kRows8 >> lg;
         const int jrow = trow & ((1 << lg) - 1), way = trow >> lg;
         const bool mine = jrow < rows;
@@ -694,53 +711,72 @@ __device__ void stream_consumer8(const AttnParams& P, StreamSmem8<DP>* sh, Walk<
           acc[c].x += f * b.x, acc[c].y += f * b.y, acc[c].z += f * b.z, acc[c].w += f * b.w;
         };
         if (mine) {
-          for (int i = way; i < parts; i += ways) {
-            const float* q = i == 0 ? p0 : p1 + (int64_t)(i - 1) * 2 * kSlot;
-            mm = fmaxf(mm, __ldcg(q + kRows8 * DP + jrow));
+          auto part = [&](int i) { return (i == 0 ? p0 : p1 + (int64_t)(i - 1) * 2 * kSlot) + hh * kPart; };
+          // (so many parts' loads in flight: one at a time, a single sequence's 37 or 74 parts took as long
+          // as its keys)
+          constexpr int kAtOnce = 4;
+          for (int i = way; i < parts; i += ways * kAtOnce) {
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u)
+              if (i + u * ways < parts) mm = fmaxf(mm, __ldcg(part(i + u * ways) + kRows8 * DP + jrow));
           }
           const float top = mm == -INFINITY ? 0.f : mm;
-          for (int i = way; i < parts; i += ways) {
-            const float* q = i == 0 ? p0 : p1 + (int64_t)(i - 1) * 2 * kSlot;
-            const float f = ex2(__ldcg(q + kRows8 * DP + jrow) - top);
-            ll += f * __ldcg(q + kRows8 * DP + kRows8 + jrow);
+          for (int i = way; i < parts; i += ways * kAtOnce) {
+            float m[kAtOnce], l1[kAtOnce];
+            float4 v[kAtOnce][kCols];
 #pragma unroll
-            for (int c = 0; c < kCols; ++c)
-              add(f, __ldcg(reinterpret_cast<const float4*>(q + jrow * DP + c * 64 + jc)), c);
+            for (int u = 0; u < kAtOnce; ++u) {
+              const float* q = part(min(i + u * ways, parts - 1));
+              m[u] = __ldcg(q + kRows8 * DP + jrow);
+              l1[u] = __ldcg(q + kRows8 * DP + kRows8 + jrow);
+#pragma unroll
+              for (int c = 0; c < kCols; ++c)
+                v[u][c] = __ldcg(reinterpret_cast<const float4*>(q + jrow * DP + c * kStep + jc));
+            }
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) {
+              if (i + u * ways >= parts) continue;
+              const float f = ex2(m[u] - top);
+              ll += f * l1[u];
+#pragma unroll
+              for (int c = 0; c < kCols; ++c) add(f, v[u][c], c);
+            }
           }
         }
         if (ways > 1) {
-          static_assert(sizeof(sh->merge) >= kRows8 * DP * sizeof(float), "the ways' sums fit");
+          static_assert(sizeof(sh->merge) >= HP * kRows8 * DP * sizeof(float) &&
+                            HP * kRows8 <= kConsumers * kRows8, "the ways' sums fit");
           float* all = &sh->merge[0][0][0];
+          float(*sums)[2] = &sh->ml[0][0];  // [head and row][2]
 #pragma unroll
           for (int c = 0; c < kCols; ++c)
-            *reinterpret_cast<float4*>(all + trow * DP + c * 64 + jc) = acc[c];
-          if (jc == 0) sh->ml[0][trow][0] = mm, sh->ml[0][trow][1] = ll;
+            *reinterpret_cast<float4*>(all + any * DP + c * kStep + jc) = acc[c];
+          if (jc == 0) sums[any][0] = mm, sums[any][1] = ll;
           named_bar(1, kConsumers * kWarp);
           if (mine && way == 0) {
-            for (int i = 1; i < ways; ++i) mm = fmaxf(mm, sh->ml[0][jrow + (i << lg)][0]);
+            for (int i = 1; i < ways; ++i) mm = fmaxf(mm, sums[any + (i << lg)][0]);
             const float top = mm == -INFINITY ? 0.f : mm;
             ll = 0.f;
 #pragma unroll
             for (int c = 0; c < kCols; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
             for (int i = 0; i < ways; ++i) {
-              const int at = jrow + (i << lg);
-              const float f = ex2(sh->ml[0][at][0] - top);
-              ll += f * sh->ml[0][at][1];
+              const int at = any + (i << lg);
+              const float f = ex2(sums[at][0] - top);
+              ll += f * sums[at][1];
 #pragma unroll
               for (int c = 0; c < kCols; ++c)
-                add(f, *reinterpret_cast<const float4*>(all + at * DP + c * 64 + jc), c);
+                add(f, *reinterpret_cast<const float4*>(all + at * DP + c * kStep + jc), c);
             }
           }
           named_bar(1, kConsumers * kWarp);  // (the next pair writes the merge buffer)
         }
         if (mine && way == 0) {
           const float inv = ll > 0.f || ll != ll ? 1.f / ll : 0.f;
-          const int row = row0 + jrow;
-          const int64_t at = (int64_t)(s.q0 + row / P.G) * P.Hq + w.head * P.G + row % P.G;
+          const int64_t at = out_row(row0 + jrow, hh);
 #pragma unroll
           for (int c = 0; c < kCols; ++c)
-            if (c * 64 + jc < P.D)
-              *reinterpret_cast<uint2*>(P.out + at * P.D + c * 64 + jc) = make_uint2(
+            if (c * kStep + jc < P.D)
+              *reinterpret_cast<uint2*>(P.out + at * P.D + c * kStep + jc) = make_uint2(
                   pack2<T>(acc[c].x * inv, acc[c].y * inv), pack2<T>(acc[c].z * inv, acc[c].w * inv));
           if (P.lse && jc == 0)
             P.lse[at] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) * 0.69314718055994531f;
@@ -752,7 +788,7 @@ __device__ void stream_consumer8(const AttnParams& P, StreamSmem8<DP>* sh, Walk<
 }
 
 template <typename T, int DP, bool C8>
-__device__ void stream_consumer(const AttnParams& P, StreamSmem<DP, C8>* sh, Walk<kRows> w, int row0,
+__device__ void stream_consumer(const AttnParams& P, StreamSmem<DP, C8>* sh, Walk<kRows, kTile> w, int row0,
                                 int64_t share) {
   constexpr int kStages = StreamSmem<DP, C8>::kStages;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -1141,12 +1177,14 @@ __device__ void stream_consumer(const AttnParams& P, StreamSmem<DP, C8>* sh, Wal
   }
 }
 
-// R: rows of a row tile. 8 is the form for few rows over a cache of bytes.
-template <typename T, int DP, bool C8, int R>
-__global__ void __launch_bounds__(kThreads, R == kRows8 ? kCtasPerSm8 : kCtasPerSm)
+// HP: the form for few rows over a cache of bytes, by so many heads; 0: the other.
+template <typename T, int DP, bool C8, int HP>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm)
     k_attn_stream(const __grid_constant__ AttnMaps M, const __grid_constant__ AttnParams P) {
   extern __shared__ uint8_t smem_raw[];
-  using Smem = typename std::conditional<R == kRows8, StreamSmem8<DP>, StreamSmem<DP, C8>>::type;
+  constexpr int R = HP ? kRows8 : kRows, KT = HP ? 64 / (HP ? HP : 1) : kTile;
+  using Smem = typename std::conditional<HP != 0, StreamSmem8<DP, HP ? HP : 1>, StreamSmem<DP, C8>>::type;
+  const int heads = HP == 2 ? P.Hkv / 2 : P.Hkv;
   Smem* sh = reinterpret_cast<Smem*>(
       smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -1170,8 +1208,8 @@ __global__ void __launch_bounds__(kThreads, R == kRows8 ? kCtasPerSm8 : kCtasPer
   bool empty = false;
   for (int b = b0; b < b1; ++b) {
     const AttnSeq s = attn_seq(P, b);
-    const PairTiles t = pair_tiles<R>(P, s, row0);
-    mine += (int64_t)(t.t1 - t.t0) * P.Hkv;
+    const PairTiles t = pair_tiles<R, KT>(P, s, row0);
+    mine += (int64_t)(t.t1 - t.t0) * heads;
     if (blockIdx.x == 0 && blockIdx.y == 0 && (s.bad_len || s.bad_rows))
       atomicOr(P.status, (s.bad_len ? kAttnBadPage : 0u) | (s.bad_rows ? kAttnBadRows : 0u));
     empty |= t.t1 == t.t0 && (int64_t)s.n * P.G > row0;
@@ -1190,13 +1228,14 @@ __global__ void __launch_bounds__(kThreads, R == kRows8 ? kCtasPerSm8 : kCtasPer
     total += sh->scan[i];
   }
   const int64_t excl = before + incl - mine;
-  const int64_t share = total > 0 ? (total + gridDim.x - 1) / gridDim.x : 1;
+  int64_t share = total > 0 ? (total + gridDim.x - 1) / gridDim.x : 1;
+  if (HP == 2 && share < 2) share = 2;  // (64 keys, as in the other forms)
   const int64_t at = share * blockIdx.x;
   if (at >= excl && at < excl + mine) {
     int64_t pos = excl;
     for (int b = b0; b < b1; ++b) {
-      const PairTiles t = pair_tiles<R>(P, attn_seq(P, b), row0);
-      const int64_t n = (int64_t)(t.t1 - t.t0) * P.Hkv;
+      const PairTiles t = pair_tiles<R, KT>(P, attn_seq(P, b), row0);
+      const int64_t n = (int64_t)(t.t1 - t.t0) * heads;
       if (at < pos + n) {
         sh->start_seq = b;
         sh->start_item = pos;
@@ -1210,7 +1249,7 @@ __global__ void __launch_bounds__(kThreads, R == kRows8 ? kCtasPerSm8 : kCtasPer
   if (any_empty) {
     for (int b = blockIdx.x; b < P.batch; b += gridDim.x) {
       const AttnSeq s = attn_seq(P, b);
-      const PairTiles t = pair_tiles<R>(P, s, row0);
+      const PairTiles t = pair_tiles<R, KT>(P, s, row0);
       const int64_t all = (int64_t)s.n * P.G - row0;
       if (t.t1 != t.t0 || all <= 0) continue;
       const int rows = all < R ? (int)all : R;
@@ -1225,33 +1264,34 @@ __global__ void __launch_bounds__(kThreads, R == kRows8 ? kCtasPerSm8 : kCtasPer
   }
   if (at >= total) return;
   const int64_t count = total - at < share ? total - at : share;
-  Walk<R> w;
-  w.start(P, row0, sh->start_seq, sh->start_item, at, count);
+  Walk<R, KT> w;
+  w.start(P, row0, sh->start_seq, sh->start_item, at, count, heads);
   if (warp == kConsumers) {
     if constexpr (C8)
-      stream_producer8(P, M, sh, w, row0);
+      stream_producer8<HP ? HP : 1>(P, M, sh, w, row0);
     else
       stream_producer<DP>(P, M, sh, w, row0);
-  } else if constexpr (R == kRows8) {
-    stream_consumer8<T, DP>(P, sh, w, row0, share);
+  } else if constexpr (HP != 0) {
+    stream_consumer8<T, DP, HP>(P, sh, w, row0, share);
   } else {
     stream_consumer<T, DP, C8>(P, sh, w, row0, share);
   }
 }
 
-template <typename T, int DP, bool C8, int R>
+template <typename T, int DP, bool C8, int HP>
 int run_stream(const AttnMaps& M, const AttnParams& P, dim3 grid, cudaStream_t stream) {
-  constexpr size_t smem = (R == kRows8 ? sizeof(StreamSmem8<DP>) : sizeof(StreamSmem<DP, C8>)) + 1024;
-  static_assert((smem + 1024) * (R == kRows8 ? kCtasPerSm8 : kCtasPerSm) <= 228 * 1024, "blocks per SM");
+  constexpr size_t smem =
+      (HP ? sizeof(StreamSmem8<DP, HP ? HP : 1>) : sizeof(StreamSmem<DP, C8>)) + 1024;
+  static_assert(smem <= 113 * 1024, "two blocks per SM");
   static std::atomic<uint64_t> done{0};
-  cudaError_t err = allow_smem(k_attn_stream<T, DP, C8, R>, smem, done);
+  cudaError_t err = allow_smem(k_attn_stream<T, DP, C8, HP>, smem, done);
   if (err != cudaSuccess) return cuda_status(err);
-  return cuda_status(launch_pdl(k_attn_stream<T, DP, C8, R>, grid, dim3(kThreads), smem, stream, M, P));
+  return cuda_status(launch_pdl(k_attn_stream<T, DP, C8, HP>, grid, dim3(kThreads), smem, stream, M, P));
 }
 
-// Blocks per row tile: so many per SM over all row tiles, at least one.
-int stream_blocks(int64_t row_tiles, int per_sm = kCtasPerSm) {
-  int64_t w = (int64_t)per_sm * sm_count() / row_tiles;
+// Blocks per row tile: two per SM over all row tiles, at least one.
+int stream_blocks(int64_t row_tiles) {
+  int64_t w = (int64_t)kCtasPerSm * sm_count() / row_tiles;
   if (w < 1) w = 1;
   return (int)w;
 }
@@ -1266,41 +1306,55 @@ size_t attn_stream_partial_bytes(int64_t rows_max, int D) {
   return (size_t)(tiles * w) * 2 * (kRows * dp + 2 * kRows) * sizeof(float);
 }
 
-template <bool C8, int R>
+template <bool C8, int HP>
 int pick_stream(const ftb_attn_args& a, const AttnMaps& M, const AttnParams& P, int dp, dim3 grid,
                 cudaStream_t stream) {
   if (a.type == FTB_TYPE_BF16)
-    return dp == 64 ? run_stream<__nv_bfloat16, 64, C8, R>(M, P, grid, stream)
-                    : run_stream<__nv_bfloat16, 128, C8, R>(M, P, grid, stream);
-  return dp == 64 ? run_stream<__half, 64, C8, R>(M, P, grid, stream)
-                  : run_stream<__half, 128, C8, R>(M, P, grid, stream);
+    return dp == 64 ? run_stream<__nv_bfloat16, 64, C8, HP>(M, P, grid, stream)
+                    : run_stream<__nv_bfloat16, 128, C8, HP>(M, P, grid, stream);
+  return dp == 64 ? run_stream<__half, 64, C8, HP>(M, P, grid, stream)
+                  : run_stream<__half, 128, C8, HP>(M, P, grid, stream);
+}
+
+// Whether the form for few rows takes kv heads by pairs. That reads memory faster, but cuts half as many
+// pairs of sequence and heads into twice as many parts each, whose join is the end of a block's chain. By
+// what the host knows of the keys: where a block has at least 1.5 times as many tiles as a pair has parts.
+// On one B200, us (one head / pairs), 32 heads of 128 over 8: 1 token at 8192 keys 18.5 / 29.5, at 131072
+// 74.9 / 86.6; 2 at 32768 48.8 / 54.0, at 131072 124 / 113; 16 at 500 12.4 / 12.9; 64 at 300 21.6 / 19.7;
+// 61 at up to 8192 98 / 87; 3 at up to 131072 152 / 134.
+bool pair_heads(const ftb_attn_args& a) {
+  if (a.Hkv % 2) return false;
+  const double blocks = stream_blocks(1), pairs = 0.5 * a.batch * a.Hkv;
+  const double tiles = (double)a.batch * a.Hkv * (double)ceil_div((int64_t)a.table_width * a.page, kTile);
+  return tiles * pairs >= 1.5 * blocks * blocks;
 }
 
 int launch_attn_stream(const ftb_attn_args& a, AttnParams P, bool fp8, cudaStream_t stream) {
   AttnMaps M;
-  const uint32_t r = a.page < kTile ? a.page : kTile;
   const int dp = a.D <= 64 ? 64 : 128;
   const uint32_t halves = a.D == dp ? dp / 64 : 1;
-  int st = fp8 ? attn_cache_map8(&M.k, a.k_cache, a, a.k_strides, r)
+  const int hp = !fp8 || (int64_t)a.max_q * P.G > kRows8 ? 0 : pair_heads(a) ? 2 : 1;
+  const uint32_t keys = hp == 2 ? kTile / 2 : kTile, r = a.page < (int)keys ? a.page : keys;
+  int st = fp8 ? attn_cache_map8(&M.k, a.k_cache, a, a.k_strides, r, hp == 2 ? 2 : 1)
                : attn_cache_map(&M.k, a.k_cache, a, a.k_strides, r, halves);
   if (!st)
-    st = fp8 ? attn_cache_map8(&M.v, a.v_cache, a, a.v_strides, r)
+    st = fp8 ? attn_cache_map8(&M.v, a.v_cache, a, a.v_strides, r, hp == 2 ? 2 : 1)
              : attn_cache_map(&M.v, a.v_cache, a, a.v_strides, r, halves);
   if (st) return st;
   M.q = M.k;  // unused
-  if (fp8 && (int64_t)a.max_q * P.G <= kRows8) {
-    // (its parts are fewer and smaller than the workspace allows: 3 blocks' of 8 rows against 2 of 16)
-    static_assert(kCtasPerSm8 * kRows8 <= kCtasPerSm * kRows, "parts fit the workspace");
-    const int64_t w = stream_blocks(1, kCtasPerSm8);
-    if (w > kAttnCounters) return FTB_ERR_SHAPE;
-    return pick_stream<true, kRows8>(a, M, P, dp, dim3((unsigned)w), stream);
+  if (hp) {
+    // (parts of 2 x 8 rows are no larger than those of 16 that the workspace is for)
+    const dim3 grid((unsigned)stream_blocks(1));
+    if ((int)grid.x > kAttnCounters) return FTB_ERR_SHAPE;
+    return hp == 2 ? pick_stream<true, 2>(a, M, P, dp, grid, stream)
+                   : pick_stream<true, 1>(a, M, P, dp, grid, stream);
   }
   const int64_t tiles = ceil_div((int64_t)a.max_q * P.G, kRows);
   const int64_t w = stream_blocks(tiles);
   if (tiles > 65535 || (w > 1 && tiles * w > kAttnCounters)) return FTB_ERR_SHAPE;
   const dim3 grid((unsigned)w, (unsigned)tiles);
-  return fp8 ? pick_stream<true, kRows>(a, M, P, dp, grid, stream)
-             : pick_stream<false, kRows>(a, M, P, dp, grid, stream);
+  return fp8 ? pick_stream<true, 0>(a, M, P, dp, grid, stream)
+             : pick_stream<false, 0>(a, M, P, dp, grid, stream);
 }
 
 }  // namespace ftb

@@ -61,6 +61,21 @@ def test_decode_long_split_over_blocks():
     check(Fp8Case([(1, 20011), (1, 3), (1, 9000)], q_heads=8, kv_heads=2, page=64, block=32, cu=False))
 
 
+@pytest.mark.parametrize("kv_heads", [1, 2, 3, 6, 8])
+@pytest.mark.parametrize("head", [64, 80, 128])
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+def test_decode_batch_by_one_head_and_by_pairs(page, head, kv_heads):
+    """Enough keys for two heads at a time (even numbers of kv heads), in any pages, with sequences
+    without keys, windows over parts of tiles and rows beyond one token."""
+    g = torch.Generator().manual_seed(page + head + kv_heads)
+    kv = torch.randint(0, 700, (90,), generator=g).tolist()
+    c = Fp8Case([(1, n) for n in kv], q_heads=4 * kv_heads, kv_heads=kv_heads, head=head, page=page,
+                cu=False, window=333 if page == 32 else 0, dtype=F16 if page == 64 else BF)
+    check(c)
+    check(Fp8Case([(2, n) for n in kv[:60]], q_heads=3 * kv_heads, kv_heads=kv_heads, head=head, page=page,
+                  block=16))
+
+
 @pytest.mark.parametrize("window", [1, 7, 64, 65, 500])
 def test_one_token_window(window):
     check(Fp8Case([(1, 700), (1, 64), (1, 5)], window=window, cu=False))
