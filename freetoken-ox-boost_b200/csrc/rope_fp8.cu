@@ -128,17 +128,27 @@ struct Column {
     }
   }
   struct Raw {
-    uint16_t a[VEC], b[VEC];
+    typename Chunk<VEC>::type a, b;
   };
   __device__ __forceinline__ Raw load(const uint16_t* head) const {
-    Raw r;
-    load_bits<VEC>(head + e0, r.a);
-    load_bits<VEC>(head + e1, r.b);
-    return r;
+    return Raw{*reinterpret_cast<const typename Chunk<VEC>::type*>(head + e0),
+               *reinterpret_cast<const typename Chunk<VEC>::type*>(head + e1)};
   }
   __device__ __forceinline__ void unpack(const Raw& r, float (&x)[2 * VEC]) const {
+    uint16_t a[VEC], b[VEC];
+    memcpy(a, &r.a, sizeof(a));
+    memcpy(b, &r.b, sizeof(b));
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) x[j] = elem_f32<T>(r.a[j]), x[VEC + j] = elem_f32<T>(r.b[j]);
+    for (int j = 0; j < VEC; ++j) x[j] = elem_f32<T>(a[j]), x[VEC + j] = elem_f32<T>(b[j]);
+  }
+  __device__ __forceinline__ Raw pack(const float (&x)[2 * VEC]) const {
+    uint16_t a[VEC], b[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) a[j] = elem_bits<T>(x[j]), b[j] = elem_bits<T>(x[VEC + j]);
+    Raw r;
+    memcpy(&r.a, a, sizeof(a));
+    memcpy(&r.b, b, sizeof(b));
+    return r;
   }
   // cos and sin of token t at this column's frequencies
   __device__ __forceinline__ void angles(const RopeParams& P, int64_t t, float (&cs)[VEC],
@@ -220,11 +230,10 @@ __device__ __forceinline__ void turn_q(const RopeParams& P, int64_t t0, int64_t 
         float x[2 * VEC];
         c.unpack(r, x);
         c.turn(P, cs, sn, x);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) r.a[j] = elem_bits<T>(x[j]), r.b[j] = elem_bits<T>(x[VEC + j]);
+        r = c.pack(x);
       }
-      store_bits<VEC>(dst + c.e0, r.a);
-      store_bits<VEC>(dst + c.e1, r.b);
+      *reinterpret_cast<typename Chunk<VEC>::type*>(dst + c.e0) = r.a;
+      *reinterpret_cast<typename Chunk<VEC>::type*>(dst + c.e1) = r.b;
     }
   }
 }

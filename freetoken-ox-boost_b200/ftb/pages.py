@@ -53,7 +53,7 @@ def _copy_args(caches, src, dst):
         if a.page_strides[i] < a.page_bytes[i]:
             raise ValueError(f"cache {i}: pages {t.stride(0)} elements apart overlap")
     a.num_pages = caches[0].shape[0]
-    return dev, a
+    return a
 
 
 def _ids(x, name, num_pages, dev):
@@ -74,31 +74,34 @@ def copy_pages(caches, src, dst) -> None:
     ``dst``: int32 or int64 device tensors of one length, or lists of ids. A pair with an id outside
     the pages (-1: padding), or twice the same, copies nothing. The copies have no order: no page may be
     in ``dst`` twice, or in ``src`` and ``dst`` (lists are checked, tensors are not)."""
-    caches = list(caches)
+    if type(caches) is not list:
+        caches = list(caches)
     if not caches:
         return
-    if not isinstance(src, torch.Tensor) and not isinstance(dst, torch.Tensor):
-        src, dst = list(src), list(dst)
-        to = [d for s, d in zip(src, dst) if s != d and s >= 0 and d >= 0]
-        if len(src) != len(dst) or len(set(to)) != len(to) or set(to) & {
-                s for s, d in zip(src, dst) if s != d and d >= 0}:
-            raise ValueError("src and dst differ in length, or a page is copied to twice, or copied "
-                             "both from and to")
-    dev = require_cuda(caches[0])
-    src = _ids(src, "src", caches[0].shape[0], dev)
-    dst = _ids(dst, "dst", caches[0].shape[0], dev)
-    most = max(t.dim() for t in caches)
-    step = min(_GROUP, max(1, 240 // (1 + 2 * most)))
+    if not isinstance(src, torch.Tensor) or not isinstance(dst, torch.Tensor):
+        if not isinstance(src, torch.Tensor) and not isinstance(dst, torch.Tensor):
+            src, dst = list(src), list(dst)
+            to = [d for s, d in zip(src, dst) if s != d and s >= 0 and d >= 0]
+            if len(src) != len(dst) or len(set(to)) != len(to) or set(to) & {
+                    s for s, d in zip(src, dst) if s != d and d >= 0}:
+                raise ValueError("src and dst differ in length, or a page is copied to twice, or copied "
+                                 "both from and to")
+        dev = require_cuda(caches[0])
+        src = _ids(src, "src", caches[0].shape[0], dev)
+        dst = _ids(dst, "dst", caches[0].shape[0], dev)
+    step = _GROUP
+    if len(caches) > step or sum(t.dim() for t in caches) > 4 * step:
+        step = min(step, max(1, 120 // (1 + max(t.dim() for t in caches))))
     for at in range(0, len(caches), step):
-        group = caches[at:at + step]
+        group = caches if len(caches) <= step else caches[at:at + step]
         key = _pycall.key(src, dst, *group)
         known = _ARGS.get(key)
         if known is None:
-            dev, a = _copy_args(group, src, dst)
-            if group[0].shape[0] != caches[0].shape[0]:
-                raise ValueError(f"cache {at}: {group[0].shape[0]} pages, expected "
-                                 f"{caches[0].shape[0]}")
-            known = remember(key, a, _OFFSETS[:len(group)] + _IDS)
+            if group[0].shape[:1] != caches[0].shape[:1]:
+                raise ValueError(f"cache {at}: shape {tuple(group[0].shape)}, expected "
+                                 f"{caches[0].shape[0]} pages in dimension 0")
+            known = remember(key, _copy_args(group, src, dst), _OFFSETS[:len(group)] + _IDS)
+        dev = group[0].device
         st = caller(dev)(_lib.entry("ftb_copy_pages"), known[0], known[1], stream_handle(dev), *group,
                          src, dst)
         if st:
