@@ -38,6 +38,13 @@
 // 9 the TMA copies, 10 clears V rows that no token of the item may see (their weight is 0, but
 // 0 x NaN is not). K and V tiles share a ring in the order of their use: K0 V0 K1 V1 ...
 //
+// A cache of bytes (C8, attn.cuh has the arithmetic of its scales): tiles land as bytes, and warps 10 and
+// 11 turn them into 16-bit operands in place; P is f16, its reference a base-2 logarithm that starts at
+// the lowest scale of V in the first tile and may lag by 2^14; the scales come by plain loads of the
+// copying warp. The chunk above takes 2.24 ms so (0.56 of a large product's rate), the prompts 129 us, 12
+// ragged chunks in f16 50 us. Of a chunk of 2048 tokens at 16384 keys (636 us) the tensor pipe is active
+// 42 %, and 58 MB come from DRAM.
+//
 // k_attn_plan lists the pieces of a call (an item, or a part of its keys where items are too few
 // or too long to fill the SMs evenly), largest first; parts leave (ref, l, O) in the workspace and
 // k_attn_join puts them together in their order in the sequence.

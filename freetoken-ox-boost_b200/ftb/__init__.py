@@ -1,6 +1,6 @@
 """ftb - a B200-native (sm_100a) NVFP4 fused-MoE layer with FreeToken's MoE backend API, and the
 operators of a decoder layer around it (norms with gated residual, rotary positions, paged
-attention).
+attention over caches in 16 or 8 bits, copies of their pages).
 
 Host code is Python/PyTorch; all device work runs in ``libftb.so`` (hand-written CUDA,
 C ABI in ``include/ftb.h``), loaded through ctypes. There is no CPU or Triton fallback.

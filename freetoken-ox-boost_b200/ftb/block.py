@@ -275,6 +275,8 @@ def _rope(q, k, v, positions, table, k_dst, v_dst, slots, sections, order, pairs
 def _rope_fp8(q, k, v, positions, table, k_cache, v_cache, slots, sections, order, pairs, q_out,
               k_scale, v_scale):
     """The call into an 8-bit cache."""
+    if slots is None or v is None:
+        raise ValueError("an 8-bit cache takes v and the slots of the tokens")
     if sections is not None:
         sections = tuple(map(int, sections))
     key = (_pycall.key(q, k, positions, table, v, k_cache, v_cache, slots, k_scale, v_scale), sections,

@@ -558,8 +558,10 @@ FTB_API int ftb_rope_fp8(const ftb_rope_fp8_args* args, ftb_stream_t stream);
 /*
  * ftb_attention() over an 8-bit cache: attn.k_cache and attn.v_cache are the caches, attn.k_strides and
  * attn.v_strides in bytes (multiples of 16), D % 16 == 0, page >= scale_block; all else as there, the
- * workspace among it. Products are those of the codes with q in f16 (a bf16 row that f16 would not hold
- * is taken times a power of two), the probabilities' operand is f16.
+ * workspace among it. Products are those of the codes: with q as it is in calls of many rows, with q in
+ * f16 in the others (a bf16 row that f16 would not hold is taken times a power of two; what f16 drops is
+ * below 2^-21 of the row's largest). The probabilities' operand is f16; where the output is f16 too, the
+ * rest of that rounding is a second operand in calls of few rows.
  */
 typedef struct ftb_attn_fp8_args {
   ftb_attn_args attn;
