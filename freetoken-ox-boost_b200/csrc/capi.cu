@@ -147,6 +147,15 @@ int cuda_status(cudaError_t err) {
   return FTB_ERR_CUDA;
 }
 
+void bind_context() {
+  static thread_local uint64_t bound = 0;  // a bit per device
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (bound & bit) return;
+  if (cudaSetDevice(dev) == cudaSuccess) bound |= bit;
+}
+
 int sm_count() {
   static std::mutex mu;
   static std::vector<int> cache;

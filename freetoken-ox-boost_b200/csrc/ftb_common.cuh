@@ -20,6 +20,10 @@ int cuda_status(cudaError_t err);
 // Number of SMs of the current device (cached per device).
 int sm_count();
 
+// Makes the current device's context current to this thread, which driver calls (tensor maps) need and
+// a thread that has made no call of the runtime yet lacks.
+void bind_context();
+
 __host__ __device__ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // ---------------------------------------------------------------------------------------

@@ -748,6 +748,7 @@ PFN_cuTensorMapEncodeTiled encode_fn() {
         q == cudaDriverEntryPointSuccess)
       fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled>(p);
   });
+  bind_context();
   return fn;
 }
 

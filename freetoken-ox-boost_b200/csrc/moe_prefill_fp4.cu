@@ -682,6 +682,7 @@ PFN_cuTensorMapEncodeTiled f4_encode_fn() {
         qr == cudaDriverEntryPointSuccess)
       fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled>(p);
   });
+  bind_context();
   return fn;
 }
 
