@@ -261,3 +261,99 @@ def test_q_in_place():
     out = ftb.rope_append(q, k, v, c["positions"].cuda(), c["table"].cuda(), kc, vc, c["slots"].cuda(),
                           k_scale=c["k_scale"].cuda(), v_scale=c["v_scale"].cuda(), q_out=q)
     assert out is q and torch.equal(q.cpu(), want)
+
+
+def test_offsets_past_32_bits():
+    """Caches of more than 2^32 bytes: the last pages are written like the first, found by a scan and by
+    the table of slots."""
+    page, heads, D = 64, 8, 128
+    pages = (1 << 32) // (page * heads * D) + 64
+    big = [torch.empty(pages, page, heads, D, dtype=torch.uint8, device="cuda") for _ in "kv"]
+    scales = [torch.zeros(pages, 1, heads, device="cuda") for _ in "kv"]
+    for tokens in (70, 2200):
+        last = -(-tokens // page) + 1
+        c = make(tokens, range(3, 3 + tokens), heads=(8, 8), D=D, rot=D, page=page, block=64, pages=last)
+        want = call(c)
+        far = slice(pages - last, pages)
+        for t, n in zip(big, ("k_cache", "v_cache")):
+            t[far] = c[n].cuda()
+        for t, n in zip(scales, ("k_scale", "v_scale")):
+            t[far] = c[n].cuda()
+        q, k, v = c["qkv"].cuda().split([8, 8, 8], 1)
+        slots = c["slots"].cuda() + (pages - last) * page
+        out = ftb.rope_append(q, k, v, c["positions"].cuda(), c["table"].cuda(), big[0].view(FP8),
+                              big[1].view(FP8), slots, k_scale=scales[0], v_scale=scales[1])
+        assert torch.equal(out.cpu(), want["q"])
+        for t, n in zip(big + scales, ("k_cache", "v_cache", "k_scale", "v_scale")):
+            assert torch.equal(t[far].cpu(), want[n]), n
+
+
+def test_calls_of_two_threads_and_two_streams():
+    """Threads on one stream, and calls on several streams at once, each with its own caches."""
+    import threading
+
+    cases = [make(n, range(5, 5 + n), pages=80, seed=n) for n in (40, 2300, 700, 2500)]
+    wants = [call(c) for c in cases]
+    errors = []
+
+    def work(c, want, stream):
+        try:
+            with torch.cuda.stream(stream):
+                for _ in range(4):
+                    got = call(c)
+                    assert all(torch.equal(got[n], want[n]) for n in want)
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    shared = torch.cuda.Stream()
+    streams = [shared, shared, torch.cuda.Stream(), torch.cuda.Stream()]
+    threads = [threading.Thread(target=work, args=a) for a in zip(cases, wants, streams)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+
+
+def test_captured_before_any_call():
+    """A call captured on a stream that has run none has a workspace of its own."""
+    c = make(2100, range(9, 2109), pages=80, seed=3)
+    dev = {n: c[n].cuda() for n in ("qkv", "positions", "table", "slots", "k_scale", "v_scale", "k_cache",
+                                    "v_cache")}
+    start = {n: x.clone() for n, x in dev.items()}
+    q, k, v = dev["qkv"].split([4, 2, 2], 1)
+    stream = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=stream):
+        out = ftb.rope_append(q, k, v, dev["positions"], dev["table"], dev["k_cache"].view(FP8),
+                              dev["v_cache"].view(FP8), dev["slots"], k_scale=dev["k_scale"],
+                              v_scale=dev["v_scale"])
+    want = call(c)
+    for _ in range(3):
+        for n in ("k_cache", "v_cache", "k_scale", "v_scale"):
+            dev[n].copy_(start[n])
+        graph.replay()
+        assert torch.equal(out.cpu(), want["q"])
+        for n in ("k_cache", "v_cache", "k_scale", "v_scale"):
+            assert torch.equal(dev[n].cpu(), want[n])
+
+
+def test_refusals():
+    c = make(4, range(4))
+    q, k, v = c["qkv"].cuda().split([4, 2, 2], 1)
+    good = dict(k_cache=c["k_cache"].cuda().view(FP8), v_cache=c["v_cache"].cuda().view(FP8),
+                slots=c["slots"].cuda(), k_scale=c["k_scale"].cuda(), v_scale=c["v_scale"].cuda())
+    pos, table = c["positions"].cuda(), c["table"].cuda()
+    ftb.rope_append(q, k, v, pos, table, **good)
+    for bad in (dict(k_scale=None), dict(v_scale=None), dict(k_cache=good["k_cache"].view(torch.uint8)),
+                dict(k_cache=good["k_cache"].view(torch.uint8).bfloat16()), dict(slots=None),
+                dict(k_scale=good["k_scale"].half()), dict(v_scale=good["v_scale"][:, :1]),
+                dict(k_scale=good["k_scale"].cpu()), dict(slots=good["slots"][:3]),
+                dict(k_scale=good["k_scale"][:, :, :1], v_scale=good["v_scale"][:, :, :1]),
+                dict(v_cache=good["v_cache"][:, :16])):
+        with pytest.raises(ValueError):
+            ftb.rope_append(q, k, v, pos, table, **{**good, **bad})
+    # (the caches are held in 8 bits, so a call without scales is refused too)
+    with pytest.raises(ValueError):
+        ftb.rope_append(q, k, v, pos, table, good["k_cache"], good["v_cache"], good["slots"])

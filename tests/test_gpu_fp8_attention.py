@@ -320,3 +320,40 @@ def test_offsets_past_32_bits():
     t["block_table"] = t["block_table"].clone()
     t["block_table"][0, :4] = far.int()
     compare(c, *ftb.paged_attention(**t, return_lse=True, check_status=True), *ref)
+
+
+def test_refusals():
+    c = Fp8Case([(1, 100)], cu=False, page=32, block=16)
+    build(c)
+    ftb.paged_attention(**c.t)
+    for bad in (dict(k_scale=None), dict(v_scale=None), dict(k_cache=c.t["k_cache"].view(torch.uint8)),
+                dict(k_scale=c.t["k_scale"].double(), v_scale=c.t["v_scale"].double()),
+                dict(v_scale=c.t["v_scale"][:, :1]), dict(k_scale=c.t["k_scale"].cpu()),
+                dict(q=c.t["q"].float()), dict(q=c.t["q"][..., :64])):
+        with pytest.raises(ValueError):
+            ftb.paged_attention(**{**c.t, **bad})
+    with pytest.raises(ValueError):  # an 8-bit cache without its scales
+        ftb.paged_attention(**{**c.t, "k_scale": None, "v_scale": None})
+
+
+def test_calls_of_two_threads():
+    import threading
+
+    cases = [Fp8Case([(1, 4000)] * 9, cu=False, page=64, block=64, seed=1),
+             Fp8Case([(600, 1500)], q_heads=16, seed=2)]
+    refs = [reference(c, *build(c)) for c in cases]
+    errors = []
+
+    def work(i):
+        try:
+            for _ in range(10):
+                compare(cases[i], *ftb.paged_attention(**cases[i].t, return_lse=True), *refs[i])
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1, 0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
