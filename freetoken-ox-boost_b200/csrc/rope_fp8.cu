@@ -14,15 +14,17 @@
 //
 // The rows of a block are spread over the call's tokens in any order, so a block has one owner: the
 // token with its lowest written row. Its thread block collects W, takes the maximum over W and writes
-// all of W. A call of few tokens finds W by a scan of all slots (kScan); a larger one by a table of the
-// token at each slot, written by a small launch before. Entries of the table are checked against the
+// all of W. In calls of up to kTogether tokens, which have few blocks or few rows in each, the written
+// tokens of a block share its heads instead. A call of few tokens finds W by a scan of all slots (kScan);
+// a larger one by a table of the token at each slot, written by a small launch before. Entries of the table are checked against the
 // slots, so what it held before does not matter; of two tokens with one slot one is kept.
 //
 // Bound: DRAM, (2 Hq + 2 Hkv) D 2 + 2 Hkv D bytes per token. The blocks are bound by latencies (the
 // table, the slots, the tokens, then the second pass over them, which comes from L1), so they come first
 // in the grid and the tokens' q, a plain stream, fills the SMs beside them: registers are kept low for
 // both. With four items a thread kept in fp32 (171 registers, one block per SM) and q in a launch of its
-// own, 20440 tokens of 32 + 8 + 8 heads of 128 took 243 us.
+// own, 20440 tokens of 32 + 8 + 8 heads of 128 took 243 us; they take 104, 4.2 TB/s, 0.67 of the measured
+// copy rate; 64 tokens of 64 sequences 6.6 us.
 #include "rope.cuh"
 
 namespace ftb {
@@ -34,9 +36,14 @@ constexpr int kKept = 1;         // items of a thread that stay in registers
 constexpr int kItems = 8;        // items of a thread that a thread block is made for
 constexpr int kMaxBlock = 128;   // tokens per scale
 constexpr int kMaxHeads = 256;   // of a thread block
-constexpr int kScan = 2048;      // tokens up to which an owner scans all slots
+// Tokens up to which the slots are scanned (one prompt of 2048 tokens 22.8 us, by the table 24.5; 2048
+// tokens of as many sequences 85 against 72), and up to which a block's tokens share its heads (a prompt
+// of 512 tokens 11.1 us, by owners 17.5, of 2048 31.7 and 22.8; 256 tokens of as many sequences 8.6 and
+// 11.8).
+constexpr int kScan = 2048, kTogether = 1024;
+static_assert(kTogether <= kScan, "what is shared is scanned for");
 constexpr int kMaxRange = 64;    // tokens per thread block beyond that, at most
-constexpr int kManyTokens = 4096;  // from here on a thread block turns q of eight tokens
+constexpr int kManyTokens = 4096;  // from here on a thread block turns q of eight tokens (30.2 us, one: 35.4)
 constexpr float kMaxScale = 0x1p40f, kMinScale = 0x1p-40f;
 
 struct AppendParams {
@@ -48,6 +55,7 @@ struct AppendParams {
   int32_t* token_at;     // the table; NULL: scan
   int block_log2;
   int splits, per_split;  // thread blocks per token range: K or V, per_split heads each
+  int together;
   int append_blocks;
   int range, q_tokens;  // tokens per thread block: of keys and values, of q
 };
@@ -241,7 +249,7 @@ __device__ __forceinline__ void turn_q(const RopeParams& P, int64_t t0, int64_t 
 struct AppendShared {
   int token[kMaxBlock];  // by row of the block: the call's token there, -1: none
   int row[kMaxBlock], tok[kMaxBlock];  // the written rows, ascending
-  int n, last;
+  int n, last, rank;
   uint32_t candidates[kMaxRange / 32];
   uint32_t top[kMaxHeads];  // by head: largest |x|, as bits
   float by[kMaxHeads];      // 1 / scale
@@ -274,6 +282,7 @@ __device__ void append_block(const AppendParams& A, AppendShared& sh, int64_t t,
     }
     __syncthreads();
   }
+  if (tid == 0) sh.rank = -1;
   if (tid < 32) {
     int n = 0, last = 0;
     for (int r0 = 0; r0 < size; r0 += 32) {
@@ -289,13 +298,23 @@ __device__ void append_block(const AppendParams& A, AppendShared& sh, int64_t t,
   for (int h = tid; h < nh; h += kThreads) sh.top[h] = 0;
   __syncthreads();
   const int n = sh.n;
-  if (n == 0 || sh.tok[0] != t) return;  // (n: another token of this slot is kept)
+  // The owner's thread block has all heads; or token r of the n written has heads r, r + n, ...
+  int h_step = 1;
+  if (A.together) {
+    if (tid < n && sh.tok[tid] == t) sh.rank = tid;
+    __syncthreads();
+    const int rank = sh.rank;
+    if (rank < 0 || rank >= nh) return;  // (below 0: another token of this slot is kept)
+    h0 += rank, h_step = n, nh = (nh - rank + n - 1) / n;
+  } else if (n == 0 || sh.tok[0] != t) {
+    return;
+  }
   const bool fresh = sh.row[0] == 0;
   // old scales, asked for early
   float* scale = A.scale[kind] + page * A.scale_st[kind][0] +
                  (int64_t)(row0 >> A.block_log2) * A.scale_st[kind][1];
   float old = 0.f;
-  if (tid < nh && !fresh) old = scale[(h0 + tid) * A.scale_st[kind][2]];
+  if (tid < nh && !fresh) old = scale[(h0 + tid * h_step) * A.scale_st[kind][2]];
 
   // A thread has a column of some heads of some rows: slot / across is its first row, slot % across its
   // first head. Where there are many rows it has all heads of a row, whose angles it takes once a pass;
@@ -321,7 +340,7 @@ __device__ void append_block(const AppendParams& A, AppendShared& sh, int64_t t,
     return it;
   };
   auto get = [&](const Item& it) {
-    return c.load(src + sh.tok[it.w] * src_st + (h0 + it.h) * src_sh);
+    return c.load(src + sh.tok[it.w] * src_st + (h0 + it.h * h_step) * src_sh);
   };
   float cs[VEC], sn[VEC];
   int angles_of = -1;
@@ -367,10 +386,10 @@ __device__ void append_block(const AppendParams& A, AppendShared& sh, int64_t t,
   }
   __syncthreads();
   for (int h = tid; h < nh; h += kThreads) {
-    if (h != tid && !fresh) old = scale[(h0 + h) * A.scale_st[kind][2]];
+    if (h != tid && !fresh) old = scale[(h0 + h * h_step) * A.scale_st[kind][2]];
     const float so_far = fresh ? 0.f : scale_so_far(old);
     const float now = fmaxf(so_far, scale_for(__uint_as_float(sh.top[h])));
-    scale[(h0 + h) * A.scale_st[kind][2]] = now;
+    scale[(h0 + h * h_step) * A.scale_st[kind][2]] = now;
     sh.by[h] = 1.f / now;
     sh.again[h] = so_far > 0.f && now != old ? old / now : 0.f;
   }
@@ -380,7 +399,7 @@ __device__ void append_block(const AppendParams& A, AppendShared& sh, int64_t t,
   auto put = [&](const Item& it, const Raw& r) {
     float x[2 * VEC];
     number(it, r, x);
-    uint8_t* to = dst + sh.row[it.w] * st_row + (h0 + it.h) * st_head;
+    uint8_t* to = dst + sh.row[it.w] * st_row + (h0 + it.h * h_step) * st_head;
     store_e4m3<VEC>(to + c.e0, x, sh.by[it.h]);
     store_e4m3<VEC>(to + c.e1, x + VEC, sh.by[it.h]);
   };
@@ -399,7 +418,7 @@ __device__ void append_block(const AppendParams& A, AppendShared& sh, int64_t t,
       const int h = item / rows, r = item - h * rows;
       const float f = sh.again[h];
       if (f == 0.f || sh.token[r] >= 0) continue;
-      uint8_t* at = dst + r * st_row + (h0 + h) * st_head;
+      uint8_t* at = dst + r * st_row + (h0 + h * h_step) * st_head;
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         uint8_t* p = at + (k ? c.e1 : c.e0);
@@ -445,7 +464,9 @@ __global__ void __launch_bounds__(kThreads, kPerSm)
     if ((int)threadIdx.x < A.range && t < P.tokens) {
       const int64_t s = slot_of(P, t);
       const bool first = (s & ((1 << A.block_log2) - 1)) == 0;
-      if (s >= 0 && !A.token_at) {
+      if (s >= 0 && A.together) {
+        can = true;
+      } else if (s >= 0 && !A.token_at) {
         can = first || t == 0 || slot_of(P, t - 1) != s - 1;
       } else if (s >= 0 && A.token_at[s] == t) {
         const int w = first ? -1 : A.token_at[s - 1];
@@ -481,14 +502,18 @@ int run_append(AppendParams A, cudaStream_t stream) {
   // heads per thread block: as many as its registers hold of a full block of tokens
   const int rows = (int)(T0 < (1 << A.block_log2) ? T0 : (1 << A.block_log2));
   int per = step * kItems / rows;
+  per = per < 1 ? 1 : per;
+  A.together = T0 <= kTogether;
+  // (shared, more heads where the blocks would not all be on the SMs at once)
+  while (A.together && per < P.Hkv && T0 * 2 * ceil_div(P.Hkv, per) > kPerSm * sm_count()) per *= 2;
   per = per > kMaxHeads ? kMaxHeads : per;
   per = per < 1 ? 1 : per > P.Hkv ? P.Hkv : per;
   A.per_split = per;
   A.splits = 2 * (int)ceil_div(P.Hkv, per);
   // Tokens of a thread block: a block of the cache, so that neighbours have one owner among them; fewer
-  // where that would not fill the SMs twice (1283 tokens, blocks of 16: 27 us with 64, 9 with this).
+  // where that would not fill the SMs twice.
   A.range = 1;
-  while (A.range < kMaxRange && A.range < (1 << A.block_log2) &&
+  while (!A.together && A.range < kMaxRange && A.range < (1 << A.block_log2) &&
          T0 * A.splits >= (int64_t)A.range * 2 * 2 * kPerSm * sm_count())
     A.range *= 2;
   int64_t blocks = ceil_div(T0, A.range) * A.splits;
