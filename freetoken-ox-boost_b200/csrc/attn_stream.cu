@@ -30,8 +30,10 @@
 // A cache of bytes (C8, attn.cuh has the arithmetic of its scales) is read by the same walk and ring: codes
 // become f16 in registers, and a stage's scales come by plain loads beside its copies. Up to 8 rows have
 // a form of their own (stream_consumer8), by one or two kv heads a block. On one B200, 32 heads of 128
-// over 8: 61 tokens at up to 8192 keys (418 MB) 87 us, 4.8 TB/s, 0.75 of the measured copy rate; 3 at up
-// to 131072 keys (720 MB) 134 us, 5.4 TB/s, 0.84; one at 901 keys 12.5 us.
+// over 8: 61 tokens at up to 8192 keys (418 MB) 89 us, 4.7 TB/s, 0.73 of the measured copy rate; 3 at up
+// to 131072 keys (719 MB) 131 us, 5.5 TB/s, 0.86; one at 901 keys 13.3 us. P is f16, whose numbers the codes
+// are, and the rest of that rounding here too, whatever the tensors' type: with P alone 87, 131 and 13.2 us in
+// bf16, where 7 to 10 outputs of 100 were rounded otherwise than the exact ones (now 1 to 2 of 1000).
 //
 // The consumers share barriers without a limit, so a warp whose wait gives up passes them all the
 // same: it takes no more tiles, makes its rows' sums NaN, and walks on through its share's joins
@@ -446,7 +448,6 @@ __device__ void stream_consumer8(const AttnParams& P, StreamSmem8<DP, HP>* sh, W
   constexpr int kWarps = kConsumers / HP, KT = 64 / HP;  // warps of a head, keys of a stage
   constexpr int kStages = Smem::kStages, VB = DP / 8;
   constexpr float kLazy = 10.f;
-  constexpr bool kRest = std::is_same<T, __half>::value;  // (as above)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t2 = (lane & 3) * 2;  // key (or columns) of the lane; its rows t2, t2 + 1
   const StreamSync<Smem> sy{sh, P.status};
@@ -571,10 +572,8 @@ __device__ void stream_consumer8(const AttnParams& P, StreamSmem8<DP, HP>* sh, W
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         pb[h] = pack2<__half>(p[2 * h], p[2 * h + 1]);
-        if constexpr (kRest) {
-          const float2 a = unpack2<__half>(pb[h]);
-          rb[h] = transpose8(pack2<__half>(p[2 * h] - a.x, p[2 * h + 1] - a.y));
-        }
+        const float2 a = unpack2<__half>(pb[h]);
+        rb[h] = transpose8(pack2<__half>(p[2 * h] - a.x, p[2 * h + 1] - a.y));
         pb[h] = transpose8(pb[h]);
       }
 #pragma unroll
@@ -593,7 +592,7 @@ __device__ void stream_consumer8(const AttnParams& P, StreamSmem8<DP, HP>* sh, W
                                  e4m3x2_to_f16x2((uint16_t)(x[1][c] & 0xffffu)),
                                  e4m3x2_to_f16x2((uint16_t)(x[1][c] >> 16))};
           mma16816<__half>(o[2 * k + c], a, pb[0], pb[1]);
-          if constexpr (kRest) mma16816<__half>(o[2 * k + c], a, rb[0], rb[1]);
+          mma16816<__half>(o[2 * k + c], a, rb[0], rb[1]);
         }
       }
       __syncwarp();
@@ -800,10 +799,8 @@ __device__ void stream_consumer(const AttnParams& P, StreamSmem<DP, C8>* sh, Wal
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t2 = (lane & 3) * 2;
   const StreamSync<StreamSmem<DP, C8>> sy{sh, P.status};
-  // P's type: the tensors', or f16 beside V's codes, which are f16 numbers. The rounding's rest goes
-  // along where the output is as fine as P.
+  // P's type: the tensors', or f16 beside V's codes, which are f16 numbers
   using TP = typename std::conditional<C8, __half, T>::type;
-  constexpr bool kRest = std::is_same<TP, T>::value;
   const int page = 1 << P.page_log2;
   const int r = page < kTile ? page : kTile;
   const int half_bytes = r * 128, box_bytes = half_bytes * (DP / 64);
@@ -922,11 +919,9 @@ __device__ void stream_consumer(const AttnParams& P, StreamSmem<DP, C8>* sh, Wal
                   : l[e] * f + ((p0 + p1) + (p2 + p3));
         pa[e] = pack2<TP>(p0, p1);
         pa[2 + e] = pack2<TP>(p2, p3);
-        if constexpr (kRest) {
-          const float2 a = unpack2<TP>(pa[e]), b = unpack2<TP>(pa[2 + e]);
-          pr[e] = pack2<TP>(p0 - a.x, p1 - a.y);
-          pr[2 + e] = pack2<TP>(p2 - b.x, p3 - b.y);
-        }
+        const float2 a = unpack2<TP>(pa[e]), b = unpack2<TP>(pa[2 + e]);
+        pr[e] = pack2<TP>(p0 - a.x, p1 - a.y);
+        pr[2 + e] = pack2<TP>(p2 - b.x, p3 - b.y);
         if (__any_sync(0xffffffffu, f != 1.f)) {
 #pragma unroll
           for (int jj = 0; jj < DP / 8; ++jj) o[jj][2 * e] *= f, o[jj][2 * e + 1] *= f;
@@ -973,7 +968,7 @@ __device__ void stream_consumer(const AttnParams& P, StreamSmem<DP, C8>* sh, Wal
             for (int h = 0; h < 2; ++h)
               b[h] = e4m3x2_to_f16x2((uint16_t)(c & 1 ? x[h][c >> 1] >> 16 : x[h][c >> 1] & 0xffffu));
             mma16816<TP>(o[4 * k + c], pa, b[0], b[1]);
-            if constexpr (kRest) mma16816<TP>(o[4 * k + c], pr, b[0], b[1]);
+            mma16816<TP>(o[4 * k + c], pr, b[0], b[1]);
           }
         }
       } else {

@@ -560,8 +560,8 @@ FTB_API int ftb_rope_fp8(const ftb_rope_fp8_args* args, ftb_stream_t stream);
  * attn.v_strides in bytes (multiples of 16), D % 16 == 0, page >= scale_block; all else as there, the
  * workspace among it. Products are those of the codes: with q as it is in calls of many rows, with q in
  * f16 in the others (a bf16 row that f16 would not hold is taken times a power of two; what f16 drops is
- * below 2^-21 of the row's largest). The probabilities' operand is f16; where the output is f16 too, the
- * rest of that rounding is a second operand in calls of few rows.
+ * below 2^-21 of the row's largest). The probabilities' operand is f16, and in calls of few rows the rest of
+ * that rounding is a second one.
  */
 typedef struct ftb_attn_fp8_args {
   ftb_attn_args attn;
