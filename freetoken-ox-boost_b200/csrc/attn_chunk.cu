@@ -668,7 +668,7 @@ __device__ void chunk_load(const AttnParams& P, const AttnMaps& M, const Plan& p
       int id = 0, row = 0;
       if (mine) {
         const int key = key0 + lane * r;
-        id = __ldg(table + (key >> P.page_log2));
+        id = table[key >> P.page_log2];
         row = key & (page - 1);
         if (id < 0 || id >= P.num_pages) {
           atomicOr(P.status, kAttnBadPage);
@@ -813,7 +813,7 @@ __device__ void chunk_load8(const AttnParams& P, const AttnMaps& M, const Plan& 
       const bool has = lane < kGroups && box_of >= b0 && box_of < b1;
       int id = 0;
       if (has) {
-        id = __ldg(table + (key >> P.page_log2));
+        id = table[key >> P.page_log2];
         if (id < 0 || id >= P.num_pages) {
           atomicOr(P.status, kAttnBadPage);
           id = (int)P.num_pages;  // outside the tensor: reads zeros
@@ -822,8 +822,8 @@ __device__ void chunk_load8(const AttnParams& P, const AttnMaps& M, const Plan& 
       float ks = 1.f, vs = 1.f;
       if (has && id < P.num_pages) {
         const int block = (key & (page - 1)) >> P.block_log2;
-        ks = __ldg(P.k_scale + id * P.ks_st[0] + block * P.ks_st[1] + p.head * P.ks_st[2]);
-        vs = __ldg(P.v_scale + id * P.vs_st[0] + block * P.vs_st[1] + p.head * P.vs_st[2]);
+        ks = P.k_scale[id * P.ks_st[0] + block * P.ks_st[1] + p.head * P.ks_st[2]];
+        vs = P.v_scale[id * P.vs_st[0] + block * P.vs_st[1] + p.head * P.vs_st[2]];
       }
       const int box_id = __shfl_sync(0xffffffffu, id, (lane * r / kGroup) & (kGroups - 1));
       const bool mine = lane >= b0 && lane < b1;

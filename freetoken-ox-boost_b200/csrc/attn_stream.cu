@@ -262,15 +262,16 @@ __device__ void stream_producer(const AttnParams& P, const AttnMaps& M, StreamSm
       if (mbar_try_wait(&sh->full[u % kStages], (u / kStages) & 1u)) break;
 }
 
-// A load that keeps its place among volatile statements: asked for before the waits that hide it.
+// A load that keeps its place among volatile statements: asked for before the waits that hide it. (Coherent:
+// the kernel before this one, which writes the scales, may run beside this one's start.)
 __device__ __forceinline__ int ldg_now(const int32_t* p) {
   int r;
-  asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(r) : "l"(p));
+  asm volatile("ld.global.b32 %0, [%1];" : "=r"(r) : "l"(p));
   return r;
 }
 __device__ __forceinline__ float ldg_now(const float* p) {
   float r;
-  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(r) : "l"(p));
+  asm volatile("ld.global.f32 %0, [%1];" : "=f"(r) : "l"(p));
   return r;
 }
 
@@ -381,7 +382,7 @@ __device__ __forceinline__ float load_q8(const uint16_t* qp, bool in, int D,
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int d = h * 64 + tig * 16 + i * 8;
-      w[h][i] = in && d < D ? __ldg(reinterpret_cast<const uint4*>(qp + d)) : make_uint4(0, 0, 0, 0);
+      w[h][i] = in && d < D ? *reinterpret_cast<const uint4*>(qp + d) : make_uint4(0, 0, 0, 0);
     }
   float back = 1.f, by = 1.f;
   if constexpr (!std::is_same<T, __half>::value) {
