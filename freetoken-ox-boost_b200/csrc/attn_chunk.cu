@@ -819,8 +819,10 @@ __device__ void chunk_load8(const AttnParams& P, const AttnMaps& M, const Plan& 
           id = (int)P.num_pages;  // outside the tensor: reads zeros
         }
       }
-      float ks = 1.f, vs = 1.f;
-      if (has && id < P.num_pages) {
+      // (a block of the same page that no token sees may have any scale: it takes no part in the lowest)
+      const bool seen = has && key < p.hi && key + kGroup > p.lo;
+      float ks = 1.f, vs = seen ? 1.f : kMaxScale;
+      if (seen && id < P.num_pages) {
         const int block = (key & (page - 1)) >> P.block_log2;
         ks = P.k_scale[id * P.ks_st[0] + block * P.ks_st[1] + p.head * P.ks_st[2]];
         vs = P.v_scale[id * P.vs_st[0] + block * P.vs_st[1] + p.head * P.vs_st[2]];
@@ -841,7 +843,7 @@ __device__ void chunk_load8(const AttnParams& P, const AttnMaps& M, const Plan& 
         if (++stage == kStages) stage = 0, parity ^= 1u;
         if (v == 0) {
           const BlockScale b = block_scale(ks, vs);
-          float low = has ? b.v_log2 : INFINITY;
+          float low = b.v_log2;
 #pragma unroll
           for (int o = 1; o < kGroups; o <<= 1) low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
           if (lane < kGroups) sh->scale[sc][lane] = make_float4(b.k, b.v_log2, b.v_inv, low);
