@@ -170,7 +170,7 @@ class PagePool:
         """Makes room for ``new[b]`` tokens behind the ``past[b]`` of sequence b, whose list ``pages[b]``
         is changed in place: pages are added, and a page that others hold too and that the new tokens
         reach is replaced by one of its own (a copy where older tokens are in it). All sequences'
-        copies are one call; a MemoryError changes nothing. Returns how many pages were copied."""
+        copies are one call; an error changes nothing. Returns how many pages were copied."""
         if not len(pages) == len(past) == len(new):
             raise ValueError(f"{len(pages)} page lists, {len(past)} pasts, {len(new)} counts")
         if len({id(ids) for ids in pages}) != len(pages):
@@ -190,20 +190,21 @@ class PagePool:
                     want += 1
             want += max(0, last - len(ids))
         fresh = self.allocate(want)
+        copies = [(ids[j], to) for (ids, j, copied), to in zip(plan, fresh) if copied]
+        if copies:
+            try:  # (before anything is changed)
+                copy_pages(self.caches, [s for s, _ in copies], [d for _, d in copies])
+            except BaseException:
+                self.free(fresh)
+                raise
         fresh.reverse()
-        src, dst = [], []
-        for ids, j, copied in plan:
-            old, ids[j] = ids[j], fresh.pop()
-            self._held[old] -= 1
-            if copied:
-                src.append(old)
-                dst.append(ids[j])
+        for ids, j, _ in plan:
+            self._held[ids[j]] -= 1
+            ids[j] = fresh.pop()
         for ids, p, n in zip(pages, past, new):
             last = -(-(p + n) // self.page) if n else 0
             ids += [fresh.pop() for _ in range(max(0, last - len(ids)))]
-        if src:
-            copy_pages(self.caches, src, dst)
-        return len(src)
+        return len(copies)
 
     def compact(self, pages: list) -> int:
         """Moves the pages in use to the lowest ids, and changes the lists of all sequences (``pages``:
