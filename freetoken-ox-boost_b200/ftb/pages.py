@@ -92,15 +92,18 @@ def copy_pages(caches, src, dst) -> None:
     step = _GROUP
     if len(caches) > step or sum(t.dim() for t in caches) > 4 * step:
         step = min(step, max(1, 120 // (1 + max(t.dim() for t in caches))))
+    groups = []  # (all checked before the first launch)
     for at in range(0, len(caches), step):
         group = caches if len(caches) <= step else caches[at:at + step]
+        if at and group[0].shape[:1] != caches[0].shape[:1]:
+            raise ValueError(f"cache {at}: shape {tuple(group[0].shape)}, expected "
+                             f"{caches[0].shape[0]} pages in dimension 0")
         key = _pycall.key(src, dst, *group)
         known = _ARGS.get(key)
         if known is None:
-            if group[0].shape[:1] != caches[0].shape[:1]:
-                raise ValueError(f"cache {at}: shape {tuple(group[0].shape)}, expected "
-                                 f"{caches[0].shape[0]} pages in dimension 0")
             known = remember(key, _copy_args(group, src, dst), _OFFSETS[:len(group)] + _IDS)
+        groups.append((group, known))
+    for group, known in groups:
         dev = group[0].device
         st = caller(dev)(_lib.entry("ftb_copy_pages"), known[0], known[1], stream_handle(dev), *group,
                          src, dst)

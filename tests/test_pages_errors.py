@@ -40,3 +40,38 @@ def test_an_extension_of_caches_that_cannot_be_copied_changes_nothing():
     with pytest.raises(ValueError, match="CUDA"):
         pool.extend([b], [6], [1])
     assert account(pool, a, b) == before
+
+
+@pytest.fixture
+def launched(monkeypatch):
+    """Calls of the entry point, which copy nothing: the caches of each."""
+    calls = []
+
+    def call(entry, template, offsets, stream, *tensors):
+        calls.append(len(tensors) - 2)
+        return 0
+
+    monkeypatch.setattr(pages, "require_cuda", lambda *t: t[0].device)
+    monkeypatch.setattr(pages, "stream_handle", lambda device: 0)
+    monkeypatch.setattr(pages, "caller", lambda device: call)
+    monkeypatch.setattr(pages, "_ARGS", {})
+    monkeypatch.setattr(pages, "remember", lambda key, args, *extra: pages._ARGS.setdefault(
+        key, (bytes(args), *extra)))
+    return calls
+
+
+def test_caches_of_several_launches_are_checked_before_the_first(launched):
+    """Whether or not a part of the caches is known from a call of its own."""
+    many, fewer = [torch.zeros(6, 4) for _ in range(24)], [torch.zeros(5, 4) for _ in range(24)]
+    bad = [torch.zeros(6, 4) for _ in range(3)] + [torch.zeros(6, 4, 4)[:, :, :2]]
+    for caches in (many + fewer, many + bad, many + [torch.zeros(6, 4), torch.tensor(1.0)]):
+        with pytest.raises(ValueError):
+            ftb.copy_pages(caches, [0], [1])
+    assert launched == []
+    ftb.copy_pages(fewer, [0], [1])
+    ftb.copy_pages(many, [0], [1])
+    with pytest.raises(ValueError, match="6 pages"):
+        ftb.copy_pages(many + fewer, [0], [1])
+    assert launched == [24, 24]
+    ftb.copy_pages(many + many[:5], [0], [1])
+    assert launched == [24, 24, 24, 5]
