@@ -78,6 +78,8 @@ def copy_pages(caches, src, dst) -> None:
         caches = list(caches)
     if not caches:
         return
+    if caches[0].dim() < 1:
+        raise ValueError("cache 0 has no dimension of pages")
     if not isinstance(src, torch.Tensor) or not isinstance(dst, torch.Tensor):
         if not isinstance(src, torch.Tensor) and not isinstance(dst, torch.Tensor):
             src, dst = list(src), list(dst)

@@ -75,3 +75,9 @@ def test_caches_of_several_launches_are_checked_before_the_first(launched):
     assert launched == [24, 24]
     ftb.copy_pages(many + many[:5], [0], [1])
     assert launched == [24, 24, 24, 5]
+
+
+def test_a_cache_without_a_dimension(launched):
+    with pytest.raises(ValueError):
+        ftb.copy_pages([torch.tensor(1.0)], [0], [1])
+    assert launched == []
