@@ -19,7 +19,7 @@ class PagedKvCache:
     """Keys and values of one layer in pages: ``k``, ``v`` [num_pages, page, kv heads, D]. With
     ``dtype=torch.float8_e4m3fn`` in 8 bits, with ``k_scale``, ``v_scale`` float32 [num_pages,
     page / scale_block, kv heads] (``scale_block`` tokens per scale: 16, 32, 64 or 128; by default the
-    page, 128 at most)."""
+    largest of them that divides the page)."""
 
     def __init__(self, num_pages: int, page: int, kv_heads: int, head_dim: int,
                  dtype=torch.bfloat16, device="cuda", scale_block: int | None = None):
@@ -29,7 +29,9 @@ class PagedKvCache:
         self.page = page
         self.k_scale = self.v_scale = None
         if dtype == FP8:
-            size = min(page, 128) if scale_block is None else scale_block
+            size = scale_block
+            if size is None:
+                size = next((s for s in (128, 64, 32, 16) if page % s == 0), page)
             if size not in (16, 32, 64, 128) or page % size:
                 raise ValueError(f"{size} tokens per scale in pages of {page}: expected 16, 32, 64 or "
                                  "128 that divide the page")
