@@ -576,6 +576,15 @@ int ftb_rope_fp8(const ftb_rope_fp8_args* args, ftb_stream_t stream) {
     if (reinterpret_cast<uintptr_t>(args->workspace) & 3u) return FTB_ERR_ALIGN;
     A.token_at = reinterpret_cast<int32_t*>(static_cast<char*>(args->workspace) + FTB_ATTN_ZERO_BYTES);
   }
+  // every element and scale has an address of its own: thread blocks write them side by side
+  if (a->k_dst == a->v_dst || args->k_scale == args->v_scale) return FTB_ERR_ARG;
+  for (int i = 0; i < 2; ++i) {
+    const int64_t pages = a->n_slots / a->page;
+    if ((pages > 1 && (A.st[i][0] == 0 || A.scale_st[i][0] == 0)) || A.st[i][1] == 0 ||
+        (a->page > size && A.scale_st[i][1] == 0) ||
+        (a->Hkv > 1 && (A.st[i][2] == 0 || A.scale_st[i][2] == 0)))
+      return FTB_ERR_SHAPE;
+  }
   // the widest chunk that divides the turned and the copied part, and that every head of every
   // operand starts aligned to (16-bit tensors, bytes, and the table's floats)
   const int half = a->rot / 2;

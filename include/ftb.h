@@ -531,7 +531,8 @@ FTB_API int ftb_attention(const ftb_attn_args* args, ftb_stream_t stream);
 
 /*
  * ftb_rope() into an 8-bit cache: rope.k_dst and rope.v_dst are the caches (their strides in bytes),
- * rope.slots is required, rope.n_slots = pages * page, Hkv <= 1024.
+ * rope.slots is required, rope.n_slots = pages * page, Hkv <= 1024. Every element and every scale has an
+ * address of its own: no stride of 0 (of more than one), nothing shared by K and V.
  * For a block and head that the call writes to, with A the largest |x| that it writes there and 2^e the
  * smallest power of two with A <= 448 * 2^e, -40 <= e <= 40: the scale becomes 2^e where the call
  * writes the block's first row or the scale is no positive finite number, else the larger of 2^e and
