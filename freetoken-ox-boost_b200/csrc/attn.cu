@@ -139,6 +139,8 @@ static int attention(const ftb_attn_args* args, const ftb_attn_fp8_args* fp8, ft
   if (!std::isfinite(a->scale)) return FTB_ERR_ARG;
   if (!aligned16(a->q) || !aligned16(a->k_cache) || !aligned16(a->v_cache) || !aligned16(a->out))
     return FTB_ERR_ALIGN;
+  if (fp8 && ((reinterpret_cast<uintptr_t>(fp8->k_scale) | reinterpret_cast<uintptr_t>(fp8->v_scale)) & 3u))
+    return FTB_ERR_ALIGN;
   for (int i = 0; i < 3; ++i)
     if (a->k_strides[i] % (fp8 ? 16 : 8) || a->v_strides[i] % (fp8 ? 16 : 8) || a->k_strides[i] < 0 ||
         a->v_strides[i] < 0)

@@ -99,6 +99,8 @@ extern "C" int ftb_copy_pages(const ftb_pages_args* a, ftb_stream_t stream) {
     return FTB_ERR_SHAPE;
   if (a->n == 0 || a->n_caches == 0 || a->num_pages == 0) return FTB_OK;
   if (!a->src || !a->dst) return FTB_ERR_ARG;
+  if ((reinterpret_cast<uintptr_t>(a->src) | reinterpret_cast<uintptr_t>(a->dst)) & (a->id64 ? 7u : 3u))
+    return FTB_ERR_ALIGN;
   PagesParams P{};
   P.src = a->src, P.dst = a->dst, P.n = a->n, P.num_pages = a->num_pages, P.id64 = a->id64;
   int64_t pieces = 0;

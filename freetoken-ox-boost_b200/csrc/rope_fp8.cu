@@ -576,6 +576,8 @@ int ftb_rope_fp8(const ftb_rope_fp8_args* args, ftb_stream_t stream) {
     if (reinterpret_cast<uintptr_t>(args->workspace) & 3u) return FTB_ERR_ALIGN;
     A.token_at = reinterpret_cast<int32_t*>(static_cast<char*>(args->workspace) + FTB_ATTN_ZERO_BYTES);
   }
+  if ((reinterpret_cast<uintptr_t>(args->k_scale) | reinterpret_cast<uintptr_t>(args->v_scale)) & 3u)
+    return FTB_ERR_ALIGN;
   // every element and scale has an address of its own: thread blocks write them side by side
   if (a->k_dst == a->v_dst || args->k_scale == args->v_scale) return FTB_ERR_ARG;
   for (int i = 0; i < 2; ++i) {
