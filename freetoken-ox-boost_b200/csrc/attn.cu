@@ -22,9 +22,9 @@ CUtensorMapDataType attn_dtype(int type) {
 // rate gives: at most 1.1 GFLOP by the bound that the host knows (every token against the whole
 // table, or its window). On one B200, us (streaming / tensor cores), 32 heads over 8 of 128: prompts
 // of 64 tokens 7.6 / 18.0, 256 (1.1 GFLOP) 19.3 / 20.2, 300 35.2 / 21.6, 384 37.7 / 22.8, 512 53.7 /
-// 22.5; 16 tokens at 2048 keys (0.5 GFLOP) 17.4 / 20.6, 64 32.0 / 24.3. Over a cache of bytes: 64 8.8 /
-// 25.6, 256 18.6 / 25.5, 300 34.6 / 26.8, 512 45.6 / 28.8; 16 tokens at 2048 keys 21.1 / 23.6, 64 31.2 /
-// 27.2. Its row tiles are a grid's rows, so that many at most.
+// 22.5; 16 tokens at 2048 keys (0.5 GFLOP) 17.4 / 20.6, 64 32.0 / 24.3. Over a cache of bytes: 64 9.5 /
+// 25.9, 256 20.5 / 26.0, 300 37.5 / 27.2, 512 51.0 / 28.6; 16 tokens at 2048 keys 22.6 / 24.2, 64 34.7 /
+// 27.7. Its row tiles are a grid's rows, so that many at most.
 constexpr int kStreamRows = 16;
 constexpr double kStreamFlops = 1.1e9;
 // Of the two, a batch beyond the tensor-core kernel's plan goes to the streaming one.

@@ -103,7 +103,8 @@ __device__ __forceinline__ float2 unpack2(uint32_t v) {
 //   With t_j = log2(e) scale q.k_j + log2(vs_j), vs_j the scale of V: P'_j = 2^(t_j - M) is the weight of
 //   the code of v_j, so no scale is left outside, P' <= 1 for M the largest t, and
 //   out = sum P'_j c_j / l,  l = sum P'_j / vs_j,  lse = M + log2(l).
-//   P' and 1 / vs stay normal numbers wherever they matter: scales 2^80 apart at most.
+//   In fp32 P' and 1 / vs stay normal numbers wherever they matter: scales 2^80 apart at most. As an operand
+//   in f16 P' is exact to 2^-25 of the largest, that is of the largest weight times scale.
 constexpr float kMaxScale = 0x1p40f, kMinScale = 0x1p-40f;
 struct BlockScale {
   float k, v_log2, v_inv;  // scale of K; log2 and reciprocal of the scale of V

@@ -41,9 +41,10 @@
 // A cache of bytes (C8, attn.cuh has the arithmetic of its scales): tiles land as bytes, and warps 10 and
 // 11 turn them into 16-bit operands in place; P is f16, its reference a base-2 logarithm that starts at
 // the lowest scale of V in the first tile and may lag by 2^14; the scales come by plain loads of the
-// copying warp. The chunk above takes 2.24 ms so (0.56 of a large product's rate), the prompts 129 us, 12
-// ragged chunks in f16 50 us. Of a chunk of 2048 tokens at 16384 keys (636 us) the tensor pipe is active
-// 42 %, and 58 MB come from DRAM.
+// copying warp. The chunk above takes 2.25 ms so (0.57 of a large product's rate; the 16-bit kernel 1.92 on
+// the same GPU), 8 causal prompts of 53.8 GFLOP 129 us, 12 ragged chunks in f16 of 3.3 GFLOP 50 us: per
+// operation 0.85, 0.75 and 0.63 of the 16-bit kernel. Of a chunk of 2048 tokens at 16384 keys (636 us) the
+// tensor pipe is active 42 %, and 58 MB come from DRAM.
 //
 // k_attn_plan lists the pieces of a call (an item, or a part of its keys where items are too few
 // or too long to fill the SMs evenly), largest first; parts leave (ref, l, O) in the workspace and

@@ -1321,9 +1321,9 @@ int pick_stream(const ftb_attn_args& a, const AttnMaps& M, const AttnParams& P, 
 // Whether the form for few rows takes kv heads by pairs. That reads memory faster, but cuts half as many
 // pairs of sequence and heads into twice as many parts each, whose join is the end of a block's chain. By
 // what the host knows of the keys: where a block has at least 1.5 times as many tiles as a pair has parts.
-// On one B200, us (one head / pairs), 32 heads of 128 over 8: 1 token at 8192 keys 18.5 / 29.5, at 131072
-// 74.9 / 86.6; 2 at 32768 48.8 / 54.0, at 131072 124 / 113; 16 at 500 12.4 / 12.9; 64 at 300 21.6 / 19.7;
-// 61 at up to 8192 98 / 87; 3 at up to 131072 152 / 134.
+// On one B200, us (one head / pairs), 32 heads of 128 over 8: 1 token at 8192 keys 18.8 / 29.8, at 131072
+// 75.7 / 86.8; 2 at 32768 47.8 / 54.4, at 131072 123 / 114; 16 at 500 12.6 / 13.3; 64 at 300 23.1 / 21.2;
+// 61 at up to 8192 97 / 89; 3 at up to 131072 150 / 130.
 bool pair_heads(const ftb_attn_args& a) {
   if (a.Hkv % 2) return false;
   const double blocks = stream_blocks(1), pairs = 0.5 * a.batch * a.Hkv;

@@ -23,8 +23,8 @@
 // table, the slots, the tokens, then the second pass over them, which comes from L1), so they come first
 // in the grid and the tokens' q, a plain stream, fills the SMs beside them: registers are kept low for
 // both. With four items a thread kept in fp32 (171 registers, one block per SM) and q in a launch of its
-// own, 20440 tokens of 32 + 8 + 8 heads of 128 took 243 us; they take 104, 4.2 TB/s, 0.67 of the measured
-// copy rate; 64 tokens of 64 sequences 6.6 us.
+// own, 19106 tokens of 32 + 8 + 8 heads of 128 took 243 us; they take 104, 4.2 TB/s, 0.66 of the measured
+// copy rate; 64 tokens of 64 sequences 6.7 us.
 #include "rope.cuh"
 
 namespace ftb {
@@ -36,10 +36,11 @@ constexpr int kKept = 1;         // items of a thread that stay in registers
 constexpr int kItems = 8;        // items of a thread that a thread block is made for
 constexpr int kMaxBlock = 128;   // tokens per scale
 constexpr int kMaxHeads = 256;   // of a thread block
-// Tokens up to which the slots are scanned (one prompt of 2048 tokens 22.8 us, by the table 24.5; 2048
-// tokens of as many sequences 85 against 72), and up to which a block's tokens share its heads (a prompt
-// of 512 tokens 11.1 us, by owners 17.5, of 2048 31.7 and 22.8; 256 tokens of as many sequences 8.6 and
-// 11.8).
+// Tokens up to which the slots are scanned (one prompt of 1280 tokens 19.8 us, by the table 21.6, of 2048
+// 24.3 and 26.5; as many sequences of one token lose: 1280 59 against 55, 2048 90 against 79), and up to
+// which a block's tokens share its heads (us, shared / by owners: a prompt of 600 tokens 12.2 / 17.3, 1024
+// 18.0 / 19.8, 1280 21.8 / 19.8, 2048 36 / 24; as many sequences of one token 600 18 / 29, 1024 28 / 43,
+// 1280 35 / 59).
 constexpr int kScan = 2048, kTogether = 1024;
 static_assert(kTogether <= kScan, "what is shared is scanned for");
 constexpr int kMaxRange = 64;    // tokens per thread block beyond that, at most

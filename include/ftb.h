@@ -525,7 +525,7 @@ FTB_API int ftb_attention(const ftb_attn_args* args, ftb_stream_t stream);
  * Keys and values in e4m3, [pages, page, Hkv, D] bytes by strides {page, row, head}, with one fp32
  * scale for each block of scale_block tokens of a page and kv head, [pages, page / scale_block, Hkv] by
  * strides {page, block, head} in floats: a byte c stands for c * scale. scale_block is a power of two,
- * 16 <= scale_block <= 128, that divides the page. Scales are positive and finite; the calls below use
+ * 16 <= scale_block <= 128, that divides the page. Scales are positive and finite; the attention uses
  * 2^-40 for a smaller one (or NaN) and 2^40 for a larger one.
  */
 
@@ -538,8 +538,10 @@ FTB_API int ftb_attention(const ftb_attn_args* args, ftb_stream_t stream);
  * writes the block's first row or the scale is no positive finite number, else the larger of 2^e and
  * the scale so far (rounded up to a power of two). The rows written are x / scale, rounded to e4m3 from
  * fp32 (infinite x to +-448, NaN stays); where the scale changed, the block's other rows below the last
- * one written are rounded again. Rows past the last one written, and blocks without one, stay as they
- * are. Tokens may come in any order; of two tokens with the same slot one is kept, whole.
+ * one written are rounded again, as their bytes times the scale that was there (bytes whose scale was no
+ * positive finite number stand for nothing, and stay). Rows past the last one written, and blocks
+ * without one, stay as they are. Tokens may come in any order; of two tokens with the same slot one is
+ * kept, whole.
  * workspace: ftb_rope_fp8_workspace_bytes() bytes, 4-byte aligned, for calls of one stream order. It
  * may be the one of ftb_attention(): its first FTB_ATTN_ZERO_BYTES bytes are not touched, and the rest
  * may hold anything. Calls of up to 2048 tokens take none (it may be NULL).
